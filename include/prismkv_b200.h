@@ -27,6 +27,8 @@
  *   pkv_lse_combine    (new) log-sum-exp merge of split-sequence partials
  *   pkv_attn_decode_xr (new) split-sequence decode with the cross-GPU merge
  *                      inside the attention kernel (pkv_xr_* set it up)
+ *   pkv_paged_attn, pkv_pages_*, pkv_tokens_* (new) attention, page selection and
+ *                      eviction over a paged code cache
  */
 #ifndef PRISMKV_B200_H
 #define PRISMKV_B200_H
@@ -305,6 +307,107 @@ PKV_API int pkv_polar_scores(const float *q_rot, const void *k_codes, int32_t co
                      int32_t B, int32_t H, int32_t Sq, int32_t Sk, int32_t dim,
                      const float *q_params, const int32_t *bits, float *out,
                      void *stream);
+
+/* ---- paged code caches --------------------------------------------------- *
+ * A pool of num_pages pages; a page holds page_size token slots of every KV
+ * head.  Slot r of KV head hk of page i starts at
+ *     k + i*page_stride + hk*head_stride + r*token_stride        (in codes)
+ * and holds the m codes of one token (the same in v).  Row b of the page
+ * table names sequence b's pages: token t sits in slot t % page_size of page
+ * table[b*table_stride + t / page_size].  page_size is a power of two, 16 to
+ * 1024; k, v and the three strides are multiples of 16 bytes.
+ * Page ids outside [0, num_pages) are never followed: their tokens count as
+ * masked and the device error word is set to 6.  Sequence lengths are read on
+ * the device, clamped to [0, max_pages * page_size].                        */
+typedef struct pkv_pages {
+    const void *k, *v;
+    int32_t code_bytes;                          /* 1 (uint8) or 2 (u/int16)     */
+    int32_t num_pages, kv_heads, page_size;
+    int64_t page_stride, head_stride, token_stride;   /* codes                   */
+    const int32_t *table;                        /* device (batch, max_pages)    */
+    int64_t table_stride;
+    int32_t batch, max_pages;
+} pkv_pages;
+
+/* Decode attention over a paged cache (the mathematics of pkv_attn_decode).
+ * selected: optional device (batch, kv_heads, n_selected) logical page indexes,
+ * strictly ascending and padded with -1; only their tokens are attended (an
+ * entry that does not ascend is skipped and sets the device error word to 6).
+ * weights / weights_out (both or neither): (batch, kv_heads, slots) f32 rows of
+ * weights_row_stride floats; every attended token t gets
+ *     weights_out[b, hk, t] = weights[b, hk, t] + sum over hk's query heads of p(t)
+ * (the two may be the same buffer); other entries are not touched.  A row with
+ * no attended token gives zeros.  The workspace needs no initialisation and
+ * belongs to one call until that call's kernels are done.                    */
+typedef struct pkv_paged_attn_args {
+    pkv_pages pages;
+    int32_t q_heads, q_dtype;
+    const void *q;                               /* (batch, q_heads, dim)        */
+    int64_t q_batch_stride, q_head_stride;
+    const int32_t *seq_lens;                     /* device (batch)               */
+    const int32_t *selected;
+    int32_t n_selected;
+    float scale;
+    void *out;                                   /* (batch, q_heads, dim) of out_dtype */
+    int32_t out_dtype;
+    int64_t out_batch_stride, out_head_stride;
+    const float *weights;
+    float *weights_out;
+    int64_t weights_row_stride;
+    int32_t weights_slots;
+} pkv_paged_attn_args;
+PKV_API size_t pkv_paged_attn_workspace_size(const pkv_codec *c, const pkv_paged_attn_args *a);
+PKV_API int pkv_paged_attn(const pkv_codec *c, const pkv_paged_attn_args *a, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
+/* Copies n rows of m codes per (sequence, KV head) -- codes (batch, kv_heads, n,
+ * m) contiguous -- into slots start[b] .. start[b] + min(n, counts[b]) - 1 of
+ * the paged K (or V) cache `dst` (the k pointer of `pages` is ignored).
+ * counts may be NULL (n each).  Slots past the table are dropped and set the
+ * device error word to 6.                                                    */
+PKV_API int pkv_pages_store(const pkv_pages *pages, int32_t m, void *dst, const void *codes, int32_t n,
+                            const int32_t *start, const int32_t *counts, void *stream);
+
+/* Summaries of K pages: for every page of sequence b that holds a token >=
+ * start[b] (start NULL: every page), per KV head and rotated channel d (3 m of
+ * them), the floor of the least and the ceiling of the greatest decoded value
+ * of the page's tokens on a grid of 1/127 of the codec's largest magnitude:
+ *     summaries + ((page * kv_heads + hk) * 2 + {0: least, 1: greatest}) * pitch + d
+ * with pitch = dim rounded up to 16 (int8; the padding is set to 0).  grid_z
+ * (2^bits_z) and grid_xy (2^bits_total, 2) are the decoded values in 1/128
+ * grid steps (int16, device).                                               */
+PKV_API int pkv_pages_summarize(const pkv_codec *c, const pkv_pages *pages, const int32_t *seq_lens,
+                                const int32_t *start, const int16_t *grid_z, const int16_t *grid_xy,
+                                int8_t *summaries, void *stream);
+
+/* Pages worth attending to: the query of every head, rotated (64 bits) and
+ * rounded to int8 on the group's common scale (largest magnitude of the KV
+ * head's query heads at 127), scores a page by
+ *     max over the group's heads of sum_d (q_d > 0 ? q_d greatest_d : q_d least_d),
+ * an upper bound of its tokens' scores.  The first `sinks` and the last
+ * `recent` pages of a sequence are always taken; the others by score, ties by
+ * the lower index.  out (batch, kv_heads, top): logical page indexes,
+ * ascending, -1 behind the last.  sinks + recent <= top.                     */
+PKV_API int pkv_pages_select(const pkv_codec *c, const pkv_pages *pages, const void *q, int32_t q_dtype,
+                             int32_t q_heads, int64_t q_batch_stride, int64_t q_head_stride,
+                             const int32_t *seq_lens, const int8_t *summaries, int32_t top, int32_t sinks,
+                             int32_t recent, int32_t *out, void *stream);
+
+/* Tokens worth keeping: of the first seq_lens[b] entries of every weight row
+ * (batch, kv_heads, slots; row stride in floats) the first `sinks`, the last
+ * `recent` and then those of the largest weight, `keep` in all; ties by the
+ * lower slot, NaN below every number.  kept (batch, kv_heads, keep): slots,
+ * ascending, -1 behind the last; kept_weights (same shape): their weights, 0
+ * behind the last.  sinks + recent <= keep.                                  */
+PKV_API int pkv_tokens_select(const float *weights, int32_t batch, int32_t kv_heads, int32_t slots,
+                              int64_t row_stride, const int32_t *seq_lens, int32_t keep, int32_t sinks,
+                              int32_t recent, int32_t *kept, float *kept_weights, void *stream);
+
+/* Copies the codes of slots kept[b, hk, i] (i < keep; negative entries are
+ * skipped) from `src` to slots i of `dst`, K and V.  The destination pages
+ * must not be among the source pages that are read.                          */
+PKV_API int pkv_tokens_gather(const pkv_pages *src, int32_t m, const int32_t *kept, int32_t keep,
+                              const pkv_pages *dst, void *dst_k, void *dst_v, void *stream);
 
 #ifdef __cplusplus
 }

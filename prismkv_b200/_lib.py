@@ -26,7 +26,9 @@ EXPORTED = ("pkv_abi_version", "pkv_strerror", "pkv_device_error", "pkv_encode",
             "pkv_attn_workspace_size", "pkv_workspace_init", "pkv_attn_decode", "pkv_lse_combine",
             "pkv_polar_scores", "pkv_attn_decode_noalloc", "pkv_attn_describe", "pkv_encode_append",
             "pkv_decode_cache", "pkv_lse_combine_gather", "pkv_xr_layout_for", "pkv_xr_alloc", "pkv_xr_open",
-            "pkv_xr_close", "pkv_xr_free", "pkv_xr_reset", "pkv_attn_decode_xr")
+            "pkv_xr_close", "pkv_xr_free", "pkv_xr_reset", "pkv_attn_decode_xr", "pkv_paged_attn_workspace_size",
+            "pkv_paged_attn", "pkv_pages_store", "pkv_pages_summarize", "pkv_pages_select", "pkv_tokens_select",
+            "pkv_tokens_gather")
 XR_MAX_RANKS = 8
 IPC_HANDLE_BYTES = 64
 
@@ -63,6 +65,22 @@ class PkvExchange(ctypes.Structure):
 
 class PkvXrLayout(ctypes.Structure):
     _fields_ = [("bytes", ctypes.c_uint64), ("out_offset", ctypes.c_uint64), ("rows", c_int32), ("units", c_int32)]
+
+
+class PkvPages(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("code_bytes", c_int32),
+                ("num_pages", c_int32), ("kv_heads", c_int32), ("page_size", c_int32),
+                ("page_stride", c_int64), ("head_stride", c_int64), ("token_stride", c_int64),
+                ("table", c_void_p), ("table_stride", c_int64), ("batch", c_int32), ("max_pages", c_int32)]
+
+
+class PkvPagedAttnArgs(ctypes.Structure):
+    _fields_ = [("pages", PkvPages), ("q_heads", c_int32), ("q_dtype", c_int32), ("q", c_void_p),
+                ("q_batch_stride", c_int64), ("q_head_stride", c_int64), ("seq_lens", c_void_p),
+                ("selected", c_void_p), ("n_selected", c_int32), ("scale", c_float),
+                ("out", c_void_p), ("out_dtype", c_int32), ("out_batch_stride", c_int64), ("out_head_stride", c_int64),
+                ("weights", c_void_p), ("weights_out", c_void_p), ("weights_row_stride", c_int64),
+                ("weights_slots", c_int32)]
 
 
 KERNEL_NAMES = {1: "attn_mha12_kernel", 2: "attn_polar_kernel", 3: "attn_lut_kernel", 4: "attn_tc_kernel",
@@ -120,6 +138,23 @@ def _declare(lib):
     lib.pkv_xr_reset.argtypes = [P(PkvCodec), P(PkvAttnArgs), P(PkvExchange), c_void_p]
     lib.pkv_attn_decode_xr.restype = c_int32
     lib.pkv_attn_decode_xr.argtypes = [P(PkvCodec), P(PkvAttnArgs), c_void_p, c_size_t, P(PkvExchange), c_void_p]
+    lib.pkv_paged_attn_workspace_size.restype = c_size_t
+    lib.pkv_paged_attn_workspace_size.argtypes = [P(PkvCodec), P(PkvPagedAttnArgs)]
+    lib.pkv_paged_attn.restype = c_int32
+    lib.pkv_paged_attn.argtypes = [P(PkvCodec), P(PkvPagedAttnArgs), c_void_p, c_size_t, c_void_p]
+    lib.pkv_pages_store.restype = c_int32
+    lib.pkv_pages_store.argtypes = [P(PkvPages), c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]
+    lib.pkv_pages_summarize.restype = c_int32
+    lib.pkv_pages_summarize.argtypes = [P(PkvCodec), P(PkvPages), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                        c_void_p]
+    lib.pkv_pages_select.restype = c_int32
+    lib.pkv_pages_select.argtypes = [P(PkvCodec), P(PkvPages), c_void_p, c_int32, c_int32, c_int64, c_int64, c_void_p,
+                                     c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p]
+    lib.pkv_tokens_select.restype = c_int32
+    lib.pkv_tokens_select.argtypes = [c_void_p, c_int32, c_int32, c_int32, c_int64, c_void_p, c_int32, c_int32, c_int32,
+                                      c_void_p, c_void_p, c_void_p]
+    lib.pkv_tokens_gather.restype = c_int32
+    lib.pkv_tokens_gather.argtypes = [P(PkvPages), c_int32, c_void_p, c_int32, P(PkvPages), c_void_p, c_void_p, c_void_p]
     lib.pkv_polar_scores.restype = c_int32
     lib.pkv_polar_scores.argtypes = [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
                                      P(c_float), P(c_int32), c_void_p, c_void_p]

@@ -3,8 +3,9 @@
 ``DeviceCodec`` owns one device copy of a quantizer's tables (rotation,
 thresholds, LUTs) and exposes the hot-path operations on CUDA tensors:
 ``encode``, ``decode``, ``attention`` (fused dequant + flash decoding) and
-``combine`` (log-sum-exp merge of split-sequence partials).  All compute runs
-in libprismkv_b200.so; torch only provides memory and streams.
+``combine`` (log-sum-exp merge of split-sequence partials), and those over a
+paged cache (``paged.PagedOps``).  All compute runs in libprismkv_b200.so;
+torch only provides memory and streams.
 """
 
 from __future__ import annotations
@@ -17,6 +18,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .paged import PagedOps
 from .tables import HostTables
 
 CODE_DTYPES = {torch.uint8: 1, torch.int16: 2, torch.uint16: 2, torch.int64: 8}
@@ -52,7 +54,7 @@ def split_bf16x3(R: np.ndarray) -> np.ndarray:
     return np.stack(parts)
 
 
-class DeviceCodec:
+class DeviceCodec(PagedOps):
     def __init__(self, host: HostTables, device: torch.device):
         self.host = host
         self.device = torch.device(device)

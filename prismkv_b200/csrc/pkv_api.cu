@@ -27,6 +27,7 @@ int launch_lse_combine_gather(const pkv_codec* c, const float* const* part_ptrs,
                               int rows, float* out, int64_t out_rs, cudaStream_t st);
 int launch_polar_scores(const float* q, const void* kc, int cb, int B, int H, int Sq, int Sk, int dim,
                         const float* qp, const int32_t* bits, float* out, cudaStream_t st);
+int paged_device_error(int32_t* flag_out, int32_t clear);     // the paged kernels' own error word
 }  // namespace pkv
 
 namespace {
@@ -74,7 +75,7 @@ const char* pkv_strerror(int status) {
         case PKV_ERR_ALIGNMENT: return "misaligned pointer or stride";
         case PKV_ERR_WORKSPACE: return "workspace missing or too small";
         case PKV_ERR_CUDA: return "CUDA runtime error";
-        case PKV_ERR_DEVICE: return "device-side error flag set (a bounded wait expired)";
+        case PKV_ERR_DEVICE: return "device-side error flag set (a bounded wait expired or a page index was out of range)";
         case PKV_ERR_SCRATCH_LIMIT:
             return "arguments need more split scratch than the static array of pkv_attn_decode_noalloc holds "
                    "(8 MiB - 64 KiB of partials, 16384 split counters); use pkv_attn_decode with a workspace";
@@ -89,7 +90,10 @@ int pkv_device_error(int32_t* flag_out, int32_t clear) {
         const int32_t zero = 0;
         if (cudaMemcpyToSymbol(pkv::g_device_error, &zero, sizeof(int32_t)) != cudaSuccess) return PKV_ERR_CUDA;
     }
-    return PKV_OK;
+    int32_t paged = 0;
+    const int rc = pkv::paged_device_error(&paged, clear);
+    if (*flag_out == 0) *flag_out = paged;
+    return rc;
 }
 
 int pkv_encode(const pkv_codec* c, const void* x, int32_t x_dtype, int64_t n, int64_t x_stride, void* codes,

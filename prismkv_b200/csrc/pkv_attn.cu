@@ -44,6 +44,7 @@
 #include <cmath>
 
 #include "pkv_common.cuh"
+#include "pkv_mma.cuh"
 
 namespace pkv {
 

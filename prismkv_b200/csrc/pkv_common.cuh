@@ -14,12 +14,15 @@
 
 namespace pkv {
 
-// Device error word: set when a bounded wait expires; read by pkv_device_error.
-__device__ int32_t g_device_error = 0;   // single definition: the library is one translation unit
+// Device error word, one per translation unit: set when a bounded wait expires or a page index is
+// out of range; pkv_device_error reads them all.
+static __device__ int32_t g_device_error = 0;
 
 // 4: a split-sequence exchange waited past its bound for the other ranks' outputs
 // 5: a kernel found its dynamic shared window at another address than its layout assumes
-enum : int32_t { kErrWaitFull = 1, kErrWaitEmpty = 2, kErrWaitDrain = 3, kErrPeerWait = 4, kErrSmemLayout = 5 };
+// 6: a page table, page list or slot list named something outside the cache
+enum : int32_t { kErrWaitFull = 1, kErrWaitEmpty = 2, kErrWaitDrain = 3, kErrPeerWait = 4, kErrSmemLayout = 5,
+                 kErrPage = 6 };
 
 __device__ __forceinline__ void flag_error(int32_t code) { atomicCAS(&g_device_error, 0, code); }
 

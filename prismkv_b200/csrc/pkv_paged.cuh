@@ -1,0 +1,209 @@
+// pkv_paged.cuh -- what the kernels over a paged code cache share: the page descriptor on the
+// device, how a sequence's tokens are found, and how attention work is cut into ranges.
+#pragma once
+
+#include "pkv_common.cuh"
+#include "pkv_mma.cuh"
+
+namespace pkv {
+
+constexpr int kGranule = 16;                  // tokens per granule; pages hold whole granules
+
+// The pages of a cache, strides in bytes.
+struct Pages {
+    const uint8_t *k, *v;
+    int64_t page_bs, head_bs, tok_bs;
+    const int32_t* table;
+    int64_t table_stride;
+    int num_pages, Hkv, ps_log2, B, max_pages;
+};
+
+__device__ __forceinline__ int clamp_len(const Pages& g, int len) {
+    const int64_t cap = (int64_t)g.max_pages << g.ps_log2;
+    return (int)min((int64_t)max(len, 0), cap);
+}
+
+// Physical page of logical page j of sequence b, or -1 (and the error word) when the table names none.
+__device__ __forceinline__ int page_of(const Pages& g, int b, int j) {
+    if ((unsigned)j >= (unsigned)g.max_pages) {
+        flag_error(kErrPage);
+        return -1;
+    }
+    const int page = __ldg(g.table + (int64_t)b * g.table_stride + j);
+    if ((unsigned)page >= (unsigned)g.num_pages) {
+        flag_error(kErrPage);
+        return -1;
+    }
+    return page;
+}
+
+__device__ __forceinline__ int64_t slot_offset(const Pages& g, int page, int hk, int r) {
+    return (int64_t)page * g.page_bs + (int64_t)hk * g.head_bs + (int64_t)r * g.tok_bs;
+}
+
+// ---- attention ---------------------------------------------------------------------------------
+// A unit is up to HQ query heads of one (sequence, KV head); units are numbered sequence-major.  Its
+// tokens are the sequence's (or the listed pages', in list order) in granules of 16.  The granules of
+// all units form one line of T granules; CTA c of `grid` takes granules [c T / Gd, (c + 1) T / Gd) with
+// Gd = min(grid, T), so ragged sequences load every CTA alike.  Each (CTA, unit) range leaves one
+// partial softmax state; range (c, u) uses partial row c + u, so a unit's rows lie side by side.
+struct PagedParams {
+    Pages pg;
+    int Hq, G, HQ, UG, UH, dim, m, cb;         // UG units per KV head, UH = Hkv * UG per sequence
+    const void* q; int qdt; int64_t q_bs, q_hs;
+    const int32_t* seq_lens;
+    const int32_t* selected; int n_sel;
+    float scale_log2;
+    void* out; int odt; int64_t out_bs, out_hs;
+    const float* w_in; float* w_out; int64_t w_rs; int w_slots;
+    const float *R, *dec_z, *dec_xy;
+    int bits_z, bits_flat, xy_per_z;
+    float* part;                               // [grid + units][HQ][dim + 2]: m (log2 units), l, o
+    float* raw; int64_t raw_us; int raw_h;     // scores of every token, [unit][granule * 16][raw_h]
+    int grid, units;
+};
+
+__device__ __forceinline__ int granules_of(const PagedParams& p, int b) {
+    if (p.selected) return p.n_sel << (p.pg.ps_log2 - 4);
+    return (clamp_len(p.pg, __ldg(p.seq_lens + b)) + kGranule - 1) / kGranule;
+}
+
+// Granules of the sequences before b, and of all of them (times UH: the line of all units).  Whole warps.
+__device__ inline void granule_line(const PagedParams& p, int b, int64_t& before, int64_t& total) {
+    int64_t sb = 0, st = 0;
+    if (p.selected) {
+        const int64_t n = (int64_t)granules_of(p, 0) * p.UH;
+        before = n * b;
+        total = n * p.pg.B;
+        return;
+    }
+    const int lane = threadIdx.x & 31;
+    for (int i = lane; i < p.pg.B; i += 32) {
+        const int n = granules_of(p, i);
+        st += n;
+        if (i < b) sb += n;
+    }
+    #pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) {
+        sb += __shfl_xor_sync(0xffffffffu, sb, off);
+        st += __shfl_xor_sync(0xffffffffu, st, off);
+    }
+    before = sb * p.UH;
+    total = st * p.UH;
+}
+
+struct PagedItem { int b, hk, hg, unit, g0, g1, row; };     // granules [g0, g1) of the unit, partial row
+
+struct PagedCursor { int64_t t, end, base; int b; };
+
+// Whole warps; every warp of the CTA walks the same items.
+__device__ inline PagedCursor paged_begin(const PagedParams& p) {
+    PagedCursor c;
+    int64_t total, before;
+    granule_line(p, 0, before, total);
+    const int64_t gd = min((int64_t)p.grid, total);
+    c.b = 0;
+    c.base = 0;
+    if ((int64_t)blockIdx.x >= gd) {
+        c.t = c.end = 0;
+        return c;
+    }
+    c.t = (int64_t)blockIdx.x * total / gd;
+    c.end = (int64_t)(blockIdx.x + 1) * total / gd;
+    // the sequence of granule t: 32 sequences at a time
+    const int lane = threadIdx.x & 31;
+    for (int b0 = 0; b0 < p.pg.B; b0 += 32) {
+        const int64_t n = (b0 + lane < p.pg.B) ? (int64_t)granules_of(p, b0 + lane) * p.UH : 0;
+        int64_t inc = n;
+        #pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, inc, off);
+            if (lane >= off) inc += v;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, c.base + inc > c.t);
+        if (past) {
+            const int f = __ffs(past) - 1;
+            c.b = b0 + f;
+            c.base += __shfl_sync(0xffffffffu, inc - n, f);
+            return c;
+        }
+        c.base += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return c;
+}
+
+__device__ inline bool paged_next(const PagedParams& p, PagedCursor& c, PagedItem& it) {
+    while (c.t < c.end) {
+        const int n = granules_of(p, c.b);
+        const int64_t off = c.t - c.base;
+        if (off >= (int64_t)n * p.UH) {
+            c.base += (int64_t)n * p.UH;
+            ++c.b;
+            continue;
+        }
+        const int u = (int)(off / n);
+        it.b = c.b;
+        it.hk = u / p.UG;
+        it.hg = u % p.UG;
+        it.unit = c.b * p.UH + u;
+        it.g0 = (int)(off - (int64_t)u * n);
+        it.g1 = (int)min((int64_t)n, it.g0 + (c.end - c.t));
+        it.row = blockIdx.x + it.unit;
+        c.t += it.g1 - it.g0;
+        return true;
+    }
+    return false;
+}
+
+// Where granule gi of (b, hk) lies: its physical page (-1: masked), the slot of its first token in the
+// page, and the token that slot holds.
+struct Granule { int page, slot, tok; };
+
+__device__ __forceinline__ Granule granule_at(const PagedParams& p, int b, int hk, int gi) {
+    const int per = p.pg.ps_log2 - 4;                       // log2 of granules per page
+    const int j = gi >> per;
+    Granule g;
+    g.slot = (gi & ((1 << per) - 1)) << 4;
+    int lp = j;
+    if (p.selected) {
+        const int32_t* s = p.selected + ((int64_t)b * p.pg.Hkv + hk) * p.n_sel + j;
+        lp = __ldg(s);
+        if (lp < 0 || (j > 0 && __ldg(s - 1) >= lp)) {      // padding, or not ascending
+            if (lp >= 0) flag_error(kErrPage);
+            lp = -1;
+        } else if (j > 0 && __ldg(s - 1) < 0) {
+            flag_error(kErrPage);
+            lp = -1;
+        }
+    }
+    g.tok = (lp << p.pg.ps_log2) + g.slot;
+    g.page = -1;
+    if (lp >= 0) {
+        if (p.selected && (int64_t)lp << p.pg.ps_log2 >= clamp_len(p.pg, __ldg(p.seq_lens + b))) {
+            flag_error(kErrPage);                           // a listed page behind the sequence's end
+            g.tok = 0x7ffffff0;
+        } else {
+            g.page = page_of(p.pg, b, lp);
+        }
+    }
+    return g;
+}
+
+template <int DT>
+__device__ __forceinline__ float load_as(const void* q, int64_t i) {
+    return Elem<DT>::load(static_cast<const typename Elem<DT>::T*>(q) + i);
+}
+
+__device__ __forceinline__ float load_any(const void* q, int dt, int64_t i) {
+    if (dt == PKV_F32) return load_as<PKV_F32>(q, i);
+    if (dt == PKV_BF16) return load_as<PKV_BF16>(q, i);
+    return load_as<PKV_F16>(q, i);
+}
+
+__device__ __forceinline__ void store_any(void* o, int dt, int64_t i, float v) {
+    if (dt == PKV_F32) Elem<PKV_F32>::store(static_cast<float*>(o) + i, v);
+    else if (dt == PKV_BF16) Elem<PKV_BF16>::store(static_cast<__nv_bfloat16*>(o) + i, v);
+    else Elem<PKV_F16>::store(static_cast<__half*>(o) + i, v);
+}
+
+}  // namespace pkv

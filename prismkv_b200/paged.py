@@ -1,0 +1,338 @@
+"""Calls over a paged cache of packed codes: the paged half of ``DeviceCodec``.
+
+A pool of pages holds K and V codes as (num_pages, kv_heads, page_size, m)
+tensors (``empty_pages`` makes one); row b of an int32 ``page_table``
+(batch, max_pages) names sequence b's pages in order and int32 ``seq_lens``
+(batch) its tokens, both on the codec's device.  Token t of sequence b sits in
+slot ``t % page_size`` of page ``page_table[b, t // page_size]``; entries past
+the last token are never read.  ``page_size`` is a power of two, 16 to 1024.
+Any strides serve whose rows start on 16-byte boundaries with unit code stride,
+so (num_pages, page_size, kv_heads, m) pools pass as transposed views.
+
+Nothing here synchronises, keeps state between calls or allocates beyond its
+outputs and a workspace from torch's allocator, so every call can be captured
+into a CUDA graph.  A page id outside the pool, a token past the table or a
+page list out of order is skipped on the device and shows in
+``_lib.device_error()`` as 6.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import numpy as np
+import torch
+
+from . import _lib
+
+PAGE_CODE_DTYPES = {torch.uint8: 1, torch.int16: 2, torch.uint16: 2}
+ROW_BYTES = 16          # code rows start on multiples of this
+
+
+def _summary_grid(dec_z: np.ndarray, dec_xy: np.ndarray, total_codes: int) -> Tuple[np.ndarray, np.ndarray]:
+    """Decoded values on the summaries' grid in 1/128 steps, the largest magnitude at 127 steps (int16)."""
+    z, xy = dec_z.astype(np.float64).reshape(-1), dec_xy.astype(np.float64).reshape(-1, 2)
+    top = max(np.abs(z).max(), np.abs(xy).max())
+    f = 127.0 * 128.0 / top if top > 0 else 0.0
+    xy = np.tile(xy, (total_codes // xy.shape[0], 1))
+    return np.rint(z * f).astype(np.int16), np.rint(xy * f).astype(np.int16)
+
+
+class PagedOps:
+    """Mixed into DeviceCodec: needs its struct, host, device, dim, m, bits_total and stream."""
+
+    # ------------------------------------------------------------------
+    def empty_pages(self, num_pages: int, kv_heads: int, page_size: int,
+                    code_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """Uninitialised (num_pages, kv_heads, page_size, m) codes with rows on 16-byte boundaries."""
+        if code_dtype is None:
+            code_dtype = torch.uint8 if self.bits_total <= 8 else torch.int16
+        if code_dtype not in PAGE_CODE_DTYPES:
+            raise ValueError("codes must be stored as uint8 or 16-bit integers")
+        per = ROW_BYTES // PAGE_CODE_DTYPES[code_dtype]
+        pitch = -(-self.m // per) * per
+        return torch.empty((num_pages, kv_heads, page_size, pitch), dtype=code_dtype, device=self.device)[..., :self.m]
+
+    @property
+    def summary_pitch(self) -> int:
+        """Bytes per summary row: dim rounded up to 16."""
+        return -(-self.dim // 16) * 16
+
+    def empty_summaries(self, num_pages: int, kv_heads: int) -> torch.Tensor:
+        """Uninitialised (num_pages, kv_heads, 2, summary_pitch) int8 page summaries."""
+        return torch.empty((num_pages, kv_heads, 2, self.summary_pitch), dtype=torch.int8, device=self.device)
+
+    # ------------------------------------------------------------------
+    def _on_device(self, t: torch.Tensor, name: str) -> None:
+        _lib.require_cuda(t, name)
+        if t.device != self._dev:
+            raise ValueError(f"{name} is on {t.device}, the codec on {self.device}")
+
+    @property
+    def _dev(self) -> torch.device:
+        d = self.device
+        return d if d.index is not None else torch.device(d.type, torch.cuda.current_device())
+
+    def _check_ints(self, t: torch.Tensor, name: str, shape) -> torch.Tensor:
+        self._on_device(t, name)
+        if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}, "
+                             f"got {t.dtype} {tuple(t.shape)}")
+        return t
+
+    def _pages(self, k: torch.Tensor, v: Optional[torch.Tensor], page_table: torch.Tensor,
+               name: str = "k_pages") -> _lib.PkvPages:
+        self._on_device(k, name)
+        if k.dim() != 4 or k.shape[3] != self.m or k.shape[1] < 1:
+            raise ValueError(f"{name} must be (num_pages, kv_heads, page_size, {self.m}), got {tuple(k.shape)}")
+        if k.dtype not in PAGE_CODE_DTYPES:
+            raise ValueError("codes must be stored as uint8 or 16-bit integers")
+        if v is not None:
+            self._on_device(v, "v_pages")
+            if v.shape != k.shape or v.dtype != k.dtype or v.stride() != k.stride():
+                raise ValueError("k_pages and v_pages must have the same shape, dtype and strides")
+        if k.stride(3) != 1:
+            raise ValueError("codes need unit stride within a row")
+        self._on_device(page_table, "page_table")
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1
+                                                                        and page_table.stride(1) != 1):
+            raise ValueError("page_table must be an int32 (batch, max_pages) tensor with unit inner stride")
+        ps = k.shape[2]
+        if ps < 16 or ps > 1024 or ps & (ps - 1):
+            raise ValueError(f"page_size must be a power of two from 16 to 1024, got {ps}")
+        g = _lib.PkvPages()
+        g.k, g.v = k.data_ptr(), v.data_ptr() if v is not None else None
+        g.code_bytes = PAGE_CODE_DTYPES[k.dtype]
+        g.num_pages, g.kv_heads, g.page_size = k.shape[0], k.shape[1], ps
+        # a dimension of one element has no stride of its own
+        g.page_stride = k.stride(0) if k.shape[0] > 1 else 0
+        g.head_stride = k.stride(1) if k.shape[1] > 1 else 0
+        g.token_stride = k.stride(2)
+        g.table = page_table.data_ptr()
+        g.batch, g.max_pages = page_table.shape
+        g.table_stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
+        return g
+
+    def _query(self, q: torch.Tensor, kv_heads: int, batch: int) -> torch.Tensor:
+        self._on_device(q, "q")
+        if q.dim() == 4:
+            if q.shape[2] != 1:
+                raise ValueError("paged attention takes one query token (Sq == 1)")
+            q = q[:, :, 0, :]
+        if q.dim() != 3 or q.shape[0] != batch or q.shape[2] != self.dim:
+            raise ValueError(f"q must be ({batch}, q_heads, {self.dim}), got {tuple(q.shape)}")
+        if q.shape[1] < 1 or q.shape[1] % kv_heads:
+            raise ValueError(f"{q.shape[1]} query heads do not divide among {kv_heads} KV heads")
+        if q.dtype not in _lib.DTYPE_CODES:
+            q = q.float()
+        return q if q.stride(2) == 1 else q.contiguous()
+
+    # ------------------------------------------------------------------
+    def paged_attention(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                        page_table: torch.Tensor, seq_lens: torch.Tensor, scale: Optional[float] = None,
+                        pages: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
+                        weights_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                        out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Decode attention over a paged cache: q (B, Hq, dim) [or (B, Hq, 1, dim)] -> (B, Hq, dim) of out_dtype.
+
+        ``pages`` (B, Hkv, n) int32 restricts each KV head to the listed logical
+        pages (``select_pages`` makes such lists): strictly ascending, -1 behind
+        the last.  ``weights`` (B, Hkv, slots) fp32: every attended token's
+        softmax weights, summed over the KV head's query heads, are added --
+        in place, or into ``weights_out`` of the same shape, whose other entries
+        are not touched; slots must cover every token.  A sequence without
+        tokens gives zeros.
+        """
+        g = self._pages(k_pages, v_pages, page_table)
+        q = self._query(q, g.kv_heads, g.batch)
+        B, Hq, _ = q.shape
+        self._check_ints(seq_lens, "seq_lens", (B,))
+        if out is None:
+            if out_dtype not in _lib.DTYPE_CODES:
+                raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+            out = torch.empty((B, Hq, self.dim), dtype=out_dtype, device=q.device)
+        else:
+            self._on_device(out, "out")
+            if out.shape != (B, Hq, self.dim) or out.dtype not in _lib.DTYPE_CODES or out.stride(2) != 1:
+                raise ValueError(f"out must be a ({B}, {Hq}, {self.dim}) float tensor with unit inner stride")
+        a = _lib.PkvPagedAttnArgs()
+        a.pages = g
+        a.q_heads, a.q_dtype, a.q = Hq, _lib.DTYPE_CODES[q.dtype], q.data_ptr()
+        a.q_batch_stride, a.q_head_stride = q.stride(0), q.stride(1)
+        a.seq_lens = seq_lens.data_ptr()
+        if pages is not None:
+            if pages.dim() != 3:
+                raise ValueError(f"pages must be ({B}, {g.kv_heads}, n), got {tuple(pages.shape)}")
+            self._check_ints(pages, "pages", (B, g.kv_heads, pages.shape[2]))
+            if pages.shape[2] == 0:
+                raise ValueError("pages lists no page; leave it out to attend to every token")
+            a.selected, a.n_selected = pages.data_ptr(), pages.shape[2]
+        a.scale = float(self.dim ** -0.5 if scale is None else scale)
+        a.out, a.out_dtype = out.data_ptr(), _lib.DTYPE_CODES[out.dtype]
+        a.out_batch_stride, a.out_head_stride = out.stride(0), out.stride(1)
+        if weights_out is not None and weights is None:
+            raise ValueError("weights_out needs weights")
+        if weights is not None:
+            w_out = weights if weights_out is None else weights_out
+            for t, n in ((weights, "weights"), (w_out, "weights_out")):
+                self._on_device(t, n)
+                if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (B, g.kv_heads) or not t.is_contiguous():
+                    raise ValueError(f"{n} must be a contiguous float32 ({B}, {g.kv_heads}, slots) tensor")
+            if w_out.shape != weights.shape:
+                raise ValueError("weights and weights_out must have the same shape")
+            a.weights, a.weights_out = weights.data_ptr(), w_out.data_ptr()
+            a.weights_slots = a.weights_row_stride = weights.shape[2]
+        lib = _lib.load()
+        with torch.cuda.device(self.device):
+            need = lib.pkv_paged_attn_workspace_size(ctypes.byref(self.struct), ctypes.byref(a))
+            ws = torch.empty(max(int(need), 256), dtype=torch.uint8, device=q.device)
+            rc = lib.pkv_paged_attn(ctypes.byref(self.struct), ctypes.byref(a), ws.data_ptr(), ws.numel(), self._stream())
+        _lib.check(rc, "pkv_paged_attn")
+        return out
+
+    # ------------------------------------------------------------------
+    def store_pages(self, codes: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor,
+                    counts: Optional[torch.Tensor] = None) -> None:
+        """Copy codes (B, Hkv, n, m) into slots start[b] .. of one pool; counts[b] < n leaves padded rows out."""
+        g = self._pages(pages, None, page_table, "pages")
+        self._on_device(codes, "codes")
+        if codes.dim() != 4 or codes.dtype != pages.dtype or (codes.shape[0], codes.shape[1], codes.shape[3]) != (
+                g.batch, g.kv_heads, self.m):
+            raise ValueError(f"codes must be ({g.batch}, {g.kv_heads}, n, {self.m}) of the pool's dtype")
+        codes = codes.contiguous()
+        self._check_ints(start, "start", (g.batch,))
+        if counts is not None:
+            self._check_ints(counts, "counts", (g.batch,))
+        with torch.cuda.device(self.device):
+            rc = _lib.load().pkv_pages_store(ctypes.byref(g), self.m, pages.data_ptr(), codes.data_ptr(), codes.shape[2],
+                                             start.data_ptr(), counts.data_ptr() if counts is not None else None,
+                                             self._stream())
+        _lib.check(rc, "pkv_pages_store")
+
+    def _grid(self):
+        """Device tables of the summaries' grid, built on first use."""
+        if getattr(self, "_grid_z", None) is None:
+            z, xy = _summary_grid(np.asarray(self.host.dec_z), np.asarray(self.host.dec_xy), 1 << self.bits_total)
+            self._grid_xy = torch.from_numpy(np.ascontiguousarray(xy)).to(self.device)
+            self._grid_z = torch.from_numpy(z).to(self.device)
+        return self._grid_z, self._grid_xy
+
+    def _check_summaries(self, t: torch.Tensor, g: _lib.PkvPages) -> None:
+        self._on_device(t, "summaries")
+        want = (g.kv_heads, 2, self.summary_pitch)
+        if t.dtype != torch.int8 or t.dim() != 4 or tuple(t.shape[1:]) != want or not t.is_contiguous():
+            raise ValueError(f"summaries must be a contiguous int8 (num_pages, {', '.join(map(str, want))}) tensor")
+
+    def summarize_pages(self, k_pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                        summaries: torch.Tensor, start: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Least and greatest decoded key per page, KV head and rotated channel, rounded outwards to int8.
+
+        Writes the summaries of the pages that hold a token >= start[b] of
+        sequence b (of every page without ``start``) into ``summaries``
+        (num_pages, Hkv, 2, summary_pitch) and returns it.  One step is 1/127 of
+        the codec's largest decoded magnitude; values within 1/256 of a step of
+        a whole number count as it.
+        """
+        g = self._pages(k_pages, None, page_table)
+        self._check_ints(seq_lens, "seq_lens", (g.batch,))
+        self._check_summaries(summaries, g)
+        if summaries.shape[0] != g.num_pages:
+            raise ValueError(f"summaries hold {summaries.shape[0]} pages, the pool {g.num_pages}")
+        if start is not None:
+            self._check_ints(start, "start", (g.batch,))
+        gz, gxy = self._grid()
+        with torch.cuda.device(self.device):
+            rc = _lib.load().pkv_pages_summarize(
+                ctypes.byref(self.struct), ctypes.byref(g), seq_lens.data_ptr(),
+                start.data_ptr() if start is not None else None, gz.data_ptr(), gxy.data_ptr(), summaries.data_ptr(),
+                self._stream())
+        _lib.check(rc, "pkv_pages_summarize")
+        return summaries
+
+    def select_pages(self, q: torch.Tensor, summaries: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                     page_size: int, top: int, sinks: int = 1, recent: int = 1,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The pages worth attending to: (B, Hkv, top) int32 logical pages, ascending, -1 behind the last.
+
+        The first ``sinks`` and last ``recent`` pages of a sequence are always
+        taken, the others by an upper bound of their tokens' scores: the KV
+        head's queries, rotated and rounded to int8 on a common scale, against
+        the summaries' greatest (positive) and least (negative) values; the
+        largest over the heads counts, ties go to the lower page.
+        """
+        if summaries.dim() != 4:
+            raise ValueError("summaries must be (num_pages, kv_heads, 2, summary_pitch)")
+        if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
+        if top < 1 or sinks < 0 or recent < 0 or sinks + recent > top:
+            raise ValueError(f"need 0 <= sinks + recent <= top and top >= 1, got {sinks}, {recent}, {top}")
+        self._on_device(page_table, "page_table")
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1
+                                                                        and page_table.stride(1) != 1):
+            raise ValueError("page_table must be an int32 (batch, max_pages) tensor with unit inner stride")
+        g = _lib.PkvPages()
+        g.code_bytes, g.num_pages, g.kv_heads, g.page_size = 1, summaries.shape[0], summaries.shape[1], page_size
+        g.token_stride = -(-self.m // ROW_BYTES) * ROW_BYTES
+        g.table = page_table.data_ptr()
+        g.batch, g.max_pages = page_table.shape
+        g.table_stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
+        self._check_summaries(summaries, g)
+        q = self._query(q, g.kv_heads, g.batch)
+        self._check_ints(seq_lens, "seq_lens", (g.batch,))
+        if out is None:
+            out = torch.empty((g.batch, g.kv_heads, top), dtype=torch.int32, device=q.device)
+        self._check_ints(out, "out", (g.batch, g.kv_heads, top))
+        with torch.cuda.device(self.device):
+            rc = _lib.load().pkv_pages_select(
+                ctypes.byref(self.struct), ctypes.byref(g), q.data_ptr(), _lib.DTYPE_CODES[q.dtype], q.shape[1],
+                q.stride(0), q.stride(1), seq_lens.data_ptr(), summaries.data_ptr(), top, sinks, recent, out.data_ptr(),
+                self._stream())
+        _lib.check(rc, "pkv_pages_select")
+        return out
+
+    # ------------------------------------------------------------------
+    def select_tokens(self, weights: torch.Tensor, seq_lens: torch.Tensor, keep: int, sinks: int = 0,
+                      recent: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Slots to keep per (sequence, KV head) by accumulated weight, and their weights: both (B, Hkv, keep).
+
+        Of the first seq_lens[b] entries of weights (B, Hkv, slots): the first
+        ``sinks``, the last ``recent``, then the largest (ties: the lower slot;
+        NaN last), ascending; -1 and 0 behind the last.
+        """
+        self._on_device(weights, "weights")
+        if weights.dim() != 3 or weights.dtype != torch.float32 or not weights.is_contiguous():
+            raise ValueError("weights must be a contiguous float32 (batch, kv_heads, slots) tensor")
+        if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
+            raise ValueError(f"need 0 <= sinks + recent <= keep and keep >= 1, got {sinks}, {recent}, {keep}")
+        B, H, T = weights.shape
+        self._check_ints(seq_lens, "seq_lens", (B,))
+        kept = torch.empty((B, H, keep), dtype=torch.int32, device=weights.device)
+        kw = torch.empty((B, H, keep), dtype=torch.float32, device=weights.device)
+        with torch.cuda.device(self.device):
+            rc = _lib.load().pkv_tokens_select(weights.data_ptr(), B, H, T, T, seq_lens.data_ptr(), keep, sinks, recent,
+                                               kept.data_ptr(), kw.data_ptr(), self._stream())
+        _lib.check(rc, "pkv_tokens_select")
+        return kept, kw
+
+    def gather_tokens(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, kept: torch.Tensor,
+                      k_out: torch.Tensor, v_out: torch.Tensor, out_table: torch.Tensor) -> None:
+        """Copy the codes of slots kept[b, hk, i] (negative: none) into slots i of out_table's pages.
+
+        The destination pages may lie in the same pool but must not be among the
+        pages that are read.
+        """
+        src = self._pages(k_pages, v_pages, page_table)
+        dst = self._pages(k_out, v_out, out_table, "k_out")
+        if k_out.dtype != k_pages.dtype or dst.batch != src.batch or dst.kv_heads != src.kv_heads:
+            raise ValueError("source and destination must agree in dtype, batch and KV heads")
+        if kept.dim() != 3:
+            raise ValueError(f"kept must be ({src.batch}, {src.kv_heads}, keep), got {tuple(kept.shape)}")
+        keep = kept.shape[2]
+        self._check_ints(kept, "kept", (src.batch, src.kv_heads, keep))
+        if keep > dst.max_pages * dst.page_size:
+            raise ValueError(f"{keep} tokens do not fit {dst.max_pages} pages of {dst.page_size}")
+        with torch.cuda.device(self.device):
+            rc = _lib.load().pkv_tokens_gather(ctypes.byref(src), self.m, kept.data_ptr(), keep, ctypes.byref(dst),
+                                               k_out.data_ptr(), v_out.data_ptr(), self._stream())
+        _lib.check(rc, "pkv_tokens_gather")
