@@ -13,119 +13,539 @@ namespace pkv {
 
 constexpr int kHQ = 4;                         // query heads per unit
 
-// One warp per granule, lanes over triplets, fp32 throughout.
-__global__ void __launch_bounds__(256) paged_attn_kernel(PagedParams p) {
-    extern __shared__ float psm[];
-    const int dim = p.dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nw = blockDim.x >> 5;
-    float* sQ = psm;                           // [4][dim] scaled rotated queries
-    float* sAcc = sQ + kHQ * dim;              // [warps][4][dim]
-    float* sM = sAcc + nw * kHQ * dim;         // [warps][4], then l
-    float* sL = sM + nw * kHQ;
+// ---------------------------------------------------------------------------------------------
+// paged_attn_kernel: both products on register-operand tensor-core tiles (mma.sync m16n8k16), the codes
+// decoded straight into operand fragments by table lookups.
+//
+// Why not tcgen05: a unit's four heads are the narrow side of both products and the operands come out of a
+// table lookup in registers; tcgen05 wants M >= 64 and operands in shared or tensor memory, and writing the
+// decoded tiles there costs more shared-memory bandwidth than the lookups themselves.
+//
+// Numbers: every operand is an fp16 pair (hi, lo) equal to its fp32 value to 2^-22; sums are fp32.
+//  * a decoded x, y (and z from a table) is a pair along the contraction: k-pair = (hi, lo);
+//  * queries and softmax weights are pairs across the eight columns: column h < 4 is head h's hi part,
+//    column h + 4 its lo part; both columns are added afterwards.  So all four cross products count.
+//  * table values are scaled by a power of two that puts the largest in [2^9, 2^10), the queries per head by
+//    one that puts theirs in [2^13, 2^14): pairs of normal fp16 whatever the ranges of the codec and the
+//    data.  Weights are 2^12 exp2(score - running max).
+//  * MODE 0 (two-byte codes, 8 bits of (r, theta), uniform z): z = z0 + i dz enters by its index -- for the
+//    scores as the exact fp16 subnormal i 2^-24, for the values as the exact i - 8, both affine parts added
+//    outside.  Centred, because an uncentred sum of p i grows with every token and the tiles' sums truncate.
+// Tables in shared memory: MODE 0 and 1 (one-byte codes, any codec) hold 256 rows of 32 copies, copy `lane`
+// for each lane: the 32 lookups of a warp never collide, and at a 64 KB-aligned address one byte permute of
+// the code word makes a lookup's address.  MODE 2 (two-byte codes of any codec) holds one copy of all 2^bits
+// (x, y) -- 32 copies of 4096 do not fit -- and pays bank conflicts; z has 32 copies per bin in each mode.
+//
+// A warp takes NG granules (16 tokens each) at a time, lane = 4 g + c:
+//  * scores: rows = tokens, k = triplets.  Lane (g, c) holds tokens rho(g), rho(g) + 8, rho(g) = (g >> 1) +
+//    4 (g & 1), and CPL triplets of each: 8c .. 8c + 7 of the first 32, then its share of the rest.
+//  * weights: two 8x8 transposes (movmatrix) turn the score tile into the B operand of p . v.
+//  * values: rows = triplets, k = tokens.  Lane (g, c) holds tokens c, c + 4, c + 8, c + 12 and CPL / 2
+//    triplets of each: 4g .. 4g + 3 of the first 32, then its share of the rest.
+// Codes go from global memory to registers, one iteration ahead: a warp's load covers whole 32-byte sectors of
+// eight or sixteen rows, no barrier and no shared-memory traffic; a page is found through the item's page list
+// in shared memory.
+// ---------------------------------------------------------------------------------------------
+template <int MODE_, int CPL_, int NG_, int W_>
+struct PA {
+    static constexpr int MODE = MODE_, CPL = CPL_, NG = NG_, W = W_;
+    static constexpr int CB = MODE == 1 ? 1 : 2;
+    static constexpr int CPV = CPL / 2;                     // triplets per lane and token (values) = (x, y) m-tiles
+    static constexpr int KW = CPL * CB / 4, VW = (CPV * CB + 3) / 4;
+    static constexpr int CHUNK = 1024;                      // pages of the list held at a time
+    static constexpr int XY_BYTES = MODE == 2 ? 4096 * 8 : 256 * 32 * 8;
+    static constexpr int Z_BYTES = MODE == 0 ? 0 : (MODE == 1 ? 65536 : 256 * 32 * 4);
+    static constexpr int THREADS = W * 32;
+};
+
+struct PASmem {                                             // offsets below the tables, in floats
+    int q, acc, wm, wl, misc, list, floats;
+};
+__host__ __device__ inline PASmem pa_smem(int dim, int warps, int chunk) {
+    PASmem s;
+    s.q = 0;                                                // [4][dim]
+    s.acc = s.q + kHQ * dim;                                // [warps][4][dim]; raw queries before the loop
+    s.wm = s.acc + warps * kHQ * dim;                       // [warps][4] max
+    s.wl = s.wm + warps * kHQ;                              // [warps][4] sum
+    s.misc = s.wl + warps * kHQ;                            // [4] su, [4] cz, [32] reduction
+    s.list = s.misc + 40;                                   // [chunk] pages
+    s.floats = s.list + chunk;
+    return s;
+}
+
+// triplet j of lane c (scores), triplet i of lane g (values)
+template <class T> __device__ __forceinline__ int k_triplet(int c, int j) {
+    if (j < 8) return 8 * c + j;
+    return 32 + (T::CPL - 8) * c + (j - 8);
+}
+template <class T> __device__ __forceinline__ int v_triplet(int g, int i) {
+    if (i < 4) return 4 * g + i;
+    return 32 + (T::CPV - 4) * g + (i - 4);
+}
+
+__device__ __forceinline__ uint4 ldg_cs4(const void* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ uint2 ldg_cs2(const void* p) { return __ldcs(reinterpret_cast<const uint2*>(p)); }
+__device__ __forceinline__ uint32_t ldg_cs1(const void* p) { return __ldcs(reinterpret_cast<const uint32_t*>(p)); }
+
+// `bytes` (4, 8 or 16) of codes at row + off into w[]; nothing past the row's last code is touched
+// beyond the 16-byte piece that holds it.
+template <int BYTES> __device__ __forceinline__ void load_codes(uint32_t* w, const uint8_t* row, int off, int row_bytes) {
+    if (off >= row_bytes) return;
+    if constexpr (BYTES == 16) {
+        const uint4 v = ldg_cs4(row + off);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (BYTES == 8) {
+        const uint2 v = ldg_cs2(row + off);
+        w[0] = v.x; w[1] = v.y;
+    } else if constexpr (BYTES == 4) {
+        w[0] = ldg_cs1(row + off);
+    } else {
+        w[0] = __ldcs(reinterpret_cast<const uint16_t*>(row + off));
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void load_k(uint32_t (&w)[T::KW], const uint8_t* row, int c, int row_bytes) {
+    load_codes<8 * T::CB>(w, row, 8 * T::CB * c, row_bytes);
+    if constexpr (T::CPL > 8)
+        load_codes<(T::CPL - 8) * T::CB>(w + 8 * T::CB / 4, row, (32 + (T::CPL - 8) * c) * T::CB, row_bytes);
+}
+template <class T>
+__device__ __forceinline__ void load_v(uint32_t (&w)[T::VW], const uint8_t* row, int g, int row_bytes) {
+    load_codes<4 * T::CB>(w, row, 4 * T::CB * g, row_bytes);
+    if constexpr (T::CPV > 4)
+        load_codes<(T::CPV - 4) * T::CB>(w + T::CB, row, (32 + (T::CPV - 4) * g) * T::CB, row_bytes);
+}
+
+// Lookups.  xy_reg / z_reg: the tables' shared addresses with the lane's copy in the low byte.
+struct Lookup { uint32_t xy, z; int zsh; uint32_t zmask, xymask; };
+
+template <class T> __device__ __forceinline__ uint2 look_xy(const Lookup& l, const uint32_t* w, int j) {
+    if constexpr (T::MODE == 0) return lds_u32x2m(__byte_perm(w[j >> 1], l.xy, (j & 1) ? 0x7624u : 0x7604u));
+    if constexpr (T::MODE == 1) return lds_u32x2m(__byte_perm(w[j >> 2], l.xy, 0x7604u + ((j & 3) << 4)));
+    const uint32_t x = (j & 1) ? w[j >> 1] >> 13 : w[j >> 1] << 3;
+    return lds_u32x2m((x & l.xymask) + l.xy);
+}
+// (z_hi, z_lo) from the table (MODE 1, 2)
+template <class T> __device__ __forceinline__ uint32_t look_z(const Lookup& l, const uint32_t* w, int j) {
+    uint32_t a, v;
+    if constexpr (T::MODE == 1) {
+        a = __byte_perm(w[j >> 2], l.z, 0x7604u + ((j & 3) << 4));
+    } else {
+        const uint32_t code = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1];
+        a = (((code >> l.zsh) & l.zmask) << 7) + l.z;
+    }
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+
+__device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
+// k with |v| 2^k in [2^top, 2^(top + 1)), held in [-lim, lim]; 0 for zero and non-finite v
+__device__ __forceinline__ int pow2_to(float v, int top, int lim) {
+    if (!(v > 0.f) || v > 3.0e38f) return 0;
+    const int e = max((int)((__float_as_uint(v) >> 23) & 0xFF) - 127, -126);
+    return max(-lim, min(lim, top - e));
+}
+
+template <class T>
+__global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p) {
+    extern __shared__ __align__(128) uint8_t pa_raw[];
+    constexpr int W = T::W, NG = T::NG, CPL = T::CPL, CPV = T::CPV, MODE = T::MODE, nthr = T::THREADS;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim;
+    const PASmem L = pa_smem(dim, W, T::CHUNK);
+    float* sm = reinterpret_cast<float*>(pa_raw);
+    float *sQ = sm + L.q, *sAcc = sm + L.acc, *sWm = sm + L.wm, *sWl = sm + L.wl, *sMisc = sm + L.misc;
+    int* sList = reinterpret_cast<int*>(sm + L.list);
+    // the tables start at the first 64 KB boundary of shared addresses behind the rest
+    const uint32_t base = smem_u32(pa_raw);
+    const uint32_t tab = (base + L.floats * 4 + 0xFFFFu) & ~0xFFFFu;
+    {
+        uint32_t have;
+        asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(have));
+        if (tab + T::XY_BYTES + T::Z_BYTES > base + have) {   // the window lies elsewhere than planned for
+            if (tid == 0) flag_error(kErrSmemLayout);
+            return;
+        }
+    }
+    uint8_t* tabp = pa_raw + (tab - base);
     PagedCursor cur = paged_begin(p);
+    if (cur.t >= cur.end) return;
+    if (tid < dim * dim * 4 / 128) prefetch_l2(reinterpret_cast<const uint8_t*>(p.R) + tid * 128);
+
+    // ---- tables -----------------------------------------------------------------------------------
+    const int bits_all = p.bits_z + p.bits_flat;
+    const float z0 = __ldg(p.dec_z), dz = __ldg(p.dec_z + 1) - z0;      // MODE 0: z = z0 + i dz
+    int tk;                                                   // the table's power of two
+    {
+        float am = 0.f;
+        const int n = MODE == 0 ? 256 : 1 << (p.xy_per_z ? bits_all : p.bits_flat);
+        for (int i = tid; i < 2 * n; i += nthr) am = fmaxf(am, fabsf(__ldg(p.dec_xy + i)));
+        if (MODE != 0)
+            for (int i = tid; i < 1 << p.bits_z; i += nthr) am = fmaxf(am, fabsf(__ldg(p.dec_z + i)));
+        #pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, off));
+        if (lane == 0) sMisc[8 + warp] = am;
+        __syncthreads();
+        am = 0.f;
+        for (int w = 0; w < W; ++w) am = fmaxf(am, sMisc[8 + w]);
+        tk = pow2_to(am, 9, 30);
+        const float ts = pow2(tk);
+        if constexpr (MODE == 2) {
+            for (int i = tid; i < 1 << bits_all; i += nthr) {
+                const float2 v = __ldg(reinterpret_cast<const float2*>(p.dec_xy) +
+                                       (p.xy_per_z ? i : i & ((1 << p.bits_flat) - 1)));
+                reinterpret_cast<uint2*>(tabp)[i] = make_uint2(h2_split(v.x * ts), h2_split(v.y * ts));
+            }
+            uint32_t* zt = reinterpret_cast<uint32_t*>(tabp + T::XY_BYTES);
+            for (int i = tid; i < 32 << p.bits_z; i += nthr) zt[i] = h2_split(__ldg(p.dec_z + (i >> 5)) * ts);
+        } else {
+            // rows of 16 pieces of 16 bytes (two copies each); codes past 2^bits read row 0's value
+            for (int i = tid; i < 256 * 16; i += nthr) {
+                const int e = i >> 4, code = e < (1 << bits_all) ? e : 0;
+                const float2 v = __ldg(reinterpret_cast<const float2*>(p.dec_xy) +
+                                       (MODE == 0 || p.xy_per_z ? (MODE == 0 ? e : code) : code & ((1 << p.bits_flat) - 1)));
+                const uint32_t x = h2_split(v.x * ts), y = h2_split(v.y * ts);
+                reinterpret_cast<uint4*>(tabp)[i] = make_uint4(x, y, x, y);
+                if constexpr (MODE == 1) {
+                    const uint32_t z = h2_split(__ldg(p.dec_z + (code >> p.bits_flat)) * ts);
+                    if ((i & 15) < 8) reinterpret_cast<uint4*>(tabp + T::XY_BYTES)[i] = make_uint4(z, z, z, z);
+                }
+            }
+        }
+    }
+    Lookup lk;
+    lk.xy = MODE == 2 ? tab : tab | ((uint32_t)lane << 3);
+    lk.z = tab + T::XY_BYTES + ((uint32_t)lane << 2);
+    lk.zsh = p.bits_flat;
+    lk.zmask = (1u << p.bits_z) - 1u;
+    lk.xymask = ((1u << bits_all) - 1u) << 3;
+
+    const int g = lane >> 2, c = lane & 3, hp = c & 1;
+    const bool lo_col = g >= 4;
+    const int qh = g & 3, rho = (g >> 1) + 4 * (g & 1);
+    const int row_bytes = p.m * T::CB, per = p.pg.ps_log2 - 4;
+    const int tokb = (int)p.pg.tok_bs;                        // (a row; checked to fit 31 bits / 16)
     PagedItem it;
     while (paged_next(p, cur, it)) {
-        __syncthreads();
-        const int L = clamp_len(p.pg, p.seq_lens[it.b]);
-        for (int i = warp; i < kHQ * dim; i += nw) {
-            const int h = i / dim, k = i % dim, hl = it.hg * kHQ + h;
-            float a = 0.f;
-            if (hl < p.G)
-                for (int d = lane; d < dim; d += 32)
-                    a = fmaf(__ldg(p.R + k * dim + d),
-                             load_any(p.q, p.qdt, it.b * p.q_bs + (int64_t)(it.hk * p.G + hl) * p.q_hs + d), a);
-            #pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) a += __shfl_xor_sync(0xffffffffu, a, off);
-            if (lane == 0) sQ[i] = a * p.scale_log2;
+        const int len = clamp_len(p.pg, __ldg(p.seq_lens + it.b));
+        // ---- q' = scale log2(e) R q, a warp per row of R ------------------------------------------
+        __syncthreads();                                      // tables written; last item's sAcc read
+        for (int i = tid; i < kHQ * dim; i += nthr) {
+            const int h = it.hg * kHQ + i / dim;
+            sAcc[i] = h < p.G ? load_any(p.q, p.qdt, it.b * p.q_bs + (int64_t)(it.hk * p.G + h) * p.q_hs + i % dim) : 0.f;
         }
         __syncthreads();
-        float M[kHQ], l[kHQ], acc[kHQ][6];
-        #pragma unroll
-        for (int h = 0; h < kHQ; ++h) {
-            M[h] = -INFINITY;
-            l[h] = 0.f;
+        #pragma unroll 2
+        for (int k = warp; k < dim; k += W) {
+            float a[kHQ] = {0.f, 0.f, 0.f, 0.f};
             #pragma unroll
-            for (int i = 0; i < 6; ++i) acc[h][i] = 0.f;
-        }
-        for (int gi = it.g0 + warp; gi < it.g1; gi += nw) {
-            const Granule g = granule_at(p, it.b, it.hk, gi);
-            if (g.page < 0) continue;
-            for (int r = 0; r < kGranule && g.tok + r < L; ++r) {
-                const int64_t off = slot_offset(p.pg, g.page, it.hk, g.slot + r);
-                float s[kHQ] = {0.f, 0.f, 0.f, 0.f}, vz[2], vx[2], vy[2];
-                #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int j = lane + 32 * i;
-                    vz[i] = vx[i] = vy[i] = 0.f;
-                    if (j >= p.m) continue;
-                    uint32_t kc, vc;
-                    if (p.cb == 1) {
-                        kc = p.pg.k[off + j];
-                        vc = p.pg.v[off + j];
-                    } else {
-                        kc = reinterpret_cast<const uint16_t*>(p.pg.k + off)[j];
-                        vc = reinterpret_cast<const uint16_t*>(p.pg.v + off)[j];
-                    }
-                    const uint32_t cm = (1u << (p.bits_z + p.bits_flat)) - 1u, fm = (1u << p.bits_flat) - 1u;
-                    kc &= cm;
-                    vc &= cm;
-                    const float kz = p.dec_z[kc >> p.bits_flat];
-                    const float2 kxy = reinterpret_cast<const float2*>(p.dec_xy)[p.xy_per_z ? kc : kc & fm];
-                    const float2 vxy = reinterpret_cast<const float2*>(p.dec_xy)[p.xy_per_z ? vc : vc & fm];
-                    vz[i] = p.dec_z[vc >> p.bits_flat];
-                    vx[i] = vxy.x;
-                    vy[i] = vxy.y;
+            for (int u = 0; u < (CPL * 12 + 31) / 32; ++u) {
+                const int d = lane + 32 * u;
+                if (d < dim) {
+                    const float r = __ldg(p.R + k * dim + d);
                     #pragma unroll
-                    for (int h = 0; h < kHQ; ++h) {
-                        const float* qv = sQ + h * dim + 3 * j;
-                        s[h] = fmaf(qv[0], kz, fmaf(qv[1], kxy.x, fmaf(qv[2], kxy.y, s[h])));
-                    }
-                }
-                #pragma unroll
-                for (int h = 0; h < kHQ; ++h)
-                    #pragma unroll
-                    for (int o = 16; o >= 1; o >>= 1) s[h] += __shfl_xor_sync(0xffffffffu, s[h], o);
-                if (p.raw && lane == 0)
-                    for (int h = 0; h < p.raw_h; ++h)
-                        p.raw[(int64_t)it.unit * p.raw_us + ((int64_t)gi * kGranule + r) * p.raw_h + h] = s[h];
-                #pragma unroll
-                for (int h = 0; h < kHQ; ++h) {
-                    const float n = fmaxf(M[h], s[h]), f = exp2f(M[h] - n), e = exp2f(s[h] - n);
-                    M[h] = n;
-                    l[h] = fmaf(l[h], f, e);
-                    #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        acc[h][3 * i] = fmaf(acc[h][3 * i], f, e * vz[i]);
-                        acc[h][3 * i + 1] = fmaf(acc[h][3 * i + 1], f, e * vx[i]);
-                        acc[h][3 * i + 2] = fmaf(acc[h][3 * i + 2], f, e * vy[i]);
-                    }
+                    for (int h = 0; h < kHQ; ++h) a[h] = fmaf(r, sAcc[h * dim + d], a[h]);
                 }
             }
+            #pragma unroll
+            for (int h = 0; h < kHQ; ++h)
+                #pragma unroll
+                for (int off = 16; off >= 1; off >>= 1) a[h] += __shfl_xor_sync(0xffffffffu, a[h], off);
+            if (lane < kHQ) sQ[lane * dim + k] = (lane == 0 ? a[0] : lane == 1 ? a[1] : lane == 2 ? a[2] : a[3]) * p.scale_log2;
         }
-        for (int h = 0; h < kHQ; ++h) {
-            for (int i = 0; i < 6; ++i) {
-                const int d = 3 * (lane + 32 * (i / 3)) + i % 3;
-                if (d < dim) sAcc[(warp * kHQ + h) * dim + d] = acc[h][i];
+        __syncthreads();
+        if (warp < kHQ) {                                     // per head: operand scale, z0 sum q_z
+            float am = 0.f, cz = 0.f;
+            for (int d = lane; d < dim; d += 32) {
+                const float v = sQ[warp * dim + d];
+                const bool isz = d % 3 == 0;
+                am = fmaxf(am, fabsf(v) * (MODE == 0 && isz ? fabsf(dz) : 1.f));
+                if (isz) cz += v;
+            }
+            #pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) {
+                am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, off));
+                cz += __shfl_xor_sync(0xffffffffu, cz, off);
             }
             if (lane == 0) {
-                sM[warp * kHQ + h] = M[h];
-                sL[warp * kHQ + h] = l[h];
+                sMisc[warp] = __int_as_float(pow2_to(am, 13, 90));
+                sMisc[4 + warp] = MODE == 0 ? cz * z0 : 0.f;
+            }
+        }
+        __syncthreads();
+        uint32_t bq[CPL][2], bz[MODE == 0 ? CPL / 4 : CPL / 2][2];
+        {
+            const float su = pow2(__float_as_int(sMisc[qh]));
+            auto qv = [&](int t, int x) { return t < p.m ? sQ[qh * dim + 3 * t + x] * su : 0.f; };
+            #pragma unroll
+            for (int j = 0; j < CPL; ++j) {
+                const int t = k_triplet<T>(c, j);
+                bq[j][0] = h2_dup_part(qv(t, 1), lo_col);
+                bq[j][1] = h2_dup_part(qv(t, 2), lo_col);
+            }
+            if constexpr (MODE == 0) {
+                // i enters as i 2^-24: the table's power of two is put on the query side
+                #pragma unroll
+                for (int j = 0; j < CPL / 4; ++j) {
+                    bz[j][0] = h2_pair_part(qv(k_triplet<T>(c, 4 * j), 0) * dz, qv(k_triplet<T>(c, 4 * j + 1), 0) * dz, lo_col);
+                    bz[j][1] = h2_pair_part(qv(k_triplet<T>(c, 4 * j + 2), 0) * dz, qv(k_triplet<T>(c, 4 * j + 3), 0) * dz, lo_col);
+                }
+            } else {
+                #pragma unroll
+                for (int j = 0; j < CPL / 2; ++j) {
+                    bz[j][0] = h2_dup_part(qv(k_triplet<T>(c, 2 * j), 0), lo_col);
+                    bz[j][1] = h2_dup_part(qv(k_triplet<T>(c, 2 * j + 1), 0), lo_col);
+                }
+            }
+        }
+        // heads 2 hp, 2 hp + 1 of this lane's score columns; log2 units
+        const int k0 = __float_as_int(sMisc[2 * hp]), k1 = __float_as_int(sMisc[2 * hp + 1]);
+        const float us0 = pow2(-k0 - tk), us1 = pow2(-k1 - tk);
+        const float cz0 = sMisc[4 + 2 * hp], cz1 = sMisc[4 + 2 * hp + 1];
+        const f32x2 uu = f2_pack(us0, us1), czz = f2_pack(cz0, cz1);
+        const float zs = pow2(24 + tk);                       // MODE 0: z sums onto the (x, y) sums' scale
+        float M0 = -INFINITY, M1 = -INFINITY;
+        float l0 = 0.f, l1 = 0.f;
+        float acc[CPV + CPV / 2][4];
+        #pragma unroll
+        for (int m = 0; m < CPV + CPV / 2; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+
+        const uint8_t* kbase = p.pg.k + (int64_t)it.hk * p.pg.head_bs + (int64_t)rho * tokb;
+        const uint8_t* vbase = p.pg.v + (int64_t)it.hk * p.pg.head_bs + (int64_t)c * tokb;
+        const int lastp = (len - 1) >> p.pg.ps_log2;         // the page that may be short, its tokens
+        const int lastn = len - (lastp << p.pg.ps_log2);
+        for (int ga = it.g0; ga < it.g1;) {
+            // ---- pages of the next granules: id, -1 (masked), or id | sign bit (the short page) ----------
+            const int j0 = ga >> per, gb = min(it.g1, (j0 + T::CHUNK) << per);
+            const int j1 = (gb - 1) >> per;
+            if (ga != it.g0) __syncthreads();                 // (the first list is ordered by the barriers above)
+            for (int j = j0 + tid; j <= j1; j += nthr) {
+                const Granule gr = granule_at(p, it.b, it.hk, j << per);
+                const int lp = p.selected ? gr.tok >> p.pg.ps_log2 : j;
+                sList[j - j0] = gr.page < 0 ? -1 : lp == lastp ? gr.page | (int)0x80000000 : gr.page;
+            }
+            __syncthreads();
+            // tokens of granule gi that count, and its byte offset
+            auto locate = [&](int gi, int64_t& off) -> int {
+                off = 0;
+                if (gi >= gb) return 0;
+                const int e = sList[(gi >> per) - j0];
+                if (e == -1) return 0;
+                const int slot = (gi & ((1 << per) - 1)) << 4;
+                off = (int64_t)(e & 0x7fffffff) * p.pg.page_bs + (int64_t)slot * tokb;
+                return e < 0 ? max(0, min(16, lastn - slot)) : 16;
+            };
+            uint32_t kw[NG][2][T::KW], vw[NG][4][T::VW];
+            #pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                #pragma unroll
+                for (int x = 0; x < T::KW; ++x) kw[i][0][x] = kw[i][1][x] = 0u;
+                #pragma unroll
+                for (int x = 0; x < T::VW; ++x) vw[i][0][x] = vw[i][1][x] = vw[i][2][x] = vw[i][3][x] = 0u;
+            }
+            int nv[NG];
+            int64_t off[NG];
+            int gi = ga + warp * NG;
+            #pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                nv[i] = locate(gi + i, off[i]);
+                if (nv[i] > 0) {
+                    load_k<T>(kw[i][0], kbase + off[i], c, row_bytes);
+                    load_k<T>(kw[i][1], kbase + off[i] + 8 * tokb, c, row_bytes);
+                    #pragma unroll
+                    for (int t = 0; t < 4; ++t) load_v<T>(vw[i][t], vbase + off[i] + t * 4 * tokb, g, row_bytes);
+                }
+            }
+            #pragma unroll 1
+            for (; gi < gb; gi += W * NG) {
+                int nn[NG];
+                #pragma unroll
+                for (int i = 0; i < NG; ++i) nn[i] = locate(gi + W * NG + i, off[i]);
+                // ---- scores ------------------------------------------------------------------------
+                float S[NG][4];
+                #pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    float xa[4] = {0.f, 0.f, 0.f, 0.f}, xb[4] = {0.f, 0.f, 0.f, 0.f}, zz[4] = {0.f, 0.f, 0.f, 0.f};
+                    #pragma unroll
+                    for (int j = 0; j < CPL; ++j) {
+                        const uint2 e0 = look_xy<T>(lk, kw[i][0], j), e1 = look_xy<T>(lk, kw[i][1], j);
+                        mma16816((j & 1) ? xb : xa, e0.x, e1.x, e0.y, e1.y, bq[j][0], bq[j][1]);
+                    }
+                    if constexpr (MODE == 0) {
+                        #pragma unroll
+                        for (int j = 0; j < CPL / 4; ++j)
+                            mma16816(zz, prmt(kw[i][0][2 * j], 0u, 0x4341u), prmt(kw[i][1][2 * j], 0u, 0x4341u),
+                                     prmt(kw[i][0][2 * j + 1], 0u, 0x4341u), prmt(kw[i][1][2 * j + 1], 0u, 0x4341u),
+                                     bz[j][0], bz[j][1]);
+                    } else {
+                        #pragma unroll
+                        for (int j = 0; j < CPL / 2; ++j)
+                            mma16816(zz, look_z<T>(lk, kw[i][0], 2 * j), look_z<T>(lk, kw[i][1], 2 * j),
+                                     look_z<T>(lk, kw[i][0], 2 * j + 1), look_z<T>(lk, kw[i][1], 2 * j + 1), bz[j][0], bz[j][1]);
+                    }
+                    #pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        S[i][x] = MODE == 0 ? fmaf(zz[x], zs, xa[x] + xb[x]) : zz[x] + (xa[x] + xb[x]);
+                        S[i][x] += __shfl_xor_sync(0xffffffffu, S[i][x], 2);             // hi + lo columns
+                    }
+                    if (nn[i] > 0) {                          // the next iteration's keys
+                        load_k<T>(kw[i][0], kbase + off[i], c, row_bytes);
+                        load_k<T>(kw[i][1], kbase + off[i] + 8 * tokb, c, row_bytes);
+                    }
+                }
+                // ---- log2 scores, kept for the weights; running maximum -------------------------------
+                float mx0 = -INFINITY, mx1 = -INFINITY;
+                #pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const float2 a = f2_unpack(f2_fma(f2_pack(S[i][0], S[i][1]), uu, czz));
+                    const float2 b = f2_unpack(f2_fma(f2_pack(S[i][2], S[i][3]), uu, czz));
+                    S[i][0] = a.x; S[i][1] = a.y; S[i][2] = b.x; S[i][3] = b.y;
+                    if (p.raw && c < 2) {
+                        float* r = p.raw + (int64_t)it.unit * p.raw_us + ((int64_t)(gi + i) * kGranule + rho) * p.raw_h + 2 * hp;
+                        #pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            if (2 * hp + x < p.raw_h) {
+                                if (rho < nv[i]) r[x] = S[i][x];
+                                if (rho + 8 < nv[i]) r[8 * p.raw_h + x] = S[i][2 + x];
+                            }
+                    }
+                    if (rho >= nv[i]) S[i][0] = S[i][1] = -INFINITY;
+                    if (rho + 8 >= nv[i]) S[i][2] = S[i][3] = -INFINITY;
+                    mx0 = fmaxf(mx0, fmaxf(S[i][0], S[i][2]));
+                    mx1 = fmaxf(mx1, fmaxf(S[i][1], S[i][3]));
+                }
+                if (__any_sync(0xffffffffu, mx0 > M0 || mx1 > M1)) {
+                    #pragma unroll
+                    for (int o = 4; o <= 16; o <<= 1) {
+                        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
+                        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
+                    }
+                    mx0 = fmaxf(mx0, M0);
+                    mx1 = fmaxf(mx1, M1);
+                    const float f0 = M0 == -INFINITY ? (l0 == 0.f ? 0.f : l0) : fast_exp2(M0 - mx0);
+                    const float f1 = M1 == -INFINITY ? (l1 == 0.f ? 0.f : l1) : fast_exp2(M1 - mx1);
+                    M0 = mx0;
+                    M1 = mx1;
+                    l0 *= f0;
+                    l1 *= f1;
+                    #pragma unroll
+                    for (int m = 0; m < CPV + CPV / 2; ++m) {
+                        acc[m][0] *= f0; acc[m][1] *= f1; acc[m][2] *= f0; acc[m][3] *= f1;
+                    }
+                }
+                // ---- weights, transposed into B operands ------------------------------------------------
+                const float n0 = M0 == -INFINITY ? 0.f : 12.f - M0, n1 = M1 == -INFINITY ? 0.f : 12.f - M1;
+                uint32_t pA[NG], pB[NG];
+                #pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const float p0 = fast_exp2(S[i][0] + n0), p1 = fast_exp2(S[i][1] + n1);
+                    const float p2 = fast_exp2(S[i][2] + n0), p3 = fast_exp2(S[i][3] + n1);
+                    l0 += p0 + p2;
+                    l1 += p1 + p3;
+                    const uint32_t hA = f2h2(p0, p1), hB = f2h2(p2, p3);
+                    const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&hA));
+                    const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hB));
+                    const uint32_t lA = f2h2(p0 - fa.x, p1 - fa.y), lB = f2h2(p2 - fb.x, p3 - fb.y);
+                    pA[i] = movmatrix_t(c >= 2 ? lA : hA);     // column g of tokens (c, c + 4)
+                    pB[i] = movmatrix_t(c >= 2 ? lB : hB);     // column g of tokens (c + 8, c + 12)
+                }
+                // ---- values ----------------------------------------------------------------------------
+                #pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const uint32_t d0 = __byte_perm(pA[i], 0u, 0x1010u), d1 = __byte_perm(pA[i], 0u, 0x3232u);
+                    const uint32_t d2 = __byte_perm(pB[i], 0u, 0x1010u), d3 = __byte_perm(pB[i], 0u, 0x3232u);
+                    #pragma unroll
+                    for (int m = 0; m < CPV; ++m) {
+                        const uint2 x0 = look_xy<T>(lk, vw[i][0], m), x1 = look_xy<T>(lk, vw[i][1], m);
+                        const uint2 x2 = look_xy<T>(lk, vw[i][2], m), x3 = look_xy<T>(lk, vw[i][3], m);
+                        mma16816(acc[m], x0.x, x0.y, x1.x, x1.y, d0, d1);
+                        mma16816(acc[m], x2.x, x2.y, x3.x, x3.y, d2, d3);
+                    }
+                    #pragma unroll
+                    for (int m = 0; m < CPV / 2; ++m) {
+                        float (&za)[4] = acc[CPV + m];
+                        if constexpr (MODE == 0) {
+                            float zt[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma16816(zt, zc8(prmt(vw[i][0][m], vw[i][1][m], 0x5511u)), zc8(prmt(vw[i][0][m], vw[i][1][m], 0x7733u)),
+                                     zc8(prmt(vw[i][2][m], vw[i][3][m], 0x5511u)), zc8(prmt(vw[i][2][m], vw[i][3][m], 0x7733u)),
+                                     pA[i], pB[i]);
+                            #pragma unroll
+                            for (int x = 0; x < 4; ++x) za[x] += zt[x];
+                        } else {
+                            mma16816(za, look_z<T>(lk, vw[i][0], 2 * m), look_z<T>(lk, vw[i][0], 2 * m + 1),
+                                     look_z<T>(lk, vw[i][1], 2 * m), look_z<T>(lk, vw[i][1], 2 * m + 1), d0, d1);
+                            mma16816(za, look_z<T>(lk, vw[i][2], 2 * m), look_z<T>(lk, vw[i][2], 2 * m + 1),
+                                     look_z<T>(lk, vw[i][3], 2 * m), look_z<T>(lk, vw[i][3], 2 * m + 1), d2, d3);
+                        }
+                    }
+                    if (nn[i] > 0) {                           // the next iteration's values
+                        #pragma unroll
+                        for (int t = 0; t < 4; ++t) load_v<T>(vw[i][t], vbase + off[i] + t * 4 * tokb, g, row_bytes);
+                    }
+                    nv[i] = nn[i];
+                }
+            }
+            ga = gb;
+        }
+        // ---- hi + lo columns, the lanes, the warps -------------------------------------------------------
+        #pragma unroll
+        for (int o = 4; o <= 16; o <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+        }
+        #pragma unroll
+        for (int m = 0; m < CPV + CPV / 2; ++m)
+            #pragma unroll
+            for (int x = 0; x < 4; ++x) acc[m][x] += __shfl_xor_sync(0xffffffffu, acc[m][x], 2);
+        if (c < 2) {
+            float* o0 = sAcc + (warp * kHQ + 2 * c) * dim;     // head 2c; head 2c + 1 at + dim
+            #pragma unroll
+            for (int m = 0; m < CPV; ++m) {
+                const int t = v_triplet<T>(g, m);
+                if (t < p.m) {
+                    o0[3 * t + 1] = acc[m][0]; o0[dim + 3 * t + 1] = acc[m][1];
+                    o0[3 * t + 2] = acc[m][2]; o0[dim + 3 * t + 2] = acc[m][3];
+                }
+            }
+            #pragma unroll
+            for (int m = 0; m < CPV / 2; ++m)
+                #pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int t = v_triplet<T>(g, 2 * m + x);
+                    if (t < p.m) {
+                        o0[3 * t] = acc[CPV + m][2 * x];
+                        o0[dim + 3 * t] = acc[CPV + m][2 * x + 1];
+                    }
+                }
+            if (g == 0) {
+                sWm[warp * kHQ + 2 * c] = M0;
+                sWm[warp * kHQ + 2 * c + 1] = M1;
+                sWl[warp * kHQ + 2 * c] = l0;
+                sWl[warp * kHQ + 2 * c + 1] = l1;
             }
         }
         __syncthreads();
         float* row = p.part + (int64_t)it.row * kHQ * (dim + 2);
-        for (int i = tid; i < kHQ * dim; i += blockDim.x) {
-            const int h = i / dim, d = i % dim;
+        const float its = pow2(-tk - 12);
+        for (int i = tid; i < kHQ * dim; i += nthr) {
+            const int h = i / dim, d = i - h * dim;
             float mx = -INFINITY, o = 0.f, ls = 0.f;
-            for (int w = 0; w < nw; ++w) mx = fmaxf(mx, sM[w * kHQ + h]);
-            for (int w = 0; w < nw; ++w) {
-                const float f = sL[w * kHQ + h] == 0.f ? 0.f : exp2f(sM[w * kHQ + h] - mx);   // (NaN sums stay)
+            #pragma unroll
+            for (int w = 0; w < W; ++w) mx = fmaxf(mx, sWm[w * kHQ + h]);
+            #pragma unroll
+            for (int w = 0; w < W; ++w) {
+                // a warp without tokens has sum 0; a NaN sum is carried on
+                const float lw = sWl[w * kHQ + h], f = lw == 0.f ? 0.f : fast_exp2(sWm[w * kHQ + h] - mx);
                 o = fmaf(f, sAcc[(w * kHQ + h) * dim + d], o);
-                ls = fmaf(f, sL[w * kHQ + h], ls);
+                ls = fmaf(f, lw, ls);
             }
+            // the weights carry 2^12, the tables 2^tk; MODE 0: sum p z = (z0 + 8 dz) l + dz sum p (i - 8)
+            if (MODE == 0 && d % 3 == 0) o = fmaf(dz, o * 0x1p-12f, fmaf(8.f, dz, z0) * (ls * 0x1p-12f));
+            else o *= its;
             row[h * (dim + 2) + 2 + d] = o;
             if (d == 0) {
                 row[h * (dim + 2)] = mx;
-                row[h * (dim + 2) + 1] = ls;
+                row[h * (dim + 2) + 1] = ls * 0x1p-12f;
             }
         }
     }
@@ -273,14 +693,36 @@ size_t paged_workspace(const pkv_codec* c, const pkv_paged_attn_args* a, Pages p
     return paged_part_bytes(p) + (a->weights ? (size_t)p.units * p.raw_us * 4 : 0);
 }
 
+template <class T>
+static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
+    // tables from the first 64 KB boundary behind the rest (the window starts at most 1 KB into the shared space)
+    const uint32_t below = 1024u + (uint32_t)pa_smem(p.dim, T::W, T::CHUNK).floats * 4u;
+    const int smem = (int)(((below + 0xFFFFu) & ~0xFFFFu) - 1024u) + T::XY_BYTES + T::Z_BYTES;
+    if (cudaFuncSetAttribute(paged_attn_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return PKV_ERR_CUDA;
+    paged_attn_kernel<T><<<p.grid, T::THREADS, smem, st>>>(p);
+    return cudaGetLastError() == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+}
+
+template <int MODE>
+static int launch_paged_mode(const PagedParams& p, cudaStream_t st) {
+    if (p.m <= 32) return launch_paged_as<PA<MODE, 8, 2, 16>>(p, st);
+    if (p.m <= 48) return launch_paged_as<PA<MODE, 12, 1, 16>>(p, st);
+    return launch_paged_as<PA<MODE, 16, 1, 12>>(p, st);
+}
+
+static int launch_paged_any(const pkv_codec* c, const PagedParams& p, cudaStream_t st) {
+    if (p.cb == 1) return launch_paged_mode<1>(p, st);
+    if (p.bits_flat == 8 && p.bits_z <= 4 && !p.xy_per_z && (c->flags & PKV_CODEC_Z_UNIFORM)) return launch_paged_mode<0>(p, st);
+    return launch_paged_mode<2>(p, st);
+}
+
 int launch_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg, int sms, void* ws, cudaStream_t st) {
     PagedParams p = paged_params(c, a, pg, sms);
     p.part = static_cast<float*>(ws);
     if (a->weights) p.raw = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + paged_part_bytes(p));
-    constexpr int threads = 256;
-    const size_t smem = (size_t)(kHQ * p.dim + threads / 32 * kHQ * (p.dim + 2)) * 4;
-    paged_attn_kernel<<<p.grid, threads, smem, st>>>(p);
-    if (cudaGetLastError() != cudaSuccess) return PKV_ERR_CUDA;
+    const int rc = launch_paged_any(c, p, st);
+    if (rc) return rc;
     const int chunks = a->weights ? (int)((p.raw_us / p.raw_h + kWeighTokens - 1) / kWeighTokens) : 0;
     const int64_t ctas = p.units + (int64_t)pg.B * pg.Hkv * chunks;
     if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
