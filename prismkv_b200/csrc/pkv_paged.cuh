@@ -59,6 +59,7 @@ struct PagedParams {
     const float *R, *dec_z, *dec_xy;
     int bits_z, bits_flat, xy_per_z;
     float* part;                               // [grid + units][HQ][dim + 2]: m (log2 units), l, o
+    uint32_t* frag; float* head;               // query operands, per-head numbers (paged_query_kernel)
     float* raw; int64_t raw_us; int raw_h;     // scores of every token, [unit][granule * 16][raw_h]
     int grid, units;
 };

@@ -3,9 +3,12 @@
 //   out[b, h] = R^T ( sum_t p_t V^(t) / sum_t p_t ),   p_t = exp(scale (R q) . K^(t) - max)
 //
 // over the sequence's tokens or those of listed pages; optionally weights_out[t] = weights[t] +
-// sum_h p_t / sum p.  Two launches: paged_attn_kernel leaves one partial state per (CTA, unit) range,
-// paged_join_kernel joins a unit's ranges, normalises and rotates back (and, in further CTAs, adds the
-// weights from the scores that the first launch kept).
+// sum_h p_t / sum p.  Three launches, each started while the one before still runs (programmatic
+// dependent launches; what does not depend on it is read ahead, the rest behind the grid dependency):
+// paged_query_kernel rotates the queries into operand fragments, paged_attn_kernel leaves one partial
+// state per (CTA, unit) range, paged_join_kernel joins a unit's ranges, normalises and rotates back (and,
+// in further CTAs, adds the weights from the scores that the second launch kept).  Small calls are bound by
+// the chain of memory round trips through the three, large ones by the issue slots of the decode.
 
 #include "pkv_paged.cuh"
 
@@ -46,9 +49,10 @@ constexpr int kHQ = 4;                         // query heads per unit
 // eight or sixteen rows, no barrier and no shared-memory traffic; a page is found through the item's page list
 // in shared memory.
 // ---------------------------------------------------------------------------------------------
-template <int MODE_, int CPL_, int NG_, int W_>
+template <int MODE_, int CPL_, int NG_, int W_, bool EX_>
 struct PA {
     static constexpr int MODE = MODE_, CPL = CPL_, NG = NG_, W = W_;
+    static constexpr bool EX = EX_;
     static constexpr int CB = MODE == 1 ? 1 : 2;
     static constexpr int CPV = CPL / 2;                     // triplets per lane and token (values) = (x, y) m-tiles
     static constexpr int KW = CPL * CB / 4, VW = (CPV * CB + 3) / 4;
@@ -56,27 +60,27 @@ struct PA {
     static constexpr int XY_BYTES = MODE == 2 ? 4096 * 8 : 256 * 32 * 8;
     static constexpr int Z_BYTES = MODE == 0 ? 0 : (MODE == 1 ? 65536 : 256 * 32 * 4);
     static constexpr int THREADS = W * 32;
+    static constexpr int NBZ = MODE == 0 ? CPL / 4 : CPL / 2;   // z steps of the scores
+    static constexpr int FRAGS = 2 * (CPL + NBZ);           // query operand registers per lane
 };
 
 struct PASmem {                                             // offsets below the tables, in floats
-    int q, acc, wm, wl, misc, list, floats;
+    int acc, wm, wl, red, list, floats;
 };
 __host__ __device__ inline PASmem pa_smem(int dim, int warps, int chunk) {
     PASmem s;
-    s.q = 0;                                                // [4][dim]
-    s.acc = s.q + kHQ * dim;                                // [warps][4][dim]; raw queries before the loop
+    s.acc = 0;                                              // [warps][4][dim]
     s.wm = s.acc + warps * kHQ * dim;                       // [warps][4] max
     s.wl = s.wm + warps * kHQ;                              // [warps][4] sum
-    s.misc = s.wl + warps * kHQ;                            // [4] su, [4] cz, [32] reduction
-    s.list = s.misc + 40;                                   // [chunk] pages
+    s.red = s.wl + warps * kHQ;                             // [32] reduction
+    s.list = s.red + 32;                                    // [chunk] pages
     s.floats = s.list + chunk;
     return s;
 }
 
 // triplet j of lane c (scores), triplet i of lane g (values)
-template <class T> __device__ __forceinline__ int k_triplet(int c, int j) {
-    if (j < 8) return 8 * c + j;
-    return 32 + (T::CPL - 8) * c + (j - 8);
+__device__ __forceinline__ int k_triplet_of(int cpl, int c, int j) {
+    return j < 8 ? 8 * c + j : 32 + (cpl - 8) * c + (j - 8);
 }
 template <class T> __device__ __forceinline__ int v_triplet(int g, int i) {
     if (i < 4) return 4 * g + i;
@@ -147,14 +151,125 @@ __device__ __forceinline__ int pow2_to(float v, int top, int lim) {
     return max(-lim, min(lim, top - e));
 }
 
+// One CTA per unit: q' = scale log2(e) R q of its four heads (zero for heads past the group), then the score
+// operands of every lane, fragment r of lane l at frag[(unit FRAGS + r) 32 + l]: pairs j < CPL of (x, y) of
+// triplet j, then z; head h's power of two and z0 sum q'_z at head[unit 8 + h], + 4.
+constexpr int kQueryThreads = 512;
+__global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams p, int mode, int cpl) {
+    extern __shared__ float qsm[];
+    cudaTriggerProgrammaticLaunchCompletion();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim, unit = blockIdx.x;
+    constexpr int NW = kQueryThreads / 32;
+    float *sRaw = qsm, *sQ = qsm + kHQ * dim;
+    __shared__ int sk[kHQ];
+    const int b = unit / p.UH, u = unit % p.UH, hk = u / p.UG, hg = u % p.UG;
+    const float z0 = __ldg(p.dec_z), dz = __ldg(p.dec_z + 1) - z0;
+    float rr[6][6];                                          // rows warp, warp + NW, ... of R, six at a time
+    auto load_rows = [&](int k0) {
+        #pragma unroll
+        for (int i = 0; i < 6; ++i)
+            #pragma unroll
+            for (int x = 0; x < 6; ++x) {
+                const int k = k0 + i * NW, d = lane + 32 * x;
+                rr[i][x] = (k < dim && d < dim) ? __ldg(p.R + k * dim + d) : 0.f;
+            }
+    };
+    load_rows(warp);
+    for (int i = tid; i < kHQ * dim; i += kQueryThreads) {
+        const int h = hg * kHQ + i / dim;
+        sRaw[i] = h < p.G ? load_any(p.q, p.qdt, b * p.q_bs + (int64_t)(hk * p.G + h) * p.q_hs + i % dim) : 0.f;
+    }
+    __syncthreads();
+    for (int k0 = warp; k0 < dim; k0 += 6 * NW) {
+        if (k0 != warp) load_rows(k0);
+        #pragma unroll
+        for (int i = 0; i < 6; ++i) {
+            const int k = k0 + i * NW;
+            if (k >= dim) break;
+            float a[kHQ] = {0.f, 0.f, 0.f, 0.f};
+            #pragma unroll
+            for (int x = 0; x < 6; ++x)
+                if (32 * x < dim) {
+                    const int d = min(lane + 32 * x, dim - 1);   // (rr is 0 behind the row)
+                    #pragma unroll
+                    for (int h = 0; h < kHQ; ++h) a[h] = fmaf(rr[i][x], sRaw[h * dim + d], a[h]);
+                }
+            // four sums over the warp: halve the lanes per head twice, then a butterfly over eight
+            const bool up16 = lane & 16, up8 = lane & 8;
+            const float b0 = (up16 ? a[2] : a[0]) + __shfl_xor_sync(0xffffffffu, up16 ? a[0] : a[2], 16);
+            const float b1 = (up16 ? a[3] : a[1]) + __shfl_xor_sync(0xffffffffu, up16 ? a[1] : a[3], 16);
+            float v = (up8 ? b1 : b0) + __shfl_xor_sync(0xffffffffu, up8 ? b0 : b1, 8);
+            v += __shfl_xor_sync(0xffffffffu, v, 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            if ((lane & 7) == 0) sQ[(lane >> 3) * dim + k] = v * p.scale_log2;
+        }
+    }
+    __syncthreads();
+    if (warp < kHQ) {
+        float am = 0.f, cz = 0.f;
+        for (int d = lane; d < dim; d += 32) {
+            const float v = sQ[warp * dim + d];
+            const bool isz = d % 3 == 0;
+            am = fmaxf(am, fabsf(v) * (mode == 0 && isz ? fabsf(dz) : 1.f));
+            if (isz) cz += v;
+        }
+        #pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) {
+            am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, off));
+            cz += __shfl_xor_sync(0xffffffffu, cz, off);
+        }
+        if (lane == 0) {
+            const int k = pow2_to(am, 13, 90);
+            sk[warp] = k;
+            p.head[unit * 8 + warp] = __int_as_float(k);
+            p.head[unit * 8 + 4 + warp] = mode == 0 ? cz * z0 : 0.f;
+        }
+    }
+    __syncthreads();
+    const int nxy = 2 * cpl, frags = nxy + (mode == 0 ? cpl / 2 : cpl);
+    const int g = lane >> 2, c = lane & 3, qh = g & 3;
+    const bool lo = g >= 4;
+    const float su = pow2(sk[qh]);
+    auto qv = [&](int t, int x) { return t < p.m ? sQ[qh * dim + 3 * t + x] * su : 0.f; };
+    for (int r = warp; r < frags; r += NW) {
+        uint32_t v;
+        if (r < nxy) {
+            v = h2_dup_part(qv(k_triplet_of(cpl, c, r >> 1), 1 + (r & 1)), lo);
+        } else if (mode == 0) {                              // two triplets' z, times the bin width
+            const int j = 2 * (r - nxy);
+            v = h2_pair_part(qv(k_triplet_of(cpl, c, j), 0) * dz, qv(k_triplet_of(cpl, c, j + 1), 0) * dz, lo);
+        } else {
+            v = h2_dup_part(qv(k_triplet_of(cpl, c, r - nxy), 0), lo);
+        }
+        p.frag[((int64_t)unit * frags + r) * 32 + lane] = v;
+    }
+}
+
+// d += a . b; EX: the tile's sum starts from zero and joins d in a rounded fp32 addition (the tensor core
+// truncates what it adds to d)
+template <bool EX>
+__device__ __forceinline__ void mma_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    if constexpr (EX) {
+        float t[4] = {0.f, 0.f, 0.f, 0.f};
+        mma16816(t, a0, a1, a2, a3, b0, b1);
+        #pragma unroll
+        for (int x = 0; x < 4; ++x) d[x] += t[x];
+    } else {
+        mma16816(d, a0, a1, a2, a3, b0, b1);
+    }
+}
+
 template <class T>
 __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p) {
     extern __shared__ __align__(128) uint8_t pa_raw[];
     constexpr int W = T::W, NG = T::NG, CPL = T::CPL, CPV = T::CPV, MODE = T::MODE, nthr = T::THREADS;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim;
+    cudaTriggerProgrammaticLaunchCompletion();
     const PASmem L = pa_smem(dim, W, T::CHUNK);
     float* sm = reinterpret_cast<float*>(pa_raw);
-    float *sQ = sm + L.q, *sAcc = sm + L.acc, *sWm = sm + L.wm, *sWl = sm + L.wl, *sMisc = sm + L.misc;
+    float *sAcc = sm + L.acc, *sWm = sm + L.wm, *sWl = sm + L.wl, *sRed = sm + L.red;
     int* sList = reinterpret_cast<int*>(sm + L.list);
     // the tables start at the first 64 KB boundary of shared addresses behind the rest
     const uint32_t base = smem_u32(pa_raw);
@@ -164,55 +279,73 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(have));
         if (tab + T::XY_BYTES + T::Z_BYTES > base + have) {   // the window lies elsewhere than planned for
             if (tid == 0) flag_error(kErrSmemLayout);
+            cudaGridDependencySynchronize();
             return;
         }
     }
     uint8_t* tabp = pa_raw + (tab - base);
-    PagedCursor cur = paged_begin(p);
-    if (cur.t >= cur.end) return;
-    if (tid < dim * dim * 4 / 128) prefetch_l2(reinterpret_cast<const uint8_t*>(p.R) + tid * 128);
 
-    // ---- tables -----------------------------------------------------------------------------------
+    // ---- tables: entries to registers, the largest magnitude, then the scaled pairs -----------------
     const int bits_all = p.bits_z + p.bits_flat;
     const float z0 = __ldg(p.dec_z), dz = __ldg(p.dec_z + 1) - z0;      // MODE 0: z = z0 + i dz
-    int tk;                                                   // the table's power of two
-    {
-        float am = 0.f;
-        const int n = MODE == 0 ? 256 : 1 << (p.xy_per_z ? bits_all : p.bits_flat);
-        for (int i = tid; i < 2 * n; i += nthr) am = fmaxf(am, fabsf(__ldg(p.dec_xy + i)));
-        if (MODE != 0)
-            for (int i = tid; i < 1 << p.bits_z; i += nthr) am = fmaxf(am, fabsf(__ldg(p.dec_z + i)));
-        #pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, off));
-        if (lane == 0) sMisc[8 + warp] = am;
-        __syncthreads();
-        am = 0.f;
-        for (int w = 0; w < W; ++w) am = fmaxf(am, sMisc[8 + w]);
-        tk = pow2_to(am, 9, 30);
+    constexpr int ENT = MODE == 2 ? 4096 : 256, EPT = (ENT + nthr - 1) / nthr;
+    float2 exy[EPT];
+    float ez[MODE == 1 ? EPT : 1];
+    float am = 0.f;
+    #pragma unroll
+    for (int x = 0; x < EPT; ++x) {
+        // codes past 2^bits (never stored by an encoder) read as code 0
+        const int e = tid + x * nthr, code = e < (1 << bits_all) ? e : 0;
+        exy[x] = __ldg(reinterpret_cast<const float2*>(p.dec_xy) +
+                       (p.xy_per_z ? code : code & ((1 << p.bits_flat) - 1)));
+        if (MODE == 1) ez[x] = __ldg(p.dec_z + (code >> p.bits_flat));
+        am = fmaxf(am, fmaxf(fabsf(exy[x].x), fabsf(exy[x].y)));
+    }
+    if (MODE != 0)
+        for (int i = tid; i < 1 << p.bits_z; i += nthr) am = fmaxf(am, fabsf(__ldg(p.dec_z + i)));
+    PagedCursor cur = paged_begin(p);
+    if (cur.t >= cur.end) {
+        cudaGridDependencySynchronize();
+        return;
+    }
+    #pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, off));
+    if (lane == 0) sRed[warp] = am;
+    __syncthreads();
+    am = 0.f;
+    for (int w = 0; w < W; ++w) am = fmaxf(am, sRed[w]);
+    const int tk = pow2_to(am, 9, 30);                        // the tables' power of two
+    auto fill_tables = [&] {
         const float ts = pow2(tk);
-        if constexpr (MODE == 2) {
-            for (int i = tid; i < 1 << bits_all; i += nthr) {
-                const float2 v = __ldg(reinterpret_cast<const float2*>(p.dec_xy) +
-                                       (p.xy_per_z ? i : i & ((1 << p.bits_flat) - 1)));
-                reinterpret_cast<uint2*>(tabp)[i] = make_uint2(h2_split(v.x * ts), h2_split(v.y * ts));
-            }
-            uint32_t* zt = reinterpret_cast<uint32_t*>(tabp + T::XY_BYTES);
-            for (int i = tid; i < 32 << p.bits_z; i += nthr) zt[i] = h2_split(__ldg(p.dec_z + (i >> 5)) * ts);
-        } else {
-            // rows of 16 pieces of 16 bytes (two copies each); codes past 2^bits read row 0's value
-            for (int i = tid; i < 256 * 16; i += nthr) {
-                const int e = i >> 4, code = e < (1 << bits_all) ? e : 0;
-                const float2 v = __ldg(reinterpret_cast<const float2*>(p.dec_xy) +
-                                       (MODE == 0 || p.xy_per_z ? (MODE == 0 ? e : code) : code & ((1 << p.bits_flat) - 1)));
-                const uint32_t x = h2_split(v.x * ts), y = h2_split(v.y * ts);
-                reinterpret_cast<uint4*>(tabp)[i] = make_uint4(x, y, x, y);
+        #pragma unroll
+        for (int x = 0; x < EPT; ++x) {
+            const int e = tid + x * nthr;
+            if (e >= ENT) break;
+            if constexpr (MODE == 2)                          // (not held in registers: 16 of them)
+                exy[x] = __ldg(reinterpret_cast<const float2*>(p.dec_xy) +
+                               (p.xy_per_z ? e & ((1 << bits_all) - 1) : e & ((1 << p.bits_flat) - 1)));
+            const uint2 v = make_uint2(h2_split(exy[x].x * ts), h2_split(exy[x].y * ts));
+            if constexpr (MODE == 2) {
+                reinterpret_cast<uint2*>(tabp)[e] = v;
+            } else {
+                // 32 copies in 16-byte pieces; a thread starts at its own piece, so that a warp's stores
+                // spread over the banks (rows are 256 bytes apart)
+                #pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    reinterpret_cast<uint4*>(tabp)[e * 16 + ((i + tid) & 15)] = make_uint4(v.x, v.y, v.x, v.y);
                 if constexpr (MODE == 1) {
-                    const uint32_t z = h2_split(__ldg(p.dec_z + (code >> p.bits_flat)) * ts);
-                    if ((i & 15) < 8) reinterpret_cast<uint4*>(tabp + T::XY_BYTES)[i] = make_uint4(z, z, z, z);
+                    const uint32_t z = h2_split(ez[x] * ts);
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        reinterpret_cast<uint4*>(tabp + T::XY_BYTES)[e * 16 + ((i + tid) & 7)] = make_uint4(z, z, z, z);
                 }
             }
         }
-    }
+        if constexpr (MODE == 2) {
+            uint32_t* zt = reinterpret_cast<uint32_t*>(tabp + T::XY_BYTES);
+            for (int i = tid; i < 32 << p.bits_z; i += nthr) zt[i] = h2_split(__ldg(p.dec_z + (i >> 5)) * ts);
+        }
+    };
     Lookup lk;
     lk.xy = MODE == 2 ? tab : tab | ((uint32_t)lane << 3);
     lk.z = tab + T::XY_BYTES + ((uint32_t)lane << 2);
@@ -221,88 +354,33 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     lk.xymask = ((1u << bits_all) - 1u) << 3;
 
     const int g = lane >> 2, c = lane & 3, hp = c & 1;
-    const bool lo_col = g >= 4;
-    const int qh = g & 3, rho = (g >> 1) + 4 * (g & 1);
+    const int rho = (g >> 1) + 4 * (g & 1);
     const int row_bytes = p.m * T::CB, per = p.pg.ps_log2 - 4;
     const int tokb = (int)p.pg.tok_bs;                        // (a row; checked to fit 31 bits / 16)
     PagedItem it;
+    bool first = true;
     while (paged_next(p, cur, it)) {
         const int len = clamp_len(p.pg, __ldg(p.seq_lens + it.b));
-        // ---- q' = scale log2(e) R q, a warp per row of R ------------------------------------------
-        __syncthreads();                                      // tables written; last item's sAcc read
-        for (int i = tid; i < kHQ * dim; i += nthr) {
-            const int h = it.hg * kHQ + i / dim;
-            sAcc[i] = h < p.G ? load_any(p.q, p.qdt, it.b * p.q_bs + (int64_t)(it.hk * p.G + h) * p.q_hs + i % dim) : 0.f;
-        }
-        __syncthreads();
-        #pragma unroll 2
-        for (int k = warp; k < dim; k += W) {
-            float a[kHQ] = {0.f, 0.f, 0.f, 0.f};
-            #pragma unroll
-            for (int u = 0; u < (CPL * 12 + 31) / 32; ++u) {
-                const int d = lane + 32 * u;
-                if (d < dim) {
-                    const float r = __ldg(p.R + k * dim + d);
-                    #pragma unroll
-                    for (int h = 0; h < kHQ; ++h) a[h] = fmaf(r, sAcc[h * dim + d], a[h]);
-                }
-            }
-            #pragma unroll
-            for (int h = 0; h < kHQ; ++h)
-                #pragma unroll
-                for (int off = 16; off >= 1; off >>= 1) a[h] += __shfl_xor_sync(0xffffffffu, a[h], off);
-            if (lane < kHQ) sQ[lane * dim + k] = (lane == 0 ? a[0] : lane == 1 ? a[1] : lane == 2 ? a[2] : a[3]) * p.scale_log2;
-        }
-        __syncthreads();
-        if (warp < kHQ) {                                     // per head: operand scale, z0 sum q_z
-            float am = 0.f, cz = 0.f;
-            for (int d = lane; d < dim; d += 32) {
-                const float v = sQ[warp * dim + d];
-                const bool isz = d % 3 == 0;
-                am = fmaxf(am, fabsf(v) * (MODE == 0 && isz ? fabsf(dz) : 1.f));
-                if (isz) cz += v;
-            }
-            #pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) {
-                am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, off));
-                cz += __shfl_xor_sync(0xffffffffu, cz, off);
-            }
-            if (lane == 0) {
-                sMisc[warp] = __int_as_float(pow2_to(am, 13, 90));
-                sMisc[4 + warp] = MODE == 0 ? cz * z0 : 0.f;
-            }
-        }
-        __syncthreads();
-        uint32_t bq[CPL][2], bz[MODE == 0 ? CPL / 4 : CPL / 2][2];
-        {
-            const float su = pow2(__float_as_int(sMisc[qh]));
-            auto qv = [&](int t, int x) { return t < p.m ? sQ[qh * dim + 3 * t + x] * su : 0.f; };
+        uint32_t bq[CPL][2], bz[T::NBZ][2];
+        float us0, us1, cz0, cz1;                              // heads 2 hp, 2 hp + 1 of this lane's score columns
+        auto load_query = [&] {
+            const uint32_t* fr = p.frag + (int64_t)it.unit * T::FRAGS * 32 + lane;
             #pragma unroll
             for (int j = 0; j < CPL; ++j) {
-                const int t = k_triplet<T>(c, j);
-                bq[j][0] = h2_dup_part(qv(t, 1), lo_col);
-                bq[j][1] = h2_dup_part(qv(t, 2), lo_col);
+                bq[j][0] = __ldcg(fr + 64 * j);
+                bq[j][1] = __ldcg(fr + 64 * j + 32);
             }
-            if constexpr (MODE == 0) {
-                // i enters as i 2^-24: the table's power of two is put on the query side
-                #pragma unroll
-                for (int j = 0; j < CPL / 4; ++j) {
-                    bz[j][0] = h2_pair_part(qv(k_triplet<T>(c, 4 * j), 0) * dz, qv(k_triplet<T>(c, 4 * j + 1), 0) * dz, lo_col);
-                    bz[j][1] = h2_pair_part(qv(k_triplet<T>(c, 4 * j + 2), 0) * dz, qv(k_triplet<T>(c, 4 * j + 3), 0) * dz, lo_col);
-                }
-            } else {
-                #pragma unroll
-                for (int j = 0; j < CPL / 2; ++j) {
-                    bz[j][0] = h2_dup_part(qv(k_triplet<T>(c, 2 * j), 0), lo_col);
-                    bz[j][1] = h2_dup_part(qv(k_triplet<T>(c, 2 * j + 1), 0), lo_col);
-                }
+            #pragma unroll
+            for (int j = 0; j < T::NBZ; ++j) {
+                bz[j][0] = __ldcg(fr + 64 * (CPL + j));
+                bz[j][1] = __ldcg(fr + 64 * (CPL + j) + 32);
             }
-        }
-        // heads 2 hp, 2 hp + 1 of this lane's score columns; log2 units
-        const int k0 = __float_as_int(sMisc[2 * hp]), k1 = __float_as_int(sMisc[2 * hp + 1]);
-        const float us0 = pow2(-k0 - tk), us1 = pow2(-k1 - tk);
-        const float cz0 = sMisc[4 + 2 * hp], cz1 = sMisc[4 + 2 * hp + 1];
-        const f32x2 uu = f2_pack(us0, us1), czz = f2_pack(cz0, cz1);
+            const float* hd = p.head + it.unit * 8 + 2 * hp;
+            us0 = pow2(-__float_as_int(__ldcg(hd)) - tk);
+            us1 = pow2(-__float_as_int(__ldcg(hd + 1)) - tk);
+            cz0 = __ldcg(hd + 4);
+            cz1 = __ldcg(hd + 5);
+        };
         const float zs = pow2(24 + tk);                       // MODE 0: z sums onto the (x, y) sums' scale
         float M0 = -INFINITY, M1 = -INFINITY;
         float l0 = 0.f, l1 = 0.f;
@@ -318,7 +396,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
             // ---- pages of the next granules: id, -1 (masked), or id | sign bit (the short page) ----------
             const int j0 = ga >> per, gb = min(it.g1, (j0 + T::CHUNK) << per);
             const int j1 = (gb - 1) >> per;
-            if (ga != it.g0) __syncthreads();                 // (the first list is ordered by the barriers above)
+            __syncthreads();                                  // the last list, and the last item's sums, are read
             for (int j = j0 + tid; j <= j1; j += nthr) {
                 const Granule gr = granule_at(p, it.b, it.hk, j << per);
                 const int lp = p.selected ? gr.tok >> p.pg.ps_log2 : j;
@@ -356,6 +434,14 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     for (int t = 0; t < 4; ++t) load_v<T>(vw[i][t], vbase + off[i] + t * 4 * tokb, g, row_bytes);
                 }
             }
+            if (first) {                                      // while the first codes are on their way
+                fill_tables();
+                __syncthreads();
+                cudaGridDependencySynchronize();              // the queries' fragments
+                first = false;
+            }
+            if (ga == it.g0) load_query();
+            const f32x2 uu = f2_pack(us0, us1), czz = f2_pack(cz0, cz1);
             #pragma unroll 1
             for (; gi < gb; gi += W * NG) {
                 int nn[NG];
@@ -369,18 +455,18 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     #pragma unroll
                     for (int j = 0; j < CPL; ++j) {
                         const uint2 e0 = look_xy<T>(lk, kw[i][0], j), e1 = look_xy<T>(lk, kw[i][1], j);
-                        mma16816((j & 1) ? xb : xa, e0.x, e1.x, e0.y, e1.y, bq[j][0], bq[j][1]);
+                        mma_add<T::EX>((j & 1) ? xb : xa, e0.x, e1.x, e0.y, e1.y, bq[j][0], bq[j][1]);
                     }
                     if constexpr (MODE == 0) {
                         #pragma unroll
                         for (int j = 0; j < CPL / 4; ++j)
-                            mma16816(zz, prmt(kw[i][0][2 * j], 0u, 0x4341u), prmt(kw[i][1][2 * j], 0u, 0x4341u),
+                            mma_add<T::EX>(zz, prmt(kw[i][0][2 * j], 0u, 0x4341u), prmt(kw[i][1][2 * j], 0u, 0x4341u),
                                      prmt(kw[i][0][2 * j + 1], 0u, 0x4341u), prmt(kw[i][1][2 * j + 1], 0u, 0x4341u),
                                      bz[j][0], bz[j][1]);
                     } else {
                         #pragma unroll
                         for (int j = 0; j < CPL / 2; ++j)
-                            mma16816(zz, look_z<T>(lk, kw[i][0], 2 * j), look_z<T>(lk, kw[i][1], 2 * j),
+                            mma_add<T::EX>(zz, look_z<T>(lk, kw[i][0], 2 * j), look_z<T>(lk, kw[i][1], 2 * j),
                                      look_z<T>(lk, kw[i][0], 2 * j + 1), look_z<T>(lk, kw[i][1], 2 * j + 1), bz[j][0], bz[j][1]);
                     }
                     #pragma unroll
@@ -434,12 +520,13 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     }
                 }
                 // ---- weights, transposed into B operands ------------------------------------------------
-                const float n0 = M0 == -INFINITY ? 0.f : 12.f - M0, n1 = M1 == -INFINITY ? 0.f : 12.f - M1;
+                // (the 2^12 is put on afterwards: score - max is exact near the maximum, + 12 would round it)
+                const float n0 = M0 == -INFINITY ? 0.f : M0, n1 = M1 == -INFINITY ? 0.f : M1;
                 uint32_t pA[NG], pB[NG];
                 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
-                    const float p0 = fast_exp2(S[i][0] + n0), p1 = fast_exp2(S[i][1] + n1);
-                    const float p2 = fast_exp2(S[i][2] + n0), p3 = fast_exp2(S[i][3] + n1);
+                    const float p0 = fast_exp2(S[i][0] - n0) * 4096.f, p1 = fast_exp2(S[i][1] - n1) * 4096.f;
+                    const float p2 = fast_exp2(S[i][2] - n0) * 4096.f, p3 = fast_exp2(S[i][3] - n1) * 4096.f;
                     l0 += p0 + p2;
                     l1 += p1 + p3;
                     const uint32_t hA = f2h2(p0, p1), hB = f2h2(p2, p3);
@@ -458,8 +545,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     for (int m = 0; m < CPV; ++m) {
                         const uint2 x0 = look_xy<T>(lk, vw[i][0], m), x1 = look_xy<T>(lk, vw[i][1], m);
                         const uint2 x2 = look_xy<T>(lk, vw[i][2], m), x3 = look_xy<T>(lk, vw[i][3], m);
-                        mma16816(acc[m], x0.x, x0.y, x1.x, x1.y, d0, d1);
-                        mma16816(acc[m], x2.x, x2.y, x3.x, x3.y, d2, d3);
+                        mma_add<T::EX>(acc[m], x0.x, x0.y, x1.x, x1.y, d0, d1);
+                        mma_add<T::EX>(acc[m], x2.x, x2.y, x3.x, x3.y, d2, d3);
                     }
                     #pragma unroll
                     for (int m = 0; m < CPV / 2; ++m) {
@@ -472,9 +559,9 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                             #pragma unroll
                             for (int x = 0; x < 4; ++x) za[x] += zt[x];
                         } else {
-                            mma16816(za, look_z<T>(lk, vw[i][0], 2 * m), look_z<T>(lk, vw[i][0], 2 * m + 1),
+                            mma_add<T::EX>(za, look_z<T>(lk, vw[i][0], 2 * m), look_z<T>(lk, vw[i][0], 2 * m + 1),
                                      look_z<T>(lk, vw[i][1], 2 * m), look_z<T>(lk, vw[i][1], 2 * m + 1), d0, d1);
-                            mma16816(za, look_z<T>(lk, vw[i][2], 2 * m), look_z<T>(lk, vw[i][2], 2 * m + 1),
+                            mma_add<T::EX>(za, look_z<T>(lk, vw[i][2], 2 * m), look_z<T>(lk, vw[i][2], 2 * m + 1),
                                      look_z<T>(lk, vw[i][3], 2 * m), look_z<T>(lk, vw[i][3], 2 * m + 1), d2, d3);
                         }
                     }
@@ -565,52 +652,100 @@ __device__ inline void unit_rows(const PagedParams& p, int unit, int& r0, int& r
     r1 = (int)(((a + n) * gd - 1) / total) + unit + 1;
 }
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 384;
 constexpr int kWeighTokens = 2048;             // tokens per CTA of the weight pass
 
 // CTAs [0, units): one unit each -- join its ranges, normalise, rotate back.  CTAs behind them (with
 // weights): kWeighTokens tokens of one (sequence, KV head) each, p = exp2(score - m) / l summed over its heads.
+// A unit is three round trips to memory: the ranges' (m, l), their sums, and R -- whose first rows are asked
+// for before the grid dependency, thread (group kg, column d) holding rows kg, kg + groups, ... of column d.
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p, int chunks) {
     extern __shared__ float jsm[];
-    const int tid = threadIdx.x, dim = p.dim, rs = dim + 2;
-    cudaGridDependencySynchronize();
+    const int tid = threadIdx.x, dim = p.dim, rs = dim + 2, warp = tid >> 5, lane = tid & 31;
     if ((int)blockIdx.x < p.units) {
         float* sO = jsm;                       // [4][dim]
+        float* sF = sO + kHQ * dim;            // [ranges][4] exp2(m_r - m), at most grid ranges
+        float* sP = sF + kHQ * p.grid;         // [groups][4][dim] partial rotations
+        __shared__ float sInv[kHQ];
+        constexpr int RB = 24;
+        const int cols = (dim + 31) / 32 * 32, groups = kJoinThreads / cols;
+        const int kg = tid / cols, d = tid - kg * cols;
+        const bool mine = kg < groups && d < dim;
+        float rr[RB];
+        auto load_r = [&](int i0) {
+            #pragma unroll
+            for (int i = 0; i < RB; ++i) {
+                const int k = kg + (i0 + i) * groups;
+                rr[i] = mine && k < dim ? __ldg(p.R + k * dim + d) : 0.f;
+            }
+        };
+        load_r(0);
         int r0, r1, n;
         const int unit = blockIdx.x;
         unit_rows(p, unit, r0, r1, n);
-        for (int i = tid; i < kHQ * dim; i += kJoinThreads) {
-            const int h = i / dim, d = i % dim;
-            const float* part = p.part + ((int64_t)r0 * kHQ + h) * rs;
-            float mx = -INFINITY, l = 0.f, o = 0.f;
-            for (int r = r0; r < r1; ++r, part += kHQ * rs) {
-                const float mr = part[0];
-                if (part[1] == 0.f) continue;       // no token (a NaN sum is carried on)
-                const float nm = fmaxf(mx, mr), f0 = l == 0.f ? 0.f : exp2f(mx - nm), f1 = exp2f(mr - nm);
-                mx = nm;
-                l = fmaf(l, f0, part[1] * f1);
-                o = fmaf(o, f0, part[2 + d] * f1);
+        cudaGridDependencySynchronize();
+        const float* part = p.part + (int64_t)r0 * kHQ * rs;
+        const int nr = r1 - r0;
+        if (warp < kHQ) {                       // a range without tokens has l = 0; a NaN sum is carried on
+            float mx = -INFINITY;
+            for (int r = lane; r < nr; r += 32) {
+                const float* q = part + ((int64_t)r * kHQ + warp) * rs;
+                if (__ldcg(q + 1) != 0.f) mx = fmaxf(mx, __ldcg(q));
             }
-            sO[i] = l == 0.f ? 0.f : o / l;
+            #pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            float l = 0.f;
+            for (int r = lane; r < nr; r += 32) {
+                const float* q = part + ((int64_t)r * kHQ + warp) * rs;
+                const float lr = __ldcg(q + 1), f = lr == 0.f ? 0.f : exp2f(__ldcg(q) - mx);
+                sF[r * kHQ + warp] = f;
+                l = fmaf(lr, f, l);
+            }
+            #pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+            if (lane == 0) sInv[warp] = l;
         }
+        __syncthreads();
+        for (int i = tid; i < kHQ * dim; i += kJoinThreads) {
+            const int h = i / dim, x = i - h * dim;
+            const float* q = part + h * rs + 2 + x;
+            float o = 0.f;
+            #pragma unroll 8
+            for (int r = 0; r < nr; ++r) o = fmaf(sF[r * kHQ + h], __ldcg(q + (int64_t)r * kHQ * rs), o);
+            sO[i] = sInv[h] == 0.f ? 0.f : o / sInv[h];
+        }
+        __syncthreads();
+        float v[kHQ] = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 * groups < dim; i0 += RB) {
+            if (i0) load_r(i0);
+            #pragma unroll
+            for (int i = 0; i < RB; ++i) {
+                const int k = min(kg + (i0 + i) * groups, dim - 1);         // (rr is 0 behind the last row)
+                #pragma unroll
+                for (int h = 0; h < kHQ; ++h) v[h] = fmaf(sO[h * dim + k], rr[i], v[h]);
+            }
+        }
+        if (mine)
+            #pragma unroll
+            for (int h = 0; h < kHQ; ++h) sP[(kg * kHQ + h) * dim + d] = v[h];
         __syncthreads();
         const int b = unit / p.UH, u = unit % p.UH, hk = u / p.UG, hg = u % p.UG;
         for (int i = tid; i < kHQ * dim; i += kJoinThreads) {
-            const int h = i / dim, d = i % dim, hl = hg * kHQ + h;
+            const int h = i / dim, hl = hg * kHQ + h;
             if (hl >= p.G) break;
-            float v = 0.f;
-            for (int k = 0; k < dim; ++k) v = fmaf(sO[h * dim + k], __ldg(p.R + k * dim + d), v);
-            store_any(p.out, p.odt, b * p.out_bs + (int64_t)(hk * p.G + hl) * p.out_hs + d, v);
+            float o = 0.f;
+            for (int x = 0; x < groups; ++x) o += sP[x * kHQ * dim + i];
+            store_any(p.out, p.odt, b * p.out_bs + (int64_t)(hk * p.G + hl) * p.out_hs + (i - h * dim), o);
         }
         return;
     }
+    cudaGridDependencySynchronize();
     // ---- weights -----------------------------------------------------------------------------
     const int w = blockIdx.x - p.units, chunk = w % chunks, bh = w / chunks, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
     const int L = clamp_len(p.pg, p.seq_lens[b]);
     const int nv = granules_of(p, b) * kGranule;   // listed or dense tokens
     if (chunk * kWeighTokens >= nv) return;
     float* sOff = jsm;                         // [G] m + log2 l
-    const int warp = tid >> 5, lane = tid & 31;
     for (int h = warp; h < p.G; h += kJoinThreads / 32) {
         int r0, r1, n;
         unit_rows(p, b * p.UH + hk * p.UG + h / kHQ, r0, r1, n);
@@ -684,59 +819,76 @@ static PagedParams paged_params(const pkv_codec* c, const pkv_paged_attn_args* a
     return p;
 }
 
-static size_t paged_part_bytes(const PagedParams& p) {
-    return ((size_t)(p.grid + p.units) * kHQ * (p.dim + 2) * 4 + 255) / 256 * 256;
-}
+// Workspace: partial rows, query fragments (48 registers at most), per-head numbers, scores.
+static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+static size_t paged_part_bytes(const PagedParams& p) { return up256((size_t)(p.grid + p.units) * kHQ * (p.dim + 2) * 4); }
+static size_t paged_frag_bytes(const PagedParams& p) { return up256((size_t)p.units * 48 * 32 * 4); }
+static size_t paged_head_bytes(const PagedParams& p) { return up256((size_t)p.units * 8 * 4); }
 
 size_t paged_workspace(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg, int sms) {
     const PagedParams p = paged_params(c, a, pg, sms);
-    return paged_part_bytes(p) + (a->weights ? (size_t)p.units * p.raw_us * 4 : 0);
+    return paged_part_bytes(p) + paged_frag_bytes(p) + paged_head_bytes(p) + (a->weights ? (size_t)p.units * p.raw_us * 4 : 0);
 }
 
-template <class T>
-static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
-    // tables from the first 64 KB boundary behind the rest (the window starts at most 1 KB into the shared space)
-    const uint32_t below = 1024u + (uint32_t)pa_smem(p.dim, T::W, T::CHUNK).floats * 4u;
-    const int smem = (int)(((below + 0xFFFFu) & ~0xFFFFu) - 1024u) + T::XY_BYTES + T::Z_BYTES;
-    if (cudaFuncSetAttribute(paged_attn_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return PKV_ERR_CUDA;
-    paged_attn_kernel<T><<<p.grid, T::THREADS, smem, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
-}
-
-template <int MODE>
-static int launch_paged_mode(const PagedParams& p, cudaStream_t st) {
-    if (p.m <= 32) return launch_paged_as<PA<MODE, 8, 2, 16>>(p, st);
-    if (p.m <= 48) return launch_paged_as<PA<MODE, 12, 1, 16>>(p, st);
-    return launch_paged_as<PA<MODE, 16, 1, 12>>(p, st);
-}
-
-static int launch_paged_any(const pkv_codec* c, const PagedParams& p, cudaStream_t st) {
-    if (p.cb == 1) return launch_paged_mode<1>(p, st);
-    if (p.bits_flat == 8 && p.bits_z <= 4 && !p.xy_per_z && (c->flags & PKV_CODEC_Z_UNIFORM)) return launch_paged_mode<0>(p, st);
-    return launch_paged_mode<2>(p, st);
-}
-
-int launch_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg, int sms, void* ws, cudaStream_t st) {
-    PagedParams p = paged_params(c, a, pg, sms);
-    p.part = static_cast<float*>(ws);
-    if (a->weights) p.raw = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + paged_part_bytes(p));
-    const int rc = launch_paged_any(c, p, st);
-    if (rc) return rc;
-    const int chunks = a->weights ? (int)((p.raw_us / p.raw_h + kWeighTokens - 1) / kWeighTokens) : 0;
-    const int64_t ctas = p.units + (int64_t)pg.B * pg.Hkv * chunks;
-    if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
+// A launch that may start while the one before it in the stream still runs.
+template <class... A, class... B>
+static int launch_behind(void (*kernel)(A...), unsigned ctas, int threads, size_t smem, cudaStream_t st, B... args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.dynamicSmemBytes = (size_t)(kHQ * p.dim > 16 ? kHQ * p.dim : 16) * 4;   // outputs, or one value per head
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_join_kernel, p, chunks) == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+}
+
+template <class T>
+static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
+    static_assert(T::FRAGS <= 48, "paged_frag_bytes");
+    // tables from the first 64 KB boundary behind the rest (the window starts at most 1 KB into the shared space)
+    const uint32_t below = 1024u + (uint32_t)pa_smem(p.dim, T::W, T::CHUNK).floats * 4u;
+    const int smem = (int)(((below + 0xFFFFu) & ~0xFFFFu) - 1024u) + T::XY_BYTES + T::Z_BYTES;
+    if (cudaFuncSetAttribute(paged_attn_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return PKV_ERR_CUDA;
+    paged_query_kernel<<<p.units, kQueryThreads, 2 * kHQ * p.dim * 4, st>>>(p, T::MODE, T::CPL);
+    if (cudaGetLastError() != cudaSuccess) return PKV_ERR_CUDA;
+    return launch_behind(paged_attn_kernel<T>, p.grid, T::THREADS, smem, st, p);
+}
+
+// fp32 results get the tiles' sums added in rounded fp32 (about an eighth more time); for 16-bit results the
+// truncation of the running sums (a few 1e-6 relative) is far below their own rounding.
+template <int MODE, bool EX>
+static int launch_paged_mode(const PagedParams& p, cudaStream_t st) {
+    if (p.m <= 32) return launch_paged_as<PA<MODE, 8, 2, 16, EX>>(p, st);
+    if (p.m <= 48) return launch_paged_as<PA<MODE, 12, 1, 16, EX>>(p, st);
+    return launch_paged_as<PA<MODE, 16, 1, 12, EX>>(p, st);
+}
+
+template <bool EX>
+static int launch_paged_any(const pkv_codec* c, const PagedParams& p, cudaStream_t st) {
+    if (p.cb == 1) return launch_paged_mode<1, EX>(p, st);
+    if (p.bits_flat == 8 && p.bits_z <= 4 && !p.xy_per_z && (c->flags & PKV_CODEC_Z_UNIFORM)) return launch_paged_mode<0, EX>(p, st);
+    return launch_paged_mode<2, EX>(p, st);
+}
+
+int launch_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg, int sms, void* ws, cudaStream_t st) {
+    PagedParams p = paged_params(c, a, pg, sms);
+    uint8_t* w = static_cast<uint8_t*>(ws);
+    p.part = reinterpret_cast<float*>(w);
+    p.frag = reinterpret_cast<uint32_t*>(w += paged_part_bytes(p));
+    p.head = reinterpret_cast<float*>(w += paged_frag_bytes(p));
+    if (a->weights) p.raw = reinterpret_cast<float*>(w + paged_head_bytes(p));
+    const int rc = a->out_dtype == PKV_F32 ? launch_paged_any<true>(c, p, st) : launch_paged_any<false>(c, p, st);
+    if (rc) return rc;
+    const int chunks = a->weights ? (int)((p.raw_us / p.raw_h + kWeighTokens - 1) / kWeighTokens) : 0;
+    const int64_t ctas = p.units + (int64_t)pg.B * pg.Hkv * chunks;
+    if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
+    const size_t smem = (size_t)(kHQ * p.dim + kHQ * p.grid + kJoinThreads / ((p.dim + 31) / 32 * 32) * kHQ * p.dim) * 4;
+    return launch_behind(paged_join_kernel, (unsigned)ctas, kJoinThreads, smem, st, p, chunks);
 }
 
 }  // namespace pkv
