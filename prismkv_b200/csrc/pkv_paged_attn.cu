@@ -32,7 +32,7 @@ constexpr int kHQ = 4;                         // query heads per unit
 //    one that puts theirs in [2^13, 2^14): pairs of normal fp16 whatever the ranges of the codec and the
 //    data.  Weights are 2^12 exp2(score - running max).
 //  * MODE 0 (two-byte codes, 8 bits of (r, theta), uniform z): z = z0 + i dz enters by its index -- for the
-//    scores as the exact fp16 subnormal i 2^-24, for the values as the exact i - 8, both affine parts added
+//    scores as the exact fp16 subnormal i 2^-24 (EX: as i - 8), for the values as the exact i - 8, both affine parts added
 //    outside.  Centred, because an uncentred sum of p i grows with every token and the tiles' sums truncate.
 // Tables in shared memory: MODE 0 and 1 (one-byte codes, any codec) hold 256 rows of 32 copies, copy `lane`
 // for each lane: the 32 lookups of a warp never collide, and at a 64 KB-aligned address one byte permute of
@@ -153,9 +153,9 @@ __device__ __forceinline__ int pow2_to(float v, int top, int lim) {
 
 // One CTA per unit: q' = scale log2(e) R q of its four heads (zero for heads past the group), then the score
 // operands of every lane, fragment r of lane l at frag[(unit FRAGS + r) 32 + l]: pairs j < CPL of (x, y) of
-// triplet j, then z; head h's power of two and z0 sum q'_z at head[unit 8 + h], + 4.
+// triplet j, then z; head h's power of two and z0 sum q'_z (EX: (z0 + 8 dz) sum q'_z) at head[unit 8 + h], + 4.
 constexpr int kQueryThreads = 512;
-__global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams p, int mode, int cpl) {
+__global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams p, int mode, int cpl, int ex) {
     extern __shared__ float qsm[];
     cudaTriggerProgrammaticLaunchCompletion();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim, unit = blockIdx.x;
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
             const int k = pow2_to(am, 13, 90);
             sk[warp] = k;
             p.head[unit * 8 + warp] = __int_as_float(k);
-            p.head[unit * 8 + 4 + warp] = mode == 0 ? cz * z0 : 0.f;
+            p.head[unit * 8 + 4 + warp] = mode == 0 ? cz * (ex ? fmaf(8.f, dz, z0) : z0) : 0.f;
         }
     }
     __syncthreads();
@@ -244,6 +244,13 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
         }
         p.frag[((int64_t)unit * frags + r) * 32 + lane] = v;
     }
+}
+
+// MODE 0: the z indexes of a word's two codes, as the subnormals i 2^-24 or (EX: sums of q (i - 8) are several
+// times smaller, and so is what they lose) as i - 8
+template <bool EX> __device__ __forceinline__ uint32_t z_index(uint32_t w) {
+    if constexpr (EX) return zc8(w >> 8);
+    return prmt(w, 0u, 0x4341u);
 }
 
 // d += a . b; EX: the tile's sum starts from zero and joins d in a rounded fp32 addition (the tensor core
@@ -381,7 +388,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
             cz0 = __ldcg(hd + 4);
             cz1 = __ldcg(hd + 5);
         };
-        const float zs = pow2(24 + tk);                       // MODE 0: z sums onto the (x, y) sums' scale
+        const float zs = pow2((T::EX ? 0 : 24) + tk);         // MODE 0: z sums onto the (x, y) sums' scale
         float M0 = -INFINITY, M1 = -INFINITY;
         float l0 = 0.f, l1 = 0.f;
         float acc[CPV + CPV / 2][4];
@@ -460,9 +467,9 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     if constexpr (MODE == 0) {
                         #pragma unroll
                         for (int j = 0; j < CPL / 4; ++j)
-                            mma_add<T::EX>(zz, prmt(kw[i][0][2 * j], 0u, 0x4341u), prmt(kw[i][1][2 * j], 0u, 0x4341u),
-                                     prmt(kw[i][0][2 * j + 1], 0u, 0x4341u), prmt(kw[i][1][2 * j + 1], 0u, 0x4341u),
-                                     bz[j][0], bz[j][1]);
+                            mma_add<T::EX>(zz, z_index<T::EX>(kw[i][0][2 * j]), z_index<T::EX>(kw[i][1][2 * j]),
+                                           z_index<T::EX>(kw[i][0][2 * j + 1]), z_index<T::EX>(kw[i][1][2 * j + 1]),
+                                           bz[j][0], bz[j][1]);
                     } else {
                         #pragma unroll
                         for (int j = 0; j < CPL / 2; ++j)
@@ -854,7 +861,7 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
     const int smem = (int)(((below + 0xFFFFu) & ~0xFFFFu) - 1024u) + T::XY_BYTES + T::Z_BYTES;
     if (cudaFuncSetAttribute(paged_attn_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return PKV_ERR_CUDA;
-    paged_query_kernel<<<p.units, kQueryThreads, 2 * kHQ * p.dim * 4, st>>>(p, T::MODE, T::CPL);
+    paged_query_kernel<<<p.units, kQueryThreads, 2 * kHQ * p.dim * 4, st>>>(p, T::MODE, T::CPL, T::EX);
     if (cudaGetLastError() != cudaSuccess) return PKV_ERR_CUDA;
     return launch_behind(paged_attn_kernel<T>, p.grid, T::THREADS, smem, st, p);
 }

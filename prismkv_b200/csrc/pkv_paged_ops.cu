@@ -108,122 +108,122 @@ __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
 }
 
 // ---- the k largest of a row, in index order ---------------------------------------------------------
-// A cluster of CTAs holds a row of n keys (unsigned, larger = better), CTA `rank` the slice [lo, hi).
-// Three digit passes (11, 11, 10 bits) of histograms narrow the k-th largest key; a last pass writes the
-// indexes of the keys above it and of the first equal ones, in index order.  Counters of all CTAs meet in
-// rank 0's shared memory.
+// A cluster of CTAs holds a row of n keys (unsigned, larger = better): CTA `rank` the slice [lo, hi), its
+// warps contiguous parts of that.  Histograms of the key's digits from the top narrow the k-th largest key;
+// then every warp counts the keys of its part above and equal to it, and writes their indexes behind those of
+// the parts before it (of the equal ones the first `need` of the row).  One cluster barrier per digit: every CTA
+// sums all CTAs' histograms for itself, and the histograms of two digits alternate.
+// What bounds it: a handful of barriers and round trips through the cluster's shared memory for short rows, the
+// passes over the keys in shared memory for long ones.
 constexpr int kTopThreads = 512;
-constexpr int kTopBins = 2048;
+constexpr int kTopWarps = kTopThreads / 32;
 
+template <int DIGIT>
 struct TopShared {
-    uint32_t hist[kTopBins];
-    uint32_t warp[2][kTopThreads / 32];
+    uint32_t hist[2][1 << DIGIT];
+    uint32_t warp[2][kTopWarps];
+    uint32_t total[2];                         // this CTA's keys above and equal to the threshold
     uint32_t bin, need;
 };
 
-template <class Key, class Put>
-__device__ void top_row(TopShared& s, int lo, int hi, int n, int k, Key key, Put put) {
+// BITS-bit keys in digits of DIGIT bits (the last one may be shorter)
+template <int BITS, int DIGIT, class Key, class Put>
+__device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key key, Put put) {
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const unsigned rank = cl.block_rank(), C = cl.num_blocks();
-    TopShared* s0 = cl.map_shared_rank(&s, 0);
-    cl.sync();                                              // every CTA of the cluster runs: its memory may be reached
+    constexpr int BINS = 1 << DIGIT, PER = BINS / kTopThreads, PASSES = (BITS + DIGIT - 1) / DIGIT;
     uint32_t prefix = 0, need = (uint32_t)min(k, n);        // keys still to take among those with this prefix
     const bool all = n <= k;
-    int shift = 32;
+    for (int i = tid; i < 2 * BINS; i += kTopThreads) (&s.hist[0][0])[i] = 0;
+    __syncthreads();
     if (!all) {
+        int shift = BITS;
         #pragma unroll 1
-        for (int pass = 0; pass < 3; ++pass) {
-            const int bits = pass < 2 ? 11 : 10, bins = 1 << bits;
-            const uint32_t above = shift == 32 ? 0u : prefix >> shift;
-            for (int i = tid; i < kTopBins; i += kTopThreads) s.hist[i] = 0;
-            cl.sync();
+        for (int pass = 0; pass < PASSES; ++pass) {
+            const int bits = min(DIGIT, shift), low = shift - bits;
+            uint32_t* hist = s.hist[pass & 1];
             for (int i = lo + tid; i < hi; i += kTopThreads) {
                 const uint32_t x = key(i);
-                if (shift == 32 || (x >> shift) == above) atomicAdd(&s.hist[(x >> (shift - bits)) & (bins - 1)], 1u);
+                if (shift == BITS || (x >> shift) == (prefix >> shift)) atomicAdd(&hist[(x >> low) & ((1u << bits) - 1u)], 1u);
             }
             cl.sync();
-            if (rank != 0)
-                for (int i = tid; i < bins; i += kTopThreads)
-                    if (s.hist[i]) atomicAdd(&s0->hist[i], s.hist[i]);
-            cl.sync();
-            // rank 0: the bin where the count from the top reaches `need`
-            if (rank == 0) {
-                const int per = bins / kTopThreads;         // 4 or 2 bins a thread, thread 0 the top ones
-                uint32_t v[4], sum = 0;
-                for (int j = 0; j < per; ++j) sum += v[j] = s.hist[bins - 1 - (tid * per + j)];
-                uint32_t inc = sum;
+            if (pass + 2 < PASSES + 1 && pass > 0)          // the other one was read before this barrier
+                for (int i = tid; i < BINS; i += kTopThreads) s.hist[(pass + 1) & 1][i] = 0;
+            // bins from the top, PER neighbouring ones a thread, summed over the cluster
+            uint32_t v[PER], sum = 0;
+            #pragma unroll
+            for (int j = 0; j < PER; ++j) v[j] = 0;
+            for (unsigned r = 0; r < C; ++r) {
+                const uint32_t* h = cl.map_shared_rank(&s, r)->hist[pass & 1];
                 #pragma unroll
-                for (int off = 1; off < 32; off <<= 1) {
-                    const uint32_t o = __shfl_up_sync(0xffffffffu, inc, off);
-                    if (lane >= off) inc += o;
-                }
-                if (lane == 31) s.warp[0][warp] = inc;
-                __syncthreads();
-                for (int w = 0; w < warp; ++w) inc += s.warp[0][w];
-                uint32_t cum = inc - sum;
-                for (int j = 0; j < per; ++j) {
-                    if (cum < need && cum + v[j] >= need) {
-                        s.bin = bins - 1 - (tid * per + j);
-                        s.need = need - cum;
-                    }
-                    cum += v[j];
-                }
+                for (int j = 0; j < PER; ++j) v[j] += h[BINS - 1 - (tid * PER + j)];
             }
-            cl.sync();
-            shift -= bits;
-            prefix |= s0->bin << shift;
-            need = s0->need;
-            cl.sync();
+            #pragma unroll
+            for (int j = 0; j < PER; ++j) sum += v[j];
+            uint32_t inc = sum;
+            #pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const uint32_t o = __shfl_up_sync(0xffffffffu, inc, off);
+                if (lane >= off) inc += o;
+            }
+            if (lane == 31) s.warp[0][warp] = inc;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) inc += s.warp[0][w];
+            uint32_t cum = inc - sum;
+            #pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (cum < need && cum + v[j] >= need) {
+                    s.bin = BINS - 1 - (tid * PER + j);
+                    s.need = need - cum;
+                }
+                cum += v[j];
+            }
+            __syncthreads();
+            prefix |= s.bin << low;
+            need = s.need;
+            shift = low;
+            __syncthreads();
         }
     }
-    // counts of this slice
+    // this warp's part, and its keys above and equal to the threshold
+    const int part = (hi - lo + kTopWarps - 1) / kTopWarps;
+    const int w0 = min(hi, lo + warp * part), w1 = min(hi, w0 + part);
     uint32_t above = 0, equal = 0;
-    for (int i = lo + tid; i < hi; i += kTopThreads) {
+    for (int i = w0 + lane; i < w1; i += 32) {
         const uint32_t x = key(i);
         above += all || x > prefix;
         equal += !all && x == prefix;
     }
-    #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-        above += __shfl_xor_sync(0xffffffffu, above, off);
-        equal += __shfl_xor_sync(0xffffffffu, equal, off);
-    }
-    __syncthreads();
+    above = __reduce_add_sync(0xffffffffu, above);
+    equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) { s.warp[0][warp] = above; s.warp[1][warp] = equal; }
     __syncthreads();
-    if (tid == 0) {
-        uint32_t a = 0, e = 0;
-        for (int w = 0; w < kTopThreads / 32; ++w) { a += s.warp[0][w]; e += s.warp[1][w]; }
-        s0->hist[2 * rank] = a;                              // the histogram is done with
-        s0->hist[2 * rank + 1] = e;
+    uint32_t pa = 0, pe = 0, ta = 0, te = 0;
+    for (int w = 0; w < kTopWarps; ++w) {
+        if (w == warp) { pa = ta; pe = te; }
+        ta += s.warp[0][w];
+        te += s.warp[1][w];
     }
+    if (tid == 0) { s.total[0] = ta; s.total[1] = te; }
     cl.sync();
-    uint32_t base_a = 0, base_e = 0;
-    for (unsigned r = 0; r < rank; ++r) { base_a += s0->hist[2 * r]; base_e += s0->hist[2 * r + 1]; }
-    cl.sync();                                               // remote reads done before anyone leaves
-    // in index order, kTopThreads keys at a time: position = keys above before + equal ones taken before
-    for (int i0 = lo; i0 < hi; i0 += kTopThreads) {
-        const int i = i0 + tid;
-        const uint32_t x = i < hi ? key(i) : 0u;
-        const bool a = i < hi && (all || x > prefix), e = i < hi && !all && x == prefix;
-        const unsigned ma = __ballot_sync(0xffffffffu, a), me = __ballot_sync(0xffffffffu, e);
-        __syncthreads();
-        if (lane == 0) { s.warp[0][warp] = __popc(ma); s.warp[1][warp] = __popc(me); }
-        __syncthreads();
-        uint32_t pa = base_a, pe = base_e, ta = 0, te = 0;
-        for (int w = 0; w < kTopThreads / 32; ++w) {
-            if (w < warp) { pa += s.warp[0][w]; pe += s.warp[1][w]; }
-            ta += s.warp[0][w];
-            te += s.warp[1][w];
-        }
-        const unsigned below = (1u << lane) - 1u;
-        pa += __popc(ma & below);
-        pe += __popc(me & below);
-        if (a || (e && pe < need)) put((int)(pa + min(pe, need)), i);
-        base_a += ta;
-        base_e += te;
+    for (unsigned r = 0; r < rank; ++r) {
+        const uint32_t* t = cl.map_shared_rank(&s, r)->total;
+        pa += t[0];
+        pe += t[1];
     }
+    const unsigned below = (1u << lane) - 1u;
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t x = i < w1 ? key(i) : 0u;
+        const bool a = i < w1 && (all || x > prefix), e = i < w1 && !all && x == prefix;
+        const unsigned ma = __ballot_sync(0xffffffffu, a), me = __ballot_sync(0xffffffffu, e);
+        const uint32_t ea = pe + __popc(me & below);
+        if (a || (e && ea < need)) put((int)(pa + __popc(ma & below) + min(ea, need)), i);
+        pa += __popc(ma);
+        pe += __popc(me);
+    }
+    cl.sync();                                               // no CTA leaves while another reads its counts
 }
 
 // this CTA's slice of n keys
@@ -246,74 +246,115 @@ struct SelectParams {
     int32_t* out;
 };
 
+// One cluster per (sequence, KV head), a slice of its pages per CTA.
+//  * The queries are rotated in 64 bits -- a rounding to int8 must not turn on how a sum was ordered -- each CTA
+//    a share of the rows of R for all heads, the results stored into every CTA's shared memory.
+//  * Four lanes score a page: a summary is 2 pitch bytes in one piece, its 16-byte pieces go round the four
+//    lanes, the int8 queries (positive parts against the greatest, negative ones against the least) lie in
+//    shared memory in the same order, and __dp4a sums 32-bit integers exactly.  The summaries' bytes bound it
+//    for long sequences; they are asked into L2 before the rotation starts.
+//  * A score is below 192 * 127 * 127 < 2^22 in magnitude: keys of 24 bits, two digits of 12.
+constexpr int kPageDigit = 12;
+constexpr uint32_t kForcedKey = 0xffffffu;
+
 __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams p) {
     extern __shared__ __align__(16) uint8_t ssm[];
-    __shared__ TopShared top;
-    __shared__ double amax_w[kTopThreads / 32];
+    __shared__ TopShared<kPageDigit> top;
+    __shared__ double amax_w[kTopWarps];
     cg::cluster_group cl = cg::this_cluster();
-    const int tid = threadIdx.x, dim = p.dim;
-    const int bh = blockIdx.x / cl.num_blocks(), b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
-    const int words = p.pitch / 4;
-    double* sq = reinterpret_cast<double*>(ssm);                       // [G][dim]
-    int8_t* qp = reinterpret_cast<int8_t*>(sq + p.G * dim);            // [G][pitch] positive, then negative parts
-    uint32_t* keys = reinterpret_cast<uint32_t*>(qp + 2 * p.G * p.pitch);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim;
+    const int rank = cl.block_rank(), C = cl.num_blocks();
+    const int bh = blockIdx.x / C, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
     const int L = clamp_len(p.pg, p.seq_lens[b]);
     const int n = (int)(((int64_t)L + (1 << p.pg.ps_log2) - 1) >> p.pg.ps_log2);
+    int8_t* qp = reinterpret_cast<int8_t*>(ssm);                       // [G][2][pitch] negative, then positive parts
+    double* sq = reinterpret_cast<double*>(qp + 2 * p.G * p.pitch);    // [G][dim] (pitch: a multiple of 16)
+    float* raw = reinterpret_cast<float*>(sq + p.G * dim);             // [G][dim]
+    uint32_t* keys = reinterpret_cast<uint32_t*>(raw + p.G * dim);
     int lo, hi;
     top_slice(n, lo, hi);
-    // rotated queries in 64 bits: a rounding to int8 must not turn on how a sum was ordered
+    for (int i = tid; i < p.G * dim; i += kTopThreads)
+        raw[i] = load_any(p.q, p.qdt, b * p.q_bs + (int64_t)(hk * p.G + i / dim) * p.q_hs + i % dim);
+    for (int j = lo + tid; j < hi; j += kTopThreads)
+        if (j >= p.sinks && j < n - p.recent) {
+            const int page = page_of(p.pg, b, j);
+            if (page >= 0)
+                for (int x = 0; x < 2 * p.pitch; x += 64)       // (64 apart: a summary need not start a line)
+                    prefetch_l2(p.sums + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch + x);
+        }
+    cl.sync();                                               // raw queries; every CTA of the cluster runs
+    for (int k = rank * kTopWarps + warp; k < dim; k += C * kTopWarps) {
+        float r[6];
+        #pragma unroll
+        for (int x = 0; x < 6; ++x) r[x] = lane + 32 * x < dim ? __ldg(p.R + k * dim + lane + 32 * x) : 0.f;
+        for (int h = 0; h < p.G; ++h) {
+            double a = 0.0;
+            #pragma unroll
+            for (int x = 0; x < 6; ++x)
+                if (32 * x < dim && lane + 32 * x < dim) a = fma((double)raw[h * dim + lane + 32 * x], (double)r[x], a);
+            #pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) a += __shfl_xor_sync(0xffffffffu, a, off);
+            if (lane < C) cl.map_shared_rank(sq, lane)[h * dim + k] = a;
+        }
+    }
+    cl.sync();
     double amax = 0.0;
     for (int i = tid; i < p.G * dim; i += kTopThreads) {
-        const int h = i / dim, k = i % dim;
-        const int64_t qo = b * p.q_bs + (int64_t)(hk * p.G + h) * p.q_hs;
-        double a = 0.0;
-        for (int d = 0; d < dim; ++d) a = fma((double)load_any(p.q, p.qdt, qo + d), (double)__ldg(p.R + k * dim + d), a);
-        sq[i] = a;
-        amax = fmax(amax, fabs(a));
-        if (!(fabs(a) <= 1e300)) amax = INFINITY;
+        const double a = fabs(sq[i]);
+        amax = a <= 1e300 ? fmax(amax, a) : INFINITY;       // NaN too
+        if (amax == INFINITY) break;
     }
     #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-    if ((tid & 31) == 0) amax_w[tid >> 5] = amax;
+    if (lane == 0) amax_w[warp] = amax;
     __syncthreads();
     amax = 0.0;
-    for (int w = 0; w < kTopThreads / 32; ++w) amax = fmax(amax, amax_w[w]);
+    for (int w = 0; w < kTopWarps; ++w) amax = fmax(amax, amax_w[w]);
     for (int i = tid; i < p.G * p.pitch; i += kTopThreads) {
         const int h = i / p.pitch, d = i % p.pitch;
         int v = 0;
         // a zero or non-finite group scores every page alike
         if (d < dim && amax > 0.0 && amax <= 1e300) v = (int)rint(sq[h * dim + d] * 127.0 / amax);
-        qp[i] = (int8_t)max(v, 0);
-        qp[p.G * p.pitch + i] = (int8_t)min(v, 0);
+        qp[2 * h * p.pitch + d] = (int8_t)min(v, 0);
+        qp[(2 * h + 1) * p.pitch + d] = (int8_t)max(v, 0);
     }
     __syncthreads();
-    const int* qpos = reinterpret_cast<const int*>(qp);
-    const int* qneg = qpos + p.G * words;
-    for (int j = lo + tid; j < hi; j += kTopThreads) {
-        uint32_t key = 0xffffffffu;
-        if (j >= p.sinks && j < n - p.recent) {
-            const int page = page_of(p.pg, b, j);
-            key = 0;
-            if (page >= 0) {
-                const int* least = reinterpret_cast<const int*>(p.sums + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch);
-                int best = INT_MIN;
-                for (int h = 0; h < p.G; ++h) {
-                    int a = 0;
-                    for (int w = 0; w < words; ++w) {
-                        a = __dp4a(least[words + w], qpos[h * words + w], a);
-                        a = __dp4a(least[w], qneg[h * words + w], a);
-                    }
-                    best = max(best, a);
-                }
-                key = (uint32_t)best ^ 0x80000000u;
-            }
+    // ---- scores: four lanes a page, pieces lane & 3, + 4, ... -------------------------------------------
+    const int pieces = 2 * p.pitch / 16, sub = lane & 3;
+    const int4* q4 = reinterpret_cast<const int4*>(qp);
+    for (int j0 = lo + warp * 8; j0 < hi; j0 += kTopWarps * 8) {
+        const int j = j0 + (lane >> 2);
+        const bool scored = j < hi && j >= p.sinks && j < n - p.recent;
+        const int page = scored ? page_of(p.pg, b, j) : -1;
+        int4 w[6];                                           // pitch <= 192: at most 24 pieces
+        #pragma unroll
+        for (int x = 0; x < 6; ++x) {
+            w[x] = make_int4(0, 0, 0, 0);
+            if (page >= 0 && sub + 4 * x < pieces)
+                w[x] = __ldcs(reinterpret_cast<const int4*>(p.sums + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch) + sub + 4 * x);
         }
-        keys[j - lo] = key;
+        int best = INT_MIN;
+        for (int h = 0; h < p.G; ++h) {
+            int a = 0;
+            #pragma unroll
+            for (int x = 0; x < 6; ++x)
+                if (sub + 4 * x < pieces) {
+                    const int4 qv = q4[h * pieces + sub + 4 * x];
+                    a = __dp4a(w[x].x, qv.x, a);
+                    a = __dp4a(w[x].y, qv.y, a);
+                    a = __dp4a(w[x].z, qv.z, a);
+                    a = __dp4a(w[x].w, qv.w, a);
+                }
+            a += __shfl_xor_sync(0xffffffffu, a, 1);
+            a += __shfl_xor_sync(0xffffffffu, a, 2);
+            best = max(best, a);
+        }
+        if (sub == 0 && j < hi) keys[j - lo] = !scored ? kForcedKey : page < 0 ? 0u : (uint32_t)(best + (1 << 22));
     }
     __syncthreads();
     int32_t* out = p.out + (int64_t)bh * p.top;
-    for (int i = min(n, p.top) + cl.block_rank() * kTopThreads + tid; i < p.top; i += cl.num_blocks() * kTopThreads) out[i] = -1;
-    top_row(top, lo, hi, n, p.top, [&](int i) { return keys[i - lo]; }, [&](int at, int i) { out[at] = i; });
+    for (int i = min(n, p.top) + rank * kTopThreads + tid; i < p.top; i += C * kTopThreads) out[i] = -1;
+    top_row<24, kPageDigit>(top, lo, hi, n, p.top, [&](int i) { return keys[i - lo]; }, [&](int at, int i) { out[at] = i; });
 }
 
 // ---- choosing tokens ----------------------------------------------------------------------------------
@@ -333,14 +374,14 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 __global__ void __launch_bounds__(kTopThreads) tokens_select_kernel(KeepParams p) {
     extern __shared__ uint32_t ksm[];
-    __shared__ TopShared top;
+    __shared__ TopShared<11> top;
     cg::cluster_group cl = cg::this_cluster();
     const int bh = blockIdx.x / cl.num_blocks(), tid = threadIdx.x;
     const int n = min(max(p.seq_lens[bh / p.Hkv], 0), p.slots);
     const float* w = p.w + (int64_t)bh * p.w_rs;
     int lo, hi;
     top_slice(n, lo, hi);
-    auto make = [&](int i) { return i < p.sinks || i >= n - p.recent ? 0xffffffffu : weight_key(__ldg(w + i)); };
+    auto make = [&](int i, float x) { return i < p.sinks || i >= n - p.recent ? 0xffffffffu : weight_key(x); };
     int32_t* kept = p.kept + (int64_t)bh * p.keep;
     float* kw = p.kept_w + (int64_t)bh * p.keep;
     for (int i = min(n, p.keep) + cl.block_rank() * kTopThreads + tid; i < p.keep; i += cl.num_blocks() * kTopThreads) {
@@ -349,11 +390,12 @@ __global__ void __launch_bounds__(kTopThreads) tokens_select_kernel(KeepParams p
     }
     auto put = [&](int at, int i) { kept[at] = i; kw[at] = __ldg(w + i); };
     if (p.cached) {
-        for (int i = lo + tid; i < hi; i += kTopThreads) ksm[i - lo] = make(i);
+        #pragma unroll 8
+        for (int i = lo + tid; i < hi; i += kTopThreads) ksm[i - lo] = make(i, __ldg(w + i));
         __syncthreads();
-        top_row(top, lo, hi, n, p.keep, [&](int i) { return ksm[i - lo]; }, put);
+        top_row<32, 11>(top, lo, hi, n, p.keep, [&](int i) { return ksm[i - lo]; }, put);
     } else {
-        top_row(top, lo, hi, n, p.keep, make, put);
+        top_row<32, 11>(top, lo, hi, n, p.keep, [&](int i) { return make(i, __ldg(w + i)); }, put);
     }
 }
 
@@ -384,7 +426,7 @@ static int launch_cluster(K kernel, const P& p, int64_t rows, int c, size_t smem
     return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
 }
 
-constexpr int64_t kKeyCap = 48 * 1024;          // keys of a slice in shared memory (192 KB)
+constexpr int64_t kKeyCap = 48 * 1024;          // weights of a slice in shared memory (192 KB)
 
 int launch_tokens_select(const float* w, int B, int Hkv, int slots, int64_t rs, const int32_t* lens, int keep, int sinks,
                          int recent, int32_t* kept, float* kept_w, int sms, cudaStream_t st) {
@@ -396,7 +438,7 @@ int launch_tokens_select(const float* w, int B, int Hkv, int slots, int64_t rs, 
     return launch_cluster(tokens_select_kernel, p, rows, c, p.cached ? (size_t)per * 4 : 0, st);
 }
 
-// Shared memory of the selection without its keys; keys of a slice take what is left of 200 KB.
+// Shared memory of the selection without its keys; keys of a slice take what is left of 190 KB.
 int launch_pages_select(const pkv_codec* c, Pages pg, const void* q, int qdt, int q_heads, int64_t q_bs, int64_t q_hs,
                         const int32_t* lens, const int8_t* sums, int top, int sinks, int recent, int32_t* out, int sms,
                         cudaStream_t st) {
@@ -411,8 +453,8 @@ int launch_pages_select(const pkv_codec* c, Pages pg, const void* q, int qdt, in
     p.sums = sums;
     p.top = top; p.sinks = sinks; p.recent = recent;
     p.out = out;
-    const int64_t fixed = (int64_t)p.G * p.dim * 8 + 2 * (int64_t)p.G * p.pitch;
-    const int64_t cap = (200 * 1024 - fixed) / 4, rows = (int64_t)pg.B * pg.Hkv;
+    const int64_t fixed = (int64_t)p.G * p.dim * 12 + 2 * (int64_t)p.G * p.pitch;
+    const int64_t cap = (190 * 1024 - fixed) / 4, rows = (int64_t)pg.B * pg.Hkv;
     const int cl = top_cluster(rows, pg.max_pages, sms, cap);
     const int64_t per = ((int64_t)pg.max_pages + cl - 1) / cl;
     if (per > cap) return PKV_ERR_UNSUPPORTED;
