@@ -120,19 +120,21 @@ constexpr int kTopWarps = kTopThreads / 32;
 
 template <int DIGIT>
 struct TopShared {
-    uint32_t hist[2][1 << DIGIT];
+    alignas(16) uint32_t hist[2][1 << DIGIT];
     uint32_t warp[2][kTopWarps];
     uint32_t total[2];                         // this CTA's keys above and equal to the threshold
     uint32_t bin, need;
 };
 
-// BITS-bit keys in digits of DIGIT bits (the last one may be shorter)
+// BITS-bit keys in digits of DIGIT bits (the last one may be shorter).  put(at, i): keys i, i + 32, i + 64,
+// i + 96 go to places at[0 .. 3] (negative: not taken).
 template <int BITS, int DIGIT, class Key, class Put>
 __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key key, Put put) {
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const unsigned rank = cl.block_rank(), C = cl.num_blocks();
     constexpr int BINS = 1 << DIGIT, PER = BINS / kTopThreads, PASSES = (BITS + DIGIT - 1) / DIGIT;
+    static_assert(PER % 4 == 0, "a thread's bins are read as 16-byte pieces");
     uint32_t prefix = 0, need = (uint32_t)min(k, n);        // keys still to take among those with this prefix
     const bool all = n <= k;
     for (int i = tid; i < 2 * BINS; i += kTopThreads) (&s.hist[0][0])[i] = 0;
@@ -143,9 +145,14 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
         for (int pass = 0; pass < PASSES; ++pass) {
             const int bits = min(DIGIT, shift), low = shift - bits;
             uint32_t* hist = s.hist[pass & 1];
-            for (int i = lo + tid; i < hi; i += kTopThreads) {
-                const uint32_t x = key(i);
-                if (shift == BITS || (x >> shift) == (prefix >> shift)) atomicAdd(&hist[(x >> low) & ((1u << bits) - 1u)], 1u);
+            for (int i0 = lo + tid; i0 < hi; i0 += 4 * kTopThreads) {
+                uint32_t x[4];
+                #pragma unroll
+                for (int u = 0; u < 4; ++u) x[u] = i0 + u * kTopThreads < hi ? key(i0 + u * kTopThreads) : 0u;
+                #pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (i0 + u * kTopThreads < hi && (shift == BITS || (x[u] >> shift) == (prefix >> shift)))
+                        atomicAdd(&hist[(x[u] >> low) & ((1u << bits) - 1u)], 1u);
             }
             cl.sync();
             if (pass + 2 < PASSES + 1 && pass > 0)          // the other one was read before this barrier
@@ -154,10 +161,14 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
             uint32_t v[PER], sum = 0;
             #pragma unroll
             for (int j = 0; j < PER; ++j) v[j] = 0;
+            #pragma unroll 2
             for (unsigned r = 0; r < C; ++r) {
-                const uint32_t* h = cl.map_shared_rank(&s, r)->hist[pass & 1];
+                const uint4* h = reinterpret_cast<const uint4*>(cl.map_shared_rank(&s, r)->hist[pass & 1]);
                 #pragma unroll
-                for (int j = 0; j < PER; ++j) v[j] += h[BINS - 1 - (tid * PER + j)];
+                for (int j = 0; j < PER; j += 4) {
+                    const uint4 x = h[(BINS - 4 - (tid * PER + j)) / 4];
+                    v[j] += x.w; v[j + 1] += x.z; v[j + 2] += x.y; v[j + 3] += x.x;
+                }
             }
             #pragma unroll
             for (int j = 0; j < PER; ++j) sum += v[j];
@@ -213,15 +224,20 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
         pe += t[1];
     }
     const unsigned below = (1u << lane) - 1u;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t x = i < w1 ? key(i) : 0u;
-        const bool a = i < w1 && (all || x > prefix), e = i < w1 && !all && x == prefix;
-        const unsigned ma = __ballot_sync(0xffffffffu, a), me = __ballot_sync(0xffffffffu, e);
-        const uint32_t ea = pe + __popc(me & below);
-        if (a || (e && ea < need)) put((int)(pa + __popc(ma & below) + min(ea, need)), i);
-        pa += __popc(ma);
-        pe += __popc(me);
+    for (int i0 = w0; i0 < w1; i0 += 128) {
+        int at[4];                                           // places of this lane's four keys, -1: not taken
+        #pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = i0 + 32 * u + lane;
+            const uint32_t x = i < w1 ? key(i) : 0u;
+            const bool a = i < w1 && (all || x > prefix), e = i < w1 && !all && x == prefix;
+            const unsigned ma = __ballot_sync(0xffffffffu, a), me = __ballot_sync(0xffffffffu, e);
+            const uint32_t ea = pe + __popc(me & below);
+            at[u] = a || (e && ea < need) ? (int)(pa + __popc(ma & below) + min(ea, need)) : -1;
+            pa += __popc(ma);
+            pe += __popc(me);
+        }
+        put(at, i0 + lane);
     }
     cl.sync();                                               // no CTA leaves while another reads its counts
 }
@@ -354,7 +370,12 @@ __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams 
     __syncthreads();
     int32_t* out = p.out + (int64_t)bh * p.top;
     for (int i = min(n, p.top) + rank * kTopThreads + tid; i < p.top; i += C * kTopThreads) out[i] = -1;
-    top_row<24, kPageDigit>(top, lo, hi, n, p.top, [&](int i) { return keys[i - lo]; }, [&](int at, int i) { out[at] = i; });
+    top_row<24, kPageDigit>(top, lo, hi, n, p.top, [&](int i) { return keys[i - lo]; },
+                              [&](const int (&at)[4], int i) {
+                                  #pragma unroll
+                                  for (int u = 0; u < 4; ++u)
+                                      if (at[u] >= 0) out[at[u]] = i + 32 * u;
+                              });
 }
 
 // ---- choosing tokens ----------------------------------------------------------------------------------
@@ -388,7 +409,17 @@ __global__ void __launch_bounds__(kTopThreads) tokens_select_kernel(KeepParams p
         kept[i] = -1;
         kw[i] = 0.f;
     }
-    auto put = [&](int at, int i) { kept[at] = i; kw[at] = __ldg(w + i); };
+    auto put = [&](const int (&at)[4], int i) {
+        float x[4];
+        #pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = at[u] >= 0 ? __ldg(w + i + 32 * u) : 0.f;
+        #pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (at[u] >= 0) {
+                kept[at[u]] = i + 32 * u;
+                kw[at[u]] = x[u];
+            }
+    };
     if (p.cached) {
         #pragma unroll 8
         for (int i = lo + tid; i < hi; i += kTopThreads) ksm[i - lo] = make(i, __ldg(w + i));
@@ -400,10 +431,10 @@ __global__ void __launch_bounds__(kTopThreads) tokens_select_kernel(KeepParams p
 }
 
 // ---- launches -------------------------------------------------------------------------------------------
-// CTAs per row: enough rows x CTAs for the SMs, slices of 2048 keys or more, and small enough to be held.
-static int top_cluster(int64_t rows, int64_t n, int sms, int64_t cap) {
+// CTAs per row: as many as the SMs hold at once while slices keep `least` keys, more where slices must be held.
+static int top_cluster(int64_t rows, int64_t n, int sms, int64_t cap, int64_t least) {
     int c = 1;
-    while (c < 8 && ((rows * c < sms && n / (2 * c) >= 2048) || (n + c - 1) / c > cap)) c *= 2;
+    while (c < 8 && ((rows * 2 * c <= sms && n / (2 * c) >= least) || (n + c - 1) / c > cap)) c *= 2;
     return c;
 }
 
@@ -432,7 +463,7 @@ int launch_tokens_select(const float* w, int B, int Hkv, int slots, int64_t rs, 
                          int recent, int32_t* kept, float* kept_w, int sms, cudaStream_t st) {
     KeepParams p{w, rs, Hkv, slots, keep, sinks, recent, 0, lens, kept, kept_w};
     const int64_t rows = (int64_t)B * Hkv;
-    const int c = top_cluster(rows, slots, sms, kKeyCap);
+    const int c = top_cluster(rows, slots, sms, kKeyCap, 2048);
     const int64_t per = ((int64_t)slots + c - 1) / c;
     p.cached = per <= kKeyCap;
     return launch_cluster(tokens_select_kernel, p, rows, c, p.cached ? (size_t)per * 4 : 0, st);
@@ -455,7 +486,7 @@ int launch_pages_select(const pkv_codec* c, Pages pg, const void* q, int qdt, in
     p.out = out;
     const int64_t fixed = (int64_t)p.G * p.dim * 12 + 2 * (int64_t)p.G * p.pitch;
     const int64_t cap = (190 * 1024 - fixed) / 4, rows = (int64_t)pg.B * pg.Hkv;
-    const int cl = top_cluster(rows, pg.max_pages, sms, cap);
+    const int cl = top_cluster(rows, pg.max_pages, sms, cap, 64);
     const int64_t per = ((int64_t)pg.max_pages + cl - 1) / cl;
     if (per > cap) return PKV_ERR_UNSUPPORTED;
     return launch_cluster(pages_select_kernel, p, rows, cl, (size_t)(fixed + per * 4), st);
