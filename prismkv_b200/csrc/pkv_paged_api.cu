@@ -34,6 +34,7 @@ int check_paged_codec(const pkv_codec* c, bool tables) {
 
 int check_pages(const pkv_pages* g, int m, bool need_codes) {
     if (!g || g->batch < 0 || g->max_pages < 0 || g->num_pages < 0 || g->kv_heads < 1 || m < 1) return PKV_ERR_INVALID;
+    if (m > 64) return PKV_ERR_UNSUPPORTED;                                        // head_dim <= 192
     if (g->code_bytes != 1 && g->code_bytes != 2) return PKV_ERR_INVALID;
     const int ps = g->page_size;
     if (ps < 16 || ps > 1024 || (ps & (ps - 1))) return PKV_ERR_INVALID;
@@ -176,7 +177,7 @@ int pkv_tokens_select(const float* weights, int32_t batch, int32_t kv_heads, int
 
 int pkv_tokens_gather(const pkv_pages* src, int32_t m, const int32_t* kept, int32_t keep, const pkv_pages* dst, void* dst_k,
                       void* dst_v, void* stream) {
-    int rc = check_pages(src, m, true), sms = 0;
+    int rc = check_pages(src, m, true);
     if (rc) return rc;
     rc = check_pages(dst, m, false);
     if (rc) return rc;
@@ -186,10 +187,8 @@ int pkv_tokens_gather(const pkv_pages* src, int32_t m, const int32_t* kept, int3
     if (src->batch == 0 || keep == 0) return PKV_OK;
     if (!kept || !dst_k || !dst_v || (src->num_pages > 0 && !src->v)) return PKV_ERR_INVALID;
     if ((reinterpret_cast<uintptr_t>(dst_k) | reinterpret_cast<uintptr_t>(dst_v)) % 16) return PKV_ERR_ALIGNMENT;
-    rc = sm_count(&sms);
-    if (rc) return rc;
     return pkv::launch_tokens_gather(device_pages(src), device_pages(dst), static_cast<uint8_t*>(dst_k),
-                                     static_cast<uint8_t*>(dst_v), m * src->code_bytes, kept, keep, sms,
+                                     static_cast<uint8_t*>(dst_v), m * src->code_bytes, kept, keep,
                                      static_cast<cudaStream_t>(stream));
 }
 

@@ -11,15 +11,27 @@ namespace pkv {
 namespace cg = cooperative_groups;
 
 // ---- copies of code rows ------------------------------------------------------------------------
-// One row of m codes = `bytes` bytes: 16-byte pieces, the last one short when bytes % 16 != 0 (rows
-// start on 16-byte boundaries).  Piece i of a row, src and dst at the rows' starts:
-__device__ __forceinline__ void copy_piece(uint8_t* dst, const uint8_t* src, int bytes, int i) {
+// Piece i of a row of m codes = `bytes` bytes: 16 bytes, the last one short when bytes % 16 != 0 (rows start on
+// 16-byte boundaries; what lies behind a row in its last 16 bytes is neither read nor written).
+__device__ __forceinline__ uint4 load_piece(const uint8_t* row, int bytes, int i) {
+    const int at = i * 16;
+    if (at + 16 <= bytes) return __ldcs(reinterpret_cast<const uint4*>(row + at));
+    uint32_t w[4] = {0, 0, 0, 0};
+    #pragma unroll
+    for (int x = 0; x < 15; ++x)
+        if (at + x < bytes) w[x >> 2] |= (uint32_t)row[at + x] << (8 * (x & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store_piece(uint8_t* row, int bytes, int i, uint4 v) {
     const int at = i * 16;
     if (at + 16 <= bytes) {
-        *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(src + at);
-    } else {
-        for (int x = at; x < bytes; ++x) dst[x] = src[x];
+        *reinterpret_cast<uint4*>(row + at) = v;
+        return;
     }
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    #pragma unroll
+    for (int x = 0; x < 15; ++x)
+        if (at + x < bytes) row[at + x] = (uint8_t)(w[x >> 2] >> (8 * (x & 3)));
 }
 
 // Rows (b, hk, i) of contiguous codes (any alignment of two bytes) into slots start[b] + i.
@@ -42,25 +54,48 @@ __global__ void pages_store_kernel(Pages g, uint8_t* dst, const uint8_t* codes, 
     for (int x = threadIdx.x & 7; x < bytes; x += 8) d[x] = s[x];
 }
 
-// Slots kept[b, hk, i] of the source pages into slots i of the destination's, K and V.  One thread per
-// 16-byte piece of a row; nothing is read twice, so the copies' bytes bound it.
-__global__ void tokens_gather_kernel(Pages s, Pages d, uint8_t* dk, uint8_t* dv, int bytes, const int32_t* kept,
-                                     int keep) {
-    const int pieces = (bytes + 15) / 16;
-    const int64_t total = (int64_t)s.B * s.Hkv * keep * pieces;
-    for (int64_t x = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; x < total; x += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = x / pieces;
-        const int pc = (int)(x - row * pieces);
-        const int i = (int)(row % keep), bh = (int)(row / keep), hk = bh % s.Hkv, b = bh / s.Hkv;
-        const int t = __ldg(kept + row);
-        if (t < 0) continue;
-        const int sp = page_of(s, b, t >> s.ps_log2), dp = page_of(d, b, i >> d.ps_log2);
-        if (sp < 0 || dp < 0) continue;
-        const int64_t so = slot_offset(s, sp, hk, t & ((1 << s.ps_log2) - 1));
-        const int64_t to = slot_offset(d, dp, hk, i & ((1 << d.ps_log2) - 1));
-        copy_piece(dk + to, s.k + so, bytes, pc);
-        copy_piece(dv + to, s.v + so, bytes, pc);
+// Slots kept[b, hk, i] of the source pages into slots i of the destination's, K and V.  A CTA takes kGatherRows
+// x (256 / pieces) neighbouring rows of one (sequence, KV head), a thread the same 16-byte piece of kGatherRows
+// of them: the three dependent steps (slot, pages, codes) of its rows overlap.  The copies' bytes bound it.
+constexpr int kGatherRows = 4;
+__global__ void __launch_bounds__(256) tokens_gather_kernel(Pages s, Pages d, uint8_t* dk, uint8_t* dv, int bytes,
+                                                            const int32_t* kept, int keep, int chunks) {
+    constexpr int U = kGatherRows;
+    const int pieces = (bytes + 15) / 16, rows = 256 / pieces;
+    const int r = threadIdx.x / pieces, pc = threadIdx.x - r * pieces;
+    const int bh = blockIdx.x / chunks, i0 = (blockIdx.x - bh * chunks) * rows * U + r;
+    const int b = bh / s.Hkv, hk = bh - b * s.Hkv;
+    if (r >= rows) return;
+    int t[U];
+    int64_t so[U], to[U];
+    #pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * rows;
+        t[u] = i < keep ? __ldg(kept + (int64_t)bh * keep + i) : -1;
     }
+    #pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * rows;
+        so[u] = to[u] = -1;
+        if (t[u] < 0) continue;
+        const int sp = page_of(s, b, t[u] >> s.ps_log2), dp = page_of(d, b, i >> d.ps_log2);
+        if (sp < 0 || dp < 0) continue;
+        so[u] = slot_offset(s, sp, hk, t[u] & ((1 << s.ps_log2) - 1));
+        to[u] = slot_offset(d, dp, hk, i & ((1 << d.ps_log2) - 1));
+    }
+    uint4 k[U], v[U];
+    #pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (so[u] >= 0) {
+            k[u] = load_piece(s.k + so[u], bytes, pc);
+            v[u] = load_piece(s.v + so[u], bytes, pc);
+        }
+    #pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (so[u] >= 0) {
+            store_piece(dk + to[u], bytes, pc, k[u]);
+            store_piece(dv + to[u], bytes, pc, v[u]);
+        }
 }
 
 // ---- page summaries -------------------------------------------------------------------------------
@@ -133,8 +168,8 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const unsigned rank = cl.block_rank(), C = cl.num_blocks();
-    constexpr int BINS = 1 << DIGIT, PER = BINS / kTopThreads, PASSES = (BITS + DIGIT - 1) / DIGIT;
-    static_assert(PER % 4 == 0, "a thread's bins are read as 16-byte pieces");
+    constexpr int BINS = 1 << DIGIT, PER = BINS >= 4 * kTopThreads ? 4 : 1, PASSES = (BITS + DIGIT - 1) / DIGIT;
+    static_assert(PER == 4 ? BINS == 4 * kTopThreads : BINS <= kTopThreads, "bins per thread");
     uint32_t prefix = 0, need = (uint32_t)min(k, n);        // keys still to take among those with this prefix
     const bool all = n <= k;
     for (int i = tid; i < 2 * BINS; i += kTopThreads) (&s.hist[0][0])[i] = 0;
@@ -161,13 +196,16 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
             uint32_t v[PER], sum = 0;
             #pragma unroll
             for (int j = 0; j < PER; ++j) v[j] = 0;
-            #pragma unroll 2
-            for (unsigned r = 0; r < C; ++r) {
-                const uint4* h = reinterpret_cast<const uint4*>(cl.map_shared_rank(&s, r)->hist[pass & 1]);
-                #pragma unroll
-                for (int j = 0; j < PER; j += 4) {
-                    const uint4 x = h[(BINS - 4 - (tid * PER + j)) / 4];
-                    v[j] += x.w; v[j + 1] += x.z; v[j + 2] += x.y; v[j + 3] += x.x;
+            if (PER * tid < BINS) {
+                #pragma unroll 4
+                for (unsigned r = 0; r < C; ++r) {
+                    const uint32_t* h = cl.map_shared_rank(&s, r)->hist[pass & 1];
+                    if constexpr (PER == 4) {
+                        const uint4 x = reinterpret_cast<const uint4*>(h)[kTopThreads - 1 - tid];
+                        v[0] += x.w; v[1] += x.z; v[2] += x.y; v[3] += x.x;
+                    } else {
+                        v[0] += h[BINS - 1 - tid];
+                    }
                 }
             }
             #pragma unroll
@@ -180,7 +218,8 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
             }
             if (lane == 31) s.warp[0][warp] = inc;
             __syncthreads();
-            for (int w = 0; w < warp; ++w) inc += s.warp[0][w];
+            #pragma unroll
+            for (int w = 0; w < kTopWarps; ++w) inc += w < warp ? s.warp[0][w] : 0u;
             uint32_t cum = inc - sum;
             #pragma unroll
             for (int j = 0; j < PER; ++j) {
@@ -269,8 +308,9 @@ struct SelectParams {
 //    lanes, the int8 queries (positive parts against the greatest, negative ones against the least) lie in
 //    shared memory in the same order, and __dp4a sums 32-bit integers exactly.  The summaries' bytes bound it
 //    for long sequences; they are asked into L2 before the rotation starts.
-//  * A score is below 192 * 127 * 127 < 2^22 in magnitude: keys of 24 bits, two digits of 12.
-constexpr int kPageDigit = 12;
+//  * A score is below 192 * 127 * 127 < 2^22 in magnitude: keys of 24 bits, three digits of 8 (a digit costs about
+//    2 us of barriers and remote reads with 256 bins, 5 us with 4096).
+constexpr int kPageDigit = 8;
 constexpr uint32_t kForcedKey = 0xffffffu;
 
 __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams p) {
@@ -303,14 +343,25 @@ __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams 
         float r[6];
         #pragma unroll
         for (int x = 0; x < 6; ++x) r[x] = lane + 32 * x < dim ? __ldg(p.R + k * dim + lane + 32 * x) : 0.f;
-        for (int h = 0; h < p.G; ++h) {
-            double a = 0.0;
+        for (int h0 = 0; h0 < p.G; h0 += 4) {
+            double a[4] = {0.0, 0.0, 0.0, 0.0};
             #pragma unroll
             for (int x = 0; x < 6; ++x)
-                if (32 * x < dim && lane + 32 * x < dim) a = fma((double)raw[h * dim + lane + 32 * x], (double)r[x], a);
-            #pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) a += __shfl_xor_sync(0xffffffffu, a, off);
-            if (lane < C) cl.map_shared_rank(sq, lane)[h * dim + k] = a;
+                if (32 * x < dim && lane + 32 * x < dim) {
+                    #pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                        if (h0 + h < p.G) a[h] = fma((double)raw[(h0 + h) * dim + lane + 32 * x], (double)r[x], a[h]);
+                }
+            // four sums over the warp: half the lanes keep two heads, a quarter one, then a butterfly over eight
+            const bool up16 = lane & 16, up8 = lane & 8;
+            const double b0 = (up16 ? a[2] : a[0]) + __shfl_xor_sync(0xffffffffu, up16 ? a[0] : a[2], 16);
+            const double b1 = (up16 ? a[3] : a[1]) + __shfl_xor_sync(0xffffffffu, up16 ? a[1] : a[3], 16);
+            double v = (up8 ? b1 : b0) + __shfl_xor_sync(0xffffffffu, up8 ? b0 : b1, 8);
+            v += __shfl_xor_sync(0xffffffffu, v, 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            const int h = h0 + (lane >> 3);
+            if ((lane & 7) < C && h < p.G) cl.map_shared_rank(sq, lane & 7)[h * dim + k] = v;
         }
     }
     cl.sync();
@@ -338,34 +389,57 @@ __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams 
     // ---- scores: four lanes a page, pieces lane & 3, + 4, ... -------------------------------------------
     const int pieces = 2 * p.pitch / 16, sub = lane & 3;
     const int4* q4 = reinterpret_cast<const int4*>(qp);
-    for (int j0 = lo + warp * 8; j0 < hi; j0 += kTopWarps * 8) {
-        const int j = j0 + (lane >> 2);
-        const bool scored = j < hi && j >= p.sinks && j < n - p.recent;
-        const int page = scored ? page_of(p.pg, b, j) : -1;
-        int4 w[6];                                           // pitch <= 192: at most 24 pieces
-        #pragma unroll
-        for (int x = 0; x < 6; ++x) {
-            w[x] = make_int4(0, 0, 0, 0);
-            if (page >= 0 && sub + 4 * x < pieces)
-                w[x] = __ldcs(reinterpret_cast<const int4*>(p.sums + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch) + sub + 4 * x);
+    for (int j0 = lo + warp * 32; j0 < hi; j0 += kTopWarps * 32) {
+        // a lane finds one page; then eight groups of four lanes score two of the 32 pages at a time
+        int mine = -1;
+        {
+            const int j = j0 + lane;
+            if (j < hi && j >= p.sinks && j < n - p.recent) mine = page_of(p.pg, b, j);
         }
-        int best = INT_MIN;
-        for (int h = 0; h < p.G; ++h) {
-            int a = 0;
+        #pragma unroll 1
+        for (int u0 = 0; u0 < 4 && j0 + 8 * u0 < hi; u0 += 2) {
+            int4 w[2][6];                                    // pitch <= 192: at most 24 pieces
             #pragma unroll
-            for (int x = 0; x < 6; ++x)
-                if (sub + 4 * x < pieces) {
-                    const int4 qv = q4[h * pieces + sub + 4 * x];
-                    a = __dp4a(w[x].x, qv.x, a);
-                    a = __dp4a(w[x].y, qv.y, a);
-                    a = __dp4a(w[x].z, qv.z, a);
-                    a = __dp4a(w[x].w, qv.w, a);
+            for (int u = 0; u < 2; ++u) {
+                const int page = __shfl_sync(0xffffffffu, mine, 8 * (u0 + u) + (lane >> 2));
+                const int4* sum = reinterpret_cast<const int4*>(p.sums + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch) + sub;
+                #pragma unroll
+                for (int x = 0; x < 6; ++x) {
+                    w[u][x] = make_int4(0, 0, 0, 0);
+                    if (page >= 0 && sub + 4 * x < pieces) w[u][x] = __ldcs(sum + 4 * x);
                 }
-            a += __shfl_xor_sync(0xffffffffu, a, 1);
-            a += __shfl_xor_sync(0xffffffffu, a, 2);
-            best = max(best, a);
+            }
+            int best[2] = {INT_MIN, INT_MIN};
+            #pragma unroll 2
+            for (int h = 0; h < p.G; ++h) {
+                int a[2] = {0, 0};
+                #pragma unroll
+                for (int x = 0; x < 6; ++x)
+                    if (sub + 4 * x < pieces) {
+                        const int4 qv = q4[h * pieces + sub + 4 * x];
+                        #pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            a[u] = __dp4a(w[u][x].x, qv.x, a[u]);
+                            a[u] = __dp4a(w[u][x].y, qv.y, a[u]);
+                            a[u] = __dp4a(w[u][x].z, qv.z, a[u]);
+                            a[u] = __dp4a(w[u][x].w, qv.w, a[u]);
+                        }
+                    }
+                #pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    a[u] += __shfl_xor_sync(0xffffffffu, a[u], 1);
+                    a[u] += __shfl_xor_sync(0xffffffffu, a[u], 2);
+                    best[u] = max(best[u], a[u]);
+                }
+            }
+            #pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int j = j0 + 8 * (u0 + u) + (lane >> 2);
+                const int page = __shfl_sync(0xffffffffu, mine, 8 * (u0 + u) + (lane >> 2));
+                if (sub == 0 && j < hi)
+                    keys[j - lo] = j < p.sinks || j >= n - p.recent ? kForcedKey : page < 0 ? 0u : (uint32_t)(best[u] + (1 << 22));
+            }
         }
-        if (sub == 0 && j < hi) keys[j - lo] = !scored ? kForcedKey : page < 0 ? 0u : (uint32_t)(best + (1 << 22));
     }
     __syncthreads();
     int32_t* out = p.out + (int64_t)bh * p.top;
@@ -394,7 +468,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 __global__ void __launch_bounds__(kTopThreads) tokens_select_kernel(KeepParams p) {
-    extern __shared__ uint32_t ksm[];
+    extern __shared__ float ksm[];
     __shared__ TopShared<11> top;
     cg::cluster_group cl = cg::this_cluster();
     const int bh = blockIdx.x / cl.num_blocks(), tid = threadIdx.x;
@@ -402,32 +476,39 @@ __global__ void __launch_bounds__(kTopThreads) tokens_select_kernel(KeepParams p
     const float* w = p.w + (int64_t)bh * p.w_rs;
     int lo, hi;
     top_slice(n, lo, hi);
-    auto make = [&](int i, float x) { return i < p.sinks || i >= n - p.recent ? 0xffffffffu : weight_key(x); };
     int32_t* kept = p.kept + (int64_t)bh * p.keep;
     float* kw = p.kept_w + (int64_t)bh * p.keep;
     for (int i = min(n, p.keep) + cl.block_rank() * kTopThreads + tid; i < p.keep; i += cl.num_blocks() * kTopThreads) {
         kept[i] = -1;
         kw[i] = 0.f;
     }
-    auto put = [&](const int (&at)[4], int i) {
-        float x[4];
-        #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = at[u] >= 0 ? __ldg(w + i + 32 * u) : 0.f;
-        #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (at[u] >= 0) {
-                kept[at[u]] = i + 32 * u;
-                kw[at[u]] = x[u];
-            }
-    };
+    // the slice's weights in shared memory, asked for sixteen at a time (32 KB in flight per CTA)
     if (p.cached) {
-        #pragma unroll 8
-        for (int i = lo + tid; i < hi; i += kTopThreads) ksm[i - lo] = make(i, __ldg(w + i));
+        constexpr int U = 16;
+        for (int i0 = lo + tid; i0 < hi; i0 += U * kTopThreads) {
+            float x[U];
+            #pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = i0 + u * kTopThreads < hi ? __ldg(w + i0 + u * kTopThreads) : 0.f;
+            #pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i0 + u * kTopThreads < hi) ksm[i0 + u * kTopThreads - lo] = x[u];
+        }
         __syncthreads();
-        top_row<32, 11>(top, lo, hi, n, p.keep, [&](int i) { return ksm[i - lo]; }, put);
-    } else {
-        top_row<32, 11>(top, lo, hi, n, p.keep, [&](int i) { return make(i, __ldg(w + i)); }, put);
     }
+    auto select = [&](auto weight) {
+        top_row<32, 11>(top, lo, hi, n, p.keep,
+                        [&](int i) { return i < p.sinks || i >= n - p.recent ? 0xffffffffu : weight_key(weight(i)); },
+                        [&](const int (&at)[4], int i) {
+                            #pragma unroll
+                            for (int u = 0; u < 4; ++u)
+                                if (at[u] >= 0) {
+                                    kept[at[u]] = i + 32 * u;
+                                    kw[at[u]] = weight(i + 32 * u);
+                                }
+                        });
+    };
+    if (p.cached) select([&](int i) { return ksm[i - lo]; });
+    else select([&](int i) { return __ldg(w + i); });
 }
 
 // ---- launches -------------------------------------------------------------------------------------------
@@ -486,7 +567,7 @@ int launch_pages_select(const pkv_codec* c, Pages pg, const void* q, int qdt, in
     p.out = out;
     const int64_t fixed = (int64_t)p.G * p.dim * 12 + 2 * (int64_t)p.G * p.pitch;
     const int64_t cap = (190 * 1024 - fixed) / 4, rows = (int64_t)pg.B * pg.Hkv;
-    const int cl = top_cluster(rows, pg.max_pages, sms, cap, 64);
+    const int cl = top_cluster(rows, pg.max_pages, sms, cap, 256);
     const int64_t per = ((int64_t)pg.max_pages + cl - 1) / cl;
     if (per > cap) return PKV_ERR_UNSUPPORTED;
     return launch_cluster(pages_select_kernel, p, rows, cl, (size_t)(fixed + per * 4), st);
@@ -511,12 +592,12 @@ int launch_pages_store(Pages pg, uint8_t* dst, const uint8_t* codes, int bytes, 
     return cudaGetLastError() == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
 }
 
-int launch_tokens_gather(Pages s, Pages d, uint8_t* dk, uint8_t* dv, int bytes, const int32_t* kept, int keep, int sms,
+int launch_tokens_gather(Pages s, Pages d, uint8_t* dk, uint8_t* dv, int bytes, const int32_t* kept, int keep,
                          cudaStream_t st) {
-    const int64_t total = (int64_t)s.B * s.Hkv * keep * ((bytes + 15) / 16);
-    const int64_t ctas = (total + 255) / 256;
-    tokens_gather_kernel<<<(unsigned)(ctas < (int64_t)sms * 16 ? ctas : (int64_t)sms * 16), 256, 0, st>>>(s, d, dk, dv, bytes,
-                                                                                                     kept, keep);
+    const int rows = 256 / ((bytes + 15) / 16) * kGatherRows, chunks = (keep + rows - 1) / rows;
+    const int64_t ctas = (int64_t)s.B * s.Hkv * chunks;
+    if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
+    tokens_gather_kernel<<<(unsigned)ctas, 256, 0, st>>>(s, d, dk, dv, bytes, kept, keep, chunks);
     return cudaGetLastError() == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
 }
 
