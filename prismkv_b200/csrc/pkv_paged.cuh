@@ -44,9 +44,16 @@ __device__ __forceinline__ int64_t slot_offset(const Pages& g, int page, int hk,
 // ---- attention ---------------------------------------------------------------------------------
 // A unit is up to HQ query heads of one (sequence, KV head); units are numbered sequence-major.  Its
 // tokens are the sequence's (or the listed pages', in list order) in granules of 16.  The granules of
-// all units form one line of T granules; CTA c of `grid` takes granules [c T / Gd, (c + 1) T / Gd) with
-// Gd = min(grid, T), so ragged sequences load every CTA alike.  Each (CTA, unit) range leaves one
-// partial softmax state; range (c, u) uses partial row c + u, so a unit's rows lie side by side.
+// all units form one line of T granules, cut among Gd CTAs: the grid, or where that is less one per unit or
+// per 16 granules, below which a CTA's warps would have nothing to share.  Two ways to cut:
+//  * evenly: CTA c takes [c T / Gd, (c + 1) T / Gd), whatever the units.  Every CTA streams the same, but most
+//    units end inside a CTA, which then sets up a second range (about 5 us).
+//  * by units, while a CTA's share is below kUnitShare granules (of which 32 take 2.7 us): a unit [a, e) goes
+//    to the CTAs [s(a), s(e)), s(t) = round(t Gd / T), in equal parts, or whole to CTA s(a) when that is none.
+// Each (CTA, unit) range leaves one partial softmax state; range (c, u) uses partial row c + u, so a
+// unit's rows lie side by side.
+constexpr int kUnitShare = 256;
+
 struct PagedParams {
     Pages pg;
     int Hq, G, HQ, UG, UH, dim, m, cb;         // UG units per KV head, UH = Hkv * UG per sequence
@@ -95,22 +102,43 @@ __device__ inline void granule_line(const PagedParams& p, int b, int64_t& before
 
 struct PagedItem { int b, hk, hg, unit, g0, g1, row; };     // granules [g0, g1) of the unit, partial row
 
-struct PagedCursor { int64_t t, end, base; int b; };
+struct PagedCut { int64_t total; int gd; bool by_unit; };
+
+__device__ __forceinline__ PagedCut paged_cut(const PagedParams& p, int64_t total) {
+    PagedCut c;
+    c.total = total;
+    c.gd = (int)min((int64_t)p.grid, min(total, max((total + 15) / 16, (int64_t)p.units)));
+    c.by_unit = total < (int64_t)kUnitShare * c.gd;
+    return c;
+}
+
+// s(t) of the cut by units
+__device__ __forceinline__ int unit_cut(const PagedCut& c, int64_t t) {
+    return (int)((2 * t * c.gd + c.total) / (2 * c.total));
+}
+
+struct PagedCursor { PagedCut cut; int64_t t, end, base; int b; };
 
 // Whole warps; every warp of the CTA walks the same items.
 __device__ inline PagedCursor paged_begin(const PagedParams& p) {
     PagedCursor c;
     int64_t total, before;
     granule_line(p, 0, before, total);
-    const int64_t gd = min((int64_t)p.grid, total);
+    c.cut = paged_cut(p, total);
     c.b = 0;
     c.base = 0;
-    if ((int64_t)blockIdx.x >= gd) {
+    const int64_t x = blockIdx.x, gd = c.cut.gd;
+    if (x >= gd) {
         c.t = c.end = 0;
         return c;
     }
-    c.t = (int64_t)blockIdx.x * total / gd;
-    c.end = (int64_t)(blockIdx.x + 1) * total / gd;
+    if (c.cut.by_unit) {                                    // units that start or lie where s may be x
+        c.t = max((int64_t)0, ((2 * x - 1) * total) / (2 * gd) - 1);
+        c.end = total;
+    } else {
+        c.t = x * total / gd;
+        c.end = (x + 1) * total / gd;
+    }
     // the sequence of granule t: 32 sequences at a time
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < p.pg.B; b0 += 32) {
@@ -126,14 +154,16 @@ __device__ inline PagedCursor paged_begin(const PagedParams& p) {
             const int f = __ffs(past) - 1;
             c.b = b0 + f;
             c.base += __shfl_sync(0xffffffffu, inc - n, f);
-            return c;
+            break;
         }
         c.base += __shfl_sync(0xffffffffu, inc, 31);
     }
+    if (c.cut.by_unit) c.t -= (c.t - c.base) % granules_of(p, c.b);      // to the start of its unit
     return c;
 }
 
 __device__ inline bool paged_next(const PagedParams& p, PagedCursor& c, PagedItem& it) {
+    const int x = blockIdx.x;
     while (c.t < c.end) {
         const int n = granules_of(p, c.b);
         const int64_t off = c.t - c.base;
@@ -147,13 +177,44 @@ __device__ inline bool paged_next(const PagedParams& p, PagedCursor& c, PagedIte
         it.hk = u / p.UG;
         it.hg = u % p.UG;
         it.unit = c.b * p.UH + u;
-        it.g0 = (int)(off - (int64_t)u * n);
-        it.g1 = (int)min((int64_t)n, it.g0 + (c.end - c.t));
-        it.row = blockIdx.x + it.unit;
-        c.t += it.g1 - it.g0;
+        it.row = x + it.unit;
+        if (c.cut.by_unit) {
+            const int sa = min(unit_cut(c.cut, c.t), c.cut.gd - 1), k = max(1, unit_cut(c.cut, c.t + n) - sa);
+            if (sa > x) {
+                c.t = c.end;
+                return false;
+            }
+            c.t += n;
+            if (x >= sa + k) continue;
+            it.g0 = (int)((int64_t)(x - sa) * n / k);
+            it.g1 = (int)((int64_t)(x - sa + 1) * n / k);
+        } else {
+            it.g0 = (int)(off - (int64_t)u * n);
+            it.g1 = (int)min((int64_t)n, it.g0 + (c.end - c.t));
+            c.t += it.g1 - it.g0;
+        }
         return true;
     }
     return false;
+}
+
+// The partial rows [r0, r1) of a unit, none without granules.  Whole warps.
+__device__ inline void unit_rows(const PagedParams& p, int unit, int& r0, int& r1) {
+    const int b = unit / p.UH, n = granules_of(p, b);
+    int64_t before, total;
+    granule_line(p, b, before, total);
+    r0 = r1 = 0;
+    if (n == 0) return;
+    const PagedCut c = paged_cut(p, total);
+    const int64_t a = before + (int64_t)(unit % p.UH) * n;
+    if (c.by_unit) {
+        const int sa = min(unit_cut(c, a), c.gd - 1);
+        r0 = sa + unit;
+        r1 = r0 + max(1, unit_cut(c, a + n) - sa);
+    } else {
+        r0 = (int)(((a + 1) * c.gd - 1) / total) + unit;
+        r1 = (int)(((a + n) * c.gd - 1) / total) + unit + 1;
+    }
 }
 
 // Where granule gi of (b, hk) lies: its physical page (-1: masked), the slot of its first token in the

@@ -56,7 +56,7 @@ struct PA {
     static constexpr int CB = MODE == 1 ? 1 : 2;
     static constexpr int CPV = CPL / 2;                     // triplets per lane and token (values) = (x, y) m-tiles
     static constexpr int KW = CPL * CB / 4, VW = (CPV * CB + 3) / 4;
-    static constexpr int CHUNK = 1024;                      // pages of the list held at a time
+    static constexpr int CHUNK = 1024;                       // pages of the list held at a time
     static constexpr int XY_BYTES = MODE == 2 ? 4096 * 8 : 256 * 32 * 8;
     static constexpr int Z_BYTES = MODE == 0 ? 0 : (MODE == 1 ? 65536 : 256 * 32 * 4);
     static constexpr int THREADS = W * 32;
@@ -73,8 +73,8 @@ __host__ __device__ inline PASmem pa_smem(int dim, int warps, int chunk) {
     s.wm = s.acc + warps * kHQ * dim;                       // [warps][4] max
     s.wl = s.wm + warps * kHQ;                              // [warps][4] sum
     s.red = s.wl + warps * kHQ;                             // [32] reduction
-    s.list = s.red + 32;                                    // [chunk] pages
-    s.floats = s.list + chunk;
+    s.list = s.red + 32;                                    // [2][chunk] pages: this range's, the next one's
+    s.floats = s.list + 2 * chunk;
     return s;
 }
 
@@ -364,13 +364,84 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     const int rho = (g >> 1) + 4 * (g & 1);
     const int row_bytes = p.m * T::CB, per = p.pg.ps_log2 - 4;
     const int tokb = (int)p.pg.tok_bs;                        // (a row; checked to fit 31 bits / 16)
+    // Pages of granules [ga, gb) of an item as id, -1 (masked), or id | sign bit (the sequence's last page)
     PagedItem it;
     bool first = true;
-    while (paged_next(p, cur, it)) {
-        const int len = clamp_len(p.pg, __ldg(p.seq_lens + it.b));
+    int len = 0, lastp = 0, lbuf = 0;
+    auto list_end = [&](const PagedItem& i, int ga) { return min(i.g1, ((ga >> per) + T::CHUNK) << per); };
+    auto list_load = [&](const PagedItem& i, int ga, int* list) {
+        const int n = clamp_len(p.pg, __ldg(p.seq_lens + i.b)), last = (n - 1) >> p.pg.ps_log2;
+        const int j0 = ga >> per, j1 = (list_end(i, ga) - 1) >> per;
+        for (int j = j0 + tid; j <= j1; j += nthr) {
+            const Granule gr = granule_at(p, i.b, i.hk, j << per);
+            const int lp = p.selected ? gr.tok >> p.pg.ps_log2 : j;
+            list[j - j0] = gr.page < 0 ? -1 : lp == last ? gr.page | (int)0x80000000 : gr.page;
+        }
+    };
+    uint32_t kw[NG][2][T::KW], vw[NG][4][T::VW];
+    int nv[NG], gi = 0, ga = 0, gb = 0;
+    int64_t off[NG] = {};
+    const uint8_t *kbase = nullptr, *vbase = nullptr;
+    // tokens of granule x that count, and its byte offset
+    auto locate = [&](int x, int64_t& o) -> int {
+        o = 0;
+        if (x >= gb) return 0;
+        const int e = sList[lbuf * T::CHUNK + (x >> per) - (ga >> per)];
+        if (e == -1) return 0;
+        const int slot = (x & ((1 << per) - 1)) << 4;
+        o = (int64_t)(e & 0x7fffffff) * p.pg.page_bs + (int64_t)slot * tokb;
+        return e < 0 ? max(0, min(16, len - (lastp << p.pg.ps_log2) - slot)) : 16;
+    };
+    auto load_keys = [&](int i) {
+        load_k<T>(kw[i][0], kbase + off[i], c, row_bytes);
+        load_k<T>(kw[i][1], kbase + off[i] + 8 * tokb, c, row_bytes);
+    };
+    auto load_values = [&](int i) {
+        #pragma unroll
+        for (int t = 0; t < 4; ++t) load_v<T>(vw[i][t], vbase + off[i] + t * 4 * tokb, g, row_bytes);
+    };
+    // the first granules of the list: warp w takes granules w and w + W, then W NG further on
+    auto start_list = [&](int from) {
+        ga = from;
+        gb = list_end(it, ga);
+        gi = ga + warp;
+        #pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            nv[i] = locate(gi + i * W, off[i]);
+            if (nv[i] > 0) {
+                load_keys(i);
+                load_values(i);
+            }
+        }
+    };
+    auto start_item = [&] {
+        len = clamp_len(p.pg, __ldg(p.seq_lens + it.b));
+        lastp = (len - 1) >> p.pg.ps_log2;                   // the page that may be short
+        kbase = p.pg.k + (int64_t)it.hk * p.pg.head_bs + (int64_t)rho * tokb;
+        vbase = p.pg.v + (int64_t)it.hk * p.pg.head_bs + (int64_t)c * tokb;
+        start_list(it.g0);
+    };
+    #pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        #pragma unroll
+        for (int x = 0; x < T::KW; ++x) kw[i][0][x] = kw[i][1][x] = 0u;
+        #pragma unroll
+        for (int x = 0; x < T::VW; ++x) vw[i][0][x] = vw[i][1][x] = vw[i][2][x] = vw[i][3][x] = 0u;
+    }
+    bool more = paged_next(p, cur, it);
+    if (more) list_load(it, it.g0, sList);
+    __syncthreads();
+    if (more) start_item();
+    while (more) {
         uint32_t bq[CPL][2], bz[T::NBZ][2];
         float us0, us1, cz0, cz1;                              // heads 2 hp, 2 hp + 1 of this lane's score columns
-        auto load_query = [&] {
+        if (first) {                                           // while the first codes are on their way
+            fill_tables();
+            __syncthreads();
+            cudaGridDependencySynchronize();                   // the queries' fragments
+            first = false;
+        }
+        {
             const uint32_t* fr = p.frag + (int64_t)it.unit * T::FRAGS * 32 + lane;
             #pragma unroll
             for (int j = 0; j < CPL; ++j) {
@@ -387,73 +458,20 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
             us1 = pow2(-__float_as_int(__ldcg(hd + 1)) - tk);
             cz0 = __ldcg(hd + 4);
             cz1 = __ldcg(hd + 5);
-        };
+        }
+        const f32x2 uu = f2_pack(us0, us1), czz = f2_pack(cz0, cz1);
         const float zs = pow2((T::EX ? 0 : 24) + tk);         // MODE 0: z sums onto the (x, y) sums' scale
         float M0 = -INFINITY, M1 = -INFINITY;
         float l0 = 0.f, l1 = 0.f;
         float acc[CPV + CPV / 2][4];
         #pragma unroll
         for (int m = 0; m < CPV + CPV / 2; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
-
-        const uint8_t* kbase = p.pg.k + (int64_t)it.hk * p.pg.head_bs + (int64_t)rho * tokb;
-        const uint8_t* vbase = p.pg.v + (int64_t)it.hk * p.pg.head_bs + (int64_t)c * tokb;
-        const int lastp = (len - 1) >> p.pg.ps_log2;         // the page that may be short, its tokens
-        const int lastn = len - (lastp << p.pg.ps_log2);
-        for (int ga = it.g0; ga < it.g1;) {
-            // ---- pages of the next granules: id, -1 (masked), or id | sign bit (the short page) ----------
-            const int j0 = ga >> per, gb = min(it.g1, (j0 + T::CHUNK) << per);
-            const int j1 = (gb - 1) >> per;
-            __syncthreads();                                  // the last list, and the last item's sums, are read
-            for (int j = j0 + tid; j <= j1; j += nthr) {
-                const Granule gr = granule_at(p, it.b, it.hk, j << per);
-                const int lp = p.selected ? gr.tok >> p.pg.ps_log2 : j;
-                sList[j - j0] = gr.page < 0 ? -1 : lp == lastp ? gr.page | (int)0x80000000 : gr.page;
-            }
-            __syncthreads();
-            // tokens of granule gi that count, and its byte offset
-            auto locate = [&](int gi, int64_t& off) -> int {
-                off = 0;
-                if (gi >= gb) return 0;
-                const int e = sList[(gi >> per) - j0];
-                if (e == -1) return 0;
-                const int slot = (gi & ((1 << per) - 1)) << 4;
-                off = (int64_t)(e & 0x7fffffff) * p.pg.page_bs + (int64_t)slot * tokb;
-                return e < 0 ? max(0, min(16, lastn - slot)) : 16;
-            };
-            uint32_t kw[NG][2][T::KW], vw[NG][4][T::VW];
-            #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                #pragma unroll
-                for (int x = 0; x < T::KW; ++x) kw[i][0][x] = kw[i][1][x] = 0u;
-                #pragma unroll
-                for (int x = 0; x < T::VW; ++x) vw[i][0][x] = vw[i][1][x] = vw[i][2][x] = vw[i][3][x] = 0u;
-            }
-            int nv[NG];
-            int64_t off[NG];
-            int gi = ga + warp * NG;
-            #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                nv[i] = locate(gi + i, off[i]);
-                if (nv[i] > 0) {
-                    load_k<T>(kw[i][0], kbase + off[i], c, row_bytes);
-                    load_k<T>(kw[i][1], kbase + off[i] + 8 * tokb, c, row_bytes);
-                    #pragma unroll
-                    for (int t = 0; t < 4; ++t) load_v<T>(vw[i][t], vbase + off[i] + t * 4 * tokb, g, row_bytes);
-                }
-            }
-            if (first) {                                      // while the first codes are on their way
-                fill_tables();
-                __syncthreads();
-                cudaGridDependencySynchronize();              // the queries' fragments
-                first = false;
-            }
-            if (ga == it.g0) load_query();
-            const f32x2 uu = f2_pack(us0, us1), czz = f2_pack(cz0, cz1);
+        for (;;) {
             #pragma unroll 1
             for (; gi < gb; gi += W * NG) {
                 int nn[NG];
                 #pragma unroll
-                for (int i = 0; i < NG; ++i) nn[i] = locate(gi + W * NG + i, off[i]);
+                for (int i = 0; i < NG; ++i) nn[i] = locate(gi + W * (NG + i), off[i]);
                 // ---- scores ------------------------------------------------------------------------
                 float S[NG][4];
                 #pragma unroll
@@ -481,10 +499,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                         S[i][x] = MODE == 0 ? fmaf(zz[x], zs, xa[x] + xb[x]) : zz[x] + (xa[x] + xb[x]);
                         S[i][x] += __shfl_xor_sync(0xffffffffu, S[i][x], 2);             // hi + lo columns
                     }
-                    if (nn[i] > 0) {                          // the next iteration's keys
-                        load_k<T>(kw[i][0], kbase + off[i], c, row_bytes);
-                        load_k<T>(kw[i][1], kbase + off[i] + 8 * tokb, c, row_bytes);
-                    }
+                    if (nn[i] > 0) load_keys(i);              // the next iteration's
                 }
                 // ---- log2 scores, kept for the weights; running maximum -------------------------------
                 float mx0 = -INFINITY, mx1 = -INFINITY;
@@ -494,7 +509,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     const float2 b = f2_unpack(f2_fma(f2_pack(S[i][2], S[i][3]), uu, czz));
                     S[i][0] = a.x; S[i][1] = a.y; S[i][2] = b.x; S[i][3] = b.y;
                     if (p.raw && c < 2) {
-                        float* r = p.raw + (int64_t)it.unit * p.raw_us + ((int64_t)(gi + i) * kGranule + rho) * p.raw_h + 2 * hp;
+                        float* r = p.raw + (int64_t)it.unit * p.raw_us + ((int64_t)(gi + i * W) * kGranule + rho) * p.raw_h + 2 * hp;
                         #pragma unroll
                         for (int x = 0; x < 2; ++x)
                             if (2 * hp + x < p.raw_h) {
@@ -572,16 +587,20 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                                      look_z<T>(lk, vw[i][3], 2 * m), look_z<T>(lk, vw[i][3], 2 * m + 1), d2, d3);
                         }
                     }
-                    if (nn[i] > 0) {                           // the next iteration's values
-                        #pragma unroll
-                        for (int t = 0; t < 4; ++t) load_v<T>(vw[i][t], vbase + off[i] + t * 4 * tokb, g, row_bytes);
-                    }
+                    if (nn[i] > 0) load_values(i);
                     nv[i] = nn[i];
                 }
             }
-            ga = gb;
+            if (gb == it.g1) break;                           // a list holds CHUNK pages; the next ones
+            __syncthreads();
+            list_load(it, gb, sList + lbuf * T::CHUNK);
+            __syncthreads();
+            start_list(gb);
         }
-        // ---- hi + lo columns, the lanes, the warps -------------------------------------------------------
+        // ---- hi + lo columns, the lanes, the warps; the next range's list and first codes meanwhile ---------
+        PagedItem nx = it;
+        more = paged_next(p, cur, nx);
+        if (more) list_load(nx, nx.g0, sList + (lbuf ^ 1) * T::CHUNK);
         #pragma unroll
         for (int o = 4; o <= 16; o <<= 1) {
             l0 += __shfl_xor_sync(0xffffffffu, l0, o);
@@ -591,6 +610,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         for (int m = 0; m < CPV + CPV / 2; ++m)
             #pragma unroll
             for (int x = 0; x < 4; ++x) acc[m][x] += __shfl_xor_sync(0xffffffffu, acc[m][x], 2);
+        __syncthreads();                                      // the last range's sums are read
         if (c < 2) {
             float* o0 = sAcc + (warp * kHQ + 2 * c) * dim;     // head 2c; head 2c + 1 at + dim
             #pragma unroll
@@ -620,6 +640,9 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         }
         __syncthreads();
         float* row = p.part + (int64_t)it.row * kHQ * (dim + 2);
+        it = nx;
+        lbuf ^= 1;
+        if (more) start_item();
         const float its = pow2(-tk - 12);
         for (int i = tid; i < kHQ * dim; i += nthr) {
             const int h = i / dim, d = i - h * dim;
@@ -645,21 +668,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     }
 }
 
-// The ranges of a unit: partial rows [r0, r1), empty for a unit without granules.  Whole warps.
-__device__ inline void unit_rows(const PagedParams& p, int unit, int& r0, int& r1, int& n) {
-    const int b = unit / p.UH;
-    int64_t before, total;
-    granule_line(p, b, before, total);
-    n = granules_of(p, b);
-    r0 = r1 = 0;
-    if (n == 0) return;
-    const int64_t gd = min((int64_t)p.grid, total);
-    const int64_t a = before + (int64_t)(unit % p.UH) * n;
-    r0 = (int)(((a + 1) * gd - 1) / total) + unit;
-    r1 = (int)(((a + n) * gd - 1) / total) + unit + 1;
-}
-
 constexpr int kJoinThreads = 384;
+constexpr int kMaxGrid = 160;                  // CTAs of the attention launch, at most
 constexpr int kWeighTokens = 2048;             // tokens per CTA of the weight pass
 
 // CTAs [0, units): one unit each -- join its ranges, normalise, rotate back.  CTAs behind them (with
@@ -687,30 +697,36 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
             }
         };
         load_r(0);
-        int r0, r1, n;
+        int r0, r1;
         const int unit = blockIdx.x;
-        unit_rows(p, unit, r0, r1, n);
+        unit_rows(p, unit, r0, r1);
         cudaGridDependencySynchronize();
         const float* part = p.part + (int64_t)r0 * kHQ * rs;
         const int nr = r1 - r0;
         if (warp < kHQ) {                       // a range without tokens has l = 0; a NaN sum is carried on
-            float mx = -INFINITY;
-            for (int r = lane; r < nr; r += 32) {
+            float m[kMaxGrid / 32], l[kMaxGrid / 32], mx = -INFINITY, sum = 0.f;
+            #pragma unroll
+            for (int i = 0; i < kMaxGrid / 32; ++i) {
+                const int r = lane + 32 * i;
                 const float* q = part + ((int64_t)r * kHQ + warp) * rs;
-                if (__ldcg(q + 1) != 0.f) mx = fmaxf(mx, __ldcg(q));
+                m[i] = r < nr ? __ldcg(q) : 0.f;
+                l[i] = r < nr ? __ldcg(q + 1) : 0.f;
             }
+            #pragma unroll
+            for (int i = 0; i < kMaxGrid / 32; ++i)
+                if (l[i] != 0.f) mx = fmaxf(mx, m[i]);
             #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            float l = 0.f;
-            for (int r = lane; r < nr; r += 32) {
-                const float* q = part + ((int64_t)r * kHQ + warp) * rs;
-                const float lr = __ldcg(q + 1), f = lr == 0.f ? 0.f : exp2f(__ldcg(q) - mx);
-                sF[r * kHQ + warp] = f;
-                l = fmaf(lr, f, l);
+            #pragma unroll
+            for (int i = 0; i < kMaxGrid / 32; ++i) {
+                const int r = lane + 32 * i;
+                const float f = l[i] == 0.f ? 0.f : exp2f(m[i] - mx);
+                if (r < nr) sF[r * kHQ + warp] = f;
+                sum = fmaf(l[i], f, sum);
             }
             #pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-            if (lane == 0) sInv[warp] = l;
+            for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            if (lane == 0) sInv[warp] = sum;
         }
         __syncthreads();
         for (int i = tid; i < kHQ * dim; i += kJoinThreads) {
@@ -754,8 +770,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
     if (chunk * kWeighTokens >= nv) return;
     float* sOff = jsm;                         // [G] m + log2 l
     for (int h = warp; h < p.G; h += kJoinThreads / 32) {
-        int r0, r1, n;
-        unit_rows(p, b * p.UH + hk * p.UG + h / kHQ, r0, r1, n);
+        int r0, r1;
+        unit_rows(p, b * p.UH + hk * p.UG + h / kHQ, r0, r1);
         float mx = -INFINITY, l = 0.f;
         for (int r = r0 + lane; r < r1; r += 32) {
             const float* part = p.part + ((int64_t)r * kHQ + h % kHQ) * rs;
@@ -819,7 +835,7 @@ static PagedParams paged_params(const pkv_codec* c, const pkv_paged_attn_args* a
     p.bits_flat = c->bits_r + c->bits_theta;
     p.xy_per_z = c->xy_per_z;
     p.units = pg.B * p.UH;
-    p.grid = sms;
+    p.grid = sms < kMaxGrid ? sms : kMaxGrid;
     p.raw_h = p.G < kHQ ? p.G : kHQ;
     // room for every slot that the table (or the list) can name
     p.raw_us = ((int64_t)(a->selected ? a->n_selected : pg.max_pages) << pg.ps_log2) * p.raw_h;
