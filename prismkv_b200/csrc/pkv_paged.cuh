@@ -251,6 +251,13 @@ __device__ __forceinline__ Granule granule_at(const PagedParams& p, int b, int h
     return g;
 }
 
+// bulk_g2s (pkv_common.cuh) to a shared address
+__device__ __forceinline__ void bulk_g2s_at(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+        :: "r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
 template <int DT>
 __device__ __forceinline__ float load_as(const void* q, int64_t i) {
     return Elem<DT>::load(static_cast<const typename Elem<DT>::T*>(q) + i);

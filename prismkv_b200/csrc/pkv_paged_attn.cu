@@ -36,18 +36,22 @@ constexpr int kHQ = 4;                         // query heads per unit
 //    outside.  Centred, because an uncentred sum of p i grows with every token and the tiles' sums truncate.
 // Tables in shared memory: MODE 0 and 1 (one-byte codes, any codec) hold 256 rows of 32 copies, copy `lane`
 // for each lane: the 32 lookups of a warp never collide, and at a 64 KB-aligned address one byte permute of
-// the code word makes a lookup's address.  MODE 2 (two-byte codes of any codec) holds one copy of all 2^bits
+// the code word makes a lookup's address (z: and a shift).  MODE 2 (two-byte codes of any codec) holds one copy of all 2^bits
 // (x, y) -- 32 copies of 4096 do not fit -- and pays bank conflicts; z has 32 copies per bin in each mode.
 //
 // A warp takes NG granules (16 tokens each) at a time, lane = 4 g + c:
-//  * scores: rows = tokens, k = triplets.  Lane (g, c) holds tokens rho(g), rho(g) + 8, rho(g) = (g >> 1) +
-//    4 (g & 1), and CPL triplets of each: 8c .. 8c + 7 of the first 32, then its share of the rest.
+//  * scores: rows = tokens, k = triplets.  Lane (g, c) holds tokens rho(g), rho(g) + 8, rho(2 x) = x, rho(2 x + 1) =
+//    (x ^ 1) + 4 (neighbouring rows of 64 bytes lie in different banks), and CPL triplets of each: 8c .. 8c + 7 of
+//    the first 32, then its share of the rest.
 //  * weights: two 8x8 transposes (movmatrix) turn the score tile into the B operand of p . v.
-//  * values: rows = triplets, k = tokens.  Lane (g, c) holds tokens c, c + 4, c + 8, c + 12 and CPL / 2
+//  * values: rows = triplets, k = tokens.  Lane (g, c) holds tokens c, (c ^ 1) + 4 and both + 8, and CPL / 2
 //    triplets of each: 4g .. 4g + 3 of the first 32, then its share of the rest.
-// Codes go from global memory to registers, one iteration ahead: a warp's load covers whole 32-byte sectors of
-// eight or sixteen rows, no barrier and no shared-memory traffic; a page is found through the item's page list
-// in shared memory.
+// Codes come through shared memory, two iterations ahead: a warp's lane 0 copies its granules (16 rows of K, 16
+// of V) by bulk copies into the warp's own two-stage ring and every warp waits on its own barriers alone, so no
+// warp waits for another inside a range.  (Loaded into registers one iteration ahead instead, the codes cost
+// spills and a quarter of the issue slots in waits: attend over 4 x 131072 tokens 184 us.)  A page is found
+// through the range's page list in shared memory.  Every bit pattern decodes to something finite, so what lies
+// behind a row or a sequence needs no clearing: its scores are masked and its weights zero.
 // ---------------------------------------------------------------------------------------------
 template <int MODE_, int CPL_, int NG_, int W_, bool EX_>
 struct PA {
@@ -56,25 +60,32 @@ struct PA {
     static constexpr int CB = MODE == 1 ? 1 : 2;
     static constexpr int CPV = CPL / 2;                     // triplets per lane and token (values) = (x, y) m-tiles
     static constexpr int KW = CPL * CB / 4, VW = (CPV * CB + 3) / 4;
-    static constexpr int CHUNK = 1024;                       // pages of the list held at a time
+    static constexpr int RP = CPL * 4 * CB;                 // bytes of a code row in the ring, at most
+    static constexpr int SLOT = 2 * 16 * RP;                // a granule: 16 rows of K, then of V
+    static constexpr int SLOTS = 2 * NG;                    // per warp: two stages
+    static constexpr int UPPER = MODE != 1 && CPL == 8 ? 3 : SLOTS;   // slots above the tables, the others below
+    static constexpr int CHUNK = 512;                        // pages of the list held at a time
     static constexpr int XY_BYTES = MODE == 2 ? 4096 * 8 : 256 * 32 * 8;
-    static constexpr int Z_BYTES = MODE == 0 ? 0 : (MODE == 1 ? 65536 : 256 * 32 * 4);
+    static constexpr int Z_BYTES = MODE == 0 ? 0 : 256 * 32 * 4;
     static constexpr int THREADS = W * 32;
     static constexpr int NBZ = MODE == 0 ? CPL / 4 : CPL / 2;   // z steps of the scores
     static constexpr int FRAGS = 2 * (CPL + NBZ);           // query operand registers per lane
 };
 
-struct PASmem {                                             // offsets below the tables, in floats
-    int acc, wm, wl, red, list, floats;
+struct PASmem {                                             // offsets below the tables, in bytes
+    int acc, wm, wl, red, bar, list, ring, end;
 };
-__host__ __device__ inline PASmem pa_smem(int dim, int warps, int chunk) {
+template <class T>
+__host__ __device__ inline PASmem pa_smem(int dim) {
     PASmem s;
     s.acc = 0;                                              // [warps][4][dim]
-    s.wm = s.acc + warps * kHQ * dim;                       // [warps][4] max
-    s.wl = s.wm + warps * kHQ;                              // [warps][4] sum
-    s.red = s.wl + warps * kHQ;                             // [32] reduction
-    s.list = s.red + 32;                                    // [2][chunk] pages: this range's, the next one's
-    s.floats = s.list + 2 * chunk;
+    s.wm = s.acc + T::W * kHQ * dim * 4;                    // [warps][4] max
+    s.wl = s.wm + T::W * kHQ * 4;                           // [warps][4] sum
+    s.red = s.wl + T::W * kHQ * 4;                          // [32] reduction
+    s.bar = (s.red + 32 * 4 + 7) / 8 * 8;                   // [warps][2 stages]
+    s.list = s.bar + T::W * 2 * 8;                          // [2][CHUNK] pages: this range's, the next one's
+    s.ring = (s.list + 2 * T::CHUNK * 4 + 127) / 128 * 128; // slots UPPER .. SLOTS - 1
+    s.end = s.ring + (T::SLOTS - T::UPPER) * T::W * T::SLOT;
     return s;
 }
 
@@ -87,38 +98,32 @@ template <class T> __device__ __forceinline__ int v_triplet(int g, int i) {
     return 32 + (T::CPV - 4) * g + (i - 4);
 }
 
-__device__ __forceinline__ uint4 ldg_cs4(const void* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
-__device__ __forceinline__ uint2 ldg_cs2(const void* p) { return __ldcs(reinterpret_cast<const uint2*>(p)); }
-__device__ __forceinline__ uint32_t ldg_cs1(const void* p) { return __ldcs(reinterpret_cast<const uint32_t*>(p)); }
-
-// `bytes` (4, 8 or 16) of codes at row + off into w[]; nothing past the row's last code is touched
-// beyond the 16-byte piece that holds it.
-template <int BYTES> __device__ __forceinline__ void load_codes(uint32_t* w, const uint8_t* row, int off, int row_bytes) {
-    if (off >= row_bytes) return;
+// `BYTES` (2 to 16) of codes at a shared address into w[]
+template <int BYTES> __device__ __forceinline__ void lds_codes(uint32_t* w, uint32_t at) {
     if constexpr (BYTES == 16) {
-        const uint4 v = ldg_cs4(row + off);
+        const uint4 v = lds_u32x4(at);
         w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
     } else if constexpr (BYTES == 8) {
-        const uint2 v = ldg_cs2(row + off);
+        const uint2 v = lds_u32x2m(at);
         w[0] = v.x; w[1] = v.y;
     } else if constexpr (BYTES == 4) {
-        w[0] = ldg_cs1(row + off);
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at));
     } else {
-        w[0] = __ldcs(reinterpret_cast<const uint16_t*>(row + off));
+        uint16_t v;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+        w[0] = v;
     }
 }
 
 template <class T>
-__device__ __forceinline__ void load_k(uint32_t (&w)[T::KW], const uint8_t* row, int c, int row_bytes) {
-    load_codes<8 * T::CB>(w, row, 8 * T::CB * c, row_bytes);
-    if constexpr (T::CPL > 8)
-        load_codes<(T::CPL - 8) * T::CB>(w + 8 * T::CB / 4, row, (32 + (T::CPL - 8) * c) * T::CB, row_bytes);
+__device__ __forceinline__ void load_k(uint32_t (&w)[T::KW], uint32_t row, int c) {
+    lds_codes<8 * T::CB>(w, row + 8 * T::CB * c);
+    if constexpr (T::CPL > 8) lds_codes<(T::CPL - 8) * T::CB>(w + 8 * T::CB / 4, row + (32 + (T::CPL - 8) * c) * T::CB);
 }
 template <class T>
-__device__ __forceinline__ void load_v(uint32_t (&w)[T::VW], const uint8_t* row, int g, int row_bytes) {
-    load_codes<4 * T::CB>(w, row, 4 * T::CB * g, row_bytes);
-    if constexpr (T::CPV > 4)
-        load_codes<(T::CPV - 4) * T::CB>(w + T::CB, row, (32 + (T::CPV - 4) * g) * T::CB, row_bytes);
+__device__ __forceinline__ void load_v(uint32_t (&w)[T::VW], uint32_t row, int g) {
+    lds_codes<4 * T::CB>(w, row + 4 * T::CB * g);
+    if constexpr (T::CPV > 4) lds_codes<(T::CPV - 4) * T::CB>(w + T::CB, row + (32 + (T::CPV - 4) * g) * T::CB);
 }
 
 // Lookups.  xy_reg / z_reg: the tables' shared addresses with the lane's copy in the low byte.
@@ -134,7 +139,7 @@ template <class T> __device__ __forceinline__ uint2 look_xy(const Lookup& l, con
 template <class T> __device__ __forceinline__ uint32_t look_z(const Lookup& l, const uint32_t* w, int j) {
     uint32_t a, v;
     if constexpr (T::MODE == 1) {
-        a = __byte_perm(w[j >> 2], l.z, 0x7604u + ((j & 3) << 4));
+        a = __byte_perm(w[j >> 2], l.z, 0x7604u + ((j & 3) << 4)) >> 1;   // rows of 128 bytes
     } else {
         const uint32_t code = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1];
         a = (((code >> l.zsh) & l.zmask) << 7) + l.z;
@@ -274,23 +279,31 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     constexpr int W = T::W, NG = T::NG, CPL = T::CPL, CPV = T::CPV, MODE = T::MODE, nthr = T::THREADS;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim;
     cudaTriggerProgrammaticLaunchCompletion();
-    const PASmem L = pa_smem(dim, W, T::CHUNK);
-    float* sm = reinterpret_cast<float*>(pa_raw);
-    float *sAcc = sm + L.acc, *sWm = sm + L.wm, *sWl = sm + L.wl, *sRed = sm + L.red;
-    int* sList = reinterpret_cast<int*>(sm + L.list);
+    const PASmem L = pa_smem<T>(dim);
+    float *sAcc = reinterpret_cast<float*>(pa_raw + L.acc), *sRed = reinterpret_cast<float*>(pa_raw + L.red);
+    float *sWm = reinterpret_cast<float*>(pa_raw + L.wm), *sWl = reinterpret_cast<float*>(pa_raw + L.wl);
+    int* sList = reinterpret_cast<int*>(pa_raw + L.list);
+    uint64_t* bar = reinterpret_cast<uint64_t*>(pa_raw + L.bar) + warp * 2;
     // the tables start at the first 64 KB boundary of shared addresses behind the rest
     const uint32_t base = smem_u32(pa_raw);
-    const uint32_t tab = (base + L.floats * 4 + 0xFFFFu) & ~0xFFFFu;
+    const uint32_t tab = (base + L.end + 0xFFFFu) & ~0xFFFFu;
+    const uint32_t upper = tab + T::XY_BYTES + T::Z_BYTES;    // the ring's upper slots
     {
         uint32_t have;
         asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(have));
-        if (tab + T::XY_BYTES + T::Z_BYTES > base + have) {   // the window lies elsewhere than planned for
+        if (upper + T::UPPER * W * T::SLOT + 128 > base + have) {   // the window lies elsewhere than planned for
             if (tid == 0) flag_error(kErrSmemLayout);
             cudaGridDependencySynchronize();
             return;
         }
     }
     uint8_t* tabp = pa_raw + (tab - base);
+    if (lane == 0) {
+        mbar_init(&bar[0], 1);
+        mbar_init(&bar[1], 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
 
     // ---- tables: entries to registers, the largest magnitude, then the scaled pairs -----------------
     const int bits_all = p.bits_z + p.bits_flat;
@@ -344,7 +357,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     const uint32_t z = h2_split(ez[x] * ts);
                     #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        reinterpret_cast<uint4*>(tabp + T::XY_BYTES)[e * 16 + ((i + tid) & 7)] = make_uint4(z, z, z, z);
+                        reinterpret_cast<uint4*>(tabp + T::XY_BYTES)[e * 8 + ((i + tid) & 7)] = make_uint4(z, z, z, z);
                 }
             }
         }
@@ -355,17 +368,18 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     };
     Lookup lk;
     lk.xy = MODE == 2 ? tab : tab | ((uint32_t)lane << 3);
-    lk.z = tab + T::XY_BYTES + ((uint32_t)lane << 2);
+    lk.z = MODE == 1 ? (tab + T::XY_BYTES) * 2 + ((uint32_t)lane << 3) : tab + T::XY_BYTES + ((uint32_t)lane << 2);
     lk.zsh = p.bits_flat;
     lk.zmask = (1u << p.bits_z) - 1u;
     lk.xymask = ((1u << bits_all) - 1u) << 3;
 
     const int g = lane >> 2, c = lane & 3, hp = c & 1;
-    const int rho = (g >> 1) + 4 * (g & 1);
-    const int row_bytes = p.m * T::CB, per = p.pg.ps_log2 - 4;
-    const int tokb = (int)p.pg.tok_bs;                        // (a row; checked to fit 31 bits / 16)
+    const int rho = ((g >> 1) ^ (g & 1)) + 4 * (g & 1);
+    const int per = p.pg.ps_log2 - 4;
+    const int pitch = (p.m * T::CB + 15) & ~15;               // bytes of a row in the ring
+    const bool whole = p.pg.tok_bs == pitch;                  // a granule's rows are one piece
     // Pages of granules [ga, gb) of an item as id, -1 (masked), or id | sign bit (the sequence's last page)
-    PagedItem it;
+    PagedItem it{};
     bool first = true;
     int len = 0, lastp = 0, lbuf = 0;
     auto list_end = [&](const PagedItem& i, int ga) { return min(i.g1, ((ga >> per) + T::CHUNK) << per); };
@@ -378,10 +392,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
             list[j - j0] = gr.page < 0 ? -1 : lp == last ? gr.page | (int)0x80000000 : gr.page;
         }
     };
-    uint32_t kw[NG][2][T::KW], vw[NG][4][T::VW];
-    int nv[NG], gi = 0, ga = 0, gb = 0;
-    int64_t off[NG] = {};
-    const uint8_t *kbase = nullptr, *vbase = nullptr;
+    int gi = 0, ga = 0, gb = 0;
     // tokens of granule x that count, and its byte offset
     auto locate = [&](int x, int64_t& o) -> int {
         o = 0;
@@ -389,45 +400,62 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         const int e = sList[lbuf * T::CHUNK + (x >> per) - (ga >> per)];
         if (e == -1) return 0;
         const int slot = (x & ((1 << per) - 1)) << 4;
-        o = (int64_t)(e & 0x7fffffff) * p.pg.page_bs + (int64_t)slot * tokb;
+        o = slot_offset(p.pg, e & 0x7fffffff, it.hk, slot);
         return e < 0 ? max(0, min(16, len - (lastp << p.pg.ps_log2) - slot)) : 16;
     };
-    auto load_keys = [&](int i) {
-        load_k<T>(kw[i][0], kbase + off[i], c, row_bytes);
-        load_k<T>(kw[i][1], kbase + off[i] + 8 * tokb, c, row_bytes);
+    // The warp's slots of the stage in turn, and those of both added up: the other stage's are sum - mine.
+    static_assert(T::SLOTS - T::UPPER <= 1, "only the last slot may lie below the tables");
+    uint32_t slot[NG], both[NG];
+    #pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        slot[i] = upper + (uint32_t)(i * W + warp) * T::SLOT;
+        both[i] = slot[i] + (NG + i < T::UPPER ? upper + (uint32_t)((NG + i) * W + warp) * T::SLOT
+                                               : base + (uint32_t)L.ring + (uint32_t)warp * T::SLOT);
+    }
+    int stage = 0;
+    uint32_t phase = 0;                                      // parities of the stages' next waits, one bit each
+    bool ok = true;                                          // no wait ran out
+    const int gpair = min(lane >> 1, NG - 1), kv = lane & 1; // lanes 2 i + {0: K, 1: V} ask for granule i
+    uint32_t my_slot = slot[0], my_both = both[0];
+    if (NG > 1 && gpair == 1) { my_slot = slot[NG - 1]; my_both = both[NG - 1]; }
+    my_slot += kv * 16 * T::RP;
+    my_both += 2 * kv * 16 * T::RP;
+    const uint8_t* const my_pool = kv ? p.pg.v : p.pg.k;
+    // Ask for granules x, x + W, ... into the stage in turn (other: into the other one), whose last reads are done;
+    // tokens that count in each, 8 bits apiece.
+    auto ask = [&](int x, bool other) -> int {
+        int64_t o = 0;
+        const int n = lane < 2 * NG && ok ? locate(x + gpair * W, o) : 0;
+        const unsigned have = __ballot_sync(0xffffffffu, n > 0);
+        if (have == 0) return 0;
+        uint64_t* b = &bar[other ? stage ^ 1 : stage];
+        if (lane == 0) mbar_arrive_expect_tx(b, (uint32_t)(__popc(have) * 16 * pitch));
+        __syncwarp();
+        if (n > 0) {
+            const uint32_t dst = other ? my_both - my_slot : my_slot;
+            if (whole) {
+                bulk_g2s_at(dst, my_pool + o, (uint32_t)(16 * pitch), b);
+            } else {                                         // strided rows: one copy each
+                for (int r = 0; r < 16; ++r) bulk_g2s_at(dst + r * pitch, my_pool + o + r * p.pg.tok_bs, (uint32_t)pitch, b);
+            }
+        }
+        const int n0 = __shfl_sync(0xffffffffu, n, 0);
+        return NG == 1 ? n0 : n0 | __shfl_sync(0xffffffffu, n, 2) << 8;
     };
-    auto load_values = [&](int i) {
-        #pragma unroll
-        for (int t = 0; t < 4; ++t) load_v<T>(vw[i][t], vbase + off[i] + t * 4 * tokb, g, row_bytes);
-    };
-    // the first granules of the list: warp w takes granules w and w + W, then W NG further on
+    // the first granules of the list: warp w takes granules w, w + W, ..., NG an iteration
+    int cnt = 0, cnt2 = 0;                                   // of this iteration and the next one
     auto start_list = [&](int from) {
         ga = from;
         gb = list_end(it, ga);
         gi = ga + warp;
-        #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            nv[i] = locate(gi + i * W, off[i]);
-            if (nv[i] > 0) {
-                load_keys(i);
-                load_values(i);
-            }
-        }
+        cnt = ask(gi, false);
+        cnt2 = ask(gi + W * NG, true);
     };
     auto start_item = [&] {
         len = clamp_len(p.pg, __ldg(p.seq_lens + it.b));
         lastp = (len - 1) >> p.pg.ps_log2;                   // the page that may be short
-        kbase = p.pg.k + (int64_t)it.hk * p.pg.head_bs + (int64_t)rho * tokb;
-        vbase = p.pg.v + (int64_t)it.hk * p.pg.head_bs + (int64_t)c * tokb;
         start_list(it.g0);
     };
-    #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        #pragma unroll
-        for (int x = 0; x < T::KW; ++x) kw[i][0][x] = kw[i][1][x] = 0u;
-        #pragma unroll
-        for (int x = 0; x < T::VW; ++x) vw[i][0][x] = vw[i][1][x] = vw[i][2][x] = vw[i][3][x] = 0u;
-    }
     bool more = paged_next(p, cur, it);
     if (more) list_load(it, it.g0, sList);
     __syncthreads();
@@ -468,38 +496,45 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         for (int m = 0; m < CPV + CPV / 2; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
         for (;;) {
             #pragma unroll 1
-            for (; gi < gb; gi += W * NG) {
-                int nn[NG];
+            while (gi < gb) {
+                if (cnt) {                                    // (uniform: something was asked for)
+                    ok = __all_sync(0xffffffffu, mbar_wait(&bar[stage], (phase >> stage) & 1u, kErrWaitFull)) && ok;
+                    phase ^= 1u << stage;
+                }
+                if (cnt && ok) {
+                int nv[NG];
                 #pragma unroll
-                for (int i = 0; i < NG; ++i) nn[i] = locate(gi + W * (NG + i), off[i]);
+                for (int i = 0; i < NG; ++i) nv[i] = (cnt >> (8 * i)) & 0xff;
                 // ---- scores ------------------------------------------------------------------------
                 float S[NG][4];
                 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
                     float xa[4] = {0.f, 0.f, 0.f, 0.f}, xb[4] = {0.f, 0.f, 0.f, 0.f}, zz[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t kw[2][T::KW];
+                    load_k<T>(kw[0], slot[i] + rho * pitch, c);
+                    load_k<T>(kw[1], slot[i] + (rho + 8) * pitch, c);
                     #pragma unroll
                     for (int j = 0; j < CPL; ++j) {
-                        const uint2 e0 = look_xy<T>(lk, kw[i][0], j), e1 = look_xy<T>(lk, kw[i][1], j);
+                        const uint2 e0 = look_xy<T>(lk, kw[0], j), e1 = look_xy<T>(lk, kw[1], j);
                         mma_add<T::EX>((j & 1) ? xb : xa, e0.x, e1.x, e0.y, e1.y, bq[j][0], bq[j][1]);
                     }
                     if constexpr (MODE == 0) {
                         #pragma unroll
                         for (int j = 0; j < CPL / 4; ++j)
-                            mma_add<T::EX>(zz, z_index<T::EX>(kw[i][0][2 * j]), z_index<T::EX>(kw[i][1][2 * j]),
-                                           z_index<T::EX>(kw[i][0][2 * j + 1]), z_index<T::EX>(kw[i][1][2 * j + 1]),
+                            mma_add<T::EX>(zz, z_index<T::EX>(kw[0][2 * j]), z_index<T::EX>(kw[1][2 * j]),
+                                           z_index<T::EX>(kw[0][2 * j + 1]), z_index<T::EX>(kw[1][2 * j + 1]),
                                            bz[j][0], bz[j][1]);
                     } else {
                         #pragma unroll
                         for (int j = 0; j < CPL / 2; ++j)
-                            mma_add<T::EX>(zz, look_z<T>(lk, kw[i][0], 2 * j), look_z<T>(lk, kw[i][1], 2 * j),
-                                     look_z<T>(lk, kw[i][0], 2 * j + 1), look_z<T>(lk, kw[i][1], 2 * j + 1), bz[j][0], bz[j][1]);
+                            mma_add<T::EX>(zz, look_z<T>(lk, kw[0], 2 * j), look_z<T>(lk, kw[1], 2 * j),
+                                     look_z<T>(lk, kw[0], 2 * j + 1), look_z<T>(lk, kw[1], 2 * j + 1), bz[j][0], bz[j][1]);
                     }
                     #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         S[i][x] = MODE == 0 ? fmaf(zz[x], zs, xa[x] + xb[x]) : zz[x] + (xa[x] + xb[x]);
                         S[i][x] += __shfl_xor_sync(0xffffffffu, S[i][x], 2);             // hi + lo columns
                     }
-                    if (nn[i] > 0) load_keys(i);              // the next iteration's
                 }
                 // ---- log2 scores, kept for the weights; running maximum -------------------------------
                 float mx0 = -INFINITY, mx1 = -INFINITY;
@@ -555,18 +590,21 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&hA));
                     const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hB));
                     const uint32_t lA = f2h2(p0 - fa.x, p1 - fa.y), lB = f2h2(p2 - fb.x, p3 - fb.y);
-                    pA[i] = movmatrix_t(c >= 2 ? lA : hA);     // column g of tokens (c, c + 4)
-                    pB[i] = movmatrix_t(c >= 2 ? lB : hB);     // column g of tokens (c + 8, c + 12)
+                    pA[i] = movmatrix_t(c >= 2 ? lA : hA);     // column g of tokens (c, (c ^ 1) + 4)
+                    pB[i] = movmatrix_t(c >= 2 ? lB : hB);     // column g of the same + 8
                 }
                 // ---- values ----------------------------------------------------------------------------
                 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
+                    uint32_t vw[4][T::VW];
+                    #pragma unroll
+                    for (int t = 0; t < 4; ++t) load_v<T>(vw[t], slot[i] + 16 * T::RP + ((t & 1 ? c ^ 1 : c) + 4 * t) * pitch, g);
                     const uint32_t d0 = __byte_perm(pA[i], 0u, 0x1010u), d1 = __byte_perm(pA[i], 0u, 0x3232u);
                     const uint32_t d2 = __byte_perm(pB[i], 0u, 0x1010u), d3 = __byte_perm(pB[i], 0u, 0x3232u);
                     #pragma unroll
                     for (int m = 0; m < CPV; ++m) {
-                        const uint2 x0 = look_xy<T>(lk, vw[i][0], m), x1 = look_xy<T>(lk, vw[i][1], m);
-                        const uint2 x2 = look_xy<T>(lk, vw[i][2], m), x3 = look_xy<T>(lk, vw[i][3], m);
+                        const uint2 x0 = look_xy<T>(lk, vw[0], m), x1 = look_xy<T>(lk, vw[1], m);
+                        const uint2 x2 = look_xy<T>(lk, vw[2], m), x3 = look_xy<T>(lk, vw[3], m);
                         mma_add<T::EX>(acc[m], x0.x, x0.y, x1.x, x1.y, d0, d1);
                         mma_add<T::EX>(acc[m], x2.x, x2.y, x3.x, x3.y, d2, d3);
                     }
@@ -575,22 +613,31 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                         float (&za)[4] = acc[CPV + m];
                         if constexpr (MODE == 0) {
                             float zt[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma16816(zt, zc8(prmt(vw[i][0][m], vw[i][1][m], 0x5511u)), zc8(prmt(vw[i][0][m], vw[i][1][m], 0x7733u)),
-                                     zc8(prmt(vw[i][2][m], vw[i][3][m], 0x5511u)), zc8(prmt(vw[i][2][m], vw[i][3][m], 0x7733u)),
+                            mma16816(zt, zc8(prmt(vw[0][m], vw[1][m], 0x5511u)), zc8(prmt(vw[0][m], vw[1][m], 0x7733u)),
+                                     zc8(prmt(vw[2][m], vw[3][m], 0x5511u)), zc8(prmt(vw[2][m], vw[3][m], 0x7733u)),
                                      pA[i], pB[i]);
                             #pragma unroll
                             for (int x = 0; x < 4; ++x) za[x] += zt[x];
                         } else {
-                            mma_add<T::EX>(za, look_z<T>(lk, vw[i][0], 2 * m), look_z<T>(lk, vw[i][0], 2 * m + 1),
-                                     look_z<T>(lk, vw[i][1], 2 * m), look_z<T>(lk, vw[i][1], 2 * m + 1), d0, d1);
-                            mma_add<T::EX>(za, look_z<T>(lk, vw[i][2], 2 * m), look_z<T>(lk, vw[i][2], 2 * m + 1),
-                                     look_z<T>(lk, vw[i][3], 2 * m), look_z<T>(lk, vw[i][3], 2 * m + 1), d2, d3);
+                            mma_add<T::EX>(za, look_z<T>(lk, vw[0], 2 * m), look_z<T>(lk, vw[0], 2 * m + 1),
+                                     look_z<T>(lk, vw[1], 2 * m), look_z<T>(lk, vw[1], 2 * m + 1), d0, d1);
+                            mma_add<T::EX>(za, look_z<T>(lk, vw[2], 2 * m), look_z<T>(lk, vw[2], 2 * m + 1),
+                                     look_z<T>(lk, vw[3], 2 * m), look_z<T>(lk, vw[3], 2 * m + 1), d2, d3);
                         }
                     }
-                    if (nn[i] > 0) load_values(i);
-                    nv[i] = nn[i];
                 }
+                }
+                __syncwarp();
+                cnt = cnt2;
+                cnt2 = ask(gi + 2 * W * NG, false);
+                gi += W * NG;
+                stage ^= 1;
+                my_slot = my_both - my_slot;
+                #pragma unroll
+                for (int i = 0; i < NG; ++i) slot[i] = both[i] - slot[i];
             }
+            if (!ok)                                          // give what was asked for some 20 ms to arrive
+                for (int x = 0; x < 4; ++x) mbar_wait(&bar[x & 1], ((phase >> (x & 1)) ^ (x >> 1)) & 1u, kErrWaitDrain, 1u << 9);
             if (gb == it.g1) break;                           // a list holds CHUNK pages; the next ones
             __syncthreads();
             list_load(it, gb, sList + lbuf * T::CHUNK);
@@ -873,8 +920,8 @@ template <class T>
 static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
     static_assert(T::FRAGS <= 48, "paged_frag_bytes");
     // tables from the first 64 KB boundary behind the rest (the window starts at most 1 KB into the shared space)
-    const uint32_t below = 1024u + (uint32_t)pa_smem(p.dim, T::W, T::CHUNK).floats * 4u;
-    const int smem = (int)(((below + 0xFFFFu) & ~0xFFFFu) - 1024u) + T::XY_BYTES + T::Z_BYTES;
+    const uint32_t below = 1024u + (uint32_t)pa_smem<T>(p.dim).end;
+    const int smem = (int)(((below + 0xFFFFu) & ~0xFFFFu) - 1024u) + T::XY_BYTES + T::Z_BYTES + T::UPPER * T::W * T::SLOT + 128;
     if (cudaFuncSetAttribute(paged_attn_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return PKV_ERR_CUDA;
     paged_query_kernel<<<p.units, kQueryThreads, 2 * kHQ * p.dim * 4, st>>>(p, T::MODE, T::CPL, T::EX);
