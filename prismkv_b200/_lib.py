@@ -203,6 +203,15 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# torch's own accessor of the current stream's handle; the public one builds a Stream object on every call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(index: int) -> int:
+    """Handle of the current stream of CUDA device ``index``."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def device_error(clear: bool = True) -> int:
     flag = c_int32(0)
     check(load().pkv_device_error(ctypes.byref(flag), int(clear)), "pkv_device_error")

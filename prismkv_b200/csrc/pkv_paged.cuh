@@ -2,6 +2,9 @@
 // device, how a sequence's tokens are found, and how attention work is cut into ranges.
 #pragma once
 
+#include <atomic>
+#include <mutex>
+
 #include "pkv_common.cuh"
 #include "pkv_mma.cuh"
 
@@ -39,6 +42,22 @@ __device__ __forceinline__ int page_of(const Pages& g, int b, int j) {
 
 __device__ __forceinline__ int64_t slot_offset(const Pages& g, int page, int hk, int r) {
     return (int64_t)page * g.page_bs + (int64_t)hk * g.head_bs + (int64_t)r * g.tok_bs;
+}
+
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device: asked of the runtime once per device
+// and growth (`seen`: the most asked for on each device, one array per kernel).
+template <class K>
+static int allow_smem(K kernel, int bytes, std::atomic<int> (&seen)[64]) {
+    static std::mutex growing;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return PKV_ERR_CUDA;
+    if (dev < 0 || dev >= 64) return PKV_ERR_UNSUPPORTED;
+    if (seen[dev].load(std::memory_order_acquire) >= bytes) return PKV_OK;
+    std::lock_guard<std::mutex> hold(growing);              // (a smaller request must not undo a larger one)
+    if (seen[dev].load(std::memory_order_acquire) >= bytes) return PKV_OK;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return PKV_ERR_CUDA;
+    seen[dev].store(bytes, std::memory_order_release);
+    return PKV_OK;
 }
 
 // ---- attention ---------------------------------------------------------------------------------

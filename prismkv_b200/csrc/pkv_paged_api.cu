@@ -1,5 +1,6 @@
 // pkv_paged_api.cu -- extern "C" entry points of the paged cache: argument checks, then the launches.
 
+#include <atomic>
 #include <cmath>
 
 #include "pkv_paged.cuh"
@@ -86,10 +87,17 @@ int check_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a) {
     return PKV_OK;
 }
 
+// SMs of the current device, asked for once per device.
 int sm_count(int* n) {
+    static std::atomic<int> known[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return PKV_ERR_CUDA;
-    return cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+    const bool kept = dev >= 0 && dev < 64;
+    *n = kept ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (*n) return PKV_OK;
+    if (cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return PKV_ERR_CUDA;
+    if (kept) known[dev].store(*n, std::memory_order_relaxed);
+    return PKV_OK;
 }
 
 }  // namespace

@@ -922,8 +922,9 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
     // tables from the first 64 KB boundary behind the rest (the window starts at most 1 KB into the shared space)
     const uint32_t below = 1024u + (uint32_t)pa_smem<T>(p.dim).end;
     const int smem = (int)(((below + 0xFFFFu) & ~0xFFFFu) - 1024u) + T::XY_BYTES + T::Z_BYTES + T::UPPER * T::W * T::SLOT + 128;
-    if (cudaFuncSetAttribute(paged_attn_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return PKV_ERR_CUDA;
+    static std::atomic<int> seen[64];
+    const int rc = allow_smem(paged_attn_kernel<T>, smem, seen);
+    if (rc) return rc;
     paged_query_kernel<<<p.units, kQueryThreads, 2 * kHQ * p.dim * 4, st>>>(p, T::MODE, T::CPL, T::EX);
     if (cudaGetLastError() != cudaSuccess) return PKV_ERR_CUDA;
     return launch_behind(paged_attn_kernel<T>, p.grid, T::THREADS, smem, st, p);

@@ -522,8 +522,9 @@ static int top_cluster(int64_t rows, int64_t n, int sms, int64_t cap, int64_t le
 template <class K, class P>
 static int launch_cluster(K kernel, const P& p, int64_t rows, int c, size_t smem, cudaStream_t st) {
     if (rows * c > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-        return PKV_ERR_CUDA;
+    static std::atomic<int> seen[64];                        // (one array per instantiation: per parameter type)
+    const int rc = allow_smem(kernel, (int)smem, seen);
+    if (rc) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * c));
     cfg.blockDim = dim3(kTopThreads);

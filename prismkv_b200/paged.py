@@ -64,55 +64,59 @@ class PagedOps:
         return torch.empty((num_pages, kv_heads, 2, self.summary_pitch), dtype=torch.int8, device=self.device)
 
     # ------------------------------------------------------------------
-    def _on_device(self, t: torch.Tensor, name: str) -> None:
-        _lib.require_cuda(t, name)
-        if t.device != self._dev:
-            raise ValueError(f"{name} is on {t.device}, the codec on {self.device}")
+    # The checks run on every call of a decode step, so they read each property of a tensor once.
+    def _index(self) -> int:
+        """The codec's CUDA device index."""
+        i = self.device.index
+        return torch.cuda.current_device() if i is None else i
 
-    @property
-    def _dev(self) -> torch.device:
-        d = self.device
-        return d if d.index is not None else torch.device(d.type, torch.cuda.current_device())
+    def _on_device(self, t: torch.Tensor, name: str) -> None:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor")
+        if t.get_device() != self._index():
+            raise ValueError(f"{name} is on {t.device}, the codec on {self.device}")
 
     def _check_ints(self, t: torch.Tensor, name: str, shape) -> torch.Tensor:
         self._on_device(t, name)
-        if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}, "
                              f"got {t.dtype} {tuple(t.shape)}")
         return t
+
+    def _check_table(self, page_table: torch.Tensor):
+        """(data pointer, row stride, batch, max_pages) of a page table."""
+        self._on_device(page_table, "page_table")
+        if page_table.dtype != torch.int32 or page_table.dim() != 2:
+            raise ValueError("page_table must be an int32 (batch, max_pages) tensor with unit inner stride")
+        B, n = page_table.shape
+        stride, inner = page_table.stride()
+        if n > 1 and inner != 1:
+            raise ValueError("page_table must be an int32 (batch, max_pages) tensor with unit inner stride")
+        return page_table.data_ptr(), stride if B > 1 else n, B, n
 
     def _pages(self, k: torch.Tensor, v: Optional[torch.Tensor], page_table: torch.Tensor,
                name: str = "k_pages") -> _lib.PkvPages:
         self._on_device(k, name)
         if k.dim() != 4 or k.shape[3] != self.m or k.shape[1] < 1:
             raise ValueError(f"{name} must be (num_pages, kv_heads, page_size, {self.m}), got {tuple(k.shape)}")
-        if k.dtype not in PAGE_CODE_DTYPES:
+        P, H, ps, _ = shape = k.shape
+        code_bytes = PAGE_CODE_DTYPES.get(k.dtype)
+        if code_bytes is None:
             raise ValueError("codes must be stored as uint8 or 16-bit integers")
+        strides = k.stride()
         if v is not None:
             self._on_device(v, "v_pages")
-            if v.shape != k.shape or v.dtype != k.dtype or v.stride() != k.stride():
+            if v.shape != shape or v.dtype != k.dtype or v.stride() != strides:
                 raise ValueError("k_pages and v_pages must have the same shape, dtype and strides")
-        if k.stride(3) != 1:
+        if strides[3] != 1:
             raise ValueError("codes need unit stride within a row")
-        self._on_device(page_table, "page_table")
-        if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1
-                                                                        and page_table.stride(1) != 1):
-            raise ValueError("page_table must be an int32 (batch, max_pages) tensor with unit inner stride")
-        ps = k.shape[2]
         if ps < 16 or ps > 1024 or ps & (ps - 1):
             raise ValueError(f"page_size must be a power of two from 16 to 1024, got {ps}")
-        g = _lib.PkvPages()
-        g.k, g.v = k.data_ptr(), v.data_ptr() if v is not None else None
-        g.code_bytes = PAGE_CODE_DTYPES[k.dtype]
-        g.num_pages, g.kv_heads, g.page_size = k.shape[0], k.shape[1], ps
-        # a dimension of one element has no stride of its own
-        g.page_stride = k.stride(0) if k.shape[0] > 1 else 0
-        g.head_stride = k.stride(1) if k.shape[1] > 1 else 0
-        g.token_stride = k.stride(2)
-        g.table = page_table.data_ptr()
-        g.batch, g.max_pages = page_table.shape
-        g.table_stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
-        return g
+        table, table_stride, B, max_pages = self._check_table(page_table)
+        # (a dimension of one element has no stride of its own)
+        return _lib.PkvPages(k.data_ptr(), v.data_ptr() if v is not None else None, code_bytes, P, H, ps,
+                             strides[0] if P > 1 else 0, strides[1] if H > 1 else 0, strides[2], table, table_stride, B,
+                             max_pages)
 
     def _query(self, q: torch.Tensor, kv_heads: int, batch: int) -> torch.Tensor:
         self._on_device(q, "q")
@@ -127,6 +131,17 @@ class PagedOps:
         if q.dtype not in _lib.DTYPE_CODES:
             q = q.float()
         return q if q.stride(2) == 1 else q.contiguous()
+
+    def _call(self, fn, what: str, *args) -> None:
+        """fn(*args, stream) with the codec's device current; a non-zero status raises."""
+        i = self._index()
+        if torch.cuda.current_device() == i:
+            rc = fn(*args, _lib.raw_stream(i))
+        else:
+            with torch.cuda.device(i):
+                rc = fn(*args, _lib.raw_stream(i))
+        if rc:
+            _lib.check(rc, what)
 
     # ------------------------------------------------------------------
     def paged_attention(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -156,40 +171,50 @@ class PagedOps:
             self._on_device(out, "out")
             if out.shape != (B, Hq, self.dim) or out.dtype not in _lib.DTYPE_CODES or out.stride(2) != 1:
                 raise ValueError(f"out must be a ({B}, {Hq}, {self.dim}) float tensor with unit inner stride")
-        a = _lib.PkvPagedAttnArgs()
-        a.pages = g
-        a.q_heads, a.q_dtype, a.q = Hq, _lib.DTYPE_CODES[q.dtype], q.data_ptr()
-        a.q_batch_stride, a.q_head_stride = q.stride(0), q.stride(1)
-        a.seq_lens = seq_lens.data_ptr()
+        selected = n_selected = 0
         if pages is not None:
             if pages.dim() != 3:
                 raise ValueError(f"pages must be ({B}, {g.kv_heads}, n), got {tuple(pages.shape)}")
-            self._check_ints(pages, "pages", (B, g.kv_heads, pages.shape[2]))
-            if pages.shape[2] == 0:
+            n_selected = pages.shape[2]
+            self._check_ints(pages, "pages", (B, g.kv_heads, n_selected))
+            if n_selected == 0:
                 raise ValueError("pages lists no page; leave it out to attend to every token")
-            a.selected, a.n_selected = pages.data_ptr(), pages.shape[2]
-        a.scale = float(self.dim ** -0.5 if scale is None else scale)
-        a.out, a.out_dtype = out.data_ptr(), _lib.DTYPE_CODES[out.dtype]
-        a.out_batch_stride, a.out_head_stride = out.stride(0), out.stride(1)
+            selected = pages.data_ptr()
+        w_in = w_out = slots = 0
         if weights_out is not None and weights is None:
             raise ValueError("weights_out needs weights")
         if weights is not None:
-            w_out = weights if weights_out is None else weights_out
-            for t, n in ((weights, "weights"), (w_out, "weights_out")):
+            to = weights if weights_out is None else weights_out
+            for t, n in ((weights, "weights"), (to, "weights_out")):
                 self._on_device(t, n)
                 if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (B, g.kv_heads) or not t.is_contiguous():
                     raise ValueError(f"{n} must be a contiguous float32 ({B}, {g.kv_heads}, slots) tensor")
-            if w_out.shape != weights.shape:
+            if to.shape != weights.shape:
                 raise ValueError("weights and weights_out must have the same shape")
-            a.weights, a.weights_out = weights.data_ptr(), w_out.data_ptr()
-            a.weights_slots = a.weights_row_stride = weights.shape[2]
+            w_in, w_out, slots = weights.data_ptr(), to.data_ptr(), weights.shape[2]
+        qs, os = q.stride(), out.stride()
+        a = _lib.PkvPagedAttnArgs(g, Hq, _lib.DTYPE_CODES[q.dtype], q.data_ptr(), qs[0], qs[1], seq_lens.data_ptr(),
+                                  selected or None, n_selected, self.dim ** -0.5 if scale is None else float(scale),
+                                  out.data_ptr(), _lib.DTYPE_CODES[out.dtype], os[0], os[1], w_in or None, w_out or None,
+                                  slots, slots)
+        args = ctypes.byref(a)
         lib = _lib.load()
-        with torch.cuda.device(self.device):
-            need = lib.pkv_paged_attn_workspace_size(ctypes.byref(self.struct), ctypes.byref(a))
-            ws = torch.empty(max(int(need), 256), dtype=torch.uint8, device=q.device)
-            rc = lib.pkv_paged_attn(ctypes.byref(self.struct), ctypes.byref(a), ws.data_ptr(), ws.numel(), self._stream())
-        _lib.check(rc, "pkv_paged_attn")
+        # the workspace's size follows from the shapes alone
+        key = (B, Hq, g.kv_heads, g.page_size, g.max_pages, n_selected, w_in != 0)
+        sizes = self.__dict__.setdefault("_paged_sizes", {})
+        need = sizes.get(key)
+        if need is None:
+            with torch.cuda.device(self._index()):
+                need = max(int(lib.pkv_paged_attn_workspace_size(self._struct_ref(), args)), 256)
+            if len(sizes) > 256:
+                sizes.clear()
+            sizes[key] = need
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        self._call(lib.pkv_paged_attn, "pkv_paged_attn", self._struct_ref(), args, ws.data_ptr(), need)
         return out
+
+    def _struct_ref(self):
+        return ctypes.byref(self.struct)
 
     # ------------------------------------------------------------------
     def store_pages(self, codes: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor,
@@ -204,11 +229,8 @@ class PagedOps:
         self._check_ints(start, "start", (g.batch,))
         if counts is not None:
             self._check_ints(counts, "counts", (g.batch,))
-        with torch.cuda.device(self.device):
-            rc = _lib.load().pkv_pages_store(ctypes.byref(g), self.m, pages.data_ptr(), codes.data_ptr(), codes.shape[2],
-                                             start.data_ptr(), counts.data_ptr() if counts is not None else None,
-                                             self._stream())
-        _lib.check(rc, "pkv_pages_store")
+        self._call(_lib.load().pkv_pages_store, "pkv_pages_store", ctypes.byref(g), self.m, pages.data_ptr(),
+                   codes.data_ptr(), codes.shape[2], start.data_ptr(), counts.data_ptr() if counts is not None else None)
 
     def _grid(self):
         """Device tables of the summaries' grid, built on first use."""
@@ -242,12 +264,9 @@ class PagedOps:
         if start is not None:
             self._check_ints(start, "start", (g.batch,))
         gz, gxy = self._grid()
-        with torch.cuda.device(self.device):
-            rc = _lib.load().pkv_pages_summarize(
-                ctypes.byref(self.struct), ctypes.byref(g), seq_lens.data_ptr(),
-                start.data_ptr() if start is not None else None, gz.data_ptr(), gxy.data_ptr(), summaries.data_ptr(),
-                self._stream())
-        _lib.check(rc, "pkv_pages_summarize")
+        self._call(_lib.load().pkv_pages_summarize, "pkv_pages_summarize", self._struct_ref(), ctypes.byref(g),
+                   seq_lens.data_ptr(), start.data_ptr() if start is not None else None, gz.data_ptr(), gxy.data_ptr(),
+                   summaries.data_ptr())
         return summaries
 
     def select_pages(self, q: torch.Tensor, summaries: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -267,28 +286,19 @@ class PagedOps:
             raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
         if top < 1 or sinks < 0 or recent < 0 or sinks + recent > top:
             raise ValueError(f"need 0 <= sinks + recent <= top and top >= 1, got {sinks}, {recent}, {top}")
-        self._on_device(page_table, "page_table")
-        if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1
-                                                                        and page_table.stride(1) != 1):
-            raise ValueError("page_table must be an int32 (batch, max_pages) tensor with unit inner stride")
-        g = _lib.PkvPages()
-        g.code_bytes, g.num_pages, g.kv_heads, g.page_size = 1, summaries.shape[0], summaries.shape[1], page_size
-        g.token_stride = -(-self.m // ROW_BYTES) * ROW_BYTES
-        g.table = page_table.data_ptr()
-        g.batch, g.max_pages = page_table.shape
-        g.table_stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
+        table, table_stride, B, max_pages = self._check_table(page_table)
+        g = _lib.PkvPages(None, None, 1, summaries.shape[0], summaries.shape[1], page_size, 0, 0,
+                          -(-self.m // ROW_BYTES) * ROW_BYTES, table, table_stride, B, max_pages)
         self._check_summaries(summaries, g)
         q = self._query(q, g.kv_heads, g.batch)
         self._check_ints(seq_lens, "seq_lens", (g.batch,))
         if out is None:
             out = torch.empty((g.batch, g.kv_heads, top), dtype=torch.int32, device=q.device)
         self._check_ints(out, "out", (g.batch, g.kv_heads, top))
-        with torch.cuda.device(self.device):
-            rc = _lib.load().pkv_pages_select(
-                ctypes.byref(self.struct), ctypes.byref(g), q.data_ptr(), _lib.DTYPE_CODES[q.dtype], q.shape[1],
-                q.stride(0), q.stride(1), seq_lens.data_ptr(), summaries.data_ptr(), top, sinks, recent, out.data_ptr(),
-                self._stream())
-        _lib.check(rc, "pkv_pages_select")
+        qs = q.stride()
+        self._call(_lib.load().pkv_pages_select, "pkv_pages_select", self._struct_ref(), ctypes.byref(g), q.data_ptr(),
+                   _lib.DTYPE_CODES[q.dtype], q.shape[1], qs[0], qs[1], seq_lens.data_ptr(), summaries.data_ptr(), top,
+                   sinks, recent, out.data_ptr())
         return out
 
     # ------------------------------------------------------------------
@@ -309,10 +319,8 @@ class PagedOps:
         self._check_ints(seq_lens, "seq_lens", (B,))
         kept = torch.empty((B, H, keep), dtype=torch.int32, device=weights.device)
         kw = torch.empty((B, H, keep), dtype=torch.float32, device=weights.device)
-        with torch.cuda.device(self.device):
-            rc = _lib.load().pkv_tokens_select(weights.data_ptr(), B, H, T, T, seq_lens.data_ptr(), keep, sinks, recent,
-                                               kept.data_ptr(), kw.data_ptr(), self._stream())
-        _lib.check(rc, "pkv_tokens_select")
+        self._call(_lib.load().pkv_tokens_select, "pkv_tokens_select", weights.data_ptr(), B, H, T, T, seq_lens.data_ptr(),
+                   keep, sinks, recent, kept.data_ptr(), kw.data_ptr())
         return kept, kw
 
     def gather_tokens(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, kept: torch.Tensor,
@@ -332,7 +340,5 @@ class PagedOps:
         self._check_ints(kept, "kept", (src.batch, src.kv_heads, keep))
         if keep > dst.max_pages * dst.page_size:
             raise ValueError(f"{keep} tokens do not fit {dst.max_pages} pages of {dst.page_size}")
-        with torch.cuda.device(self.device):
-            rc = _lib.load().pkv_tokens_gather(ctypes.byref(src), self.m, kept.data_ptr(), keep, ctypes.byref(dst),
-                                               k_out.data_ptr(), v_out.data_ptr(), self._stream())
-        _lib.check(rc, "pkv_tokens_gather")
+        self._call(_lib.load().pkv_tokens_gather, "pkv_tokens_gather", ctypes.byref(src), self.m, kept.data_ptr(), keep,
+                   ctypes.byref(dst), k_out.data_ptr(), v_out.data_ptr())
