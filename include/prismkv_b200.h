@@ -374,8 +374,8 @@ PKV_API int pkv_pages_store(const pkv_pages *pages, int32_t m, void *dst, const 
  * of the page's tokens on a grid of 1/127 of the codec's largest magnitude:
  *     summaries + ((page * kv_heads + hk) * 2 + {0: least, 1: greatest}) * pitch + d
  * with pitch = dim rounded up to 16 (int8; the padding is set to 0).  grid_z
- * (2^bits_z) and grid_xy (2^bits_total, 2) are the decoded values in 1/128
- * grid steps (int16, device).                                               */
+ * (2^bits_z; rising with the bin) and grid_xy (2^bits_total, 2) are the decoded
+ * values in 1/128 grid steps (int16, device, 16-byte aligned).              */
 PKV_API int pkv_pages_summarize(const pkv_codec *c, const pkv_pages *pages, const int32_t *seq_lens,
                                 const int32_t *start, const int16_t *grid_z, const int16_t *grid_xy,
                                 int8_t *summaries, void *stream);

@@ -143,7 +143,7 @@ int pkv_pages_summarize(const pkv_codec* c, const pkv_pages* pages, const int32_
     if (pages->code_bytes == 1 && c->bits_z + c->bits_r + c->bits_theta > 8) return PKV_ERR_INVALID;
     if (pages->batch == 0 || pages->max_pages == 0) return PKV_OK;
     if (!seq_lens || !grid_z || !grid_xy || !summaries) return PKV_ERR_INVALID;
-    if (reinterpret_cast<uintptr_t>(summaries) % 16) return PKV_ERR_ALIGNMENT;
+    if ((reinterpret_cast<uintptr_t>(summaries) | reinterpret_cast<uintptr_t>(grid_xy)) % 16) return PKV_ERR_ALIGNMENT;
     rc = sm_count(&sms);
     if (rc) return rc;
     return pkv::launch_pages_summarize(c, device_pages(pages), pages->code_bytes, seq_lens, start, grid_z, grid_xy, summaries,

@@ -1,6 +1,7 @@
 // pkv_paged_ops.cu -- the kernels around attention over a paged code cache: storing rows, page
 // summaries, choosing pages, choosing tokens to keep, and moving them.
 
+#include <algorithm>
 #include <climits>
 
 #include <cooperative_groups.h>
@@ -100,46 +101,100 @@ __global__ void __launch_bounds__(256) tokens_gather_kernel(Pages s, Pages d, ui
 
 // ---- page summaries -------------------------------------------------------------------------------
 // Per page, KV head and channel the least and greatest grid value of the page's tokens; a step is 128
-// grid values, so the floor is a shift and the ceiling a shift of the value + 127.  One warp per (page,
-// KV head), lanes over triplets.
+// grid values, so the floor is a shift and the ceiling a shift of the value + 127.
+// One warp per (page, KV head).  LPT lanes hold a token's row, one 4-byte word (two or four codes) each, so a
+// load covers 32 / LPT tokens; a lane keeps, per code, the least and greatest (x, y) as packed 16-bit pairs and
+// of z the least and greatest bin (grid values rise with the bin).  (x, y) come from shared memory: up to 256
+// entries in 32 copies, one per lane, so that lookups never collide; more entries in one copy, with conflicts.
+// The codes' bytes bound it.
 struct SummaryParams {
     Pages pg;
     const int32_t *seq_lens, *start;
     const int16_t *grid_z, *grid_xy;
     int8_t* out;
-    int m, cb, pitch, bits_flat, code_mask;
+    int m, pitch, bits_z, bits_flat, index_mask, code_mask, entries, chunk, chunks;
 };
 
+template <int CB, int LPT, bool COPIES>
 __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
-    const int lane = threadIdx.x & 31;
-    const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    if (w >= (int64_t)p.pg.B * p.pg.max_pages * p.pg.Hkv) return;
-    const int hk = (int)(w % p.pg.Hkv), j = (int)(w / p.pg.Hkv % p.pg.max_pages), b = (int)(w / p.pg.Hkv / p.pg.max_pages);
-    const int L = clamp_len(p.pg, p.seq_lens[b]);
-    const int t0 = j << p.pg.ps_log2, n = min(L - t0, 1 << p.pg.ps_log2);
-    if (n <= 0 || (p.start && t0 + n <= p.start[b])) return;
-    const int page = page_of(p.pg, b, j);
-    if (page < 0) return;
-    int8_t* o = p.out + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch;
-    for (int i = lane; i < p.m; i += 32) {
-        int lo[3] = {1 << 20, 1 << 20, 1 << 20}, hi[3] = {-(1 << 20), -(1 << 20), -(1 << 20)};
-        for (int r = 0; r < n; ++r) {
-            const uint8_t* row = p.pg.k + slot_offset(p.pg, page, hk, r);
-            const int c = (p.cb == 1 ? row[i] : reinterpret_cast<const uint16_t*>(row)[i]) & p.code_mask;
-            const int v[3] = {p.grid_z[c >> p.bits_flat], p.grid_xy[2 * c], p.grid_xy[2 * c + 1]};
+    extern __shared__ __align__(16) uint32_t lut[];
+    constexpr int CW = 4 / CB, TPL = 32 / LPT, U = 8;       // codes per word, tokens per load, loads in flight
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int chunk = blockIdx.x % p.chunks, bh = blockIdx.x / p.chunks, b = bh / p.pg.Hkv, hk = bh - b * p.pg.Hkv;
+    const int L = clamp_len(p.pg, __ldg(p.seq_lens + b)), ps = 1 << p.pg.ps_log2;
+    const int first = p.start ? max(__ldg(p.start + b), 0) >> p.pg.ps_log2 : 0;
+    const int j0 = first + chunk * p.chunk, j1 = min(j0 + p.chunk, (int)(((int64_t)L + ps - 1) >> p.pg.ps_log2));
+    if (j0 >= j1 || (p.start && p.start[b] >= L)) return;
+    const uint32_t* xy = reinterpret_cast<const uint32_t*>(p.grid_xy);
+    if constexpr (COPIES) {                                  // 16-byte pieces of four copies, spread over the banks
+        for (int e = tid; e < p.entries; e += 256) {
+            const uint32_t v = __ldg(xy + e);
             #pragma unroll
-            for (int x = 0; x < 3; ++x) {
-                lo[x] = min(lo[x], v[x]);
-                hi[x] = max(hi[x], v[x]);
+            for (int k = 0; k < 8; ++k) reinterpret_cast<uint4*>(lut)[e * 8 + ((k + e) & 7)] = make_uint4(v, v, v, v);
+        }
+    } else {
+        for (int i = tid; i < p.entries; i += 256) lut[i] = __ldg(xy + i);
+    }
+    __syncthreads();
+    const int word = lane % LPT, tok = lane / LPT;
+    const bool have = word * 4 < p.m * CB;                   // this lane's word holds codes of the row
+    const uint32_t field = CB == 2 ? 0xffffu : 0xffu;
+    for (int j = j0 + warp; j < j1; j += 8) {
+        const int page = page_of(p.pg, b, j);
+        if (page < 0) continue;
+        const int n = min(L - (j << p.pg.ps_log2), ps);
+        const uint8_t* row = p.pg.k + slot_offset(p.pg, page, hk, 0) + word * 4;
+        uint32_t lo[CW], hi[CW], zl[CW], zh[CW];
+        #pragma unroll
+        for (int x = 0; x < CW; ++x) { lo[x] = 0x7fff7fffu; hi[x] = 0x80008000u; zl[x] = 0xffffu; zh[x] = 0u; }
+        for (int r0 = 0; r0 < n; r0 += U * TPL) {
+            uint32_t w[U];
+            #pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * TPL + tok;
+                w[u] = have && r < n ? __ldcs(reinterpret_cast<const uint32_t*>(row + (int64_t)r * p.pg.tok_bs)) : 0u;
+            }
+            #pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (r0 + u * TPL + tok >= n) break;
+                #pragma unroll
+                for (int x = 0; x < CW; ++x) {
+                    const uint32_t code = (w[u] >> (8 * CB * x)) & field, idx = code & p.index_mask;
+                    const uint32_t v = COPIES ? lut[idx * 32 + lane] : lut[idx];
+                    lo[x] = __vmins2(lo[x], v);
+                    hi[x] = __vmaxs2(hi[x], v);
+                    const uint32_t z = (code & p.code_mask) >> p.bits_flat;
+                    zl[x] = min(zl[x], z);
+                    zh[x] = max(zh[x], z);
+                }
             }
         }
         #pragma unroll
-        for (int x = 0; x < 3; ++x) {
-            o[3 * i + x] = (int8_t)(lo[x] >> 7);
-            o[p.pitch + 3 * i + x] = (int8_t)((hi[x] + 127) >> 7);
+        for (int off = LPT; off < 32; off <<= 1)
+            #pragma unroll
+            for (int x = 0; x < CW; ++x) {
+                lo[x] = __vmins2(lo[x], __shfl_xor_sync(0xffffffffu, lo[x], off));
+                hi[x] = __vmaxs2(hi[x], __shfl_xor_sync(0xffffffffu, hi[x], off));
+                zl[x] = min(zl[x], __shfl_xor_sync(0xffffffffu, zl[x], off));
+                zh[x] = max(zh[x], __shfl_xor_sync(0xffffffffu, zh[x], off));
+            }
+        int8_t* o = p.out + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch;
+        if (tok == 0 && have) {
+            #pragma unroll
+            for (int x = 0; x < CW; ++x) {
+                const int i = word * CW + x;
+                if (i >= p.m) break;
+                const int l[3] = {__ldg(p.grid_z + zl[x]), (int16_t)lo[x], (int16_t)(lo[x] >> 16)};
+                const int h[3] = {__ldg(p.grid_z + zh[x]), (int16_t)hi[x], (int16_t)(hi[x] >> 16)};
+                #pragma unroll
+                for (int y = 0; y < 3; ++y) {
+                    o[3 * i + y] = (int8_t)(l[y] >> 7);
+                    o[p.pitch + 3 * i + y] = (int8_t)((h[y] + 127) >> 7);
+                }
+            }
         }
+        for (int d = 3 * p.m + lane; d < p.pitch; d += 32) o[d] = o[p.pitch + d] = 0;
     }
-    for (int d = 3 * p.m + lane; d < p.pitch; d += 32) o[d] = o[p.pitch + d] = 0;
 }
 
 // ---- the k largest of a row, in index order ---------------------------------------------------------
@@ -574,15 +629,36 @@ int launch_pages_select(const pkv_codec* c, Pages pg, const void* q, int qdt, in
     return launch_cluster(pages_select_kernel, p, rows, cl, (size_t)(fixed + per * 4), st);
 }
 
+template <int CB, int LPT>
+static int launch_summaries(const SummaryParams& p, cudaStream_t st) {
+    const int64_t ctas = (int64_t)p.pg.B * p.pg.Hkv * p.chunks;
+    if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
+    if (p.entries <= 256) pages_summarize_kernel<CB, LPT, true><<<(unsigned)ctas, 256, p.entries * 128, st>>>(p);
+    else pages_summarize_kernel<CB, LPT, false><<<(unsigned)ctas, 256, p.entries * 4, st>>>(p);
+    return cudaGetLastError() == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+}
+
 int launch_pages_summarize(const pkv_codec* c, Pages pg, int cb, const int32_t* lens, const int32_t* start,
                            const int16_t* gz, const int16_t* gxy, int8_t* out, int sms, cudaStream_t st) {
-    SummaryParams p{pg, lens, start, gz, gxy, out, c->dim / 3, cb, (c->dim + 15) / 16 * 16,
-                    c->bits_r + c->bits_theta, (1 << (c->bits_z + c->bits_r + c->bits_theta)) - 1};
-    const int64_t warps = (int64_t)pg.B * pg.max_pages * pg.Hkv;
-    const int64_t ctas = (warps + 7) / 8;
-    if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-    pages_summarize_kernel<<<(unsigned)ctas, 256, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+    SummaryParams p{};
+    p.pg = pg;
+    p.seq_lens = lens; p.start = start;
+    p.grid_z = gz; p.grid_xy = gxy;
+    p.out = out;
+    p.m = c->dim / 3;
+    p.pitch = (c->dim + 15) / 16 * 16;
+    p.bits_z = c->bits_z;
+    p.bits_flat = c->bits_r + c->bits_theta;
+    p.code_mask = (1 << (p.bits_z + p.bits_flat)) - 1;
+    p.index_mask = c->xy_per_z ? p.code_mask : (1 << p.bits_flat) - 1;
+    p.entries = p.index_mask + 1;
+    // pages per CTA: about eight CTAs per SM when every page is asked for, so that the table's fill is shared
+    const int64_t all = (int64_t)pg.B * pg.Hkv * pg.max_pages;
+    p.chunk = (int)std::min<int64_t>(512, std::max<int64_t>(8, all / (8 * sms)));
+    p.chunks = (pg.max_pages + p.chunk - 1) / p.chunk;
+    const int words = (p.m * cb + 3) / 4;
+    if (cb == 1) return words <= 8 ? launch_summaries<1, 8>(p, st) : launch_summaries<1, 16>(p, st);
+    return words <= 16 ? launch_summaries<2, 16>(p, st) : launch_summaries<2, 32>(p, st);
 }
 
 int launch_pages_store(Pages pg, uint8_t* dst, const uint8_t* codes, int bytes, int n, const int32_t* start,

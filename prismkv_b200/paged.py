@@ -236,6 +236,8 @@ class PagedOps:
         """Device tables of the summaries' grid, built on first use."""
         if getattr(self, "_grid_z", None) is None:
             z, xy = _summary_grid(np.asarray(self.host.dec_z), np.asarray(self.host.dec_xy), 1 << self.bits_total)
+            if (np.diff(z.astype(np.int64)) < 0).any():
+                raise ValueError("page summaries need decoded z values that rise with the bin")
             self._grid_xy = torch.from_numpy(np.ascontiguousarray(xy)).to(self.device)
             self._grid_z = torch.from_numpy(z).to(self.device)
         return self._grid_z, self._grid_xy
