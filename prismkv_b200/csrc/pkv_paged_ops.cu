@@ -112,7 +112,7 @@ struct SummaryParams {
     const int32_t *seq_lens, *start;
     const int16_t *grid_z, *grid_xy;
     int8_t* out;
-    int m, pitch, bits_z, bits_flat, index_mask, code_mask, entries, chunk, chunks;
+    int m, pitch, bits_z, bits_flat, index_mask, entries, chunk, chunks;
 };
 
 template <int CB, int LPT, bool COPIES>
@@ -138,36 +138,50 @@ __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
     __syncthreads();
     const int word = lane % LPT, tok = lane / LPT;
     const bool have = word * 4 < p.m * CB;                   // this lane's word holds codes of the row
-    const uint32_t field = CB == 2 ? 0xffffu : 0xffu;
+    // byte address of a lookup: the index on the table's pitch (128 bytes of copies, or 4), plus the lane's copy
+    constexpr int SH = COPIES ? 7 : 2;
+    const uint32_t imask = (uint32_t)p.index_mask << SH, lane4 = COPIES ? lane * 4 : 0;
+    const uint32_t zm = (1u << p.bits_z) - 1u, zmask = CB == 2 ? zm * 0x00010001u : zm * 0x01010101u;
+    const char* const lutb = reinterpret_cast<const char*>(lut);
     for (int j = j0 + warp; j < j1; j += 8) {
         const int page = page_of(p.pg, b, j);
         if (page < 0) continue;
         const int n = min(L - (j << p.pg.ps_log2), ps);
-        const uint8_t* row = p.pg.k + slot_offset(p.pg, page, hk, 0) + word * 4;
-        uint32_t lo[CW], hi[CW], zl[CW], zh[CW];
+        const uint8_t* row = p.pg.k + slot_offset(p.pg, page, hk, tok) + word * 4;
+        const int64_t step = TPL * p.pg.tok_bs;
+        uint32_t lo[CW], hi[CW], zl[CW / 2], zh[CW / 2];     // z bins: two codes to a word
         #pragma unroll
-        for (int x = 0; x < CW; ++x) { lo[x] = 0x7fff7fffu; hi[x] = 0x80008000u; zl[x] = 0xffffu; zh[x] = 0u; }
-        for (int r0 = 0; r0 < n; r0 += U * TPL) {
-            uint32_t w[U];
+        for (int x = 0; x < CW; ++x) { lo[x] = 0x7fff7fffu; hi[x] = 0x80008000u; }
+        #pragma unroll
+        for (int x = 0; x < CW / 2; ++x) { zl[x] = 0xffffffffu; zh[x] = 0u; }
+        auto take = [&](uint32_t w) {
             #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int r = r0 + u * TPL + tok;
-                w[u] = have && r < n ? __ldcs(reinterpret_cast<const uint32_t*>(row + (int64_t)r * p.pg.tok_bs)) : 0u;
+            for (int x = 0; x < CW; ++x) {
+                const int at = 8 * CB * x - SH;              // the code's lowest bit comes to bit SH
+                const uint32_t a = (at < 0 ? w << -at : w >> at) & imask;
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(lutb + (a | lane4));
+                lo[x] = __vmins2(lo[x], v);
+                hi[x] = __vmaxs2(hi[x], v);
             }
+            const uint32_t z = (w >> p.bits_flat) & zmask;
             #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (r0 + u * TPL + tok >= n) break;
+            for (int x = 0; x < CW / 2; ++x) {               // CB 1: codes 0, 2 and codes 1, 3
+                const uint32_t y = CB == 2 ? z : (z >> (8 * x)) & 0x00ff00ffu;
+                zl[x] = __vminu2(zl[x], y);
+                zh[x] = __vmaxu2(zh[x], y);
+            }
+        };
+        if (have) {
+            int r0 = 0;
+            for (; r0 + U * TPL <= n; r0 += U * TPL) {       // U loads of whole groups of tokens in flight
+                uint32_t w[U];
                 #pragma unroll
-                for (int x = 0; x < CW; ++x) {
-                    const uint32_t code = (w[u] >> (8 * CB * x)) & field, idx = code & p.index_mask;
-                    const uint32_t v = COPIES ? lut[idx * 32 + lane] : lut[idx];
-                    lo[x] = __vmins2(lo[x], v);
-                    hi[x] = __vmaxs2(hi[x], v);
-                    const uint32_t z = (code & p.code_mask) >> p.bits_flat;
-                    zl[x] = min(zl[x], z);
-                    zh[x] = max(zh[x], z);
-                }
+                for (int u = 0; u < U; ++u) w[u] = __ldcs(reinterpret_cast<const uint32_t*>(row + u * step));
+                row += U * step;
+                #pragma unroll
+                for (int u = 0; u < U; ++u) take(w[u]);
             }
+            for (r0 += tok; r0 < n; r0 += TPL, row += step) take(__ldcs(reinterpret_cast<const uint32_t*>(row)));
         }
         #pragma unroll
         for (int off = LPT; off < 32; off <<= 1)
@@ -175,8 +189,10 @@ __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
             for (int x = 0; x < CW; ++x) {
                 lo[x] = __vmins2(lo[x], __shfl_xor_sync(0xffffffffu, lo[x], off));
                 hi[x] = __vmaxs2(hi[x], __shfl_xor_sync(0xffffffffu, hi[x], off));
-                zl[x] = min(zl[x], __shfl_xor_sync(0xffffffffu, zl[x], off));
-                zh[x] = max(zh[x], __shfl_xor_sync(0xffffffffu, zh[x], off));
+                if (x < CW / 2) {
+                    zl[x] = __vminu2(zl[x], __shfl_xor_sync(0xffffffffu, zl[x], off));
+                    zh[x] = __vmaxu2(zh[x], __shfl_xor_sync(0xffffffffu, zh[x], off));
+                }
             }
         int8_t* o = p.out + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch;
         if (tok == 0 && have) {
@@ -184,8 +200,10 @@ __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
             for (int x = 0; x < CW; ++x) {
                 const int i = word * CW + x;
                 if (i >= p.m) break;
-                const int l[3] = {__ldg(p.grid_z + zl[x]), (int16_t)lo[x], (int16_t)(lo[x] >> 16)};
-                const int h[3] = {__ldg(p.grid_z + zh[x]), (int16_t)hi[x], (int16_t)(hi[x] >> 16)};
+                // code x's bins: CB 2: half x; CB 1: half x / 2 of word x % 2
+                const int zw = CB == 2 ? 0 : x & 1, zs = CB == 2 ? 16 * x : 16 * (x >> 1);
+                const int l[3] = {__ldg(p.grid_z + ((zl[zw] >> zs) & 0xffffu)), (int16_t)lo[x], (int16_t)(lo[x] >> 16)};
+                const int h[3] = {__ldg(p.grid_z + ((zh[zw] >> zs) & 0xffffu)), (int16_t)hi[x], (int16_t)(hi[x] >> 16)};
                 #pragma unroll
                 for (int y = 0; y < 3; ++y) {
                     o[3 * i + y] = (int8_t)(l[y] >> 7);
@@ -205,29 +223,26 @@ __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
 // sums all CTAs' histograms for itself, and the histograms of two digits alternate.
 // What bounds it: a handful of barriers and round trips through the cluster's shared memory for short rows, the
 // passes over the keys in shared memory for long ones.
-constexpr int kTopThreads = 512;
-constexpr int kTopWarps = kTopThreads / 32;
-
-template <int DIGIT>
+template <int THREADS, int DIGIT>
 struct TopShared {
     alignas(16) uint32_t hist[2][1 << DIGIT];
-    uint32_t warp[2][kTopWarps];
+    uint32_t warp[2][THREADS / 32];
     uint32_t total[2];                         // this CTA's keys above and equal to the threshold
     uint32_t bin, need;
 };
 
-// BITS-bit keys in digits of DIGIT bits (the last one may be shorter).  put(at, i): keys i, i + 32, i + 64,
-// i + 96 go to places at[0 .. 3] (negative: not taken).
-template <int BITS, int DIGIT, class Key, class Put>
-__device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key key, Put put) {
+// BITS-bit keys in digits of DIGIT bits (the last one may be shorter).  put(at, x, i): keys i, i + 32, i + 64,
+// i + 96 (x[0 .. 3]) go to places at[0 .. 3] (negative: not taken).
+template <int BITS, int THREADS, int DIGIT, class Key, class Put>
+__device__ void top_row(TopShared<THREADS, DIGIT>& s, int lo, int hi, int n, int k, Key key, Put put) {
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const unsigned rank = cl.block_rank(), C = cl.num_blocks();
-    constexpr int BINS = 1 << DIGIT, PER = BINS >= 4 * kTopThreads ? 4 : 1, PASSES = (BITS + DIGIT - 1) / DIGIT;
-    static_assert(PER == 4 ? BINS == 4 * kTopThreads : BINS <= kTopThreads, "bins per thread");
+    constexpr int BINS = 1 << DIGIT, PER = BINS >= 4 * THREADS ? 4 : 1, PASSES = (BITS + DIGIT - 1) / DIGIT;
+    static_assert(PER == 4 ? BINS == 4 * THREADS : BINS <= THREADS, "bins per thread");
     uint32_t prefix = 0, need = (uint32_t)min(k, n);        // keys still to take among those with this prefix
     const bool all = n <= k;
-    for (int i = tid; i < 2 * BINS; i += kTopThreads) (&s.hist[0][0])[i] = 0;
+    for (int i = tid; i < 2 * BINS; i += THREADS) (&s.hist[0][0])[i] = 0;
     __syncthreads();
     if (!all) {
         int shift = BITS;
@@ -235,18 +250,18 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
         for (int pass = 0; pass < PASSES; ++pass) {
             const int bits = min(DIGIT, shift), low = shift - bits;
             uint32_t* hist = s.hist[pass & 1];
-            for (int i0 = lo + tid; i0 < hi; i0 += 4 * kTopThreads) {
+            for (int i0 = lo + tid; i0 < hi; i0 += 4 * THREADS) {
                 uint32_t x[4];
                 #pragma unroll
-                for (int u = 0; u < 4; ++u) x[u] = i0 + u * kTopThreads < hi ? key(i0 + u * kTopThreads) : 0u;
+                for (int u = 0; u < 4; ++u) x[u] = i0 + u * THREADS < hi ? key(i0 + u * THREADS) : 0u;
                 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    if (i0 + u * kTopThreads < hi && (shift == BITS || (x[u] >> shift) == (prefix >> shift)))
+                    if (i0 + u * THREADS < hi && (shift == BITS || (x[u] >> shift) == (prefix >> shift)))
                         atomicAdd(&hist[(x[u] >> low) & ((1u << bits) - 1u)], 1u);
             }
             cl.sync();
             if (pass + 2 < PASSES + 1 && pass > 0)          // the other one was read before this barrier
-                for (int i = tid; i < BINS; i += kTopThreads) s.hist[(pass + 1) & 1][i] = 0;
+                for (int i = tid; i < BINS; i += THREADS) s.hist[(pass + 1) & 1][i] = 0;
             // bins from the top, PER neighbouring ones a thread, summed over the cluster
             uint32_t v[PER], sum = 0;
             #pragma unroll
@@ -256,7 +271,7 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
                 for (unsigned r = 0; r < C; ++r) {
                     const uint32_t* h = cl.map_shared_rank(&s, r)->hist[pass & 1];
                     if constexpr (PER == 4) {
-                        const uint4 x = reinterpret_cast<const uint4*>(h)[kTopThreads - 1 - tid];
+                        const uint4 x = reinterpret_cast<const uint4*>(h)[THREADS - 1 - tid];
                         v[0] += x.w; v[1] += x.z; v[2] += x.y; v[3] += x.x;
                     } else {
                         v[0] += h[BINS - 1 - tid];
@@ -274,7 +289,7 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
             if (lane == 31) s.warp[0][warp] = inc;
             __syncthreads();
             #pragma unroll
-            for (int w = 0; w < kTopWarps; ++w) inc += w < warp ? s.warp[0][w] : 0u;
+            for (int w = 0; w < (THREADS / 32); ++w) inc += w < warp ? s.warp[0][w] : 0u;
             uint32_t cum = inc - sum;
             #pragma unroll
             for (int j = 0; j < PER; ++j) {
@@ -292,20 +307,26 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
         }
     }
     // this warp's part, and its keys above and equal to the threshold
-    const int part = (hi - lo + kTopWarps - 1) / kTopWarps;
+    const int part = (hi - lo + (THREADS / 32) - 1) / (THREADS / 32);
     const int w0 = min(hi, lo + warp * part), w1 = min(hi, w0 + part);
     uint32_t above = 0, equal = 0;
-    for (int i = w0 + lane; i < w1; i += 32) {
-        const uint32_t x = key(i);
-        above += all || x > prefix;
-        equal += !all && x == prefix;
+    for (int i0 = w0 + lane; i0 < w1; i0 += 128) {
+        uint32_t x[4];
+        #pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = i0 + 32 * u < w1 ? key(i0 + 32 * u) : 0u;
+        #pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i0 + 32 * u < w1) {
+                above += all || x[u] > prefix;
+                equal += !all && x[u] == prefix;
+            }
     }
     above = __reduce_add_sync(0xffffffffu, above);
     equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) { s.warp[0][warp] = above; s.warp[1][warp] = equal; }
     __syncthreads();
     uint32_t pa = 0, pe = 0, ta = 0, te = 0;
-    for (int w = 0; w < kTopWarps; ++w) {
+    for (int w = 0; w < (THREADS / 32); ++w) {
         if (w == warp) { pa = ta; pe = te; }
         ta += s.warp[0][w];
         te += s.warp[1][w];
@@ -320,18 +341,25 @@ __device__ void top_row(TopShared<DIGIT>& s, int lo, int hi, int n, int k, Key k
     const unsigned below = (1u << lane) - 1u;
     for (int i0 = w0; i0 < w1; i0 += 128) {
         int at[4];                                           // places of this lane's four keys, -1: not taken
+        uint32_t x[4];
+        #pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = i0 + 32 * u + lane < w1 ? key(i0 + 32 * u + lane) : 0u;
+        bool some = false;
         #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int i = i0 + 32 * u + lane;
-            const uint32_t x = i < w1 ? key(i) : 0u;
-            const bool a = i < w1 && (all || x > prefix), e = i < w1 && !all && x == prefix;
+            const bool in = i0 + 32 * u + lane < w1;
+            const bool a = in && (all || x[u] > prefix), e = in && !all && x[u] == prefix;
             const unsigned ma = __ballot_sync(0xffffffffu, a), me = __ballot_sync(0xffffffffu, e);
-            const uint32_t ea = pe + __popc(me & below);
-            at[u] = a || (e && ea < need) ? (int)(pa + __popc(ma & below) + min(ea, need)) : -1;
-            pa += __popc(ma);
-            pe += __popc(me);
+            at[u] = -1;
+            if (ma | me) {                                   // (uniform; most groups hold nothing to take)
+                const uint32_t ea = pe + __popc(me & below);
+                if (a || (e && ea < need)) at[u] = (int)(pa + __popc(ma & below) + min(ea, need));
+                pa += __popc(ma);
+                pe += __popc(me);
+                some = true;
+            }
         }
-        put(at, i0 + lane);
+        if (some) put(at, x, i0 + lane);
     }
     cl.sync();                                               // no CTA leaves while another reads its counts
 }
@@ -366,12 +394,16 @@ struct SelectParams {
 //  * A score is below 192 * 127 * 127 < 2^22 in magnitude: keys of 24 bits, three digits of 8 (a digit costs about
 //    2 us of barriers and remote reads with 256 bins, 5 us with 4096).
 constexpr int kPageDigit = 8;
+constexpr int kPageThreads = 512, kPageWarps = kPageThreads / 32;
 constexpr uint32_t kForcedKey = 0xffffffu;
 
-__global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams p) {
+// PPL: 16-byte pieces of a summary per lane, at most
+template <int PPL>
+__global__ void __launch_bounds__(kPageThreads) pages_select_kernel(SelectParams p) {
+    constexpr int U = PPL <= 3 ? 4 : 2;                      // pages a lane group has in flight
     extern __shared__ __align__(16) uint8_t ssm[];
-    __shared__ TopShared<kPageDigit> top;
-    __shared__ double amax_w[kTopWarps];
+    __shared__ TopShared<kPageThreads, kPageDigit> top;
+    __shared__ double amax_w[kPageWarps];
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim;
     const int rank = cl.block_rank(), C = cl.num_blocks();
@@ -384,9 +416,9 @@ __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams 
     uint32_t* keys = reinterpret_cast<uint32_t*>(raw + p.G * dim);
     int lo, hi;
     top_slice(n, lo, hi);
-    for (int i = tid; i < p.G * dim; i += kTopThreads)
+    for (int i = tid; i < p.G * dim; i += kPageThreads)
         raw[i] = load_any(p.q, p.qdt, b * p.q_bs + (int64_t)(hk * p.G + i / dim) * p.q_hs + i % dim);
-    for (int j = lo + tid; j < hi; j += kTopThreads)
+    for (int j = lo + tid; j < hi; j += kPageThreads)
         if (j >= p.sinks && j < n - p.recent) {
             const int page = page_of(p.pg, b, j);
             if (page >= 0)
@@ -394,7 +426,7 @@ __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams 
                     prefetch_l2(p.sums + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch + x);
         }
     cl.sync();                                               // raw queries; every CTA of the cluster runs
-    for (int k = rank * kTopWarps + warp; k < dim; k += C * kTopWarps) {
+    for (int k = rank * kPageWarps + warp; k < dim; k += C * kPageWarps) {
         float r[6];
         #pragma unroll
         for (int x = 0; x < 6; ++x) r[x] = lane + 32 * x < dim ? __ldg(p.R + k * dim + lane + 32 * x) : 0.f;
@@ -421,7 +453,7 @@ __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams 
     }
     cl.sync();
     double amax = 0.0;
-    for (int i = tid; i < p.G * dim; i += kTopThreads) {
+    for (int i = tid; i < p.G * dim; i += kPageThreads) {
         const double a = fabs(sq[i]);
         amax = a <= 1e300 ? fmax(amax, a) : INFINITY;       // NaN too
         if (amax == INFINITY) break;
@@ -431,8 +463,8 @@ __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams 
     if (lane == 0) amax_w[warp] = amax;
     __syncthreads();
     amax = 0.0;
-    for (int w = 0; w < kTopWarps; ++w) amax = fmax(amax, amax_w[w]);
-    for (int i = tid; i < p.G * p.pitch; i += kTopThreads) {
+    for (int w = 0; w < kPageWarps; ++w) amax = fmax(amax, amax_w[w]);
+    for (int i = tid; i < p.G * p.pitch; i += kPageThreads) {
         const int h = i / p.pitch, d = i % p.pitch;
         int v = 0;
         // a zero or non-finite group scores every page alike
@@ -444,36 +476,38 @@ __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams 
     // ---- scores: four lanes a page, pieces lane & 3, + 4, ... -------------------------------------------
     const int pieces = 2 * p.pitch / 16, sub = lane & 3;
     const int4* q4 = reinterpret_cast<const int4*>(qp);
-    for (int j0 = lo + warp * 32; j0 < hi; j0 += kTopWarps * 32) {
-        // a lane finds one page; then eight groups of four lanes score two of the 32 pages at a time
+    for (int j0 = lo + warp * 32; j0 < hi; j0 += kPageWarps * 32) {
+        // a lane finds one page; then eight groups of four lanes score U of the 32 pages at a time
         int mine = -1;
         {
             const int j = j0 + lane;
             if (j < hi && j >= p.sinks && j < n - p.recent) mine = page_of(p.pg, b, j);
         }
         #pragma unroll 1
-        for (int u0 = 0; u0 < 4 && j0 + 8 * u0 < hi; u0 += 2) {
-            int4 w[2][6];                                    // pitch <= 192: at most 24 pieces
+        for (int u0 = 0; u0 < 4 && j0 + 8 * u0 < hi; u0 += U) {
+            int4 w[U][PPL];
             #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const int page = __shfl_sync(0xffffffffu, mine, 8 * (u0 + u) + (lane >> 2));
                 const int4* sum = reinterpret_cast<const int4*>(p.sums + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch) + sub;
                 #pragma unroll
-                for (int x = 0; x < 6; ++x) {
+                for (int x = 0; x < PPL; ++x) {
                     w[u][x] = make_int4(0, 0, 0, 0);
                     if (page >= 0 && sub + 4 * x < pieces) w[u][x] = __ldcs(sum + 4 * x);
                 }
             }
-            int best[2] = {INT_MIN, INT_MIN};
+            int best[U];
+            #pragma unroll
+            for (int u = 0; u < U; ++u) best[u] = INT_MIN;
             #pragma unroll 2
             for (int h = 0; h < p.G; ++h) {
-                int a[2] = {0, 0};
+                int a[U] = {};
                 #pragma unroll
-                for (int x = 0; x < 6; ++x)
+                for (int x = 0; x < PPL; ++x)
                     if (sub + 4 * x < pieces) {
                         const int4 qv = q4[h * pieces + sub + 4 * x];
                         #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
+                        for (int u = 0; u < U; ++u) {
                             a[u] = __dp4a(w[u][x].x, qv.x, a[u]);
                             a[u] = __dp4a(w[u][x].y, qv.y, a[u]);
                             a[u] = __dp4a(w[u][x].z, qv.z, a[u]);
@@ -481,14 +515,14 @@ __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams 
                         }
                     }
                 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < U; ++u) {
                     a[u] += __shfl_xor_sync(0xffffffffu, a[u], 1);
                     a[u] += __shfl_xor_sync(0xffffffffu, a[u], 2);
                     best[u] = max(best[u], a[u]);
                 }
             }
             #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const int j = j0 + 8 * (u0 + u) + (lane >> 2);
                 const int page = __shfl_sync(0xffffffffu, mine, 8 * (u0 + u) + (lane >> 2));
                 if (sub == 0 && j < hi)
@@ -498,9 +532,9 @@ __global__ void __launch_bounds__(kTopThreads) pages_select_kernel(SelectParams 
     }
     __syncthreads();
     int32_t* out = p.out + (int64_t)bh * p.top;
-    for (int i = min(n, p.top) + rank * kTopThreads + tid; i < p.top; i += C * kTopThreads) out[i] = -1;
-    top_row<24, kPageDigit>(top, lo, hi, n, p.top, [&](int i) { return keys[i - lo]; },
-                              [&](const int (&at)[4], int i) {
+    for (int i = min(n, p.top) + rank * kPageThreads + tid; i < p.top; i += C * kPageThreads) out[i] = -1;
+    top_row<24, kPageThreads, kPageDigit>(top, lo, hi, n, p.top, [&](int i) { return keys[i - lo]; },
+                              [&](const int (&at)[4], const uint32_t (&)[4], int i) {
                                   #pragma unroll
                                   for (int u = 0; u < 4; ++u)
                                       if (at[u] >= 0) out[at[u]] = i + 32 * u;
@@ -522,48 +556,53 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kTopThreads) tokens_select_kernel(KeepParams p) {
-    extern __shared__ float ksm[];
-    __shared__ TopShared<11> top;
+// the weight of a key; keys of NaN, of either zero and of forced tokens do not tell theirs
+__device__ __forceinline__ bool key_tells(uint32_t k) { return k != 0u && k != 0x80000000u && k != 0xffffffffu; }
+__device__ __forceinline__ float key_weight(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+// One cluster per (sequence, KV head).  The slice's keys lie in shared memory, computed once (a weight is read
+// back from its key); where a slice does not fit they are computed from the weights on every pass.
+constexpr int kKeepThreads = 1024, kKeepDigit = 12;
+
+__global__ void __launch_bounds__(kKeepThreads) tokens_select_kernel(KeepParams p) {
+    extern __shared__ uint32_t ksm[];
+    __shared__ TopShared<kKeepThreads, kKeepDigit> top;
     cg::cluster_group cl = cg::this_cluster();
     const int bh = blockIdx.x / cl.num_blocks(), tid = threadIdx.x;
     const int n = min(max(p.seq_lens[bh / p.Hkv], 0), p.slots);
     const float* w = p.w + (int64_t)bh * p.w_rs;
     int lo, hi;
     top_slice(n, lo, hi);
+    auto make = [&](int i, float x) { return i < p.sinks || i >= n - p.recent ? 0xffffffffu : weight_key(x); };
     int32_t* kept = p.kept + (int64_t)bh * p.keep;
     float* kw = p.kept_w + (int64_t)bh * p.keep;
-    for (int i = min(n, p.keep) + cl.block_rank() * kTopThreads + tid; i < p.keep; i += cl.num_blocks() * kTopThreads) {
+    for (int i = min(n, p.keep) + cl.block_rank() * kKeepThreads + tid; i < p.keep; i += cl.num_blocks() * kKeepThreads) {
         kept[i] = -1;
         kw[i] = 0.f;
     }
-    // the slice's weights in shared memory, asked for sixteen at a time (32 KB in flight per CTA)
+    auto put = [&](const int (&at)[4], const uint32_t (&x)[4], int i) {
+        #pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (at[u] >= 0) {
+                kept[at[u]] = i + 32 * u;
+                kw[at[u]] = key_tells(x[u]) ? key_weight(x[u]) : __ldg(w + i + 32 * u);
+            }
+    };
     if (p.cached) {
-        constexpr int U = 16;
-        for (int i0 = lo + tid; i0 < hi; i0 += U * kTopThreads) {
+        constexpr int U = 16;                                // 64 KB of weights in flight per CTA
+        for (int i0 = lo + tid; i0 < hi; i0 += U * kKeepThreads) {
             float x[U];
             #pragma unroll
-            for (int u = 0; u < U; ++u) x[u] = i0 + u * kTopThreads < hi ? __ldg(w + i0 + u * kTopThreads) : 0.f;
+            for (int u = 0; u < U; ++u) x[u] = i0 + u * kKeepThreads < hi ? __ldg(w + i0 + u * kKeepThreads) : 0.f;
             #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (i0 + u * kTopThreads < hi) ksm[i0 + u * kTopThreads - lo] = x[u];
+                if (i0 + u * kKeepThreads < hi) ksm[i0 + u * kKeepThreads - lo] = make(i0 + u * kKeepThreads, x[u]);
         }
         __syncthreads();
+        top_row<32, kKeepThreads, kKeepDigit>(top, lo, hi, n, p.keep, [&](int i) { return ksm[i - lo]; }, put);
+    } else {
+        top_row<32, kKeepThreads, kKeepDigit>(top, lo, hi, n, p.keep, [&](int i) { return make(i, __ldg(w + i)); }, put);
     }
-    auto select = [&](auto weight) {
-        top_row<32, 11>(top, lo, hi, n, p.keep,
-                        [&](int i) { return i < p.sinks || i >= n - p.recent ? 0xffffffffu : weight_key(weight(i)); },
-                        [&](const int (&at)[4], int i) {
-                            #pragma unroll
-                            for (int u = 0; u < 4; ++u)
-                                if (at[u] >= 0) {
-                                    kept[at[u]] = i + 32 * u;
-                                    kw[at[u]] = weight(i + 32 * u);
-                                }
-                        });
-    };
-    if (p.cached) select([&](int i) { return ksm[i - lo]; });
-    else select([&](int i) { return __ldg(w + i); });
 }
 
 // ---- launches -------------------------------------------------------------------------------------------
@@ -575,14 +614,14 @@ static int top_cluster(int64_t rows, int64_t n, int sms, int64_t cap, int64_t le
 }
 
 template <class K, class P>
-static int launch_cluster(K kernel, const P& p, int64_t rows, int c, size_t smem, cudaStream_t st) {
+static int launch_cluster(K kernel, const P& p, int64_t rows, int c, int threads, size_t smem, cudaStream_t st,
+                          std::atomic<int> (&seen)[64]) {
     if (rows * c > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-    static std::atomic<int> seen[64];                        // (one array per instantiation: per parameter type)
     const int rc = allow_smem(kernel, (int)smem, seen);
     if (rc) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * c));
-    cfg.blockDim = dim3(kTopThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at{};
@@ -594,7 +633,7 @@ static int launch_cluster(K kernel, const P& p, int64_t rows, int c, size_t smem
     return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
 }
 
-constexpr int64_t kKeyCap = 48 * 1024;          // weights of a slice in shared memory (192 KB)
+constexpr int64_t kKeyCap = 46 * 1024;          // keys of a slice in shared memory (184 KB, beside 33 KB of counters)
 
 int launch_tokens_select(const float* w, int B, int Hkv, int slots, int64_t rs, const int32_t* lens, int keep, int sinks,
                          int recent, int32_t* kept, float* kept_w, int sms, cudaStream_t st) {
@@ -603,7 +642,8 @@ int launch_tokens_select(const float* w, int B, int Hkv, int slots, int64_t rs, 
     const int c = top_cluster(rows, slots, sms, kKeyCap, 2048);
     const int64_t per = ((int64_t)slots + c - 1) / c;
     p.cached = per <= kKeyCap;
-    return launch_cluster(tokens_select_kernel, p, rows, c, p.cached ? (size_t)per * 4 : 0, st);
+    static std::atomic<int> seen[64];
+    return launch_cluster(tokens_select_kernel, p, rows, c, kKeepThreads, p.cached ? (size_t)per * 4 : 0, st, seen);
 }
 
 // Shared memory of the selection without its keys; keys of a slice take what is left of 190 KB.
@@ -623,10 +663,13 @@ int launch_pages_select(const pkv_codec* c, Pages pg, const void* q, int qdt, in
     p.out = out;
     const int64_t fixed = (int64_t)p.G * p.dim * 12 + 2 * (int64_t)p.G * p.pitch;
     const int64_t cap = (190 * 1024 - fixed) / 4, rows = (int64_t)pg.B * pg.Hkv;
-    const int cl = top_cluster(rows, pg.max_pages, sms, cap, 256);
+    const int cl = top_cluster(rows, pg.max_pages, sms, cap, 32);
     const int64_t per = ((int64_t)pg.max_pages + cl - 1) / cl;
     if (per > cap) return PKV_ERR_UNSUPPORTED;
-    return launch_cluster(pages_select_kernel, p, rows, cl, (size_t)(fixed + per * 4), st);
+    static std::atomic<int> seen3[64], seen6[64];
+    const size_t smem = (size_t)(fixed + per * 4);
+    if (2 * p.pitch <= 16 * 4 * 3) return launch_cluster(pages_select_kernel<3>, p, rows, cl, kPageThreads, smem, st, seen3);
+    return launch_cluster(pages_select_kernel<6>, p, rows, cl, kPageThreads, smem, st, seen6);
 }
 
 template <int CB, int LPT>
@@ -649,8 +692,7 @@ int launch_pages_summarize(const pkv_codec* c, Pages pg, int cb, const int32_t* 
     p.pitch = (c->dim + 15) / 16 * 16;
     p.bits_z = c->bits_z;
     p.bits_flat = c->bits_r + c->bits_theta;
-    p.code_mask = (1 << (p.bits_z + p.bits_flat)) - 1;
-    p.index_mask = c->xy_per_z ? p.code_mask : (1 << p.bits_flat) - 1;
+    p.index_mask = (1 << (c->xy_per_z ? p.bits_z + p.bits_flat : p.bits_flat)) - 1;
     p.entries = p.index_mask + 1;
     // pages per CTA: about eight CTAs per SM when every page is asked for, so that the table's fill is shared
     const int64_t all = (int64_t)pg.B * pg.Hkv * pg.max_pages;
