@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include <cooperative_groups.h>
 
@@ -117,15 +118,19 @@ struct SummaryParams {
 
 template <int CB, int LPT, bool COPIES>
 __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
-    extern __shared__ __align__(16) uint32_t lut[];
+    __shared__ __align__(16) uint32_t lut[COPIES ? 256 * 32 : 4096];   // (x, y) grid values
+    __shared__ int gz[256];
     constexpr int CW = 4 / CB, TPL = 32 / LPT, U = 8;       // codes per word, tokens per load, loads in flight
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int chunk = blockIdx.x % p.chunks, bh = blockIdx.x / p.chunks, b = bh / p.pg.Hkv, hk = bh - b * p.pg.Hkv;
     const int L = clamp_len(p.pg, __ldg(p.seq_lens + b)), ps = 1 << p.pg.ps_log2;
-    const int first = p.start ? max(__ldg(p.start + b), 0) >> p.pg.ps_log2 : 0;
-    const int j0 = first + chunk * p.chunk, j1 = min(j0 + p.chunk, (int)(((int64_t)L + ps - 1) >> p.pg.ps_log2));
-    if (j0 >= j1 || (p.start && p.start[b] >= L)) return;
+    const int start = p.start ? max(__ldg(p.start + b), 0) : 0;
+    const int j0 = (start >> p.pg.ps_log2) + chunk * p.chunk;
+    const int j1 = min(j0 + p.chunk, (int)(((int64_t)L + ps - 1) >> p.pg.ps_log2));
+    if (j0 >= j1 || start >= L) return;
     const uint32_t* xy = reinterpret_cast<const uint32_t*>(p.grid_xy);
+    int next = j0 + warp < j1 ? page_of(p.pg, b, j0 + warp) : -1;
+    for (int i = tid; i < 1 << p.bits_z; i += 256) gz[i] = __ldg(p.grid_z + i);
     if constexpr (COPIES) {                                  // 16-byte pieces of four copies, spread over the banks
         for (int e = tid; e < p.entries; e += 256) {
             const uint32_t v = __ldg(xy + e);
@@ -143,11 +148,13 @@ __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
     const uint32_t imask = (uint32_t)p.index_mask << SH, lane4 = COPIES ? lane * 4 : 0;
     const uint32_t zm = (1u << p.bits_z) - 1u, zmask = CB == 2 ? zm * 0x00010001u : zm * 0x01010101u;
     const char* const lutb = reinterpret_cast<const char*>(lut);
+    const uint8_t* const mine = p.pg.k + (int64_t)hk * p.pg.head_bs + (int64_t)tok * p.pg.tok_bs + word * 4;
     for (int j = j0 + warp; j < j1; j += 8) {
-        const int page = page_of(p.pg, b, j);
+        const int page = next;
+        if (j + 8 < j1) next = page_of(p.pg, b, j + 8);
         if (page < 0) continue;
         const int n = min(L - (j << p.pg.ps_log2), ps);
-        const uint8_t* row = p.pg.k + slot_offset(p.pg, page, hk, tok) + word * 4;
+        const uint8_t* row = mine + (int64_t)page * p.pg.page_bs;
         const int64_t step = TPL * p.pg.tok_bs;
         uint32_t lo[CW], hi[CW], zl[CW / 2], zh[CW / 2];     // z bins: two codes to a word
         #pragma unroll
@@ -195,20 +202,35 @@ __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
                 }
             }
         int8_t* o = p.out + ((int64_t)page * p.pg.Hkv + hk) * 2 * p.pitch;
-        if (tok == 0 && have) {
+        // lanes of the first token write the least, those of the next (or the same) the greatest: 3 CW bytes
+        #pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            if (!have || tok != (TPL > 1 ? side : 0)) continue;
+            int8_t v[3 * CW];
             #pragma unroll
             for (int x = 0; x < CW; ++x) {
-                const int i = word * CW + x;
-                if (i >= p.m) break;
-                // code x's bins: CB 2: half x; CB 1: half x / 2 of word x % 2
+                // code x's bin: CB 2: half x; CB 1: half x / 2 of word x % 2
                 const int zw = CB == 2 ? 0 : x & 1, zs = CB == 2 ? 16 * x : 16 * (x >> 1);
-                const int l[3] = {__ldg(p.grid_z + ((zl[zw] >> zs) & 0xffffu)), (int16_t)lo[x], (int16_t)(lo[x] >> 16)};
-                const int h[3] = {__ldg(p.grid_z + ((zh[zw] >> zs) & 0xffffu)), (int16_t)hi[x], (int16_t)(hi[x] >> 16)};
+                const uint32_t xyv = side ? hi[x] : lo[x];
+                const int up = side ? 127 : 0;
+                v[3 * x] = (int8_t)((gz[((side ? zh[zw] : zl[zw]) >> zs) & 0xffu] + up) >> 7);
+                v[3 * x + 1] = (int8_t)(((int16_t)xyv + up) >> 7);
+                v[3 * x + 2] = (int8_t)(((int16_t)(xyv >> 16) + up) >> 7);
+            }
+            int8_t* d = o + side * p.pitch + 3 * CW * word;
+            if ((word + 1) * CW <= p.m) {
+                using Out = typename std::conditional<CB == 2, uint16_t, uint32_t>::type;   // 3 CW bytes as three
                 #pragma unroll
                 for (int y = 0; y < 3; ++y) {
-                    o[3 * i + y] = (int8_t)(l[y] >> 7);
-                    o[p.pitch + 3 * i + y] = (int8_t)((h[y] + 127) >> 7);
+                    Out t = 0;
+                    #pragma unroll
+                    for (int z = 0; z < (int)sizeof(Out); ++z) t |= (Out)((Out)(uint8_t)v[y * (int)sizeof(Out) + z] << (8 * z));
+                    reinterpret_cast<Out*>(d)[y] = t;
                 }
+            } else {                                         // the row's last word, not full
+                #pragma unroll
+                for (int y = 0; y < 3 * CW; ++y)
+                    if (word * CW + y / 3 < p.m) d[y] = v[y];
             }
         }
         for (int d = 3 * p.m + lane; d < p.pitch; d += 32) o[d] = o[p.pitch + d] = 0;
@@ -231,8 +253,8 @@ struct TopShared {
     uint32_t bin, need;
 };
 
-// BITS-bit keys in digits of DIGIT bits (the last one may be shorter).  put(at, x, i): keys i, i + 32, i + 64,
-// i + 96 (x[0 .. 3]) go to places at[0 .. 3] (negative: not taken).
+// BITS-bit keys in digits of DIGIT bits (the last one may be shorter).  put(at, x, i): key i, which is x, goes to
+// place at.
 template <int BITS, int THREADS, int DIGIT, class Key, class Put>
 __device__ void top_row(TopShared<THREADS, DIGIT>& s, int lo, int hi, int n, int k, Key key, Put put) {
     cg::cluster_group cl = cg::this_cluster();
@@ -339,27 +361,39 @@ __device__ void top_row(TopShared<THREADS, DIGIT>& s, int lo, int hi, int n, int
         pe += t[1];
     }
     const unsigned below = (1u << lane) - 1u;
-    for (int i0 = w0; i0 < w1; i0 += 128) {
-        int at[4];                                           // places of this lane's four keys, -1: not taken
+    for (int i0 = w0; i0 < w1; i0 += 128) {                  // four neighbouring keys a lane
+        const int i = i0 + 4 * lane;
         uint32_t x[4];
         #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = i0 + 32 * u + lane < w1 ? key(i0 + 32 * u + lane) : 0u;
-        bool some = false;
+        for (int u = 0; u < 4; ++u) x[u] = i + u < w1 ? key(i + u) : 0u;
+        uint32_t take = 0, same = 0;                         // keys above the threshold, and equal to it
         #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const bool in = i0 + 32 * u + lane < w1;
-            const bool a = in && (all || x[u] > prefix), e = in && !all && x[u] == prefix;
-            const unsigned ma = __ballot_sync(0xffffffffu, a), me = __ballot_sync(0xffffffffu, e);
-            at[u] = -1;
-            if (ma | me) {                                   // (uniform; most groups hold nothing to take)
-                const uint32_t ea = pe + __popc(me & below);
-                if (a || (e && ea < need)) at[u] = (int)(pa + __popc(ma & below) + min(ea, need));
-                pa += __popc(ma);
-                pe += __popc(me);
-                some = true;
+        for (int u = 0; u < 4; ++u)
+            if (i + u < w1) {
+                take |= (uint32_t)(all || x[u] > prefix) << u;
+                same |= (uint32_t)(!all && x[u] == prefix) << u;
+            }
+        // counts of the lanes below, bit by bit (a count is 0 to 4)
+        const uint32_t ca = __popc(take), ce = __popc(same);
+        const unsigned a0 = __ballot_sync(0xffffffffu, ca & 1), a1 = __ballot_sync(0xffffffffu, ca & 2),
+                       a2 = __ballot_sync(0xffffffffu, ca & 4);
+        uint32_t at = pa + __popc(a0 & below) + 2 * __popc(a1 & below) + 4 * __popc(a2 & below), ea = pe;
+        if (__any_sync(0xffffffffu, ce)) {
+            const unsigned e0 = __ballot_sync(0xffffffffu, ce & 1), e1 = __ballot_sync(0xffffffffu, ce & 2),
+                           e2 = __ballot_sync(0xffffffffu, ce & 4);
+            ea = pe + __popc(e0 & below) + 2 * __popc(e1 & below) + 4 * __popc(e2 & below);
+            pe += __popc(e0) + 2 * __popc(e1) + 4 * __popc(e2);
+        }
+        pa += __popc(a0) + 2 * __popc(a1) + 4 * __popc(a2);
+        if (take | same) {
+            #pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool a = take >> u & 1, e = same >> u & 1;
+                if (a || (e && ea < need)) put((int)(at + min(ea, need)), x[u], i + u);
+                at += a;
+                ea += e;
             }
         }
-        if (some) put(at, x, i0 + lane);
     }
     cl.sync();                                               // no CTA leaves while another reads its counts
 }
@@ -534,11 +568,7 @@ __global__ void __launch_bounds__(kPageThreads) pages_select_kernel(SelectParams
     int32_t* out = p.out + (int64_t)bh * p.top;
     for (int i = min(n, p.top) + rank * kPageThreads + tid; i < p.top; i += C * kPageThreads) out[i] = -1;
     top_row<24, kPageThreads, kPageDigit>(top, lo, hi, n, p.top, [&](int i) { return keys[i - lo]; },
-                              [&](const int (&at)[4], const uint32_t (&)[4], int i) {
-                                  #pragma unroll
-                                  for (int u = 0; u < 4; ++u)
-                                      if (at[u] >= 0) out[at[u]] = i + 32 * u;
-                              });
+                              [&](int at, uint32_t, int i) { out[at] = i; });
 }
 
 // ---- choosing tokens ----------------------------------------------------------------------------------
@@ -561,12 +591,15 @@ __device__ __forceinline__ bool key_tells(uint32_t k) { return k != 0u && k != 0
 __device__ __forceinline__ float key_weight(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
 // One cluster per (sequence, KV head).  The slice's keys lie in shared memory, computed once (a weight is read
-// back from its key); where a slice does not fit they are computed from the weights on every pass.
-constexpr int kKeepThreads = 1024, kKeepDigit = 12;
+// back from its key); where a slice does not fit they are computed from the weights on every pass.  Two sizes:
+// 1024 threads and digits of 12 bits for long slices (3 passes over the keys), 512 threads and digits of 8 bits
+// (4 passes, but 256 counters to clear, read and scan) up to kShortSlice keys: 8 rows of 1024 take 8 us, not 14.
+constexpr int kShortSlice = 4096;
 
-__global__ void __launch_bounds__(kKeepThreads) tokens_select_kernel(KeepParams p) {
+template <int THREADS, int DIGIT>
+__global__ void __launch_bounds__(THREADS) tokens_select_kernel(KeepParams p) {
     extern __shared__ uint32_t ksm[];
-    __shared__ TopShared<kKeepThreads, kKeepDigit> top;
+    __shared__ TopShared<THREADS, DIGIT> top;
     cg::cluster_group cl = cg::this_cluster();
     const int bh = blockIdx.x / cl.num_blocks(), tid = threadIdx.x;
     const int n = min(max(p.seq_lens[bh / p.Hkv], 0), p.slots);
@@ -576,32 +609,28 @@ __global__ void __launch_bounds__(kKeepThreads) tokens_select_kernel(KeepParams 
     auto make = [&](int i, float x) { return i < p.sinks || i >= n - p.recent ? 0xffffffffu : weight_key(x); };
     int32_t* kept = p.kept + (int64_t)bh * p.keep;
     float* kw = p.kept_w + (int64_t)bh * p.keep;
-    for (int i = min(n, p.keep) + cl.block_rank() * kKeepThreads + tid; i < p.keep; i += cl.num_blocks() * kKeepThreads) {
+    for (int i = min(n, p.keep) + cl.block_rank() * THREADS + tid; i < p.keep; i += cl.num_blocks() * THREADS) {
         kept[i] = -1;
         kw[i] = 0.f;
     }
-    auto put = [&](const int (&at)[4], const uint32_t (&x)[4], int i) {
-        #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (at[u] >= 0) {
-                kept[at[u]] = i + 32 * u;
-                kw[at[u]] = key_tells(x[u]) ? key_weight(x[u]) : __ldg(w + i + 32 * u);
-            }
+    auto put = [&](int at, uint32_t x, int i) {
+        kept[at] = i;
+        kw[at] = key_tells(x) ? key_weight(x) : __ldg(w + i);
     };
     if (p.cached) {
         constexpr int U = 16;                                // 64 KB of weights in flight per CTA
-        for (int i0 = lo + tid; i0 < hi; i0 += U * kKeepThreads) {
+        for (int i0 = lo + tid; i0 < hi; i0 += U * THREADS) {
             float x[U];
             #pragma unroll
-            for (int u = 0; u < U; ++u) x[u] = i0 + u * kKeepThreads < hi ? __ldg(w + i0 + u * kKeepThreads) : 0.f;
+            for (int u = 0; u < U; ++u) x[u] = i0 + u * THREADS < hi ? __ldg(w + i0 + u * THREADS) : 0.f;
             #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (i0 + u * kKeepThreads < hi) ksm[i0 + u * kKeepThreads - lo] = make(i0 + u * kKeepThreads, x[u]);
+                if (i0 + u * THREADS < hi) ksm[i0 + u * THREADS - lo] = make(i0 + u * THREADS, x[u]);
         }
         __syncthreads();
-        top_row<32, kKeepThreads, kKeepDigit>(top, lo, hi, n, p.keep, [&](int i) { return ksm[i - lo]; }, put);
+        top_row<32, THREADS, DIGIT>(top, lo, hi, n, p.keep, [&](int i) { return ksm[i - lo]; }, put);
     } else {
-        top_row<32, kKeepThreads, kKeepDigit>(top, lo, hi, n, p.keep, [&](int i) { return make(i, __ldg(w + i)); }, put);
+        top_row<32, THREADS, DIGIT>(top, lo, hi, n, p.keep, [&](int i) { return make(i, __ldg(w + i)); }, put);
     }
 }
 
@@ -642,8 +671,10 @@ int launch_tokens_select(const float* w, int B, int Hkv, int slots, int64_t rs, 
     const int c = top_cluster(rows, slots, sms, kKeyCap, 2048);
     const int64_t per = ((int64_t)slots + c - 1) / c;
     p.cached = per <= kKeyCap;
-    static std::atomic<int> seen[64];
-    return launch_cluster(tokens_select_kernel, p, rows, c, kKeepThreads, p.cached ? (size_t)per * 4 : 0, st, seen);
+    const size_t smem = p.cached ? (size_t)per * 4 : 0;
+    static std::atomic<int> seen_short[64], seen_long[64];
+    if (per <= kShortSlice) return launch_cluster(tokens_select_kernel<512, 8>, p, rows, c, 512, smem, st, seen_short);
+    return launch_cluster(tokens_select_kernel<1024, 12>, p, rows, c, 1024, smem, st, seen_long);
 }
 
 // Shared memory of the selection without its keys; keys of a slice take what is left of 190 KB.
@@ -676,8 +707,8 @@ template <int CB, int LPT>
 static int launch_summaries(const SummaryParams& p, cudaStream_t st) {
     const int64_t ctas = (int64_t)p.pg.B * p.pg.Hkv * p.chunks;
     if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-    if (p.entries <= 256) pages_summarize_kernel<CB, LPT, true><<<(unsigned)ctas, 256, p.entries * 128, st>>>(p);
-    else pages_summarize_kernel<CB, LPT, false><<<(unsigned)ctas, 256, p.entries * 4, st>>>(p);
+    if (p.entries <= 256) pages_summarize_kernel<CB, LPT, true><<<(unsigned)ctas, 256, 0, st>>>(p);
+    else pages_summarize_kernel<CB, LPT, false><<<(unsigned)ctas, 256, 0, st>>>(p);
     return cudaGetLastError() == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
 }
 
@@ -694,9 +725,9 @@ int launch_pages_summarize(const pkv_codec* c, Pages pg, int cb, const int32_t* 
     p.bits_flat = c->bits_r + c->bits_theta;
     p.index_mask = (1 << (c->xy_per_z ? p.bits_z + p.bits_flat : p.bits_flat)) - 1;
     p.entries = p.index_mask + 1;
-    // pages per CTA: about eight CTAs per SM when every page is asked for, so that the table's fill is shared
-    const int64_t all = (int64_t)pg.B * pg.Hkv * pg.max_pages;
-    p.chunk = (int)std::min<int64_t>(512, std::max<int64_t>(8, all / (8 * sms)));
+    // CTAs: one wave of six per SM (33 KB of tables each), or one per (sequence, KV head) where those are more
+    const int64_t rows = (int64_t)pg.B * pg.Hkv, per = std::max<int64_t>(1, 6 * (int64_t)sms / rows);
+    p.chunk = (int)std::max<int64_t>(8, (pg.max_pages + per - 1) / per);
     p.chunks = (pg.max_pages + p.chunk - 1) / p.chunk;
     const int words = (p.m * cb + 3) / 4;
     if (cb == 1) return words <= 8 ? launch_summaries<1, 8>(p, st) : launch_summaries<1, 16>(p, st);
