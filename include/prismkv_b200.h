@@ -315,7 +315,8 @@ PKV_API int pkv_polar_scores(const float *q_rot, const void *k_codes, int32_t co
  * and holds the m codes of one token (the same in v).  Row b of the page
  * table names sequence b's pages: token t sits in slot t % page_size of page
  * table[b*table_stride + t / page_size].  page_size is a power of two, 16 to
- * 1024; k, v and the three strides are multiples of 16 bytes.
+ * 1024; k, v and the three strides are multiples of 16 bytes; a page_stride of
+ * 2 GiB or a token_stride of 2 MiB and more is PKV_ERR_UNSUPPORTED.
  * Page ids outside [0, num_pages) are never followed: their tokens count as
  * masked and the device error word is set to 6.  Sequence lengths are read on
  * the device, clamped to [0, max_pages * page_size].                        */

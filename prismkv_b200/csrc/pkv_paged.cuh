@@ -10,8 +10,6 @@
 
 namespace pkv {
 
-constexpr int kGranule = 16;                  // tokens per granule; pages hold whole granules
-
 // The pages of a cache, strides in bytes.
 struct Pages {
     const uint8_t *k, *v;
@@ -62,20 +60,20 @@ static int allow_smem(K kernel, int bytes, std::atomic<int> (&seen)[64]) {
 
 // ---- attention ---------------------------------------------------------------------------------
 // A unit is up to HQ query heads of one (sequence, KV head); units are numbered sequence-major.  Its
-// tokens are the sequence's (or the listed pages', in list order) in granules of 16.  The granules of
-// all units form one line of T granules, cut among Gd CTAs: the grid, or where that is less one per unit or
-// per 16 granules, below which a CTA's warps would have nothing to share.  Two ways to cut:
+// tokens are the sequence's (or the listed pages', in list order) in granules of what a warp takes at a time,
+// 2^gran_log2 = 16 or 32.  The granules of all units form one line of T granules, cut among Gd CTAs: the grid, or
+// where that is less one per unit or per 256 tokens, below which a CTA's warps would have little to share.  Two ways to cut:
 //  * evenly: CTA c takes [c T / Gd, (c + 1) T / Gd), whatever the units.  Every CTA streams the same, but most
 //    units end inside a CTA, which then sets up a second range (about 5 us).
-//  * by units, while a CTA's share is below kUnitShare granules (of which 32 take 2.7 us): a unit [a, e) goes
+//  * by units, while a CTA's share is below kUnitShare tokens (of which 512 take 2.7 us): a unit [a, e) goes
 //    to the CTAs [s(a), s(e)), s(t) = round(t Gd / T), in equal parts, or whole to CTA s(a) when that is none.
 // Each (CTA, unit) range leaves one partial softmax state; range (c, u) uses partial row c + u, so a
 // unit's rows lie side by side.
-constexpr int kUnitShare = 256;
+constexpr int kUnitShare = 4096;
 
 struct PagedParams {
     Pages pg;
-    int Hq, G, HQ, UG, UH, dim, m, cb;         // UG units per KV head, UH = Hkv * UG per sequence
+    int Hq, G, HQ, UG, UH, dim, m, cb, gran_log2;   // UG units per KV head, UH = Hkv * UG per sequence
     const void* q; int qdt; int64_t q_bs, q_hs;
     const int32_t* seq_lens;
     const int32_t* selected; int n_sel;
@@ -91,8 +89,8 @@ struct PagedParams {
 };
 
 __device__ __forceinline__ int granules_of(const PagedParams& p, int b) {
-    if (p.selected) return p.n_sel << (p.pg.ps_log2 - 4);
-    return (clamp_len(p.pg, __ldg(p.seq_lens + b)) + kGranule - 1) / kGranule;
+    const int n = p.selected ? p.n_sel << p.pg.ps_log2 : clamp_len(p.pg, __ldg(p.seq_lens + b));
+    return (n + (1 << p.gran_log2) - 1) >> p.gran_log2;
 }
 
 // Granules of the sequences before b, and of all of them (times UH: the line of all units).  Whole warps.
@@ -126,8 +124,9 @@ struct PagedCut { int64_t total; int gd; bool by_unit; };
 __device__ __forceinline__ PagedCut paged_cut(const PagedParams& p, int64_t total) {
     PagedCut c;
     c.total = total;
-    c.gd = (int)min((int64_t)p.grid, min(total, max((total + 15) / 16, (int64_t)p.units)));
-    c.by_unit = total < (int64_t)kUnitShare * c.gd;
+    const int64_t tokens = total << p.gran_log2;
+    c.gd = (int)min((int64_t)p.grid, min(total, max((tokens + 255) / 256, (int64_t)p.units)));
+    c.by_unit = tokens < (int64_t)kUnitShare * c.gd;
     return c;
 }
 
@@ -236,38 +235,21 @@ __device__ inline void unit_rows(const PagedParams& p, int unit, int& r0, int& r
     }
 }
 
-// Where granule gi of (b, hk) lies: its physical page (-1: masked), the slot of its first token in the
-// page, and the token that slot holds.
-struct Granule { int page, slot, tok; };
+// Page j of an attention range: the sequence's logical page (j itself, or entry j of its list) and the physical one;
+// -1 for what is masked.
+struct RangePage { int logical, page; };
 
-__device__ __forceinline__ Granule granule_at(const PagedParams& p, int b, int hk, int gi) {
-    const int per = p.pg.ps_log2 - 4;                       // log2 of granules per page
-    const int j = gi >> per;
-    Granule g;
-    g.slot = (gi & ((1 << per) - 1)) << 4;
-    int lp = j;
-    if (p.selected) {
-        const int32_t* s = p.selected + ((int64_t)b * p.pg.Hkv + hk) * p.n_sel + j;
-        lp = __ldg(s);
-        if (lp < 0 || (j > 0 && __ldg(s - 1) >= lp)) {      // padding, or not ascending
-            if (lp >= 0) flag_error(kErrPage);
-            lp = -1;
-        } else if (j > 0 && __ldg(s - 1) < 0) {
-            flag_error(kErrPage);
-            lp = -1;
-        }
+__device__ __forceinline__ RangePage range_page(const PagedParams& p, int b, int hk, int j) {
+    if (!p.selected) return {j, page_of(p.pg, b, j)};
+    const int32_t* s = p.selected + ((int64_t)b * p.pg.Hkv + hk) * p.n_sel + j;
+    const int lp = __ldg(s), before = j > 0 ? __ldg(s - 1) : -1;
+    if (lp < 0) return {-1, -1};                            // padding
+    if ((j > 0 && (before < 0 || before >= lp)) ||          // not ascending, or behind the sequence's end
+        (int64_t)lp << p.pg.ps_log2 >= clamp_len(p.pg, __ldg(p.seq_lens + b))) {
+        flag_error(kErrPage);
+        return {-1, -1};
     }
-    g.tok = (lp << p.pg.ps_log2) + g.slot;
-    g.page = -1;
-    if (lp >= 0) {
-        if (p.selected && (int64_t)lp << p.pg.ps_log2 >= clamp_len(p.pg, __ldg(p.seq_lens + b))) {
-            flag_error(kErrPage);                           // a listed page behind the sequence's end
-            g.tok = 0x7ffffff0;
-        } else {
-            g.page = page_of(p.pg, b, lp);
-        }
-    }
-    return g;
+    return {lp, page_of(p.pg, b, lp)};
 }
 
 // bulk_g2s (pkv_common.cuh) to a shared address

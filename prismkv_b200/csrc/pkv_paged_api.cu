@@ -45,6 +45,8 @@ int check_pages(const pkv_pages* g, int m, bool need_codes) {
     if (need_codes && g->num_pages > 0 && !g->k) return PKV_ERR_INVALID;
     const int64_t cb = g->code_bytes;
     if ((g->token_stride * cb | g->head_stride * cb | g->page_stride * cb) % 16) return PKV_ERR_ALIGNMENT;
+    // byte strides of a page and of a page's tokens are 32-bit factors in the kernels
+    if (g->page_stride * cb > 0x7fffffff || g->token_stride * cb > 0x7fffffff / 1024) return PKV_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(g->k) | reinterpret_cast<uintptr_t>(g->v)) % 16) return PKV_ERR_ALIGNMENT;
     return PKV_OK;
 }

@@ -31,24 +31,25 @@ constexpr int kHQ = 4;                         // query heads per unit
 //  * table values are scaled by a power of two that puts the largest in [2^9, 2^10), the queries per head by
 //    one that puts theirs in [2^13, 2^14): pairs of normal fp16 whatever the ranges of the codec and the
 //    data.  Weights are 2^12 exp2(score - running max).
-//  * MODE 0 (two-byte codes, 8 bits of (r, theta), uniform z): z = z0 + i dz enters by its index -- for the
+//  * MODE 0 (two-byte codes, 8 bits of (r, theta)) and 3 (one-byte codes), both with uniform z of up to 4 bits and
+//    one polar grid: z = z0 + i dz enters by its index -- for the
 //    scores as the exact fp16 subnormal i 2^-24 (EX: as i - 8), for the values as the exact i - 8, both affine parts added
 //    outside.  Centred, because an uncentred sum of p i grows with every token and the tiles' sums truncate.
-// Tables in shared memory: MODE 0 and 1 (one-byte codes, any codec) hold 256 rows of 32 copies, copy `lane`
+// Tables in shared memory: MODE 0, 3 and 1 (one-byte codes, any codec) hold 256 rows of 32 copies, copy `lane`
 // for each lane: the 32 lookups of a warp never collide, and at a 64 KB-aligned address one byte permute of
 // the code word makes a lookup's address (z: and a shift).  MODE 2 (two-byte codes of any codec) holds one copy of all 2^bits
-// (x, y) -- 32 copies of 4096 do not fit -- and pays bank conflicts; z has 32 copies per bin in each mode.
+// (x, y) -- 32 copies of 4096 do not fit -- and pays bank conflicts; a z table has 32 copies per bin.
 //
-// A warp takes NG granules (16 tokens each) at a time, lane = 4 g + c:
+// A warp takes a granule of NG times 16 tokens at a time; for 16 of them, lane = 4 g + c:
 //  * scores: rows = tokens, k = triplets.  Lane (g, c) holds tokens rho(g), rho(g) + 8, rho(2 x) = x, rho(2 x + 1) =
 //    (x ^ 1) + 4 (neighbouring rows of 64 bytes lie in different banks), and CPL triplets of each: 8c .. 8c + 7 of
 //    the first 32, then its share of the rest.
 //  * weights: two 8x8 transposes (movmatrix) turn the score tile into the B operand of p . v.
 //  * values: rows = triplets, k = tokens.  Lane (g, c) holds tokens c, (c ^ 1) + 4 and both + 8, and CPL / 2
 //    triplets of each: 4g .. 4g + 3 of the first 32, then its share of the rest.
-// Codes come through shared memory, two iterations ahead: a warp's lane 0 copies its granules (16 rows of K, 16
-// of V) by bulk copies into the warp's own two-stage ring and every warp waits on its own barriers alone, so no
-// warp waits for another inside a range.  (Loaded into registers one iteration ahead instead, the codes cost
+// Codes come through shared memory, two iterations ahead: a warp's lane 0 brings its granules' rows of K and V by
+// bulk copies into the warp's own two-stage ring and every warp waits on its own barriers alone, so no warp
+// waits for another inside a range.  (Loaded into registers one iteration ahead instead, the codes cost
 // spills and a quarter of the issue slots in waits: attend over 4 x 131072 tokens 184 us.)  A page is found
 // through the range's page list in shared memory.  Every bit pattern decodes to something finite, so what lies
 // behind a row or a sequence needs no clearing: its scores are masked and its weights zero.
@@ -57,18 +58,18 @@ template <int MODE_, int CPL_, int NG_, int W_, bool EX_>
 struct PA {
     static constexpr int MODE = MODE_, CPL = CPL_, NG = NG_, W = W_;
     static constexpr bool EX = EX_;
-    static constexpr int CB = MODE == 1 ? 1 : 2;
+    static constexpr bool AFF = MODE == 0 || MODE == 3;     // z by its index
+    static constexpr int CB = MODE & 1 ? 1 : 2;
     static constexpr int CPV = CPL / 2;                     // triplets per lane and token (values) = (x, y) m-tiles
     static constexpr int KW = CPL * CB / 4, VW = (CPV * CB + 3) / 4;
     static constexpr int RP = CPL * 4 * CB;                 // bytes of a code row in the ring, at most
-    static constexpr int SLOT = 2 * 16 * RP;                // a granule: 16 rows of K, then of V
-    static constexpr int SLOTS = 2 * NG;                    // per warp: two stages
-    static constexpr int UPPER = MODE != 1 && CPL == 8 ? 3 : SLOTS;   // slots above the tables, the others below
+    static constexpr int SLOT = NG * 16 * RP;               // a granule's rows of K, or of V
+    static constexpr int UPPER = CB == 2 && CPL == 8 ? 3 : 4;   // slots (K, V of two stages) above the tables
     static constexpr int CHUNK = 512;                        // pages of the list held at a time
     static constexpr int XY_BYTES = MODE == 2 ? 4096 * 8 : 256 * 32 * 8;
-    static constexpr int Z_BYTES = MODE == 0 ? 0 : 256 * 32 * 4;
+    static constexpr int Z_BYTES = AFF ? 0 : 256 * 32 * 4;
     static constexpr int THREADS = W * 32;
-    static constexpr int NBZ = MODE == 0 ? CPL / 4 : CPL / 2;   // z steps of the scores
+    static constexpr int NBZ = AFF ? CPL / 4 : CPL / 2;   // z steps of the scores
     static constexpr int FRAGS = 2 * (CPL + NBZ);           // query operand registers per lane
 };
 
@@ -84,8 +85,8 @@ __host__ __device__ inline PASmem pa_smem(int dim) {
     s.red = s.wl + T::W * kHQ * 4;                          // [32] reduction
     s.bar = (s.red + 32 * 4 + 7) / 8 * 8;                   // [warps][2 stages]
     s.list = s.bar + T::W * 2 * 8;                          // [2][CHUNK] pages: this range's, the next one's
-    s.ring = (s.list + 2 * T::CHUNK * 4 + 127) / 128 * 128; // slots UPPER .. SLOTS - 1
-    s.end = s.ring + (T::SLOTS - T::UPPER) * T::W * T::SLOT;
+    s.ring = (s.list + 2 * T::CHUNK * 4 + 127) / 128 * 128; // slots UPPER .. 3
+    s.end = s.ring + (4 - T::UPPER) * T::W * T::SLOT;
     return s;
 }
 
@@ -131,7 +132,7 @@ struct Lookup { uint32_t xy, z; int zsh; uint32_t zmask, xymask; };
 
 template <class T> __device__ __forceinline__ uint2 look_xy(const Lookup& l, const uint32_t* w, int j) {
     if constexpr (T::MODE == 0) return lds_u32x2m(__byte_perm(w[j >> 1], l.xy, (j & 1) ? 0x7624u : 0x7604u));
-    if constexpr (T::MODE == 1) return lds_u32x2m(__byte_perm(w[j >> 2], l.xy, 0x7604u + ((j & 3) << 4)));
+    if constexpr (T::MODE & 1) return lds_u32x2m(__byte_perm(w[j >> 2], l.xy, 0x7604u + ((j & 3) << 4)));
     const uint32_t x = (j & 1) ? w[j >> 1] >> 13 : w[j >> 1] << 3;
     return lds_u32x2m((x & l.xymask) + l.xy);
 }
@@ -160,7 +161,7 @@ __device__ __forceinline__ int pow2_to(float v, int top, int lim) {
 // operands of every lane, fragment r of lane l at frag[(unit FRAGS + r) 32 + l]: pairs j < CPL of (x, y) of
 // triplet j, then z; head h's power of two and z0 sum q'_z (EX: (z0 + 8 dz) sum q'_z) at head[unit 8 + h], + 4.
 constexpr int kQueryThreads = 512;
-__global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams p, int mode, int cpl, int ex) {
+__global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams p, int affine, int cpl, int ex) {
     extern __shared__ float qsm[];
     cudaTriggerProgrammaticLaunchCompletion();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim, unit = blockIdx.x;
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
         for (int d = lane; d < dim; d += 32) {
             const float v = sQ[warp * dim + d];
             const bool isz = d % 3 == 0;
-            am = fmaxf(am, fabsf(v) * (mode == 0 && isz ? fabsf(dz) : 1.f));
+            am = fmaxf(am, fabsf(v) * (affine && isz ? fabsf(dz) : 1.f));
             if (isz) cz += v;
         }
         #pragma unroll
@@ -228,11 +229,11 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
             const int k = pow2_to(am, 13, 90);
             sk[warp] = k;
             p.head[unit * 8 + warp] = __int_as_float(k);
-            p.head[unit * 8 + 4 + warp] = mode == 0 ? cz * (ex ? fmaf(8.f, dz, z0) : z0) : 0.f;
+            p.head[unit * 8 + 4 + warp] = affine ? cz * (ex ? fmaf(8.f, dz, z0) : z0) : 0.f;
         }
     }
     __syncthreads();
-    const int nxy = 2 * cpl, frags = nxy + (mode == 0 ? cpl / 2 : cpl);
+    const int nxy = 2 * cpl, frags = nxy + (affine ? cpl / 2 : cpl);
     const int g = lane >> 2, c = lane & 3, qh = g & 3;
     const bool lo = g >= 4;
     const float su = pow2(sk[qh]);
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
         uint32_t v;
         if (r < nxy) {
             v = h2_dup_part(qv(k_triplet_of(cpl, c, r >> 1), 1 + (r & 1)), lo);
-        } else if (mode == 0) {                              // two triplets' z, times the bin width
+        } else if (affine) {                              // two triplets' z, times the bin width
             const int j = 2 * (r - nxy);
             v = h2_pair_part(qv(k_triplet_of(cpl, c, j), 0) * dz, qv(k_triplet_of(cpl, c, j + 1), 0) * dz, lo);
         } else {
@@ -251,21 +252,44 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
     }
 }
 
-// MODE 0: the z indexes of a word's two codes, as the subnormals i 2^-24 or (EX: sums of q (i - 8) are several
-// times smaller, and so is what they lose) as i - 8
-template <bool EX> __device__ __forceinline__ uint32_t z_index(uint32_t w) {
-    if constexpr (EX) return zc8(w >> 8);
-    return prmt(w, 0u, 0x4341u);
+// z by index, scores: the indexes of codes 4 j + 2 h, + 1 of a row's words, as the subnormals i 2^-24 or (EX: sums of
+// q (i - 8) are several times smaller, and so is what they lose) as i - 8
+template <class T> __device__ __forceinline__ uint32_t k_index(const Lookup& l, const uint32_t* w, int j, int h) {
+    if constexpr (T::MODE == 0) {
+        if constexpr (T::EX) return zc8(w[2 * j + h] >> 8);
+        return prmt(w[2 * j + h], 0u, 0x4341u);
+    } else {
+        const uint32_t t = prmt((w[j] >> l.zsh) & l.zmask, 0u, h ? 0x4342u : 0x4140u);
+        return T::EX ? zc8(t) : t;
+    }
+}
+// values: i - 8 of triplet i's code for two tokens' words
+template <class T> __device__ __forceinline__ uint32_t v_index(const Lookup& l, const uint32_t* wa, const uint32_t* wb, int i) {
+    if constexpr (T::MODE == 0) return zc8(prmt(wa[i >> 1], wb[i >> 1], (i & 1) ? 0x7733u : 0x5511u));
+    const int x = i & 3;
+    return zc8(prmt((wa[i >> 2] >> l.zsh) & l.zmask, (wb[i >> 2] >> l.zsh) & l.zmask,
+                    (uint32_t)(x | x << 4 | (x + 4) << 8 | (x + 4) << 12)));
 }
 
-// d += a . b; EX: the tile's sum starts from zero and joins d in a rounded fp32 addition (the tensor core
-// truncates what it adds to d)
+// a . b on one tile, its sums started from zero
+__device__ __forceinline__ void mma_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// d (+)= a . b (first: from zero); EX: the tile's sum joins d in a rounded fp32 addition (the tensor core truncates
+// what it adds to d)
 template <bool EX>
 __device__ __forceinline__ void mma_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-    if constexpr (EX) {
-        float t[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816(t, a0, a1, a2, a3, b0, b1);
+                                        uint32_t b1, bool first = false) {
+    if (first) {
+        mma_zero(d, a0, a1, a2, a3, b0, b1);
+    } else if constexpr (EX) {
+        float t[4];
+        mma_zero(t, a0, a1, a2, a3, b0, b1);
         #pragma unroll
         for (int x = 0; x < 4; ++x) d[x] += t[x];
     } else {
@@ -277,6 +301,7 @@ template <class T>
 __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p) {
     extern __shared__ __align__(128) uint8_t pa_raw[];
     constexpr int W = T::W, NG = T::NG, CPL = T::CPL, CPV = T::CPV, MODE = T::MODE, nthr = T::THREADS;
+    constexpr bool AFF = T::AFF;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim;
     cudaTriggerProgrammaticLaunchCompletion();
     const PASmem L = pa_smem<T>(dim);
@@ -307,7 +332,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
 
     // ---- tables: entries to registers, the largest magnitude, then the scaled pairs -----------------
     const int bits_all = p.bits_z + p.bits_flat;
-    const float z0 = __ldg(p.dec_z), dz = __ldg(p.dec_z + 1) - z0;      // MODE 0: z = z0 + i dz
+    const float z0 = __ldg(p.dec_z), dz = __ldg(p.dec_z + 1) - z0;      // AFF: z = z0 + i dz
     constexpr int ENT = MODE == 2 ? 4096 : 256, EPT = (ENT + nthr - 1) / nthr;
     float2 exy[EPT];
     float ez[MODE == 1 ? EPT : 1];
@@ -321,7 +346,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         if (MODE == 1) ez[x] = __ldg(p.dec_z + (code >> p.bits_flat));
         am = fmaxf(am, fmaxf(fabsf(exy[x].x), fabsf(exy[x].y)));
     }
-    if (MODE != 0)
+    if (!AFF)
         for (int i = tid; i < 1 << p.bits_z; i += nthr) am = fmaxf(am, fabsf(__ldg(p.dec_z + i)));
     PagedCursor cur = paged_begin(p);
     if (cur.t >= cur.end) {
@@ -370,90 +395,106 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     lk.xy = MODE == 2 ? tab : tab | ((uint32_t)lane << 3);
     lk.z = MODE == 1 ? (tab + T::XY_BYTES) * 2 + ((uint32_t)lane << 3) : tab + T::XY_BYTES + ((uint32_t)lane << 2);
     lk.zsh = p.bits_flat;
-    lk.zmask = (1u << p.bits_z) - 1u;
+    lk.zmask = ((1u << p.bits_z) - 1u) * (MODE == 3 ? 0x01010101u : 1u);
     lk.xymask = ((1u << bits_all) - 1u) << 3;
 
     const int g = lane >> 2, c = lane & 3, hp = c & 1;
     const int rho = ((g >> 1) ^ (g & 1)) + 4 * (g & 1);
-    const int per = p.pg.ps_log2 - 4;
+    const int psl = p.pg.ps_log2, tokb = (int)p.pg.tok_bs;
     const int pitch = (p.m * T::CB + 15) & ~15;               // bytes of a row in the ring
     const bool whole = p.pg.tok_bs == pitch;                  // a granule's rows are one piece
     // Pages of granules [ga, gb) of an item as id, -1 (masked), or id | sign bit (the sequence's last page)
     PagedItem it{};
     bool first = true;
-    int len = 0, lastp = 0, lbuf = 0;
-    auto list_end = [&](const PagedItem& i, int ga) { return min(i.g1, ((ga >> per) + T::CHUNK) << per); };
+    int lbuf = 0;
+    constexpr int GL = NG == 2 ? 5 : 4;                       // log2 of a granule's tokens (CHUNK is even)
+    auto list_end = [&](const PagedItem& i, int ga) {
+        return (int)min((int64_t)i.g1, ((int64_t)((ga << GL >> psl) + T::CHUNK) << psl) >> GL);
+    };
+    // pages that the item's sequence (or list) has
+    auto page_end = [&](const PagedItem& i, int n) { return p.selected ? p.n_sel : (n + (1 << psl) - 1) >> psl; };
     auto list_load = [&](const PagedItem& i, int ga, int* list) {
-        const int n = clamp_len(p.pg, __ldg(p.seq_lens + i.b)), last = (n - 1) >> p.pg.ps_log2;
-        const int j0 = ga >> per, j1 = (list_end(i, ga) - 1) >> per;
+        const int n = clamp_len(p.pg, __ldg(p.seq_lens + i.b)), last = (n - 1) >> psl;
+        const int j0 = ga << GL >> psl, j1 = ((list_end(i, ga) << GL) - 1) >> psl, je = page_end(i, n);
         for (int j = j0 + tid; j <= j1; j += nthr) {
-            const Granule gr = granule_at(p, i.b, i.hk, j << per);
-            const int lp = p.selected ? gr.tok >> p.pg.ps_log2 : j;
-            list[j - j0] = gr.page < 0 ? -1 : lp == last ? gr.page | (int)0x80000000 : gr.page;
+            const RangePage r = j < je ? range_page(p, i.b, i.hk, j) : RangePage{-1, -1};
+            list[j - j0] = r.page < 0 ? -1 : r.logical == last ? r.page | (int)0x80000000 : r.page;
         }
     };
-    int gi = 0, ga = 0, gb = 0;
-    // tokens of granule x that count, and its byte offset
-    auto locate = [&](int x, int64_t& o) -> int {
-        o = 0;
-        if (x >= gb) return 0;
-        const int e = sList[lbuf * T::CHUNK + (x >> per) - (ga >> per)];
-        if (e == -1) return 0;
-        const int slot = (x & ((1 << per) - 1)) << 4;
-        o = slot_offset(p.pg, e & 0x7fffffff, it.hk, slot);
-        return e < 0 ? max(0, min(16, len - (lastp << p.pg.ps_log2) - slot)) : 16;
-    };
+    int gi = 0, ga = 0, gb = 0, lastn = 0;
+    const uint8_t *kpool = nullptr, *vpool = nullptr;        // the item's KV head of page 0
     // The warp's slots of the stage in turn, and those of both added up: the other stage's are sum - mine.
-    static_assert(T::SLOTS - T::UPPER <= 1, "only the last slot may lie below the tables");
-    uint32_t slot[NG], both[NG];
-    #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        slot[i] = upper + (uint32_t)(i * W + warp) * T::SLOT;
-        both[i] = slot[i] + (NG + i < T::UPPER ? upper + (uint32_t)((NG + i) * W + warp) * T::SLOT
-                                               : base + (uint32_t)L.ring + (uint32_t)warp * T::SLOT);
-    }
+    auto slot_at = [&](int x) {
+        return x < T::UPPER ? upper + (uint32_t)(x * W + warp) * T::SLOT : base + (uint32_t)L.ring + (uint32_t)warp * T::SLOT;
+    };
+    uint32_t sk = slot_at(0), sv = slot_at(1);
+    const uint32_t bothk = sk + slot_at(2), bothv = sv + slot_at(3);
     int stage = 0;
     uint32_t phase = 0;                                      // parities of the stages' next waits, one bit each
     bool ok = true;                                          // no wait ran out
-    const int gpair = min(lane >> 1, NG - 1), kv = lane & 1; // lanes 2 i + {0: K, 1: V} ask for granule i
-    uint32_t my_slot = slot[0], my_both = both[0];
-    if (NG > 1 && gpair == 1) { my_slot = slot[NG - 1]; my_both = both[NG - 1]; }
-    my_slot += kv * 16 * T::RP;
-    my_both += 2 * kv * 16 * T::RP;
-    const uint8_t* const my_pool = kv ? p.pg.v : p.pg.k;
-    // Ask for granules x, x + W, ... into the stage in turn (other: into the other one), whose last reads are done;
-    // tokens that count in each, 8 bits apiece.
+    // Ask for granule x into the stage in turn (other: into the other one), whose last reads are done; tokens that
+    // count in each of its sixteens, 8 bits apiece.
     auto ask = [&](int x, bool other) -> int {
-        int64_t o = 0;
-        const int n = lane < 2 * NG && ok ? locate(x + gpair * W, o) : 0;
-        const unsigned have = __ballot_sync(0xffffffffu, n > 0);
+        if (x >= gb || !ok) return 0;
+        int n[NG], cnt = 0, have = 0;
+        int64_t o[NG];
+        #pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int t = (x << GL) + 16 * i, slot = t & ((1 << psl) - 1);
+            const int e = sList[lbuf * T::CHUNK + (t >> psl) - (ga << GL >> psl)];
+            n[i] = e == -1 ? 0 : e < 0 ? max(0, min(16, lastn - slot)) : 16;
+            o[i] = (int64_t)(e & 0x7fffffff) * (int)p.pg.page_bs + slot * tokb;
+            cnt |= n[i] << (8 * i);
+            have += n[i] > 0;
+        }
         if (have == 0) return 0;
         uint64_t* b = &bar[other ? stage ^ 1 : stage];
-        if (lane == 0) mbar_arrive_expect_tx(b, (uint32_t)(__popc(have) * 16 * pitch));
-        __syncwarp();
-        if (n > 0) {
-            const uint32_t dst = other ? my_both - my_slot : my_slot;
-            if (whole) {
-                bulk_g2s_at(dst, my_pool + o, (uint32_t)(16 * pitch), b);
-            } else {                                         // strided rows: one copy each
-                for (int r = 0; r < 16; ++r) bulk_g2s_at(dst + r * pitch, my_pool + o + r * p.pg.tok_bs, (uint32_t)pitch, b);
+        const uint32_t dk = other ? bothk - sk : sk, dv = other ? bothv - sv : sv;
+        const uint32_t bytes = (uint32_t)(16 * pitch);
+        if (whole) {
+            if (lane == 0) {
+                mbar_arrive_expect_tx(b, 2 * have * bytes);
+                if (NG == 2 && n[NG - 1] > 0 && o[NG - 1] == o[0] + (int)bytes) {   // 32 rows in one piece
+                    bulk_g2s_at(dk, kpool + o[0], 2 * bytes, b);
+                    bulk_g2s_at(dv, vpool + o[0], 2 * bytes, b);
+                } else {
+                    #pragma unroll
+                    for (int i = 0; i < NG; ++i)
+                        if (n[i] > 0) {
+                            bulk_g2s_at(dk + i * bytes, kpool + o[i], bytes, b);
+                            bulk_g2s_at(dv + i * bytes, vpool + o[i], bytes, b);
+                        }
+                }
+            }
+        } else {                                             // strided rows: one copy each, lane r for row r
+            if (lane == 0) mbar_arrive_expect_tx(b, 2 * have * bytes);
+            __syncwarp();
+            if (lane < 16) {
+                #pragma unroll
+                for (int i = 0; i < NG; ++i)
+                    if (n[i] > 0) {
+                        const int64_t at = o[i] + lane * tokb;
+                        bulk_g2s_at(dk + i * bytes + lane * pitch, kpool + at, (uint32_t)pitch, b);
+                        bulk_g2s_at(dv + i * bytes + lane * pitch, vpool + at, (uint32_t)pitch, b);
+                    }
             }
         }
-        const int n0 = __shfl_sync(0xffffffffu, n, 0);
-        return NG == 1 ? n0 : n0 | __shfl_sync(0xffffffffu, n, 2) << 8;
+        return cnt;
     };
-    // the first granules of the list: warp w takes granules w, w + W, ..., NG an iteration
+    // the first granules of the list: warp w takes granules w, w + W, ...
     int cnt = 0, cnt2 = 0;                                   // of this iteration and the next one
     auto start_list = [&](int from) {
         ga = from;
         gb = list_end(it, ga);
         gi = ga + warp;
         cnt = ask(gi, false);
-        cnt2 = ask(gi + W * NG, true);
+        cnt2 = ask(gi + W, true);
     };
     auto start_item = [&] {
-        len = clamp_len(p.pg, __ldg(p.seq_lens + it.b));
-        lastp = (len - 1) >> p.pg.ps_log2;                   // the page that may be short
+        const int len = clamp_len(p.pg, __ldg(p.seq_lens + it.b));
+        lastn = len - ((len - 1) >> psl << psl);             // tokens of the sequence's last page
+        kpool = p.pg.k + (int64_t)it.hk * p.pg.head_bs;
+        vpool = p.pg.v + (int64_t)it.hk * p.pg.head_bs;
         start_list(it.g0);
     };
     bool more = paged_next(p, cur, it);
@@ -488,7 +529,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
             cz1 = __ldcg(hd + 5);
         }
         const f32x2 uu = f2_pack(us0, us1), czz = f2_pack(cz0, cz1);
-        const float zs = pow2((T::EX ? 0 : 24) + tk);         // MODE 0: z sums onto the (x, y) sums' scale
+        const float zs = pow2((T::EX ? 0 : 24) + tk);         // AFF: z sums onto the (x, y) sums' scale
         float M0 = -INFINITY, M1 = -INFINITY;
         float l0 = 0.f, l1 = 0.f;
         float acc[CPV + CPV / 2][4];
@@ -509,30 +550,28 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                 float S[NG][4];
                 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
-                    float xa[4] = {0.f, 0.f, 0.f, 0.f}, xb[4] = {0.f, 0.f, 0.f, 0.f}, zz[4] = {0.f, 0.f, 0.f, 0.f};
+                    float xa[4], xb[4], zz[4];
                     uint32_t kw[2][T::KW];
-                    load_k<T>(kw[0], slot[i] + rho * pitch, c);
-                    load_k<T>(kw[1], slot[i] + (rho + 8) * pitch, c);
+                    load_k<T>(kw[0], sk + (16 * i + rho) * pitch, c);
+                    load_k<T>(kw[1], sk + (16 * i + rho + 8) * pitch, c);
                     #pragma unroll
                     for (int j = 0; j < CPL; ++j) {
                         const uint2 e0 = look_xy<T>(lk, kw[0], j), e1 = look_xy<T>(lk, kw[1], j);
-                        mma_add<T::EX>((j & 1) ? xb : xa, e0.x, e1.x, e0.y, e1.y, bq[j][0], bq[j][1]);
+                        mma_add<T::EX>((j & 1) ? xb : xa, e0.x, e1.x, e0.y, e1.y, bq[j][0], bq[j][1], j < 2);
                     }
-                    if constexpr (MODE == 0) {
-                        #pragma unroll
-                        for (int j = 0; j < CPL / 4; ++j)
-                            mma_add<T::EX>(zz, z_index<T::EX>(kw[0][2 * j]), z_index<T::EX>(kw[1][2 * j]),
-                                           z_index<T::EX>(kw[0][2 * j + 1]), z_index<T::EX>(kw[1][2 * j + 1]),
-                                           bz[j][0], bz[j][1]);
-                    } else {
-                        #pragma unroll
-                        for (int j = 0; j < CPL / 2; ++j)
+                    #pragma unroll
+                    for (int j = 0; j < T::NBZ; ++j) {
+                        if constexpr (AFF)
+                            mma_add<T::EX>(zz, k_index<T>(lk, kw[0], j, 0), k_index<T>(lk, kw[1], j, 0),
+                                           k_index<T>(lk, kw[0], j, 1), k_index<T>(lk, kw[1], j, 1), bz[j][0], bz[j][1], j == 0);
+                        else
                             mma_add<T::EX>(zz, look_z<T>(lk, kw[0], 2 * j), look_z<T>(lk, kw[1], 2 * j),
-                                     look_z<T>(lk, kw[0], 2 * j + 1), look_z<T>(lk, kw[1], 2 * j + 1), bz[j][0], bz[j][1]);
+                                           look_z<T>(lk, kw[0], 2 * j + 1), look_z<T>(lk, kw[1], 2 * j + 1), bz[j][0], bz[j][1],
+                                           j == 0);
                     }
                     #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        S[i][x] = MODE == 0 ? fmaf(zz[x], zs, xa[x] + xb[x]) : zz[x] + (xa[x] + xb[x]);
+                        S[i][x] = AFF ? fmaf(zz[x], zs, xa[x] + xb[x]) : zz[x] + (xa[x] + xb[x]);
                         S[i][x] += __shfl_xor_sync(0xffffffffu, S[i][x], 2);             // hi + lo columns
                     }
                 }
@@ -544,7 +583,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     const float2 b = f2_unpack(f2_fma(f2_pack(S[i][2], S[i][3]), uu, czz));
                     S[i][0] = a.x; S[i][1] = a.y; S[i][2] = b.x; S[i][3] = b.y;
                     if (p.raw && c < 2) {
-                        float* r = p.raw + (int64_t)it.unit * p.raw_us + ((int64_t)(gi + i * W) * kGranule + rho) * p.raw_h + 2 * hp;
+                        float* r = p.raw + (int64_t)it.unit * p.raw_us + ((int64_t)(gi << GL) + 16 * i + rho) * p.raw_h + 2 * hp;
                         #pragma unroll
                         for (int x = 0; x < 2; ++x)
                             if (2 * hp + x < p.raw_h) {
@@ -598,7 +637,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                 for (int i = 0; i < NG; ++i) {
                     uint32_t vw[4][T::VW];
                     #pragma unroll
-                    for (int t = 0; t < 4; ++t) load_v<T>(vw[t], slot[i] + 16 * T::RP + ((t & 1 ? c ^ 1 : c) + 4 * t) * pitch, g);
+                    for (int t = 0; t < 4; ++t) load_v<T>(vw[t], sv + (16 * i + (t & 1 ? c ^ 1 : c) + 4 * t) * pitch, g);
                     const uint32_t d0 = __byte_perm(pA[i], 0u, 0x1010u), d1 = __byte_perm(pA[i], 0u, 0x3232u);
                     const uint32_t d2 = __byte_perm(pB[i], 0u, 0x1010u), d3 = __byte_perm(pB[i], 0u, 0x3232u);
                     #pragma unroll
@@ -611,11 +650,10 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     #pragma unroll
                     for (int m = 0; m < CPV / 2; ++m) {
                         float (&za)[4] = acc[CPV + m];
-                        if constexpr (MODE == 0) {
-                            float zt[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma16816(zt, zc8(prmt(vw[0][m], vw[1][m], 0x5511u)), zc8(prmt(vw[0][m], vw[1][m], 0x7733u)),
-                                     zc8(prmt(vw[2][m], vw[3][m], 0x5511u)), zc8(prmt(vw[2][m], vw[3][m], 0x7733u)),
-                                     pA[i], pB[i]);
+                        if constexpr (AFF) {
+                            float zt[4];
+                            mma_zero(zt, v_index<T>(lk, vw[0], vw[1], 2 * m), v_index<T>(lk, vw[0], vw[1], 2 * m + 1),
+                                     v_index<T>(lk, vw[2], vw[3], 2 * m), v_index<T>(lk, vw[2], vw[3], 2 * m + 1), pA[i], pB[i]);
                             #pragma unroll
                             for (int x = 0; x < 4; ++x) za[x] += zt[x];
                         } else {
@@ -629,12 +667,11 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                 }
                 __syncwarp();
                 cnt = cnt2;
-                cnt2 = ask(gi + 2 * W * NG, false);
-                gi += W * NG;
+                cnt2 = ask(gi + 2 * W, false);
+                gi += W;
                 stage ^= 1;
-                my_slot = my_both - my_slot;
-                #pragma unroll
-                for (int i = 0; i < NG; ++i) slot[i] = both[i] - slot[i];
+                sk = bothk - sk;
+                sv = bothv - sv;
             }
             if (!ok)                                          // give what was asked for some 20 ms to arrive
                 for (int x = 0; x < 4; ++x) mbar_wait(&bar[x & 1], ((phase >> (x & 1)) ^ (x >> 1)) & 1u, kErrWaitDrain, 1u << 9);
@@ -703,8 +740,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                 o = fmaf(f, sAcc[(w * kHQ + h) * dim + d], o);
                 ls = fmaf(f, lw, ls);
             }
-            // the weights carry 2^12, the tables 2^tk; MODE 0: sum p z = (z0 + 8 dz) l + dz sum p (i - 8)
-            if (MODE == 0 && d % 3 == 0) o = fmaf(dz, o * 0x1p-12f, fmaf(8.f, dz, z0) * (ls * 0x1p-12f));
+            // the weights carry 2^12, the tables 2^tk; AFF: sum p z = (z0 + 8 dz) l + dz sum p (i - 8)
+            if (AFF && d % 3 == 0) o = fmaf(dz, o * 0x1p-12f, fmaf(8.f, dz, z0) * (ls * 0x1p-12f));
             else o *= its;
             row[h * (dim + 2) + 2 + d] = o;
             if (d == 0) {
@@ -717,7 +754,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
 
 constexpr int kJoinThreads = 384;
 constexpr int kMaxGrid = 160;                  // CTAs of the attention launch, at most
-constexpr int kWeighTokens = 2048;             // tokens per CTA of the weight pass
+constexpr int kWeighBatch = 4;
+constexpr int kWeighTokens = kWeighBatch * kJoinThreads;   // tokens per CTA of the weight pass
 
 // CTAs [0, units): one unit each -- join its ranges, normalise, rotate back.  CTAs behind them (with
 // weights): kWeighTokens tokens of one (sequence, KV head) each, p = exp2(score - m) / l summed over its heads.
@@ -813,7 +851,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
     // ---- weights -----------------------------------------------------------------------------
     const int w = blockIdx.x - p.units, chunk = w % chunks, bh = w / chunks, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
     const int L = clamp_len(p.pg, p.seq_lens[b]);
-    const int nv = granules_of(p, b) * kGranule;   // listed or dense tokens
+    const int nv = p.selected ? p.n_sel << p.pg.ps_log2 : L;   // listed or dense tokens
     if (chunk * kWeighTokens >= nv) return;
     float* sOff = jsm;                         // [G] m + log2 l
     for (int h = warp; h < p.G; h += kJoinThreads / 32) {
@@ -838,24 +876,36 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
         if (lane == 0) sOff[h] = mx + log2f(l);
     }
     __syncthreads();
+    // a thread's tokens kWeighBatch at a time: their pages, scores and weights are all on their way before the first
+    // is used
     const int end = min(nv, (chunk + 1) * kWeighTokens);
-    for (int i = chunk * kWeighTokens + tid; i < end; i += kJoinThreads) {
-        int t = i;
-        if (p.selected) {
-            const Granule g = granule_at(p, b, hk, i >> 4);
-            if (g.page < 0) continue;
-            t = g.tok + (i & 15);
-        } else if (t < L && page_of(p.pg, b, t >> p.pg.ps_log2) < 0) {
-            continue;
+    const float* raw = p.raw + ((int64_t)b * p.UH + hk * p.UG) * p.raw_us;
+    const int64_t row = ((int64_t)b * p.pg.Hkv + hk) * p.w_rs;
+    for (int i0 = chunk * kWeighTokens + tid; i0 < end; i0 += kWeighBatch * kJoinThreads) {
+        int t[kWeighBatch];
+        float s[kWeighBatch], w0[kWeighBatch];
+        #pragma unroll
+        for (int u = 0; u < kWeighBatch; ++u) {
+            const int i = i0 + u * kJoinThreads;
+            t[u] = -1;
+            if (i >= end) continue;
+            const RangePage r = range_page(p, b, hk, i >> p.pg.ps_log2);
+            const int tok = (r.logical << p.pg.ps_log2) + (i & ((1 << p.pg.ps_log2) - 1));
+            if (r.page >= 0 && tok < min(L, p.w_slots)) t[u] = tok;
         }
-        if (t >= L || t >= p.w_slots) continue;
-        float sum = 0.f;
-        for (int h = 0; h < p.G; ++h) {
-            const int64_t u = (int64_t)b * p.UH + hk * p.UG + h / kHQ;
-            sum += exp2f(p.raw[u * p.raw_us + (int64_t)i * p.raw_h + h % kHQ] - sOff[h]);
+        #pragma unroll
+        for (int u = 0; u < kWeighBatch; ++u) {
+            s[u] = t[u] >= 0 ? __ldcg(raw + (int64_t)(i0 + u * kJoinThreads) * p.raw_h) : 0.f;
+            w0[u] = t[u] >= 0 ? __ldcg(p.w_in + row + t[u]) : 0.f;
         }
-        const int64_t at = ((int64_t)b * p.pg.Hkv + hk) * p.w_rs + t;
-        p.w_out[at] = p.w_in[at] + sum;
+        #pragma unroll
+        for (int u = 0; u < kWeighBatch; ++u) {
+            if (t[u] < 0) continue;
+            float sum = exp2f(s[u] - sOff[0]);
+            for (int h = 1; h < p.G; ++h)
+                sum += exp2f(__ldcg(raw + h / kHQ * p.raw_us + (int64_t)(i0 + u * kJoinThreads) * p.raw_h + h % kHQ) - sOff[h]);
+            p.w_out[row + t[u]] = w0[u] + sum;
+        }
     }
 }
 
@@ -883,6 +933,7 @@ static PagedParams paged_params(const pkv_codec* c, const pkv_paged_attn_args* a
     p.xy_per_z = c->xy_per_z;
     p.units = pg.B * p.UH;
     p.grid = sms < kMaxGrid ? sms : kMaxGrid;
+    p.gran_log2 = p.m <= 32 ? 5 : 4;           // (launch_paged_mode)
     p.raw_h = p.G < kHQ ? p.G : kHQ;
     // room for every slot that the table (or the list) can name
     p.raw_us = ((int64_t)(a->selected ? a->n_selected : pg.max_pages) << pg.ps_log2) * p.raw_h;
@@ -925,7 +976,7 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
     static std::atomic<int> seen[64];
     const int rc = allow_smem(paged_attn_kernel<T>, smem, seen);
     if (rc) return rc;
-    paged_query_kernel<<<p.units, kQueryThreads, 2 * kHQ * p.dim * 4, st>>>(p, T::MODE, T::CPL, T::EX);
+    paged_query_kernel<<<p.units, kQueryThreads, 2 * kHQ * p.dim * 4, st>>>(p, T::AFF, T::CPL, T::EX);
     if (cudaGetLastError() != cudaSuccess) return PKV_ERR_CUDA;
     return launch_behind(paged_attn_kernel<T>, p.grid, T::THREADS, smem, st, p);
 }
@@ -941,8 +992,9 @@ static int launch_paged_mode(const PagedParams& p, cudaStream_t st) {
 
 template <bool EX>
 static int launch_paged_any(const pkv_codec* c, const PagedParams& p, cudaStream_t st) {
-    if (p.cb == 1) return launch_paged_mode<1, EX>(p, st);
-    if (p.bits_flat == 8 && p.bits_z <= 4 && !p.xy_per_z && (c->flags & PKV_CODEC_Z_UNIFORM)) return launch_paged_mode<0, EX>(p, st);
+    const bool affine = p.bits_z <= 4 && !p.xy_per_z && (c->flags & PKV_CODEC_Z_UNIFORM);
+    if (p.cb == 1) return affine ? launch_paged_mode<3, EX>(p, st) : launch_paged_mode<1, EX>(p, st);
+    if (affine && p.bits_flat == 8) return launch_paged_mode<0, EX>(p, st);
     return launch_paged_mode<2, EX>(p, st);
 }
 
