@@ -986,7 +986,7 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
 template <int MODE, bool EX>
 static int launch_paged_mode(const PagedParams& p, cudaStream_t st) {
     if (p.m <= 32) return launch_paged_as<PA<MODE, 8, 2, 16, EX>>(p, st);
-    if (p.m <= 48) return launch_paged_as<PA<MODE, 12, 1, 16, EX>>(p, st);
+    if (p.m <= 48) return launch_paged_as<PA<MODE, 12, 1, 12, EX>>(p, st);
     return launch_paged_as<PA<MODE, 16, 1, 12, EX>>(p, st);
 }
 
