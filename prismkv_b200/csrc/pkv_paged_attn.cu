@@ -32,9 +32,10 @@ constexpr int kHQ = 4;                         // query heads per unit
 //    one that puts theirs in [2^13, 2^14): pairs of normal fp16 whatever the ranges of the codec and the
 //    data.  Weights are 2^12 exp2(score - running max).
 //  * MODE 0 (two-byte codes, 8 bits of (r, theta)) and 3 (one-byte codes), both with uniform z of up to 4 bits and
-//    one polar grid: z = z0 + i dz enters by its index -- for the
-//    scores as the exact fp16 subnormal i 2^-24 (EX: as i - 8), for the values as the exact i - 8, both affine parts added
-//    outside.  Centred, because an uncentred sum of p i grows with every token and the tiles' sums truncate.
+//    one polar grid: z = zc + (i - c) dz, c the middle bin, enters by its index -- for the scores as the exact fp16
+//    subnormal i 2^-24 (EX: as i - c), for the values as the exact i - c; what does not depend on i is added outside.
+//    Centred, because an uncentred sum of p i grows with every token and the tiles' sums truncate; dz is taken
+//    over all bins, since neighbours' difference carries their rounding.
 // Tables in shared memory: MODE 0, 3 and 1 (one-byte codes, any codec) hold 256 rows of 32 copies, copy `lane`
 // for each lane: the 32 lookups of a warp never collide, and at a 64 KB-aligned address one byte permute of
 // the code word makes a lookup's address (z: and a shift).  MODE 2 (two-byte codes of any codec) holds one copy of all 2^bits
@@ -90,6 +91,13 @@ __host__ __device__ inline PASmem pa_smem(int dim) {
     return s;
 }
 
+// Uniform z bins: the middle bin c, its value and the bin width.
+struct AffineZ { int c; float zc, dz; };
+__device__ __forceinline__ AffineZ affine_z(const PagedParams& p) {
+    const int n = 1 << p.bits_z, c = n >> 1;
+    return {c, __ldg(p.dec_z + c), (__ldg(p.dec_z + n - 1) - __ldg(p.dec_z)) / (float)(n - 1)};
+}
+
 // triplet j of lane c (scores), triplet i of lane g (values)
 __device__ __forceinline__ int k_triplet_of(int cpl, int c, int j) {
     return j < 8 ? 8 * c + j : 32 + (cpl - 8) * c + (j - 8);
@@ -128,7 +136,7 @@ __device__ __forceinline__ void load_v(uint32_t (&w)[T::VW], uint32_t row, int g
 }
 
 // Lookups.  xy_reg / z_reg: the tables' shared addresses with the lane's copy in the low byte.
-struct Lookup { uint32_t xy, z; int zsh; uint32_t zmask, xymask; };
+struct Lookup { uint32_t xy, z; int zsh; uint32_t zmask, xymask, mid; };   // mid: 1024 + c in both fp16 halves
 
 template <class T> __device__ __forceinline__ uint2 look_xy(const Lookup& l, const uint32_t* w, int j) {
     if constexpr (T::MODE == 0) return lds_u32x2m(__byte_perm(w[j >> 1], l.xy, (j & 1) ? 0x7624u : 0x7604u));
@@ -159,7 +167,7 @@ __device__ __forceinline__ int pow2_to(float v, int top, int lim) {
 
 // One CTA per unit: q' = scale log2(e) R q of its four heads (zero for heads past the group), then the score
 // operands of every lane, fragment r of lane l at frag[(unit FRAGS + r) 32 + l]: pairs j < CPL of (x, y) of
-// triplet j, then z; head h's power of two and z0 sum q'_z (EX: (z0 + 8 dz) sum q'_z) at head[unit 8 + h], + 4.
+// triplet j, then z; head h's power of two and the index-free part of its z sum at head[unit 8 + h], + 4.
 constexpr int kQueryThreads = 512;
 __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams p, int affine, int cpl, int ex) {
     extern __shared__ float qsm[];
@@ -169,7 +177,8 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
     float *sRaw = qsm, *sQ = qsm + kHQ * dim;
     __shared__ int sk[kHQ];
     const int b = unit / p.UH, u = unit % p.UH, hk = u / p.UG, hg = u % p.UG;
-    const float z0 = __ldg(p.dec_z), dz = __ldg(p.dec_z + 1) - z0;
+    const AffineZ az = affine_z(p);
+    const float dz = az.dz;
     float rr[6][6];                                          // rows warp, warp + NW, ... of R, six at a time
     auto load_rows = [&](int k0) {
         #pragma unroll
@@ -229,7 +238,7 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
             const int k = pow2_to(am, 13, 90);
             sk[warp] = k;
             p.head[unit * 8 + warp] = __int_as_float(k);
-            p.head[unit * 8 + 4 + warp] = affine ? cz * (ex ? fmaf(8.f, dz, z0) : z0) : 0.f;
+            p.head[unit * 8 + 4 + warp] = affine ? cz * (ex ? az.zc : fmaf(-(float)az.c, dz, az.zc)) : 0.f;
         }
     }
     __syncthreads();
@@ -252,23 +261,29 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
     }
 }
 
+// (i_a - c, i_b - c) as fp16 from the low nibbles of bytes 0 and 2
+__device__ __forceinline__ uint32_t centred(uint32_t t, uint32_t mid) {
+    const uint32_t h = (t & 0x000F000Fu) | 0x64006400u;      // 1024 + i, exact
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&mid));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
 // z by index, scores: the indexes of codes 4 j + 2 h, + 1 of a row's words, as the subnormals i 2^-24 or (EX: sums of
-// q (i - 8) are several times smaller, and so is what they lose) as i - 8
+// q (i - c) are several times smaller, and so is what they lose) as i - c
 template <class T> __device__ __forceinline__ uint32_t k_index(const Lookup& l, const uint32_t* w, int j, int h) {
     if constexpr (T::MODE == 0) {
-        if constexpr (T::EX) return zc8(w[2 * j + h] >> 8);
+        if constexpr (T::EX) return centred(w[2 * j + h] >> 8, l.mid);
         return prmt(w[2 * j + h], 0u, 0x4341u);
     } else {
         const uint32_t t = prmt((w[j] >> l.zsh) & l.zmask, 0u, h ? 0x4342u : 0x4140u);
-        return T::EX ? zc8(t) : t;
+        return T::EX ? centred(t, l.mid) : t;
     }
 }
-// values: i - 8 of triplet i's code for two tokens' words
+// values: i - c of triplet i's code for two tokens' words
 template <class T> __device__ __forceinline__ uint32_t v_index(const Lookup& l, const uint32_t* wa, const uint32_t* wb, int i) {
-    if constexpr (T::MODE == 0) return zc8(prmt(wa[i >> 1], wb[i >> 1], (i & 1) ? 0x7733u : 0x5511u));
+    if constexpr (T::MODE == 0) return centred(prmt(wa[i >> 1], wb[i >> 1], (i & 1) ? 0x7733u : 0x5511u), l.mid);
     const int x = i & 3;
-    return zc8(prmt((wa[i >> 2] >> l.zsh) & l.zmask, (wb[i >> 2] >> l.zsh) & l.zmask,
-                    (uint32_t)(x | x << 4 | (x + 4) << 8 | (x + 4) << 12)));
+    return centred(prmt((wa[i >> 2] >> l.zsh) & l.zmask, (wb[i >> 2] >> l.zsh) & l.zmask,
+                        (uint32_t)(x | x << 4 | (x + 4) << 8 | (x + 4) << 12)), l.mid);
 }
 
 // a . b on one tile, its sums started from zero
@@ -332,7 +347,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
 
     // ---- tables: entries to registers, the largest magnitude, then the scaled pairs -----------------
     const int bits_all = p.bits_z + p.bits_flat;
-    const float z0 = __ldg(p.dec_z), dz = __ldg(p.dec_z + 1) - z0;      // AFF: z = z0 + i dz
+    const AffineZ az = affine_z(p);                           // (AFF)
     constexpr int ENT = MODE == 2 ? 4096 : 256, EPT = (ENT + nthr - 1) / nthr;
     float2 exy[EPT];
     float ez[MODE == 1 ? EPT : 1];
@@ -395,6 +410,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     lk.xy = MODE == 2 ? tab : tab | ((uint32_t)lane << 3);
     lk.z = MODE == 1 ? (tab + T::XY_BYTES) * 2 + ((uint32_t)lane << 3) : tab + T::XY_BYTES + ((uint32_t)lane << 2);
     lk.zsh = p.bits_flat;
+    lk.mid = (0x6400u + (uint32_t)az.c) * 0x10001u;
     lk.zmask = ((1u << p.bits_z) - 1u) * (MODE == 3 ? 0x01010101u : 1u);
     lk.xymask = ((1u << bits_all) - 1u) << 3;
 
@@ -740,8 +756,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                 o = fmaf(f, sAcc[(w * kHQ + h) * dim + d], o);
                 ls = fmaf(f, lw, ls);
             }
-            // the weights carry 2^12, the tables 2^tk; AFF: sum p z = (z0 + 8 dz) l + dz sum p (i - 8)
-            if (AFF && d % 3 == 0) o = fmaf(dz, o * 0x1p-12f, fmaf(8.f, dz, z0) * (ls * 0x1p-12f));
+            // the weights carry 2^12, the tables 2^tk; AFF: sum p z = zc l + dz sum p (i - c)
+            if (AFF && d % 3 == 0) o = fmaf(az.dz, o * 0x1p-12f, az.zc * (ls * 0x1p-12f));
             else o *= its;
             row[h * (dim + 2) + 2 + d] = o;
             if (d == 0) {
