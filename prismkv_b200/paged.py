@@ -64,82 +64,97 @@ class PagedOps:
         return torch.empty((num_pages, kv_heads, 2, self.summary_pitch), dtype=torch.int8, device=self.device)
 
     # ------------------------------------------------------------------
-    # The checks run on every call of a decode step, so they read each property of a tensor once.
+    # The checks run on every call of a decode step, where the GPU may need less than 20 us: each property of a
+    # tensor is read once, and the device is compared as an index (-1 for CPU tensors).
     def _index(self) -> int:
         """The codec's CUDA device index."""
         i = self.device.index
         return torch.cuda.current_device() if i is None else i
 
-    def _on_device(self, t: torch.Tensor, name: str) -> None:
+    def _elsewhere(self, t: torch.Tensor, name: str) -> Exception:
         if not t.is_cuda:
-            raise RuntimeError(f"{name} must be a CUDA tensor")
-        if t.get_device() != self._index():
-            raise ValueError(f"{name} is on {t.device}, the codec on {self.device}")
+            return RuntimeError(f"{name} must be a CUDA tensor")
+        return ValueError(f"{name} is on {t.device}, the codec on {self.device}")
 
-    def _check_ints(self, t: torch.Tensor, name: str, shape) -> torch.Tensor:
-        self._on_device(t, name)
-        if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+    def _check_ints(self, t: torch.Tensor, name: str, shape, dev: int) -> int:
+        """Data pointer of a contiguous int32 tensor of that shape."""
+        if t.get_device() != dev:
+            raise self._elsewhere(t, name)
+        if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}, "
                              f"got {t.dtype} {tuple(t.shape)}")
-        return t
+        return t.data_ptr()
 
-    def _check_table(self, page_table: torch.Tensor):
+    def _check_table(self, page_table: torch.Tensor, dev: int):
         """(data pointer, row stride, batch, max_pages) of a page table."""
-        self._on_device(page_table, "page_table")
-        if page_table.dtype != torch.int32 or page_table.dim() != 2:
-            raise ValueError("page_table must be an int32 (batch, max_pages) tensor with unit inner stride")
-        B, n = page_table.shape
-        stride, inner = page_table.stride()
-        if n > 1 and inner != 1:
-            raise ValueError("page_table must be an int32 (batch, max_pages) tensor with unit inner stride")
-        return page_table.data_ptr(), stride if B > 1 else n, B, n
+        if page_table.get_device() != dev:
+            raise self._elsewhere(page_table, "page_table")
+        shape = page_table.shape
+        if page_table.dtype is torch.int32 and len(shape) == 2:
+            B, n = shape
+            stride, inner = page_table.stride()
+            if n <= 1 or inner == 1:
+                return page_table.data_ptr(), stride if B > 1 else n, B, n
+        raise ValueError("page_table must be an int32 (batch, max_pages) tensor with unit inner stride")
 
-    def _pages(self, k: torch.Tensor, v: Optional[torch.Tensor], page_table: torch.Tensor,
+    def _pages(self, k: torch.Tensor, v: Optional[torch.Tensor], page_table: torch.Tensor, dev: int,
                name: str = "k_pages") -> _lib.PkvPages:
-        self._on_device(k, name)
-        if k.dim() != 4 or k.shape[3] != self.m or k.shape[1] < 1:
-            raise ValueError(f"{name} must be (num_pages, kv_heads, page_size, {self.m}), got {tuple(k.shape)}")
-        P, H, ps, _ = shape = k.shape
-        code_bytes = PAGE_CODE_DTYPES.get(k.dtype)
+        if k.get_device() != dev:
+            raise self._elsewhere(k, name)
+        shape = k.shape
+        if len(shape) != 4 or shape[3] != self.m or shape[1] < 1:
+            raise ValueError(f"{name} must be (num_pages, kv_heads, page_size, {self.m}), got {tuple(shape)}")
+        P, H, ps, _ = shape
+        dtype = k.dtype
+        code_bytes = PAGE_CODE_DTYPES.get(dtype)
         if code_bytes is None:
             raise ValueError("codes must be stored as uint8 or 16-bit integers")
         strides = k.stride()
+        vp = None
         if v is not None:
-            self._on_device(v, "v_pages")
-            if v.shape != shape or v.dtype != k.dtype or v.stride() != strides:
+            if v.get_device() != dev:
+                raise self._elsewhere(v, "v_pages")
+            if v.shape != shape or v.dtype is not dtype or v.stride() != strides:
                 raise ValueError("k_pages and v_pages must have the same shape, dtype and strides")
+            vp = v.data_ptr()
         if strides[3] != 1:
             raise ValueError("codes need unit stride within a row")
         if ps < 16 or ps > 1024 or ps & (ps - 1):
             raise ValueError(f"page_size must be a power of two from 16 to 1024, got {ps}")
-        table, table_stride, B, max_pages = self._check_table(page_table)
+        table, table_stride, B, max_pages = self._check_table(page_table, dev)
         # (a dimension of one element has no stride of its own)
-        return _lib.PkvPages(k.data_ptr(), v.data_ptr() if v is not None else None, code_bytes, P, H, ps,
-                             strides[0] if P > 1 else 0, strides[1] if H > 1 else 0, strides[2], table, table_stride, B,
-                             max_pages)
+        return _lib.PkvPages(k.data_ptr(), vp, code_bytes, P, H, ps, strides[0] if P > 1 else 0,
+                             strides[1] if H > 1 else 0, strides[2], table, table_stride, B, max_pages)
 
-    def _query(self, q: torch.Tensor, kv_heads: int, batch: int) -> torch.Tensor:
-        self._on_device(q, "q")
+    def _query(self, q: torch.Tensor, kv_heads: int, batch: int, dev: int):
+        """(q, its shape, strides and dtype code) with unit inner stride, in a type the kernels read."""
+        if q.get_device() != dev:
+            raise self._elsewhere(q, "q")
         if q.dim() == 4:
             if q.shape[2] != 1:
                 raise ValueError("paged attention takes one query token (Sq == 1)")
             q = q[:, :, 0, :]
-        if q.dim() != 3 or q.shape[0] != batch or q.shape[2] != self.dim:
-            raise ValueError(f"q must be ({batch}, q_heads, {self.dim}), got {tuple(q.shape)}")
-        if q.shape[1] < 1 or q.shape[1] % kv_heads:
-            raise ValueError(f"{q.shape[1]} query heads do not divide among {kv_heads} KV heads")
-        if q.dtype not in _lib.DTYPE_CODES:
-            q = q.float()
-        return q if q.stride(2) == 1 else q.contiguous()
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != batch or shape[2] != self.dim:
+            raise ValueError(f"q must be ({batch}, q_heads, {self.dim}), got {tuple(shape)}")
+        if shape[1] < 1 or shape[1] % kv_heads:
+            raise ValueError(f"{shape[1]} query heads do not divide among {kv_heads} KV heads")
+        code = _lib.DTYPE_CODES.get(q.dtype)
+        if code is None:
+            q, code = q.float(), _lib.PKV_F32
+        strides = q.stride()
+        if strides[2] != 1:
+            q = q.contiguous()
+            strides = q.stride()
+        return q, shape, strides, code
 
-    def _call(self, fn, what: str, *args) -> None:
-        """fn(*args, stream) with the codec's device current; a non-zero status raises."""
-        i = self._index()
-        if torch.cuda.current_device() == i:
-            rc = fn(*args, _lib.raw_stream(i))
+    def _call(self, fn, what: str, dev: int, *args) -> None:
+        """fn(*args, stream) with CUDA device ``dev`` current; a non-zero status raises."""
+        if torch.cuda.current_device() == dev:
+            rc = fn(*args, _lib.raw_stream(dev))
         else:
-            with torch.cuda.device(i):
-                rc = fn(*args, _lib.raw_stream(i))
+            with torch.cuda.device(dev):
+                rc = fn(*args, _lib.raw_stream(dev))
         if rc:
             _lib.check(rc, what)
 
@@ -159,58 +174,63 @@ class PagedOps:
         are not touched; slots must cover every token.  A sequence without
         tokens gives zeros.
         """
-        g = self._pages(k_pages, v_pages, page_table)
-        q = self._query(q, g.kv_heads, g.batch)
-        B, Hq, _ = q.shape
-        self._check_ints(seq_lens, "seq_lens", (B,))
+        dev = self._index()
+        g = self._pages(k_pages, v_pages, page_table, dev)
+        B, kv_heads = g.batch, g.kv_heads
+        q, shape, qs, q_code = self._query(q, kv_heads, B, dev)
+        Hq = shape[1]
+        lens = self._check_ints(seq_lens, "seq_lens", (B,), dev)
         if out is None:
-            if out_dtype not in _lib.DTYPE_CODES:
+            out_code = _lib.DTYPE_CODES.get(out_dtype)
+            if out_code is None:
                 raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
-            out = torch.empty((B, Hq, self.dim), dtype=out_dtype, device=q.device)
+            out = q.new_empty(shape, dtype=out_dtype)
         else:
-            self._on_device(out, "out")
-            if out.shape != (B, Hq, self.dim) or out.dtype not in _lib.DTYPE_CODES or out.stride(2) != 1:
+            if out.get_device() != dev:
+                raise self._elsewhere(out, "out")
+            out_code = _lib.DTYPE_CODES.get(out.dtype)
+            if out.shape != shape or out_code is None or out.stride(2) != 1:
                 raise ValueError(f"out must be a ({B}, {Hq}, {self.dim}) float tensor with unit inner stride")
-        selected = n_selected = 0
+        os = out.stride()
+        selected, n_selected = None, 0
         if pages is not None:
             if pages.dim() != 3:
-                raise ValueError(f"pages must be ({B}, {g.kv_heads}, n), got {tuple(pages.shape)}")
+                raise ValueError(f"pages must be ({B}, {kv_heads}, n), got {tuple(pages.shape)}")
             n_selected = pages.shape[2]
-            self._check_ints(pages, "pages", (B, g.kv_heads, n_selected))
+            selected = self._check_ints(pages, "pages", (B, kv_heads, n_selected), dev)
             if n_selected == 0:
                 raise ValueError("pages lists no page; leave it out to attend to every token")
-            selected = pages.data_ptr()
-        w_in = w_out = slots = 0
+        w_in = w_out = None
+        slots = 0
         if weights_out is not None and weights is None:
             raise ValueError("weights_out needs weights")
         if weights is not None:
             to = weights if weights_out is None else weights_out
             for t, n in ((weights, "weights"), (to, "weights_out")):
-                self._on_device(t, n)
-                if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (B, g.kv_heads) or not t.is_contiguous():
-                    raise ValueError(f"{n} must be a contiguous float32 ({B}, {g.kv_heads}, slots) tensor")
+                if t.get_device() != dev:
+                    raise self._elsewhere(t, n)
+                if t.dtype is not torch.float32 or t.dim() != 3 or t.shape[:2] != (B, kv_heads) or not t.is_contiguous():
+                    raise ValueError(f"{n} must be a contiguous float32 ({B}, {kv_heads}, slots) tensor")
             if to.shape != weights.shape:
                 raise ValueError("weights and weights_out must have the same shape")
             w_in, w_out, slots = weights.data_ptr(), to.data_ptr(), weights.shape[2]
-        qs, os = q.stride(), out.stride()
-        a = _lib.PkvPagedAttnArgs(g, Hq, _lib.DTYPE_CODES[q.dtype], q.data_ptr(), qs[0], qs[1], seq_lens.data_ptr(),
-                                  selected or None, n_selected, self.dim ** -0.5 if scale is None else float(scale),
-                                  out.data_ptr(), _lib.DTYPE_CODES[out.dtype], os[0], os[1], w_in or None, w_out or None,
-                                  slots, slots)
-        args = ctypes.byref(a)
+        args = ctypes.byref(_lib.PkvPagedAttnArgs(
+            g, Hq, q_code, q.data_ptr(), qs[0], qs[1], lens, selected, n_selected,
+            self.dim ** -0.5 if scale is None else float(scale), out.data_ptr(), out_code, os[0], os[1], w_in, w_out, slots,
+            slots))
         lib = _lib.load()
         # the workspace's size follows from the shapes alone
-        key = (B, Hq, g.kv_heads, g.page_size, g.max_pages, n_selected, w_in != 0)
+        key = (B, Hq, kv_heads, g.page_size, g.max_pages, n_selected, w_in is None)
         sizes = self.__dict__.setdefault("_paged_sizes", {})
         need = sizes.get(key)
         if need is None:
-            with torch.cuda.device(self._index()):
+            with torch.cuda.device(dev):
                 need = max(int(lib.pkv_paged_attn_workspace_size(self._struct_ref(), args)), 256)
             if len(sizes) > 256:
                 sizes.clear()
             sizes[key] = need
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        self._call(lib.pkv_paged_attn, "pkv_paged_attn", self._struct_ref(), args, ws.data_ptr(), need)
+        ws = q.new_empty(need, dtype=torch.uint8)
+        self._call(lib.pkv_paged_attn, "pkv_paged_attn", dev, self._struct_ref(), args, ws.data_ptr(), need)
         return out
 
     def _struct_ref(self):
@@ -220,17 +240,18 @@ class PagedOps:
     def store_pages(self, codes: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor,
                     counts: Optional[torch.Tensor] = None) -> None:
         """Copy codes (B, Hkv, n, m) into slots start[b] .. of one pool; counts[b] < n leaves padded rows out."""
-        g = self._pages(pages, None, page_table, "pages")
-        self._on_device(codes, "codes")
+        dev = self._index()
+        g = self._pages(pages, None, page_table, dev, "pages")
+        if codes.get_device() != dev:
+            raise self._elsewhere(codes, "codes")
         if codes.dim() != 4 or codes.dtype != pages.dtype or (codes.shape[0], codes.shape[1], codes.shape[3]) != (
                 g.batch, g.kv_heads, self.m):
             raise ValueError(f"codes must be ({g.batch}, {g.kv_heads}, n, {self.m}) of the pool's dtype")
         codes = codes.contiguous()
-        self._check_ints(start, "start", (g.batch,))
-        if counts is not None:
-            self._check_ints(counts, "counts", (g.batch,))
-        self._call(_lib.load().pkv_pages_store, "pkv_pages_store", ctypes.byref(g), self.m, pages.data_ptr(),
-                   codes.data_ptr(), codes.shape[2], start.data_ptr(), counts.data_ptr() if counts is not None else None)
+        first = self._check_ints(start, "start", (g.batch,), dev)
+        taken = None if counts is None else self._check_ints(counts, "counts", (g.batch,), dev)
+        self._call(_lib.load().pkv_pages_store, "pkv_pages_store", dev, ctypes.byref(g), self.m, pages.data_ptr(),
+                   codes.data_ptr(), codes.shape[2], first, taken)
 
     def _grid(self):
         """Device tables of the summaries' grid, built on first use."""
@@ -242,11 +263,14 @@ class PagedOps:
             self._grid_z = torch.from_numpy(z).to(self.device)
         return self._grid_z, self._grid_xy
 
-    def _check_summaries(self, t: torch.Tensor, g: _lib.PkvPages) -> None:
-        self._on_device(t, "summaries")
-        want = (g.kv_heads, 2, self.summary_pitch)
-        if t.dtype != torch.int8 or t.dim() != 4 or tuple(t.shape[1:]) != want or not t.is_contiguous():
-            raise ValueError(f"summaries must be a contiguous int8 (num_pages, {', '.join(map(str, want))}) tensor")
+    def _check_summaries(self, t: torch.Tensor, g: _lib.PkvPages, dev: int) -> int:
+        """Data pointer of the pool's summaries."""
+        if t.get_device() != dev:
+            raise self._elsewhere(t, "summaries")
+        want = (g.num_pages, g.kv_heads, 2, self.summary_pitch)
+        if t.dtype is not torch.int8 or t.shape != want or not t.is_contiguous():
+            raise ValueError(f"summaries must be a contiguous int8 {want} tensor, got {t.dtype} {tuple(t.shape)}")
+        return t.data_ptr()
 
     def summarize_pages(self, k_pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
                         summaries: torch.Tensor, start: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -258,17 +282,14 @@ class PagedOps:
         the codec's largest decoded magnitude; values within 1/256 of a step of
         a whole number count as it.
         """
-        g = self._pages(k_pages, None, page_table)
-        self._check_ints(seq_lens, "seq_lens", (g.batch,))
-        self._check_summaries(summaries, g)
-        if summaries.shape[0] != g.num_pages:
-            raise ValueError(f"summaries hold {summaries.shape[0]} pages, the pool {g.num_pages}")
-        if start is not None:
-            self._check_ints(start, "start", (g.batch,))
+        dev = self._index()
+        g = self._pages(k_pages, None, page_table, dev)
+        lens = self._check_ints(seq_lens, "seq_lens", (g.batch,), dev)
+        to = self._check_summaries(summaries, g, dev)
+        first = None if start is None else self._check_ints(start, "start", (g.batch,), dev)
         gz, gxy = self._grid()
-        self._call(_lib.load().pkv_pages_summarize, "pkv_pages_summarize", self._struct_ref(), ctypes.byref(g),
-                   seq_lens.data_ptr(), start.data_ptr() if start is not None else None, gz.data_ptr(), gxy.data_ptr(),
-                   summaries.data_ptr())
+        self._call(_lib.load().pkv_pages_summarize, "pkv_pages_summarize", dev, self._struct_ref(), ctypes.byref(g), lens,
+                   first, gz.data_ptr(), gxy.data_ptr(), to)
         return summaries
 
     def select_pages(self, q: torch.Tensor, summaries: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -288,19 +309,20 @@ class PagedOps:
             raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
         if top < 1 or sinks < 0 or recent < 0 or sinks + recent > top:
             raise ValueError(f"need 0 <= sinks + recent <= top and top >= 1, got {sinks}, {recent}, {top}")
-        table, table_stride, B, max_pages = self._check_table(page_table)
+        dev = self._index()
+        table, table_stride, B, max_pages = self._check_table(page_table, dev)
         g = _lib.PkvPages(None, None, 1, summaries.shape[0], summaries.shape[1], page_size, 0, 0,
                           -(-self.m // ROW_BYTES) * ROW_BYTES, table, table_stride, B, max_pages)
-        self._check_summaries(summaries, g)
-        q = self._query(q, g.kv_heads, g.batch)
-        self._check_ints(seq_lens, "seq_lens", (g.batch,))
+        sums = self._check_summaries(summaries, g, dev)
+        q, shape, qs, q_code = self._query(q, g.kv_heads, B, dev)
+        lens = self._check_ints(seq_lens, "seq_lens", (B,), dev)
         if out is None:
-            out = torch.empty((g.batch, g.kv_heads, top), dtype=torch.int32, device=q.device)
-        self._check_ints(out, "out", (g.batch, g.kv_heads, top))
-        qs = q.stride()
-        self._call(_lib.load().pkv_pages_select, "pkv_pages_select", self._struct_ref(), ctypes.byref(g), q.data_ptr(),
-                   _lib.DTYPE_CODES[q.dtype], q.shape[1], qs[0], qs[1], seq_lens.data_ptr(), summaries.data_ptr(), top,
-                   sinks, recent, out.data_ptr())
+            out = q.new_empty((B, g.kv_heads, top), dtype=torch.int32)
+            to = out.data_ptr()
+        else:
+            to = self._check_ints(out, "out", (B, g.kv_heads, top), dev)
+        self._call(_lib.load().pkv_pages_select, "pkv_pages_select", dev, self._struct_ref(), ctypes.byref(g), q.data_ptr(),
+                   q_code, shape[1], qs[0], qs[1], lens, sums, top, sinks, recent, to)
         return out
 
     # ------------------------------------------------------------------
@@ -312,17 +334,19 @@ class PagedOps:
         ``sinks``, the last ``recent``, then the largest (ties: the lower slot;
         NaN last), ascending; -1 and 0 behind the last.
         """
-        self._on_device(weights, "weights")
-        if weights.dim() != 3 or weights.dtype != torch.float32 or not weights.is_contiguous():
+        dev = self._index()
+        if weights.get_device() != dev:
+            raise self._elsewhere(weights, "weights")
+        if weights.dim() != 3 or weights.dtype is not torch.float32 or not weights.is_contiguous():
             raise ValueError("weights must be a contiguous float32 (batch, kv_heads, slots) tensor")
         if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
             raise ValueError(f"need 0 <= sinks + recent <= keep and keep >= 1, got {sinks}, {recent}, {keep}")
         B, H, T = weights.shape
-        self._check_ints(seq_lens, "seq_lens", (B,))
-        kept = torch.empty((B, H, keep), dtype=torch.int32, device=weights.device)
-        kw = torch.empty((B, H, keep), dtype=torch.float32, device=weights.device)
-        self._call(_lib.load().pkv_tokens_select, "pkv_tokens_select", weights.data_ptr(), B, H, T, T, seq_lens.data_ptr(),
-                   keep, sinks, recent, kept.data_ptr(), kw.data_ptr())
+        lens = self._check_ints(seq_lens, "seq_lens", (B,), dev)
+        kept = weights.new_empty((B, H, keep), dtype=torch.int32)
+        kw = weights.new_empty((B, H, keep))
+        self._call(_lib.load().pkv_tokens_select, "pkv_tokens_select", dev, weights.data_ptr(), B, H, T, T, lens, keep,
+                   sinks, recent, kept.data_ptr(), kw.data_ptr())
         return kept, kw
 
     def gather_tokens(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, kept: torch.Tensor,
@@ -332,15 +356,16 @@ class PagedOps:
         The destination pages may lie in the same pool but must not be among the
         pages that are read.
         """
-        src = self._pages(k_pages, v_pages, page_table)
-        dst = self._pages(k_out, v_out, out_table, "k_out")
-        if k_out.dtype != k_pages.dtype or dst.batch != src.batch or dst.kv_heads != src.kv_heads:
+        dev = self._index()
+        src = self._pages(k_pages, v_pages, page_table, dev)
+        dst = self._pages(k_out, v_out, out_table, dev, "k_out")
+        if k_out.dtype is not k_pages.dtype or dst.batch != src.batch or dst.kv_heads != src.kv_heads:
             raise ValueError("source and destination must agree in dtype, batch and KV heads")
         if kept.dim() != 3:
             raise ValueError(f"kept must be ({src.batch}, {src.kv_heads}, keep), got {tuple(kept.shape)}")
         keep = kept.shape[2]
-        self._check_ints(kept, "kept", (src.batch, src.kv_heads, keep))
+        slots = self._check_ints(kept, "kept", (src.batch, src.kv_heads, keep), dev)
         if keep > dst.max_pages * dst.page_size:
             raise ValueError(f"{keep} tokens do not fit {dst.max_pages} pages of {dst.page_size}")
-        self._call(_lib.load().pkv_tokens_gather, "pkv_tokens_gather", ctypes.byref(src), self.m, kept.data_ptr(), keep,
-                   ctypes.byref(dst), k_out.data_ptr(), v_out.data_ptr())
+        self._call(_lib.load().pkv_tokens_gather, "pkv_tokens_gather", dev, ctypes.byref(src), self.m, slots, keep,
+                   ctypes.byref(dst), dst.k, dst.v)
