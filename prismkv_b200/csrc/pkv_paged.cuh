@@ -58,6 +58,26 @@ static int allow_smem(K kernel, int bytes, std::atomic<int> (&seen)[64]) {
     return PKV_OK;
 }
 
+// A launch whose CTAs may come up while the launch before it in the stream drains: every kernel started this way
+// waits for the grid dependency before it touches anything but its codec's constant tables.
+template <class... A, class... B>
+static int launch_behind(void (*kernel)(A...), unsigned ctas, int threads, size_t smem, int cluster, cudaStream_t st, B... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+}
+
 // ---- attention ---------------------------------------------------------------------------------
 // A unit is up to HQ query heads of one (sequence, KV head); units are numbered sequence-major.  Its
 // tokens are the sequence's (or the listed pages', in list order) in granules of what a warp takes at a time,

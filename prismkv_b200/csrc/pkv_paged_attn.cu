@@ -171,7 +171,6 @@ __device__ __forceinline__ int pow2_to(float v, int top, int lim) {
 constexpr int kQueryThreads = 512;
 __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams p, int affine, int cpl, int ex) {
     extern __shared__ float qsm[];
-    cudaTriggerProgrammaticLaunchCompletion();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim, unit = blockIdx.x;
     constexpr int NW = kQueryThreads / 32;
     float *sRaw = qsm, *sQ = qsm + kHQ * dim;
@@ -190,6 +189,10 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
             }
     };
     load_rows(warp);
+    // What the call reads is there from here on -- for the attention launch too, which comes up once every CTA of
+    // this one is past this point, and reads pages and lengths before it waits for this one's results.
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
     for (int i = tid; i < kHQ * dim; i += kQueryThreads) {
         const int h = hg * kHQ + i / dim;
         sRaw[i] = h < p.G ? load_any(p.q, p.qdt, b * p.q_bs + (int64_t)(hk * p.G + h) * p.q_hs + i % dim) : 0.f;
@@ -967,22 +970,6 @@ size_t paged_workspace(const pkv_codec* c, const pkv_paged_attn_args* a, Pages p
     return paged_part_bytes(p) + paged_frag_bytes(p) + paged_head_bytes(p) + (a->weights ? (size_t)p.units * p.raw_us * 4 : 0);
 }
 
-// A launch that may start while the one before it in the stream still runs.
-template <class... A, class... B>
-static int launch_behind(void (*kernel)(A...), unsigned ctas, int threads, size_t smem, cudaStream_t st, B... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
-}
-
 template <class T>
 static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
     static_assert(T::FRAGS <= 48, "paged_frag_bytes");
@@ -990,11 +977,12 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
     const uint32_t below = 1024u + (uint32_t)pa_smem<T>(p.dim).end;
     const int smem = (int)(((below + 0xFFFFu) & ~0xFFFFu) - 1024u) + T::XY_BYTES + T::Z_BYTES + T::UPPER * T::W * T::SLOT + 128;
     static std::atomic<int> seen[64];
-    const int rc = allow_smem(paged_attn_kernel<T>, smem, seen);
+    int rc = allow_smem(paged_attn_kernel<T>, smem, seen);
     if (rc) return rc;
-    paged_query_kernel<<<p.units, kQueryThreads, 2 * kHQ * p.dim * 4, st>>>(p, T::AFF, T::CPL, T::EX);
-    if (cudaGetLastError() != cudaSuccess) return PKV_ERR_CUDA;
-    return launch_behind(paged_attn_kernel<T>, p.grid, T::THREADS, smem, st, p);
+    rc = launch_behind(paged_query_kernel, (unsigned)p.units, kQueryThreads, (size_t)2 * kHQ * p.dim * 4, 0, st, p,
+                       (int)T::AFF, T::CPL, (int)T::EX);
+    if (rc) return rc;
+    return launch_behind(paged_attn_kernel<T>, (unsigned)p.grid, T::THREADS, (size_t)smem, 0, st, p);
 }
 
 // fp32 results get the tiles' sums added in rounded fp32 (about an eighth more time); for 16-bit results the
@@ -1027,7 +1015,7 @@ int launch_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg
     const int64_t ctas = p.units + (int64_t)pg.B * pg.Hkv * chunks;
     if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
     const size_t smem = (size_t)(kHQ * p.dim + kHQ * p.grid + kJoinThreads / ((p.dim + 31) / 32 * 32) * kHQ * p.dim) * 4;
-    return launch_behind(paged_join_kernel, (unsigned)ctas, kJoinThreads, smem, st, p, chunks);
+    return launch_behind(paged_join_kernel, (unsigned)ctas, kJoinThreads, smem, 0, st, p, chunks);
 }
 
 }  // namespace pkv

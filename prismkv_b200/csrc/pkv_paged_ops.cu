@@ -39,6 +39,7 @@ __device__ __forceinline__ void store_piece(uint8_t* row, int bytes, int i, uint
 // Rows (b, hk, i) of contiguous codes (any alignment of two bytes) into slots start[b] + i.
 __global__ void pages_store_kernel(Pages g, uint8_t* dst, const uint8_t* codes, int bytes, int n,
                                    const int32_t* start, const int32_t* counts) {
+    cudaGridDependencySynchronize();
     const int64_t rows = (int64_t)g.B * g.Hkv * n;
     const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;   // eight threads a row
     if (row >= rows) return;
@@ -67,6 +68,7 @@ __global__ void __launch_bounds__(256) tokens_gather_kernel(Pages s, Pages d, ui
     const int r = threadIdx.x / pieces, pc = threadIdx.x - r * pieces;
     const int bh = blockIdx.x / chunks, i0 = (blockIdx.x - bh * chunks) * rows * U + r;
     const int b = bh / s.Hkv, hk = bh - b * s.Hkv;
+    cudaGridDependencySynchronize();
     if (r >= rows) return;
     int t[U];
     int64_t so[U], to[U];
@@ -123,6 +125,7 @@ __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
     constexpr int CW = 4 / CB, TPL = 32 / LPT, U = 8;       // codes per word, tokens per load, loads in flight
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int chunk = blockIdx.x % p.chunks, bh = blockIdx.x / p.chunks, b = bh / p.pg.Hkv, hk = bh - b * p.pg.Hkv;
+    cudaGridDependencySynchronize();
     const int L = clamp_len(p.pg, __ldg(p.seq_lens + b)), ps = 1 << p.pg.ps_log2;
     const int start = p.start ? max(__ldg(p.start + b), 0) : 0;
     const int j0 = (start >> p.pg.ps_log2) + chunk * p.chunk;
@@ -442,6 +445,7 @@ __global__ void __launch_bounds__(kPageThreads) pages_select_kernel(SelectParams
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim;
     const int rank = cl.block_rank(), C = cl.num_blocks();
     const int bh = blockIdx.x / C, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
+    cudaGridDependencySynchronize();
     const int L = clamp_len(p.pg, p.seq_lens[b]);
     const int n = (int)(((int64_t)L + (1 << p.pg.ps_log2) - 1) >> p.pg.ps_log2);
     int8_t* qp = reinterpret_cast<int8_t*>(ssm);                       // [G][2][pitch] negative, then positive parts
@@ -602,6 +606,7 @@ __global__ void __launch_bounds__(THREADS) tokens_select_kernel(KeepParams p) {
     __shared__ TopShared<THREADS, DIGIT> top;
     cg::cluster_group cl = cg::this_cluster();
     const int bh = blockIdx.x / cl.num_blocks(), tid = threadIdx.x;
+    cudaGridDependencySynchronize();
     const int n = min(max(p.seq_lens[bh / p.Hkv], 0), p.slots);
     const float* w = p.w + (int64_t)bh * p.w_rs;
     int lo, hi;
@@ -648,18 +653,7 @@ static int launch_cluster(K kernel, const P& p, int64_t rows, int c, int threads
     if (rows * c > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
     const int rc = allow_smem(kernel, (int)smem, seen);
     if (rc) return rc;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(rows * c));
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = c;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+    return launch_behind(kernel, (unsigned)(rows * c), threads, smem, c, st, p);
 }
 
 constexpr int64_t kKeyCap = 46 * 1024;          // keys of a slice in shared memory (184 KB, beside 33 KB of counters)
@@ -707,9 +701,8 @@ template <int CB, int LPT>
 static int launch_summaries(const SummaryParams& p, cudaStream_t st) {
     const int64_t ctas = (int64_t)p.pg.B * p.pg.Hkv * p.chunks;
     if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-    if (p.entries <= 256) pages_summarize_kernel<CB, LPT, true><<<(unsigned)ctas, 256, 0, st>>>(p);
-    else pages_summarize_kernel<CB, LPT, false><<<(unsigned)ctas, 256, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+    if (p.entries <= 256) return launch_behind(pages_summarize_kernel<CB, LPT, true>, (unsigned)ctas, 256, 0, 0, st, p);
+    return launch_behind(pages_summarize_kernel<CB, LPT, false>, (unsigned)ctas, 256, 0, 0, st, p);
 }
 
 int launch_pages_summarize(const pkv_codec* c, Pages pg, int cb, const int32_t* lens, const int32_t* start,
@@ -738,8 +731,7 @@ int launch_pages_store(Pages pg, uint8_t* dst, const uint8_t* codes, int bytes, 
                        const int32_t* counts, cudaStream_t st) {
     const int64_t threads = (int64_t)pg.B * pg.Hkv * n * 8, ctas = (threads + 255) / 256;
     if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-    pages_store_kernel<<<(unsigned)ctas, 256, 0, st>>>(pg, dst, codes, bytes, n, start, counts);
-    return cudaGetLastError() == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+    return launch_behind(pages_store_kernel, (unsigned)ctas, 256, 0, 0, st, pg, dst, codes, bytes, n, start, counts);
 }
 
 int launch_tokens_gather(Pages s, Pages d, uint8_t* dk, uint8_t* dv, int bytes, const int32_t* kept, int keep,
@@ -747,8 +739,7 @@ int launch_tokens_gather(Pages s, Pages d, uint8_t* dk, uint8_t* dv, int bytes, 
     const int rows = 256 / ((bytes + 15) / 16) * kGatherRows, chunks = (keep + rows - 1) / rows;
     const int64_t ctas = (int64_t)s.B * s.Hkv * chunks;
     if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-    tokens_gather_kernel<<<(unsigned)ctas, 256, 0, st>>>(s, d, dk, dv, bytes, kept, keep, chunks);
-    return cudaGetLastError() == cudaSuccess ? PKV_OK : PKV_ERR_CUDA;
+    return launch_behind(tokens_gather_kernel, (unsigned)ctas, 256, 0, 0, st, s, d, dk, dv, bytes, kept, keep, chunks);
 }
 
 }  // namespace pkv
