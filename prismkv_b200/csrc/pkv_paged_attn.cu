@@ -75,7 +75,7 @@ struct PA {
 };
 
 struct PASmem {                                             // offsets below the tables, in bytes
-    int acc, wm, wl, red, bar, list, ring, end;
+    int acc, wm, wl, red, next, bar, list, ring, end;
 };
 template <class T>
 __host__ __device__ inline PASmem pa_smem(int dim) {
@@ -84,7 +84,8 @@ __host__ __device__ inline PASmem pa_smem(int dim) {
     s.wm = s.acc + T::W * kHQ * dim * 4;                    // [warps][4] max
     s.wl = s.wm + T::W * kHQ * 4;                           // [warps][4] sum
     s.red = s.wl + T::W * kHQ * 4;                          // [32] reduction
-    s.bar = (s.red + 32 * 4 + 7) / 8 * 8;                   // [warps][2 stages]
+    s.next = s.red + 32 * 4;                                // the next range
+    s.bar = (s.next + (int)sizeof(PagedItem) + 7) / 8 * 8;                   // [warps][2 stages]
     s.list = s.bar + T::W * 2 * 8;                          // [2][CHUNK] pages: this range's, the next one's
     s.ring = (s.list + 2 * T::CHUNK * 4 + 127) / 128 * 128; // slots UPPER .. 3
     s.end = s.ring + (4 - T::UPPER) * T::W * T::SLOT;
@@ -326,6 +327,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     float *sAcc = reinterpret_cast<float*>(pa_raw + L.acc), *sRed = reinterpret_cast<float*>(pa_raw + L.red);
     float *sWm = reinterpret_cast<float*>(pa_raw + L.wm), *sWl = reinterpret_cast<float*>(pa_raw + L.wl);
     int* sList = reinterpret_cast<int*>(pa_raw + L.list);
+    PagedItem* sNext = reinterpret_cast<PagedItem*>(pa_raw + L.next);
     uint64_t* bar = reinterpret_cast<uint64_t*>(pa_raw + L.bar) + warp * 2;
     // the tables start at the first 64 KB boundary of shared addresses behind the rest
     const uint32_t base = smem_u32(pa_raw);
@@ -424,7 +426,6 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     const bool whole = p.pg.tok_bs == pitch;                  // a granule's rows are one piece
     // Pages of granules [ga, gb) of an item as id, -1 (masked), or id | sign bit (the sequence's last page)
     PagedItem it{};
-    bool first = true;
     int lbuf = 0;
     constexpr int GL = NG == 2 ? 5 : 4;                       // log2 of a granule's tokens (CHUNK is even)
     auto list_end = [&](const PagedItem& i, int ga) {
@@ -516,36 +517,41 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         vpool = p.pg.v + (int64_t)it.hk * p.pg.head_bs;
         start_list(it.g0);
     };
+    uint32_t bq[CPL][2], bz[T::NBZ][2];
+    float us0 = 0.f, us1 = 0.f, cz0 = 0.f, cz1 = 0.f;          // heads 2 hp, 2 hp + 1 of this lane's score columns
+    auto load_query = [&] {
+        const uint32_t* fr = p.frag + (int64_t)it.unit * T::FRAGS * 32 + lane;
+        #pragma unroll
+        for (int j = 0; j < CPL; ++j) {
+            bq[j][0] = __ldcg(fr + 64 * j);
+            bq[j][1] = __ldcg(fr + 64 * j + 32);
+        }
+        #pragma unroll
+        for (int j = 0; j < T::NBZ; ++j) {
+            bz[j][0] = __ldcg(fr + 64 * (CPL + j));
+            bz[j][1] = __ldcg(fr + 64 * (CPL + j) + 32);
+        }
+        const float* hd = p.head + it.unit * 8 + 2 * hp;
+        us0 = pow2(-__float_as_int(__ldcg(hd)) - tk);
+        us1 = pow2(-__float_as_int(__ldcg(hd + 1)) - tk);
+        cz0 = __ldcg(hd + 4);
+        cz1 = __ldcg(hd + 5);
+    };
     bool more = paged_next(p, cur, it);
     if (more) list_load(it, it.g0, sList);
     __syncthreads();
     if (more) start_item();
+    fill_tables();                                            // while the first codes are on their way
+    __syncthreads();
+    cudaGridDependencySynchronize();                          // the queries' fragments
+    if (more) load_query();
     while (more) {
-        uint32_t bq[CPL][2], bz[T::NBZ][2];
-        float us0, us1, cz0, cz1;                              // heads 2 hp, 2 hp + 1 of this lane's score columns
-        if (first) {                                           // while the first codes are on their way
-            fill_tables();
-            __syncthreads();
-            cudaGridDependencySynchronize();                   // the queries' fragments
-            first = false;
-        }
-        {
-            const uint32_t* fr = p.frag + (int64_t)it.unit * T::FRAGS * 32 + lane;
-            #pragma unroll
-            for (int j = 0; j < CPL; ++j) {
-                bq[j][0] = __ldcg(fr + 64 * j);
-                bq[j][1] = __ldcg(fr + 64 * j + 32);
-            }
-            #pragma unroll
-            for (int j = 0; j < T::NBZ; ++j) {
-                bz[j][0] = __ldcg(fr + 64 * (CPL + j));
-                bz[j][1] = __ldcg(fr + 64 * (CPL + j) + 32);
-            }
-            const float* hd = p.head + it.unit * 8 + 2 * hp;
-            us0 = pow2(-__float_as_int(__ldcg(hd)) - tk);
-            us1 = pow2(-__float_as_int(__ldcg(hd + 1)) - tk);
-            cz0 = __ldcg(hd + 4);
-            cz1 = __ldcg(hd + 5);
+        // the next range's page list, while this one's codes are on their way; its item rests in shared memory
+        PagedItem nx = it;
+        const bool next = paged_next(p, cur, nx);
+        if (next) {
+            list_load(nx, nx.g0, sList + (lbuf ^ 1) * T::CHUNK);
+            if (tid == 0) *sNext = nx;
         }
         const f32x2 uu = f2_pack(us0, us1), czz = f2_pack(cz0, cz1);
         const float zs = pow2((T::EX ? 0 : 24) + tk);         // AFF: z sums onto the (x, y) sums' scale
@@ -700,10 +706,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
             __syncthreads();
             start_list(gb);
         }
-        // ---- hi + lo columns, the lanes, the warps; the next range's list and first codes meanwhile ---------
-        PagedItem nx = it;
-        more = paged_next(p, cur, nx);
-        if (more) list_load(nx, nx.g0, sList + (lbuf ^ 1) * T::CHUNK);
+        // ---- hi + lo columns, the lanes, the warps ----------------------------------------------------------
         #pragma unroll
         for (int o = 4; o <= 16; o <<= 1) {
             l0 += __shfl_xor_sync(0xffffffffu, l0, o);
@@ -713,7 +716,15 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         for (int m = 0; m < CPV + CPV / 2; ++m)
             #pragma unroll
             for (int x = 0; x < 4; ++x) acc[m][x] += __shfl_xor_sync(0xffffffffu, acc[m][x], 2);
-        __syncthreads();                                      // the last range's sums are read
+        __syncthreads();                                      // the last range's sums are read, the next one's list is there
+        float* row = p.part + (int64_t)it.row * kHQ * (dim + 2);
+        if (next) {                                           // its first codes and its queries, before the merge
+            it = *sNext;
+            lbuf ^= 1;
+            start_item();
+            load_query();
+        }
+        more = next;
         if (c < 2) {
             float* o0 = sAcc + (warp * kHQ + 2 * c) * dim;     // head 2c; head 2c + 1 at + dim
             #pragma unroll
@@ -742,10 +753,6 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
             }
         }
         __syncthreads();
-        float* row = p.part + (int64_t)it.row * kHQ * (dim + 2);
-        it = nx;
-        lbuf ^= 1;
-        if (more) start_item();
         const float its = pow2(-tk - 12);
         for (int i = tid; i < kHQ * dim; i += nthr) {
             const int h = i / dim, d = i - h * dim;
