@@ -373,13 +373,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         cudaGridDependencySynchronize();
         return;
     }
-    #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, off));
-    if (lane == 0) sRed[warp] = am;
-    __syncthreads();
-    am = 0.f;
-    for (int w = 0; w < W; ++w) am = fmaxf(am, sRed[w]);
-    const int tk = pow2_to(am, 9, 30);                        // the tables' power of two
+    int tk = 0;                                               // the tables' power of two (set below)
     auto fill_tables = [&] {
         const float ts = pow2(tk);
         #pragma unroll
@@ -539,8 +533,14 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     };
     bool more = paged_next(p, cur, it);
     if (more) list_load(it, it.g0, sList);
+    #pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, off));
+    if (lane == 0) sRed[warp] = am;
     __syncthreads();
     if (more) start_item();
+    #pragma unroll
+    for (int w = 0; w < W; ++w) am = fmaxf(am, sRed[w]);
+    tk = pow2_to(am, 9, 30);
     fill_tables();                                            // while the first codes are on their way
     __syncthreads();
     cudaGridDependencySynchronize();                          // the queries' fragments
@@ -721,8 +721,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         if (next) {                                           // its first codes and its queries, before the merge
             it = *sNext;
             lbuf ^= 1;
+            load_query();                                     // (first: the codes' copies fill the memory's queues)
             start_item();
-            load_query();
         }
         more = next;
         if (c < 2) {
