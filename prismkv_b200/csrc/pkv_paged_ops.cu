@@ -263,8 +263,8 @@ __device__ void top_row(TopShared<THREADS, DIGIT>& s, int lo, int hi, int n, int
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const unsigned rank = cl.block_rank(), C = cl.num_blocks();
-    constexpr int BINS = 1 << DIGIT, PER = BINS >= 4 * THREADS ? 4 : 1, PASSES = (BITS + DIGIT - 1) / DIGIT;
-    static_assert(PER == 4 ? BINS == 4 * THREADS : BINS <= THREADS, "bins per thread");
+    constexpr int BINS = 1 << DIGIT, PER = BINS > THREADS ? 2 : 1, PASSES = (BITS + DIGIT - 1) / DIGIT;
+    static_assert(BINS <= 2 * THREADS, "bins per thread");
     uint32_t prefix = 0, need = (uint32_t)min(k, n);        // keys still to take among those with this prefix
     const bool all = n <= k;
     for (int i = tid; i < 2 * BINS; i += THREADS) (&s.hist[0][0])[i] = 0;
@@ -295,9 +295,9 @@ __device__ void top_row(TopShared<THREADS, DIGIT>& s, int lo, int hi, int n, int
                 #pragma unroll 4
                 for (unsigned r = 0; r < C; ++r) {
                     const uint32_t* h = cl.map_shared_rank(&s, r)->hist[pass & 1];
-                    if constexpr (PER == 4) {
-                        const uint4 x = reinterpret_cast<const uint4*>(h)[THREADS - 1 - tid];
-                        v[0] += x.w; v[1] += x.z; v[2] += x.y; v[3] += x.x;
+                    if constexpr (PER == 2) {
+                        const uint2 x = reinterpret_cast<const uint2*>(h)[BINS / 2 - 1 - tid];
+                        v[0] += x.y; v[1] += x.x;
                     } else {
                         v[0] += h[BINS - 1 - tid];
                     }
@@ -363,39 +363,36 @@ __device__ void top_row(TopShared<THREADS, DIGIT>& s, int lo, int hi, int n, int
         pa += t[0];
         pe += t[1];
     }
+    pa += min(pe, need);                                     // places before this part
     const unsigned below = (1u << lane) - 1u;
     for (int i0 = w0; i0 < w1; i0 += 128) {                  // four neighbouring keys a lane
         const int i = i0 + 4 * lane;
-        uint32_t x[4];
-        #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = i + u < w1 ? key(i + u) : 0u;
         uint32_t take = 0, same = 0;                         // keys above the threshold, and equal to it
         #pragma unroll
         for (int u = 0; u < 4; ++u)
             if (i + u < w1) {
-                take |= (uint32_t)(all || x[u] > prefix) << u;
-                same |= (uint32_t)(!all && x[u] == prefix) << u;
+                const uint32_t x = key(i + u);
+                take |= (uint32_t)(all || x > prefix) << u;
+                same |= (uint32_t)(!all && x == prefix) << u;
             }
-        // counts of the lanes below, bit by bit (a count is 0 to 4)
-        const uint32_t ca = __popc(take), ce = __popc(same);
-        const unsigned a0 = __ballot_sync(0xffffffffu, ca & 1), a1 = __ballot_sync(0xffffffffu, ca & 2),
-                       a2 = __ballot_sync(0xffffffffu, ca & 4);
-        uint32_t at = pa + __popc(a0 & below) + 2 * __popc(a1 & below) + 4 * __popc(a2 & below), ea = pe;
-        if (__any_sync(0xffffffffu, ce)) {
+        if (__any_sync(0xffffffffu, same)) {                 // of the equal ones the first `need` of the row
+            const uint32_t ce = __popc(same);
             const unsigned e0 = __ballot_sync(0xffffffffu, ce & 1), e1 = __ballot_sync(0xffffffffu, ce & 2),
                            e2 = __ballot_sync(0xffffffffu, ce & 4);
-            ea = pe + __popc(e0 & below) + 2 * __popc(e1 & below) + 4 * __popc(e2 & below);
+            uint32_t ea = pe + __popc(e0 & below) + 2 * __popc(e1 & below) + 4 * __popc(e2 & below);
             pe += __popc(e0) + 2 * __popc(e1) + 4 * __popc(e2);
+            for (; same; same &= same - 1, ++ea)
+                if (ea < need) take |= same & (0u - same);
         }
+        // places: counts (0 to 4) of the lanes below, bit by bit
+        const uint32_t ca = __popc(take);
+        const unsigned a0 = __ballot_sync(0xffffffffu, ca & 1), a1 = __ballot_sync(0xffffffffu, ca & 2),
+                       a2 = __ballot_sync(0xffffffffu, ca & 4);
+        uint32_t at = pa + __popc(a0 & below) + 2 * __popc(a1 & below) + 4 * __popc(a2 & below);
         pa += __popc(a0) + 2 * __popc(a1) + 4 * __popc(a2);
-        if (take | same) {
-            #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const bool a = take >> u & 1, e = same >> u & 1;
-                if (a || (e && ea < need)) put((int)(at + min(ea, need)), x[u], i + u);
-                at += a;
-                ea += e;
-            }
+        for (; take; take &= take - 1, ++at) {               // (few lanes have more than one)
+            const int k = i + __ffs(take) - 1;
+            put((int)at, key(k), k);
         }
     }
     cl.sync();                                               // no CTA leaves while another reads its counts
@@ -596,7 +593,7 @@ __device__ __forceinline__ float key_weight(uint32_t k) { return __uint_as_float
 
 // One cluster per (sequence, KV head).  The slice's keys lie in shared memory, computed once (a weight is read
 // back from its key); where a slice does not fit they are computed from the weights on every pass.  Two sizes:
-// 1024 threads and digits of 12 bits for long slices (3 passes over the keys), 512 threads and digits of 8 bits
+// 1024 threads and digits of 11 bits for long slices (3 passes over the keys), 512 threads and digits of 8 bits
 // (4 passes, but 256 counters to clear, read and scan) up to kShortSlice keys: 8 rows of 1024 take 8 us, not 14.
 constexpr int kShortSlice = 4096;
 
@@ -656,7 +653,7 @@ static int launch_cluster(K kernel, const P& p, int64_t rows, int c, int threads
     return launch_behind(kernel, (unsigned)(rows * c), threads, smem, c, st, p);
 }
 
-constexpr int64_t kKeyCap = 46 * 1024;          // keys of a slice in shared memory (184 KB, beside 33 KB of counters)
+constexpr int64_t kKeyCap = 46 * 1024;          // keys of a slice in shared memory (184 KB, beside 17 KB of counters)
 
 int launch_tokens_select(const float* w, int B, int Hkv, int slots, int64_t rs, const int32_t* lens, int keep, int sinks,
                          int recent, int32_t* kept, float* kept_w, int sms, cudaStream_t st) {
@@ -668,7 +665,7 @@ int launch_tokens_select(const float* w, int B, int Hkv, int slots, int64_t rs, 
     const size_t smem = p.cached ? (size_t)per * 4 : 0;
     static std::atomic<int> seen_short[64], seen_long[64];
     if (per <= kShortSlice) return launch_cluster(tokens_select_kernel<512, 8>, p, rows, c, 512, smem, st, seen_short);
-    return launch_cluster(tokens_select_kernel<1024, 12>, p, rows, c, 1024, smem, st, seen_long);
+    return launch_cluster(tokens_select_kernel<1024, 11>, p, rows, c, 1024, smem, st, seen_long);
 }
 
 // Shared memory of the selection without its keys; keys of a slice take what is left of 190 KB.
