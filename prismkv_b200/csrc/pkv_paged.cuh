@@ -24,13 +24,18 @@ __device__ __forceinline__ int clamp_len(const Pages& g, int len) {
     return (int)min((int64_t)max(len, 0), cap);
 }
 
+// What a call reads was written by earlier kernels of its stream, whose last one may still run when this one's
+// CTAs come up (launch_behind): such inputs are read by ordinary loads, which stay behind the grid dependency. The
+// read-only path (__ldg), which need not, is for the codec's constant tables.
+template <class T> __device__ __forceinline__ T input(const T* p) { return *p; }
+
 // Physical page of logical page j of sequence b, or -1 (and the error word) when the table names none.
 __device__ __forceinline__ int page_of(const Pages& g, int b, int j) {
     if ((unsigned)j >= (unsigned)g.max_pages) {
         flag_error(kErrPage);
         return -1;
     }
-    const int page = __ldg(g.table + (int64_t)b * g.table_stride + j);
+    const int page = input(g.table + (int64_t)b * g.table_stride + j);
     if ((unsigned)page >= (unsigned)g.num_pages) {
         flag_error(kErrPage);
         return -1;
@@ -109,7 +114,7 @@ struct PagedParams {
 };
 
 __device__ __forceinline__ int granules_of(const PagedParams& p, int b) {
-    const int n = p.selected ? p.n_sel << p.pg.ps_log2 : clamp_len(p.pg, __ldg(p.seq_lens + b));
+    const int n = p.selected ? p.n_sel << p.pg.ps_log2 : clamp_len(p.pg, input(p.seq_lens + b));
     return (n + (1 << p.gran_log2) - 1) >> p.gran_log2;
 }
 
@@ -262,10 +267,10 @@ struct RangePage { int logical, page; };
 __device__ __forceinline__ RangePage range_page(const PagedParams& p, int b, int hk, int j) {
     if (!p.selected) return {j, page_of(p.pg, b, j)};
     const int32_t* s = p.selected + ((int64_t)b * p.pg.Hkv + hk) * p.n_sel + j;
-    const int lp = __ldg(s), before = j > 0 ? __ldg(s - 1) : -1;
+    const int lp = input(s), before = j > 0 ? input(s - 1) : -1;
     if (lp < 0) return {-1, -1};                            // padding
     if ((j > 0 && (before < 0 || before >= lp)) ||          // not ascending, or behind the sequence's end
-        (int64_t)lp << p.pg.ps_log2 >= clamp_len(p.pg, __ldg(p.seq_lens + b))) {
+        (int64_t)lp << p.pg.ps_log2 >= clamp_len(p.pg, input(p.seq_lens + b))) {
         flag_error(kErrPage);
         return {-1, -1};
     }
@@ -279,15 +284,10 @@ __device__ __forceinline__ void bulk_g2s_at(uint32_t dst, const void* src, uint3
         :: "r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
-template <int DT>
-__device__ __forceinline__ float load_as(const void* q, int64_t i) {
-    return Elem<DT>::load(static_cast<const typename Elem<DT>::T*>(q) + i);
-}
-
 __device__ __forceinline__ float load_any(const void* q, int dt, int64_t i) {
-    if (dt == PKV_F32) return load_as<PKV_F32>(q, i);
-    if (dt == PKV_BF16) return load_as<PKV_BF16>(q, i);
-    return load_as<PKV_F16>(q, i);
+    if (dt == PKV_F32) return input(static_cast<const float*>(q) + i);
+    if (dt == PKV_BF16) return __bfloat162float(input(static_cast<const __nv_bfloat16*>(q) + i));
+    return __half2float(input(static_cast<const __half*>(q) + i));
 }
 
 __device__ __forceinline__ void store_any(void* o, int dt, int64_t i, float v) {

@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     // pages that the item's sequence (or list) has
     auto page_end = [&](const PagedItem& i, int n) { return p.selected ? p.n_sel : (n + (1 << psl) - 1) >> psl; };
     auto list_load = [&](const PagedItem& i, int ga, int* list) {
-        const int n = clamp_len(p.pg, __ldg(p.seq_lens + i.b)), last = (n - 1) >> psl;
+        const int n = clamp_len(p.pg, input(p.seq_lens + i.b)), last = (n - 1) >> psl;
         const int j0 = ga << GL >> psl, j1 = ((list_end(i, ga) << GL) - 1) >> psl, je = page_end(i, n);
         for (int j = j0 + tid; j <= j1; j += nthr) {
             const RangePage r = j < je ? range_page(p, i.b, i.hk, j) : RangePage{-1, -1};
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         cnt2 = ask(gi + W, true);
     };
     auto start_item = [&] {
-        const int len = clamp_len(p.pg, __ldg(p.seq_lens + it.b));
+        const int len = clamp_len(p.pg, input(p.seq_lens + it.b));
         lastn = len - ((len - 1) >> psl << psl);             // tokens of the sequence's last page
         kpool = p.pg.k + (int64_t)it.hk * p.pg.head_bs;
         vpool = p.pg.v + (int64_t)it.hk * p.pg.head_bs;
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
     cudaGridDependencySynchronize();
     // ---- weights -----------------------------------------------------------------------------
     const int w = blockIdx.x - p.units, chunk = w % chunks, bh = w / chunks, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
-    const int L = clamp_len(p.pg, p.seq_lens[b]);
+    const int L = clamp_len(p.pg, input(p.seq_lens + b));
     const int nv = p.selected ? p.n_sel << p.pg.ps_log2 : L;   // listed or dense tokens
     if (chunk * kWeighTokens >= nv) return;
     float* sOff = jsm;                         // [G] m + log2 l

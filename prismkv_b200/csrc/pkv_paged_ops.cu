@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) tokens_gather_kernel(Pages s, Pages d, ui
     #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int i = i0 + u * rows;
-        t[u] = i < keep ? __ldg(kept + (int64_t)bh * keep + i) : -1;
+        t[u] = i < keep ? input(kept + (int64_t)bh * keep + i) : -1;
     }
     #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -126,8 +126,8 @@ __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int chunk = blockIdx.x % p.chunks, bh = blockIdx.x / p.chunks, b = bh / p.pg.Hkv, hk = bh - b * p.pg.Hkv;
     cudaGridDependencySynchronize();
-    const int L = clamp_len(p.pg, __ldg(p.seq_lens + b)), ps = 1 << p.pg.ps_log2;
-    const int start = p.start ? max(__ldg(p.start + b), 0) : 0;
+    const int L = clamp_len(p.pg, input(p.seq_lens + b)), ps = 1 << p.pg.ps_log2;
+    const int start = p.start ? max(input(p.start + b), 0) : 0;
     const int j0 = (start >> p.pg.ps_log2) + chunk * p.chunk;
     const int j1 = min(j0 + p.chunk, (int)(((int64_t)L + ps - 1) >> p.pg.ps_log2));
     if (j0 >= j1 || start >= L) return;
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kPageThreads) pages_select_kernel(SelectParams
     const int rank = cl.block_rank(), C = cl.num_blocks();
     const int bh = blockIdx.x / C, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
     cudaGridDependencySynchronize();
-    const int L = clamp_len(p.pg, p.seq_lens[b]);
+    const int L = clamp_len(p.pg, input(p.seq_lens + b));
     const int n = (int)(((int64_t)L + (1 << p.pg.ps_log2) - 1) >> p.pg.ps_log2);
     int8_t* qp = reinterpret_cast<int8_t*>(ssm);                       // [G][2][pitch] negative, then positive parts
     double* sq = reinterpret_cast<double*>(qp + 2 * p.G * p.pitch);    // [G][dim] (pitch: a multiple of 16)
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(THREADS) tokens_select_kernel(KeepParams p) {
     cg::cluster_group cl = cg::this_cluster();
     const int bh = blockIdx.x / cl.num_blocks(), tid = threadIdx.x;
     cudaGridDependencySynchronize();
-    const int n = min(max(p.seq_lens[bh / p.Hkv], 0), p.slots);
+    const int n = min(max(input(p.seq_lens + bh / p.Hkv), 0), p.slots);
     const float* w = p.w + (int64_t)bh * p.w_rs;
     int lo, hi;
     top_slice(n, lo, hi);
@@ -617,14 +617,14 @@ __global__ void __launch_bounds__(THREADS) tokens_select_kernel(KeepParams p) {
     }
     auto put = [&](int at, uint32_t x, int i) {
         kept[at] = i;
-        kw[at] = key_tells(x) ? key_weight(x) : __ldg(w + i);
+        kw[at] = key_tells(x) ? key_weight(x) : input(w + i);
     };
     if (p.cached) {
         constexpr int U = 16;                                // 64 KB of weights in flight per CTA
         for (int i0 = lo + tid; i0 < hi; i0 += U * THREADS) {
             float x[U];
             #pragma unroll
-            for (int u = 0; u < U; ++u) x[u] = i0 + u * THREADS < hi ? __ldg(w + i0 + u * THREADS) : 0.f;
+            for (int u = 0; u < U; ++u) x[u] = i0 + u * THREADS < hi ? input(w + i0 + u * THREADS) : 0.f;
             #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (i0 + u * THREADS < hi) ksm[i0 + u * THREADS - lo] = make(i0 + u * THREADS, x[u]);
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(THREADS) tokens_select_kernel(KeepParams p) {
         __syncthreads();
         top_row<32, THREADS, DIGIT>(top, lo, hi, n, p.keep, [&](int i) { return ksm[i - lo]; }, put);
     } else {
-        top_row<32, THREADS, DIGIT>(top, lo, hi, n, p.keep, [&](int i) { return make(i, __ldg(w + i)); }, put);
+        top_row<32, THREADS, DIGIT>(top, lo, hi, n, p.keep, [&](int i) { return make(i, input(w + i)); }, put);
     }
 }
 

@@ -278,11 +278,12 @@ def test_non_finite_queries_stay_in_their_rows(cuda_ready):
     ref, tol, _, _ = c.reference(q)
     q[0, 1, 5] = float("nan")
     q[1, 6, 0] = float("inf")
-    out = c.codec.paged_attention(q, c.k, c.v, c.table, c.lens)
-    assert torch.isnan(out[0, 1]).all() and torch.isnan(out[1, 6]).all()
-    for b, h in ((0, 1), (1, 6)):
-        out[b, h], ref[b, h] = 0, 0
-    _close(out, ref, tol)
+    for dt in (F32, BF):
+        out = c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, out_dtype=dt)
+        assert torch.isnan(out[0, 1]).all() and torch.isnan(out[1, 6]).all()
+        for b, h in ((0, 1), (1, 6)):
+            out[b, h], ref[b, h] = 0, 0
+        _close(out, ref, tol)
 
 
 def test_shared_prefix_pages(cuda_ready):
@@ -313,6 +314,86 @@ def test_attention_long_pool_offsets(cuda_ready):
     out = codec.paged_attention(query, k, v, table, small.lens)
     del k, v
     _close(out, ref, tol)
+    _no_error()
+
+
+@pytest.mark.parametrize("qdt,odt,ps", [(BF, BF, 16), (F32, F32, 64)])
+def test_attention_long_ranges(cuda_ready, qdt, odt, ps):
+    """Ranges of more pages than a CTA's list holds at a time, cut evenly: most CTAs serve parts of two units."""
+    c = Cache(_quantizer("v1", (3, 3, 2)), [43210], 32, ps, seed=11)
+    q = _query(1, 32, 96, qdt)
+    ref, tol, w, wt = c.reference(q)
+    w_in = torch.zeros(w.shape, device=DEV)
+    _close(c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=w_in, out_dtype=odt), ref, tol)
+    assert ((w_in.double() - w).abs() <= wt + 4 * U * w).all()
+    lists = torch.arange(0, -(-43210 // ps), 1, dtype=torch.int32, device=DEV)
+    lists = lists[lists % 7 != 3].expand(1, 32, -1).contiguous()
+    ref, tol, _, _ = c.reference(q, pages=lists)
+    _close(c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, pages=lists, out_dtype=odt), ref, tol)
+    _no_error()
+
+
+@pytest.mark.parametrize("size", [2.0 ** -20, 3e-3, 1e3, 2.0 ** 20])
+@pytest.mark.parametrize("bits", [(4, 4, 4), (3, 3, 2), (2, 5, 5)])
+def test_attention_other_ranges(cuda_ready, size, bits):
+    """Codecs calibrated to small and large values, queries the other way round: the operands are rescaled."""
+    quant = StackedPlaneQuantizer(96, *bits, seed=42, z_min=-7.0 * size, z_max=9.0 * size, r_max=8.0 * size)
+    c = Cache(quant, [300, 21], 2, 16, seed=2, spread=size)
+    q = _query(2, 8, 96) / size
+    ref, tol, _, _ = c.reference(q)
+    _close(c.codec.paged_attention(q, c.k, c.v, c.table, c.lens), ref, tol)
+    small = q * 2.0 ** -30                                               # scores of almost nothing
+    ref, tol, _, _ = c.reference(small)
+    _close(c.codec.paged_attention(small, c.k, c.v, c.table, c.lens), ref, tol)
+    sums = c.codec.summarize_pages(c.k, c.table, c.lens, c.codec.empty_summaries(c.k.shape[0], 2))
+    got = c.codec.select_pages(q, sums, c.table, c.lens, 16, 5)
+    assert torch.equal(got, _ref_select(c, q, sums, 5, 1, 1))
+
+
+def test_inputs_written_just_before_the_call(cuda_ready):
+    """Every input of every call is rewritten by the kernel right before it (launches may come up while it runs)."""
+    c = Cache(_quantizer(), [900, 700, 64], 2, 16, seed=5)
+    sums = c.codec.summarize_pages(c.k, c.table, c.lens, c.codec.empty_summaries(c.k.shape[0], 2))
+    g = torch.Generator(device=DEV).manual_seed(3)
+    rounds = []
+    for _ in range(20):
+        lens = torch.stack([torch.randint(1, n + 1, (), generator=g, device=DEV) for n in c.lens_host]).to(torch.int32)
+        rounds.append((torch.randn(3, 8, 96, generator=g, device=DEV), lens, torch.rand(3, 2, 960, generator=g, device=DEV)))
+
+    def calls(q, lens, w, settle):
+        wait = torch.cuda.synchronize if settle else (lambda: None)
+        wait()
+        pages = c.codec.select_pages(q, sums, c.table, lens, 16, 9)
+        wait()
+        a = c.codec.paged_attention(q, c.k, c.v, c.table, lens, pages=pages)
+        wait()
+        b = c.codec.paged_attention(q, c.k, c.v, c.table, lens, weights=w)
+        wait()
+        kept, kw = c.codec.select_tokens(w, lens, 50, recent=3)
+        return pages, a, b, w.clone(), kept, kw
+
+    want = [calls(q, lens.clone(), w.clone(), True) for q, lens, w in rounds]
+    bufs = [torch.empty_like(t) for t in rounds[0]]
+    got = []
+    for q, lens, w in rounds:
+        bufs[0].copy_(q * 1.0), torch.add(lens, 0, out=bufs[1]), torch.mul(w, 1.0, out=bufs[2])
+        bufs[0].mul_(1.0)
+        got.append(calls(*bufs, False))
+    torch.cuda.synchronize()
+    for x, y in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(x, y))
+    # the same, captured once and replayed on new contents
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        bufs[0].mul_(1.0)
+        held = calls(*bufs, False)
+    for (q, lens, w), y in zip(rounds, want):
+        for b, t in zip(bufs, (q, lens, w)):
+            b.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, y))
     _no_error()
 
 
