@@ -84,7 +84,8 @@ static int launch_behind(void (*kernel)(A...), unsigned ctas, int threads, size_
 }
 
 // ---- attention ---------------------------------------------------------------------------------
-// A unit is up to HQ query heads of one (sequence, KV head); units are numbered sequence-major.  Its
+// A unit is NB blocks of four query heads of one (sequence, KV head); units are numbered sequence-major, block x of
+// unit u is block u NB + x.  Its
 // tokens are the sequence's (or the listed pages', in list order) in granules of what a warp takes at a time,
 // 2^gran_log2 = 16 or 32.  The granules of all units form one line of T granules, cut among Gd CTAs: the grid, or
 // where that is less one per unit or per 256 tokens, below which a CTA's warps would have little to share.  Two ways to cut:
@@ -98,7 +99,7 @@ constexpr int kUnitShare = 4096;
 
 struct PagedParams {
     Pages pg;
-    int Hq, G, HQ, UG, UH, dim, m, cb, gran_log2;   // UG units per KV head, UH = Hkv * UG per sequence
+    int Hq, G, NB, UG, UH, dim, m, cb, gran_log2;   // NB blocks of four heads to a unit, UG units per KV head, UH = Hkv UG
     const void* q; int qdt; int64_t q_bs, q_hs;
     const int32_t* seq_lens;
     const int32_t* selected; int n_sel;
@@ -107,9 +108,9 @@ struct PagedParams {
     const float* w_in; float* w_out; int64_t w_rs; int w_slots;
     const float *R, *dec_z, *dec_xy;
     int bits_z, bits_flat, xy_per_z;
-    float* part;                               // [grid + units][HQ][dim + 2]: m (log2 units), l, o
+    float* part;                               // [grid + units][NB][4][dim + 2]: m (log2 units), l, o
     uint32_t* frag; float* head;               // query operands, per-head numbers (paged_query_kernel)
-    float* raw; int64_t raw_us; int raw_h;     // scores of every token, [unit][granule * 16][raw_h]
+    float* raw; int64_t raw_us; int raw_h;     // scores of every token, [block][token][raw_h]
     int grid, units;
 };
 

@@ -14,7 +14,7 @@
 
 namespace pkv {
 
-constexpr int kHQ = 4;                         // query heads per unit
+constexpr int kHQ = 4;                         // query heads per block: with their hi and lo parts a tile's eight columns
 
 // ---------------------------------------------------------------------------------------------
 // paged_attn_kernel: both products on register-operand tensor-core tiles (mma.sync m16n8k16), the codes
@@ -55,9 +55,9 @@ constexpr int kHQ = 4;                         // query heads per unit
 // through the range's page list in shared memory.  Every bit pattern decodes to something finite, so what lies
 // behind a row or a sequence needs no clearing: its scores are masked and its weights zero.
 // ---------------------------------------------------------------------------------------------
-template <int MODE_, int CPL_, int NG_, int W_, bool EX_>
+template <int MODE_, int CPL_, int NG_, int W_, int NB_, bool EX_>
 struct PA {
-    static constexpr int MODE = MODE_, CPL = CPL_, NG = NG_, W = W_;
+    static constexpr int MODE = MODE_, CPL = CPL_, NG = NG_, W = W_, NB = NB_, HQ = kHQ * NB;
     static constexpr bool EX = EX_;
     static constexpr bool AFF = MODE == 0 || MODE == 3;     // z by its index
     static constexpr int CB = MODE & 1 ? 1 : 2;
@@ -65,7 +65,7 @@ struct PA {
     static constexpr int KW = CPL * CB / 4, VW = (CPV * CB + 3) / 4;
     static constexpr int RP = CPL * 4 * CB;                 // bytes of a code row in the ring, at most
     static constexpr int SLOT = NG * 16 * RP;               // a granule's rows of K, or of V
-    static constexpr int UPPER = CB == 2 && CPL == 8 ? 3 : 4;   // slots (K, V of two stages) above the tables
+    static constexpr int UPPER = 4 * W * SLOT > 98304 ? 3 : 4;  // slots (K, V of two stages) above the tables
     static constexpr int CHUNK = 512;                        // pages of the list held at a time
     static constexpr int XY_BYTES = MODE == 2 ? 4096 * 8 : 256 * 32 * 8;
     static constexpr int Z_BYTES = AFF ? 0 : 256 * 32 * 4;
@@ -80,10 +80,10 @@ struct PASmem {                                             // offsets below the
 template <class T>
 __host__ __device__ inline PASmem pa_smem(int dim) {
     PASmem s;
-    s.acc = 0;                                              // [warps][4][dim]
-    s.wm = s.acc + T::W * kHQ * dim * 4;                    // [warps][4] max
-    s.wl = s.wm + T::W * kHQ * 4;                           // [warps][4] sum
-    s.red = s.wl + T::W * kHQ * 4;                          // [32] reduction
+    s.acc = 0;                                              // [warps][HQ][dim]
+    s.wm = s.acc + T::W * T::HQ * dim * 4;                  // [warps][HQ] max
+    s.wl = s.wm + T::W * T::HQ * 4;                         // [warps][HQ] sum
+    s.red = s.wl + T::W * T::HQ * 4;                          // [32] reduction
     s.next = s.red + 32 * 4;                                // the next range
     s.bar = (s.next + (int)sizeof(PagedItem) + 7) / 8 * 8;                   // [warps][2 stages]
     s.list = s.bar + T::W * 2 * 8;                          // [2][CHUNK] pages: this range's, the next one's
@@ -166,9 +166,9 @@ __device__ __forceinline__ int pow2_to(float v, int top, int lim) {
     return max(-lim, min(lim, top - e));
 }
 
-// One CTA per unit: q' = scale log2(e) R q of its four heads (zero for heads past the group), then the score
-// operands of every lane, fragment r of lane l at frag[(unit FRAGS + r) 32 + l]: pairs j < CPL of (x, y) of
-// triplet j, then z; head h's power of two and the index-free part of its z sum at head[unit 8 + h], + 4.
+// One CTA per block: q' = scale log2(e) R q of its four heads (zero for heads past the group), then the score
+// operands of every lane, fragment r of lane l at frag[(block FRAGS + r) 32 + l]: pairs j < CPL of (x, y) of
+// triplet j, then z; head h's power of two and the index-free part of its z sum at head[block 8 + h], + 4.
 constexpr int kQueryThreads = 512;
 __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams p, int affine, int cpl, int ex) {
     extern __shared__ float qsm[];
@@ -176,7 +176,8 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
     constexpr int NW = kQueryThreads / 32;
     float *sRaw = qsm, *sQ = qsm + kHQ * dim;
     __shared__ int sk[kHQ];
-    const int b = unit / p.UH, u = unit % p.UH, hk = u / p.UG, hg = u % p.UG;
+    const int per = p.UG * p.NB;                             // blocks per KV head
+    const int b = unit / (p.pg.Hkv * per), u = unit % (p.pg.Hkv * per), hk = u / per, hg = u % per;
     const AffineZ az = affine_z(p);
     const float dz = az.dz;
     float rr[6][6];                                          // rows warp, warp + NW, ... of R, six at a time
@@ -321,6 +322,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     extern __shared__ __align__(128) uint8_t pa_raw[];
     constexpr int W = T::W, NG = T::NG, CPL = T::CPL, CPV = T::CPV, MODE = T::MODE, nthr = T::THREADS;
     constexpr bool AFF = T::AFF;
+    constexpr int NB = T::NB, HQ = T::HQ;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, dim = p.dim;
     cudaTriggerProgrammaticLaunchCompletion();
     const PASmem L = pa_smem<T>(dim);
@@ -511,25 +513,28 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         vpool = p.pg.v + (int64_t)it.hk * p.pg.head_bs;
         start_list(it.g0);
     };
-    uint32_t bq[CPL][2], bz[T::NBZ][2];
-    float us0 = 0.f, us1 = 0.f, cz0 = 0.f, cz1 = 0.f;          // heads 2 hp, 2 hp + 1 of this lane's score columns
+    uint32_t bq[NB][CPL][2], bz[NB][T::NBZ][2];
+    // heads 2 hp, 2 hp + 1 of each block, those of this lane's score columns: scale of the score tile, index-free part
+    f32x2 uu[NB], czz[NB];
     auto load_query = [&] {
-        const uint32_t* fr = p.frag + (int64_t)it.unit * T::FRAGS * 32 + lane;
         #pragma unroll
-        for (int j = 0; j < CPL; ++j) {
-            bq[j][0] = __ldcg(fr + 64 * j);
-            bq[j][1] = __ldcg(fr + 64 * j + 32);
+        for (int x = 0; x < NB; ++x) {
+            const int64_t block = (int64_t)it.unit * NB + x;
+            const uint32_t* fr = p.frag + block * T::FRAGS * 32 + lane;
+            #pragma unroll
+            for (int j = 0; j < CPL; ++j) {
+                bq[x][j][0] = __ldcg(fr + 64 * j);
+                bq[x][j][1] = __ldcg(fr + 64 * j + 32);
+            }
+            #pragma unroll
+            for (int j = 0; j < T::NBZ; ++j) {
+                bz[x][j][0] = __ldcg(fr + 64 * (CPL + j));
+                bz[x][j][1] = __ldcg(fr + 64 * (CPL + j) + 32);
+            }
+            const float* hd = p.head + block * 8 + 2 * hp;
+            uu[x] = f2_pack(pow2(-__float_as_int(__ldcg(hd)) - tk), pow2(-__float_as_int(__ldcg(hd + 1)) - tk));
+            czz[x] = f2_pack(__ldcg(hd + 4), __ldcg(hd + 5));
         }
-        #pragma unroll
-        for (int j = 0; j < T::NBZ; ++j) {
-            bz[j][0] = __ldcg(fr + 64 * (CPL + j));
-            bz[j][1] = __ldcg(fr + 64 * (CPL + j) + 32);
-        }
-        const float* hd = p.head + it.unit * 8 + 2 * hp;
-        us0 = pow2(-__float_as_int(__ldcg(hd)) - tk);
-        us1 = pow2(-__float_as_int(__ldcg(hd + 1)) - tk);
-        cz0 = __ldcg(hd + 4);
-        cz1 = __ldcg(hd + 5);
     };
     bool more = paged_next(p, cur, it);
     if (more) list_load(it, it.g0, sList);
@@ -553,13 +558,16 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
             list_load(nx, nx.g0, sList + (lbuf ^ 1) * T::CHUNK);
             if (tid == 0) *sNext = nx;
         }
-        const f32x2 uu = f2_pack(us0, us1), czz = f2_pack(cz0, cz1);
         const float zs = pow2((T::EX ? 0 : 24) + tk);         // AFF: z sums onto the (x, y) sums' scale
-        float M0 = -INFINITY, M1 = -INFINITY;
-        float l0 = 0.f, l1 = 0.f;
-        float acc[CPV + CPV / 2][4];
+        float M0[NB], M1[NB], l0[NB], l1[NB];
+        float acc[NB][CPV + CPV / 2][4];
         #pragma unroll
-        for (int m = 0; m < CPV + CPV / 2; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+        for (int x = 0; x < NB; ++x) {
+            M0[x] = M1[x] = -INFINITY;
+            l0[x] = l1[x] = 0.f;
+            #pragma unroll
+            for (int m = 0; m < CPV + CPV / 2; ++m) acc[x][m][0] = acc[x][m][1] = acc[x][m][2] = acc[x][m][3] = 0.f;
+        }
         for (;;) {
             #pragma unroll 1
             while (gi < gb) {
@@ -572,90 +580,104 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                 #pragma unroll
                 for (int i = 0; i < NG; ++i) nv[i] = (cnt >> (8 * i)) & 0xff;
                 // ---- scores ------------------------------------------------------------------------
-                float S[NG][4];
+                float S[NB][NG][4];
                 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
-                    float xa[4], xb[4], zz[4];
+                    float xa[NB][4], xb[NB][4], zz[NB][4];
                     uint32_t kw[2][T::KW];
                     load_k<T>(kw[0], sk + (16 * i + rho) * pitch, c);
                     load_k<T>(kw[1], sk + (16 * i + rho + 8) * pitch, c);
                     #pragma unroll
                     for (int j = 0; j < CPL; ++j) {
                         const uint2 e0 = look_xy<T>(lk, kw[0], j), e1 = look_xy<T>(lk, kw[1], j);
-                        mma_add<T::EX>((j & 1) ? xb : xa, e0.x, e1.x, e0.y, e1.y, bq[j][0], bq[j][1], j < 2);
+                        #pragma unroll
+                        for (int x = 0; x < NB; ++x)
+                            mma_add<T::EX>((j & 1) ? xb[x] : xa[x], e0.x, e1.x, e0.y, e1.y, bq[x][j][0], bq[x][j][1], j < 2);
                     }
                     #pragma unroll
                     for (int j = 0; j < T::NBZ; ++j) {
-                        if constexpr (AFF)
-                            mma_add<T::EX>(zz, k_index<T>(lk, kw[0], j, 0), k_index<T>(lk, kw[1], j, 0),
-                                           k_index<T>(lk, kw[0], j, 1), k_index<T>(lk, kw[1], j, 1), bz[j][0], bz[j][1], j == 0);
-                        else
-                            mma_add<T::EX>(zz, look_z<T>(lk, kw[0], 2 * j), look_z<T>(lk, kw[1], 2 * j),
-                                           look_z<T>(lk, kw[0], 2 * j + 1), look_z<T>(lk, kw[1], 2 * j + 1), bz[j][0], bz[j][1],
-                                           j == 0);
-                    }
-                    #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        S[i][x] = AFF ? fmaf(zz[x], zs, xa[x] + xb[x]) : zz[x] + (xa[x] + xb[x]);
-                        S[i][x] += __shfl_xor_sync(0xffffffffu, S[i][x], 2);             // hi + lo columns
-                    }
-                }
-                // ---- log2 scores, kept for the weights; running maximum -------------------------------
-                float mx0 = -INFINITY, mx1 = -INFINITY;
-                #pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    const float2 a = f2_unpack(f2_fma(f2_pack(S[i][0], S[i][1]), uu, czz));
-                    const float2 b = f2_unpack(f2_fma(f2_pack(S[i][2], S[i][3]), uu, czz));
-                    S[i][0] = a.x; S[i][1] = a.y; S[i][2] = b.x; S[i][3] = b.y;
-                    if (p.raw && c < 2) {
-                        float* r = p.raw + (int64_t)it.unit * p.raw_us + ((int64_t)(gi << GL) + 16 * i + rho) * p.raw_h + 2 * hp;
+                        uint32_t z[4];
+                        if constexpr (AFF) {
+                            z[0] = k_index<T>(lk, kw[0], j, 0); z[1] = k_index<T>(lk, kw[1], j, 0);
+                            z[2] = k_index<T>(lk, kw[0], j, 1); z[3] = k_index<T>(lk, kw[1], j, 1);
+                        } else {
+                            z[0] = look_z<T>(lk, kw[0], 2 * j); z[1] = look_z<T>(lk, kw[1], 2 * j);
+                            z[2] = look_z<T>(lk, kw[0], 2 * j + 1); z[3] = look_z<T>(lk, kw[1], 2 * j + 1);
+                        }
                         #pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            if (2 * hp + x < p.raw_h) {
-                                if (rho < nv[i]) r[x] = S[i][x];
-                                if (rho + 8 < nv[i]) r[8 * p.raw_h + x] = S[i][2 + x];
-                            }
+                        for (int x = 0; x < NB; ++x) mma_add<T::EX>(zz[x], z[0], z[1], z[2], z[3], bz[x][j][0], bz[x][j][1], j == 0);
                     }
-                    if (rho >= nv[i]) S[i][0] = S[i][1] = -INFINITY;
-                    if (rho + 8 >= nv[i]) S[i][2] = S[i][3] = -INFINITY;
-                    mx0 = fmaxf(mx0, fmaxf(S[i][0], S[i][2]));
-                    mx1 = fmaxf(mx1, fmaxf(S[i][1], S[i][3]));
-                }
-                if (__any_sync(0xffffffffu, mx0 > M0 || mx1 > M1)) {
                     #pragma unroll
-                    for (int o = 4; o <= 16; o <<= 1) {
-                        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
-                        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
-                    }
-                    mx0 = fmaxf(mx0, M0);
-                    mx1 = fmaxf(mx1, M1);
-                    const float f0 = M0 == -INFINITY ? (l0 == 0.f ? 0.f : l0) : fast_exp2(M0 - mx0);
-                    const float f1 = M1 == -INFINITY ? (l1 == 0.f ? 0.f : l1) : fast_exp2(M1 - mx1);
-                    M0 = mx0;
-                    M1 = mx1;
-                    l0 *= f0;
-                    l1 *= f1;
-                    #pragma unroll
-                    for (int m = 0; m < CPV + CPV / 2; ++m) {
-                        acc[m][0] *= f0; acc[m][1] *= f1; acc[m][2] *= f0; acc[m][3] *= f1;
-                    }
+                    for (int x = 0; x < NB; ++x)
+                        #pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const float t = AFF ? fmaf(zz[x][y], zs, xa[x][y] + xb[x][y]) : zz[x][y] + (xa[x][y] + xb[x][y]);
+                            S[x][i][y] = t + __shfl_xor_sync(0xffffffffu, t, 2);         // hi + lo columns
+                        }
                 }
-                // ---- weights, transposed into B operands ------------------------------------------------
-                // (the 2^12 is put on afterwards: score - max is exact near the maximum, + 12 would round it)
-                const float n0 = M0 == -INFINITY ? 0.f : M0, n1 = M1 == -INFINITY ? 0.f : M1;
-                uint32_t pA[NG], pB[NG];
+                // ---- log2 scores, kept for the weights; running maximum; weights as B operands --------------
+                uint32_t pA[NB][NG], pB[NB][NG];
                 #pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    const float p0 = fast_exp2(S[i][0] - n0) * 4096.f, p1 = fast_exp2(S[i][1] - n1) * 4096.f;
-                    const float p2 = fast_exp2(S[i][2] - n0) * 4096.f, p3 = fast_exp2(S[i][3] - n1) * 4096.f;
-                    l0 += p0 + p2;
-                    l1 += p1 + p3;
-                    const uint32_t hA = f2h2(p0, p1), hB = f2h2(p2, p3);
-                    const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&hA));
-                    const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hB));
-                    const uint32_t lA = f2h2(p0 - fa.x, p1 - fa.y), lB = f2h2(p2 - fb.x, p3 - fb.y);
-                    pA[i] = movmatrix_t(c >= 2 ? lA : hA);     // column g of tokens (c, (c ^ 1) + 4)
-                    pB[i] = movmatrix_t(c >= 2 ? lB : hB);     // column g of the same + 8
+                for (int x = 0; x < NB; ++x) {
+                    float mx0 = -INFINITY, mx1 = -INFINITY;
+                    #pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        float (&s)[4] = S[x][i];
+                        const float2 a = f2_unpack(f2_fma(f2_pack(s[0], s[1]), uu[x], czz[x]));
+                        const float2 b = f2_unpack(f2_fma(f2_pack(s[2], s[3]), uu[x], czz[x]));
+                        s[0] = a.x; s[1] = a.y; s[2] = b.x; s[3] = b.y;
+                        if (p.raw && c < 2) {
+                            float* r = p.raw + ((int64_t)it.unit * NB + x) * p.raw_us +
+                                       ((int64_t)(gi << GL) + 16 * i + rho) * p.raw_h + 2 * hp;
+                            #pragma unroll
+                            for (int y = 0; y < 2; ++y)
+                                if (2 * hp + y < p.raw_h) {
+                                    if (rho < nv[i]) r[y] = s[y];
+                                    if (rho + 8 < nv[i]) r[8 * p.raw_h + y] = s[2 + y];
+                                }
+                        }
+                        if (rho >= nv[i]) s[0] = s[1] = -INFINITY;
+                        if (rho + 8 >= nv[i]) s[2] = s[3] = -INFINITY;
+                        mx0 = fmaxf(mx0, fmaxf(s[0], s[2]));
+                        mx1 = fmaxf(mx1, fmaxf(s[1], s[3]));
+                    }
+                    if (__any_sync(0xffffffffu, mx0 > M0[x] || mx1 > M1[x])) {
+                        #pragma unroll
+                        for (int o = 4; o <= 16; o <<= 1) {
+                            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
+                            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
+                        }
+                        mx0 = fmaxf(mx0, M0[x]);
+                        mx1 = fmaxf(mx1, M1[x]);
+                        // (before the first token the sums are zero, or NaN from a query that is)
+                        const float f0 = M0[x] == -INFINITY ? (l0[x] == 0.f ? 0.f : l0[x]) : fast_exp2(M0[x] - mx0);
+                        const float f1 = M1[x] == -INFINITY ? (l1[x] == 0.f ? 0.f : l1[x]) : fast_exp2(M1[x] - mx1);
+                        M0[x] = mx0;
+                        M1[x] = mx1;
+                        l0[x] *= f0;
+                        l1[x] *= f1;
+                        #pragma unroll
+                        for (int m = 0; m < CPV + CPV / 2; ++m) {
+                            float (&a)[4] = acc[x][m];
+                            a[0] *= f0; a[1] *= f1; a[2] *= f0; a[3] *= f1;
+                        }
+                    }
+                    // (the 2^12 is put on afterwards: score - max is exact near the maximum, + 12 would round it)
+                    const float n0 = M0[x] == -INFINITY ? 0.f : M0[x], n1 = M1[x] == -INFINITY ? 0.f : M1[x];
+                    #pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        const float (&s)[4] = S[x][i];
+                        const float p0 = fast_exp2(s[0] - n0) * 4096.f, p1 = fast_exp2(s[1] - n1) * 4096.f;
+                        const float p2 = fast_exp2(s[2] - n0) * 4096.f, p3 = fast_exp2(s[3] - n1) * 4096.f;
+                        l0[x] += p0 + p2;
+                        l1[x] += p1 + p3;
+                        const uint32_t hA = f2h2(p0, p1), hB = f2h2(p2, p3);
+                        const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&hA));
+                        const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hB));
+                        const uint32_t lA = f2h2(p0 - fa.x, p1 - fa.y), lB = f2h2(p2 - fb.x, p3 - fb.y);
+                        pA[x][i] = movmatrix_t(c >= 2 ? lA : hA);  // column g of tokens (c, (c ^ 1) + 4)
+                        pB[x][i] = movmatrix_t(c >= 2 ? lB : hB);  // column g of the same + 8
+                    }
                 }
                 // ---- values ----------------------------------------------------------------------------
                 #pragma unroll
@@ -663,29 +685,44 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                     uint32_t vw[4][T::VW];
                     #pragma unroll
                     for (int t = 0; t < 4; ++t) load_v<T>(vw[t], sv + (16 * i + (t & 1 ? c ^ 1 : c) + 4 * t) * pitch, g);
-                    const uint32_t d0 = __byte_perm(pA[i], 0u, 0x1010u), d1 = __byte_perm(pA[i], 0u, 0x3232u);
-                    const uint32_t d2 = __byte_perm(pB[i], 0u, 0x1010u), d3 = __byte_perm(pB[i], 0u, 0x3232u);
+                    uint32_t d[NB][4];
+                    #pragma unroll
+                    for (int x = 0; x < NB; ++x) {
+                        d[x][0] = __byte_perm(pA[x][i], 0u, 0x1010u); d[x][1] = __byte_perm(pA[x][i], 0u, 0x3232u);
+                        d[x][2] = __byte_perm(pB[x][i], 0u, 0x1010u); d[x][3] = __byte_perm(pB[x][i], 0u, 0x3232u);
+                    }
                     #pragma unroll
                     for (int m = 0; m < CPV; ++m) {
                         const uint2 x0 = look_xy<T>(lk, vw[0], m), x1 = look_xy<T>(lk, vw[1], m);
                         const uint2 x2 = look_xy<T>(lk, vw[2], m), x3 = look_xy<T>(lk, vw[3], m);
-                        mma_add<T::EX>(acc[m], x0.x, x0.y, x1.x, x1.y, d0, d1);
-                        mma_add<T::EX>(acc[m], x2.x, x2.y, x3.x, x3.y, d2, d3);
+                        #pragma unroll
+                        for (int x = 0; x < NB; ++x) {
+                            mma_add<T::EX>(acc[x][m], x0.x, x0.y, x1.x, x1.y, d[x][0], d[x][1]);
+                            mma_add<T::EX>(acc[x][m], x2.x, x2.y, x3.x, x3.y, d[x][2], d[x][3]);
+                        }
                     }
                     #pragma unroll
                     for (int m = 0; m < CPV / 2; ++m) {
-                        float (&za)[4] = acc[CPV + m];
                         if constexpr (AFF) {
-                            float zt[4];
-                            mma_zero(zt, v_index<T>(lk, vw[0], vw[1], 2 * m), v_index<T>(lk, vw[0], vw[1], 2 * m + 1),
-                                     v_index<T>(lk, vw[2], vw[3], 2 * m), v_index<T>(lk, vw[2], vw[3], 2 * m + 1), pA[i], pB[i]);
+                            const uint32_t z0 = v_index<T>(lk, vw[0], vw[1], 2 * m), z1 = v_index<T>(lk, vw[0], vw[1], 2 * m + 1);
+                            const uint32_t z2 = v_index<T>(lk, vw[2], vw[3], 2 * m), z3 = v_index<T>(lk, vw[2], vw[3], 2 * m + 1);
                             #pragma unroll
-                            for (int x = 0; x < 4; ++x) za[x] += zt[x];
+                            for (int x = 0; x < NB; ++x) {
+                                float zt[4];
+                                mma_zero(zt, z0, z1, z2, z3, pA[x][i], pB[x][i]);
+                                #pragma unroll
+                                for (int y = 0; y < 4; ++y) acc[x][CPV + m][y] += zt[y];
+                            }
                         } else {
-                            mma_add<T::EX>(za, look_z<T>(lk, vw[0], 2 * m), look_z<T>(lk, vw[0], 2 * m + 1),
-                                     look_z<T>(lk, vw[1], 2 * m), look_z<T>(lk, vw[1], 2 * m + 1), d0, d1);
-                            mma_add<T::EX>(za, look_z<T>(lk, vw[2], 2 * m), look_z<T>(lk, vw[2], 2 * m + 1),
-                                     look_z<T>(lk, vw[3], 2 * m), look_z<T>(lk, vw[3], 2 * m + 1), d2, d3);
+                            const uint32_t z0 = look_z<T>(lk, vw[0], 2 * m), z1 = look_z<T>(lk, vw[0], 2 * m + 1);
+                            const uint32_t z2 = look_z<T>(lk, vw[1], 2 * m), z3 = look_z<T>(lk, vw[1], 2 * m + 1);
+                            const uint32_t z4 = look_z<T>(lk, vw[2], 2 * m), z5 = look_z<T>(lk, vw[2], 2 * m + 1);
+                            const uint32_t z6 = look_z<T>(lk, vw[3], 2 * m), z7 = look_z<T>(lk, vw[3], 2 * m + 1);
+                            #pragma unroll
+                            for (int x = 0; x < NB; ++x) {
+                                mma_add<T::EX>(acc[x][CPV + m], z0, z1, z2, z3, d[x][0], d[x][1]);
+                                mma_add<T::EX>(acc[x][CPV + m], z4, z5, z6, z7, d[x][2], d[x][3]);
+                            }
                         }
                     }
                 }
@@ -708,16 +745,19 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         }
         // ---- hi + lo columns, the lanes, the warps ----------------------------------------------------------
         #pragma unroll
-        for (int o = 4; o <= 16; o <<= 1) {
-            l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-        }
-        #pragma unroll
-        for (int m = 0; m < CPV + CPV / 2; ++m)
+        for (int x = 0; x < NB; ++x) {
             #pragma unroll
-            for (int x = 0; x < 4; ++x) acc[m][x] += __shfl_xor_sync(0xffffffffu, acc[m][x], 2);
+            for (int o = 4; o <= 16; o <<= 1) {
+                l0[x] += __shfl_xor_sync(0xffffffffu, l0[x], o);
+                l1[x] += __shfl_xor_sync(0xffffffffu, l1[x], o);
+            }
+            #pragma unroll
+            for (int m = 0; m < CPV + CPV / 2; ++m)
+                #pragma unroll
+                for (int y = 0; y < 4; ++y) acc[x][m][y] += __shfl_xor_sync(0xffffffffu, acc[x][m][y], 2);
+        }
         __syncthreads();                                      // the last range's sums are read, the next one's list is there
-        float* row = p.part + (int64_t)it.row * kHQ * (dim + 2);
+        float* row = p.part + (int64_t)it.row * HQ * (dim + 2);
         if (next) {                                           // its first codes and its queries, before the merge
             it = *sNext;
             lbuf ^= 1;
@@ -726,44 +766,46 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
         }
         more = next;
         if (c < 2) {
-            float* o0 = sAcc + (warp * kHQ + 2 * c) * dim;     // head 2c; head 2c + 1 at + dim
             #pragma unroll
-            for (int m = 0; m < CPV; ++m) {
-                const int t = v_triplet<T>(g, m);
-                if (t < p.m) {
-                    o0[3 * t + 1] = acc[m][0]; o0[dim + 3 * t + 1] = acc[m][1];
-                    o0[3 * t + 2] = acc[m][2]; o0[dim + 3 * t + 2] = acc[m][3];
-                }
-            }
-            #pragma unroll
-            for (int m = 0; m < CPV / 2; ++m)
+            for (int x = 0; x < NB; ++x) {
+                const int h0 = warp * HQ + kHQ * x + 2 * c;    // head 2c of the block; head 2c + 1 at + dim
+                float* o0 = sAcc + h0 * dim;
                 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int t = v_triplet<T>(g, 2 * m + x);
+                for (int m = 0; m < CPV; ++m) {
+                    const int t = v_triplet<T>(g, m);
                     if (t < p.m) {
-                        o0[3 * t] = acc[CPV + m][2 * x];
-                        o0[dim + 3 * t] = acc[CPV + m][2 * x + 1];
+                        o0[3 * t + 1] = acc[x][m][0]; o0[dim + 3 * t + 1] = acc[x][m][1];
+                        o0[3 * t + 2] = acc[x][m][2]; o0[dim + 3 * t + 2] = acc[x][m][3];
                     }
                 }
-            if (g == 0) {
-                sWm[warp * kHQ + 2 * c] = M0;
-                sWm[warp * kHQ + 2 * c + 1] = M1;
-                sWl[warp * kHQ + 2 * c] = l0;
-                sWl[warp * kHQ + 2 * c + 1] = l1;
+                #pragma unroll
+                for (int m = 0; m < CPV / 2; ++m)
+                    #pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const int t = v_triplet<T>(g, 2 * m + y);
+                        if (t < p.m) {
+                            o0[3 * t] = acc[x][CPV + m][2 * y];
+                            o0[dim + 3 * t] = acc[x][CPV + m][2 * y + 1];
+                        }
+                    }
+                if (g == 0) {
+                    sWm[h0] = M0[x]; sWm[h0 + 1] = M1[x];
+                    sWl[h0] = l0[x]; sWl[h0 + 1] = l1[x];
+                }
             }
         }
         __syncthreads();
         const float its = pow2(-tk - 12);
-        for (int i = tid; i < kHQ * dim; i += nthr) {
+        for (int i = tid; i < HQ * dim; i += nthr) {
             const int h = i / dim, d = i - h * dim;
             float mx = -INFINITY, o = 0.f, ls = 0.f;
             #pragma unroll
-            for (int w = 0; w < W; ++w) mx = fmaxf(mx, sWm[w * kHQ + h]);
+            for (int w = 0; w < W; ++w) mx = fmaxf(mx, sWm[w * HQ + h]);
             #pragma unroll
             for (int w = 0; w < W; ++w) {
                 // a warp without tokens has sum 0; a NaN sum is carried on
-                const float lw = sWl[w * kHQ + h], f = lw == 0.f ? 0.f : fast_exp2(sWm[w * kHQ + h] - mx);
-                o = fmaf(f, sAcc[(w * kHQ + h) * dim + d], o);
+                const float lw = sWl[w * HQ + h], f = lw == 0.f ? 0.f : fast_exp2(sWm[w * HQ + h] - mx);
+                o = fmaf(f, sAcc[(w * HQ + h) * dim + d], o);
                 ls = fmaf(f, lw, ls);
             }
             // the weights carry 2^12, the tables 2^tk; AFF: sum p z = zc l + dz sum p (i - c)
@@ -783,14 +825,15 @@ constexpr int kMaxGrid = 160;                  // CTAs of the attention launch, 
 constexpr int kWeighBatch = 4;
 constexpr int kWeighTokens = kWeighBatch * kJoinThreads;   // tokens per CTA of the weight pass
 
-// CTAs [0, units): one unit each -- join its ranges, normalise, rotate back.  CTAs behind them (with
+// CTAs [0, blocks): one block each -- join its ranges, normalise, rotate back.  CTAs behind them (with
 // weights): kWeighTokens tokens of one (sequence, KV head) each, p = exp2(score - m) / l summed over its heads.
 // A unit is three round trips to memory: the ranges' (m, l), their sums, and R -- whose first rows are asked
 // for before the grid dependency, thread (group kg, column d) holding rows kg, kg + groups, ... of column d.
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p, int chunks) {
     extern __shared__ float jsm[];
     const int tid = threadIdx.x, dim = p.dim, rs = dim + 2, warp = tid >> 5, lane = tid & 31;
-    if ((int)blockIdx.x < p.units) {
+    const int blocks = p.units * p.NB;
+    if ((int)blockIdx.x < blocks) {
         float* sO = jsm;                       // [4][dim]
         float* sF = sO + kHQ * dim;            // [ranges][4] exp2(m_r - m), at most grid ranges
         float* sP = sF + kHQ * p.grid;         // [groups][4][dim] partial rotations
@@ -809,17 +852,18 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
         };
         load_r(0);
         int r0, r1;
-        const int unit = blockIdx.x;
+        const int unit = blockIdx.x / p.NB, blk = blockIdx.x - unit * p.NB;
         unit_rows(p, unit, r0, r1);
         cudaGridDependencySynchronize();
-        const float* part = p.part + (int64_t)r0 * kHQ * rs;
+        const float* part = p.part + ((int64_t)r0 * p.NB + blk) * kHQ * rs;
+        const int64_t next = (int64_t)p.NB * kHQ * rs;         // from a range to the next
         const int nr = r1 - r0;
         if (warp < kHQ) {                       // a range without tokens has l = 0; a NaN sum is carried on
             float m[kMaxGrid / 32], l[kMaxGrid / 32], mx = -INFINITY, sum = 0.f;
             #pragma unroll
             for (int i = 0; i < kMaxGrid / 32; ++i) {
                 const int r = lane + 32 * i;
-                const float* q = part + ((int64_t)r * kHQ + warp) * rs;
+                const float* q = part + r * next + warp * rs;
                 m[i] = r < nr ? __ldcg(q) : 0.f;
                 l[i] = r < nr ? __ldcg(q + 1) : 0.f;
             }
@@ -845,7 +889,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
             const float* q = part + h * rs + 2 + x;
             float o = 0.f;
             #pragma unroll 8
-            for (int r = 0; r < nr; ++r) o = fmaf(sF[r * kHQ + h], __ldcg(q + (int64_t)r * kHQ * rs), o);
+            for (int r = 0; r < nr; ++r) o = fmaf(sF[r * kHQ + h], __ldcg(q + r * next), o);
             sO[i] = sInv[h] == 0.f ? 0.f : o / sInv[h];
         }
         __syncthreads();
@@ -863,7 +907,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
             #pragma unroll
             for (int h = 0; h < kHQ; ++h) sP[(kg * kHQ + h) * dim + d] = v[h];
         __syncthreads();
-        const int b = unit / p.UH, u = unit % p.UH, hk = u / p.UG, hg = u % p.UG;
+        const int b = unit / p.UH, u = unit % p.UH, hk = u / p.UG, hg = u % p.UG * p.NB + blk;
         for (int i = tid; i < kHQ * dim; i += kJoinThreads) {
             const int h = i / dim, hl = hg * kHQ + h;
             if (hl >= p.G) break;
@@ -875,17 +919,18 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
     }
     cudaGridDependencySynchronize();
     // ---- weights -----------------------------------------------------------------------------
-    const int w = blockIdx.x - p.units, chunk = w % chunks, bh = w / chunks, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
+    const int w = blockIdx.x - blocks, chunk = w % chunks, bh = w / chunks, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
     const int L = clamp_len(p.pg, input(p.seq_lens + b));
     const int nv = p.selected ? p.n_sel << p.pg.ps_log2 : L;   // listed or dense tokens
     if (chunk * kWeighTokens >= nv) return;
     float* sOff = jsm;                         // [G] m + log2 l
     for (int h = warp; h < p.G; h += kJoinThreads / 32) {
         int r0, r1;
-        unit_rows(p, b * p.UH + hk * p.UG + h / kHQ, r0, r1);
+        const int hb = h / kHQ;                // its block within the KV head
+        unit_rows(p, b * p.UH + hk * p.UG + hb / p.NB, r0, r1);
         float mx = -INFINITY, l = 0.f;
         for (int r = r0 + lane; r < r1; r += 32) {
-            const float* part = p.part + ((int64_t)r * kHQ + h % kHQ) * rs;
+            const float* part = p.part + (((int64_t)r * p.NB + hb % p.NB) * kHQ + h % kHQ) * rs;
             const float mr = part[0];
             if (part[1] == 0.f) continue;
             const float nm = fmaxf(mx, mr);
@@ -905,7 +950,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
     // a thread's tokens kWeighBatch at a time: their pages, scores and weights are all on their way before the first
     // is used
     const int end = min(nv, (chunk + 1) * kWeighTokens);
-    const float* raw = p.raw + ((int64_t)b * p.UH + hk * p.UG) * p.raw_us;
+    const float* raw = p.raw + ((int64_t)b * p.UH + hk * p.UG) * p.NB * p.raw_us;
     const int64_t row = ((int64_t)b * p.pg.Hkv + hk) * p.w_rs;
     for (int i0 = chunk * kWeighTokens + tid; i0 < end; i0 += kWeighBatch * kJoinThreads) {
         int t[kWeighBatch];
@@ -941,8 +986,11 @@ static PagedParams paged_params(const pkv_codec* c, const pkv_paged_attn_args* a
     p.pg = pg;
     p.Hq = a->q_heads;
     p.G = a->q_heads / pg.Hkv;
-    p.HQ = kHQ;
-    p.UG = (p.G + kHQ - 1) / kHQ;
+    // Two blocks to a unit decode each code once for eight heads, on 8 warps of 255 registers: 64 query heads over 8 KV
+    // heads of 4 x 131072 tokens take 255 us, with one block on 16 warps 295 (learned codebooks 342, 542; on 12 warps of
+    // 168 registers, with spills, 271 and 449).  Larger head sizes have no registers for it.
+    p.NB = p.G > kHQ && c->dim <= 96 ? 2 : 1;
+    p.UG = (p.G + p.NB * kHQ - 1) / (p.NB * kHQ);
     p.UH = pg.Hkv * p.UG;
     p.dim = c->dim;
     p.m = c->dim / 3;
@@ -968,13 +1016,13 @@ static PagedParams paged_params(const pkv_codec* c, const pkv_paged_attn_args* a
 
 // Workspace: partial rows, query fragments (48 registers at most), per-head numbers, scores.
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-static size_t paged_part_bytes(const PagedParams& p) { return up256((size_t)(p.grid + p.units) * kHQ * (p.dim + 2) * 4); }
-static size_t paged_frag_bytes(const PagedParams& p) { return up256((size_t)p.units * 48 * 32 * 4); }
-static size_t paged_head_bytes(const PagedParams& p) { return up256((size_t)p.units * 8 * 4); }
+static size_t paged_part_bytes(const PagedParams& p) { return up256((size_t)(p.grid + p.units) * p.NB * kHQ * (p.dim + 2) * 4); }
+static size_t paged_frag_bytes(const PagedParams& p) { return up256((size_t)p.units * p.NB * 48 * 32 * 4); }
+static size_t paged_head_bytes(const PagedParams& p) { return up256((size_t)p.units * p.NB * 8 * 4); }
 
 size_t paged_workspace(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg, int sms) {
     const PagedParams p = paged_params(c, a, pg, sms);
-    return paged_part_bytes(p) + paged_frag_bytes(p) + paged_head_bytes(p) + (a->weights ? (size_t)p.units * p.raw_us * 4 : 0);
+    return paged_part_bytes(p) + paged_frag_bytes(p) + paged_head_bytes(p) + (a->weights ? (size_t)p.units * p.NB * p.raw_us * 4 : 0);
 }
 
 template <class T>
@@ -986,7 +1034,7 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
     static std::atomic<int> seen[64];
     int rc = allow_smem(paged_attn_kernel<T>, smem, seen);
     if (rc) return rc;
-    rc = launch_behind(paged_query_kernel, (unsigned)p.units, kQueryThreads, (size_t)2 * kHQ * p.dim * 4, 0, st, p,
+    rc = launch_behind(paged_query_kernel, (unsigned)(p.units * p.NB), kQueryThreads, (size_t)2 * kHQ * p.dim * 4, 0, st, p,
                        (int)T::AFF, T::CPL, (int)T::EX);
     if (rc) return rc;
     return launch_behind(paged_attn_kernel<T>, (unsigned)p.grid, T::THREADS, (size_t)smem, 0, st, p);
@@ -996,9 +1044,10 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
 // truncation of the running sums (a few 1e-6 relative) is far below their own rounding.
 template <int MODE, bool EX>
 static int launch_paged_mode(const PagedParams& p, cudaStream_t st) {
-    if (p.m <= 32) return launch_paged_as<PA<MODE, 8, 2, 16, EX>>(p, st);
-    if (p.m <= 48) return launch_paged_as<PA<MODE, 12, 1, 12, EX>>(p, st);
-    return launch_paged_as<PA<MODE, 16, 1, 12, EX>>(p, st);
+    if (p.m <= 32)
+        return p.NB == 2 ? launch_paged_as<PA<MODE, 8, 2, 8, 2, EX>>(p, st) : launch_paged_as<PA<MODE, 8, 2, 16, 1, EX>>(p, st);
+    if (p.m <= 48) return launch_paged_as<PA<MODE, 12, 1, 12, 1, EX>>(p, st);
+    return launch_paged_as<PA<MODE, 16, 1, 12, 1, EX>>(p, st);
 }
 
 template <bool EX>
@@ -1019,7 +1068,7 @@ int launch_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg
     const int rc = a->out_dtype == PKV_F32 ? launch_paged_any<true>(c, p, st) : launch_paged_any<false>(c, p, st);
     if (rc) return rc;
     const int chunks = a->weights ? (int)((p.raw_us / p.raw_h + kWeighTokens - 1) / kWeighTokens) : 0;
-    const int64_t ctas = p.units + (int64_t)pg.B * pg.Hkv * chunks;
+    const int64_t ctas = (int64_t)p.units * p.NB + (int64_t)pg.B * pg.Hkv * chunks;
     if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
     const size_t smem = (size_t)(kHQ * p.dim + kHQ * p.grid + kJoinThreads / ((p.dim + 31) / 32 * 32) * kHQ * p.dim) * 4;
     return launch_behind(paged_join_kernel, (unsigned)ctas, kJoinThreads, smem, 0, st, p, chunks);
