@@ -986,10 +986,10 @@ static PagedParams paged_params(const pkv_codec* c, const pkv_paged_attn_args* a
     p.pg = pg;
     p.Hq = a->q_heads;
     p.G = a->q_heads / pg.Hkv;
-    // Two blocks to a unit decode each code once for eight heads, on 8 warps of 255 registers: 64 query heads over 8 KV
-    // heads of 4 x 131072 tokens take 255 us, with one block on 16 warps 295 (learned codebooks 342, 542; on 12 warps of
-    // 168 registers, with spills, 271 and 449).  Larger head sizes have no registers for it.
-    p.NB = p.G > kHQ && c->dim <= 96 ? 2 : 1;
+    // Two blocks to a unit decode each code once for eight heads, on 8 warps of 255 registers.  64 query heads over 8 KV
+    // heads, one block against two: head size 96, 4 x 131072 tokens 295 -> 255 us (learned codebooks 542 -> 342); head
+    // size 129, 4 x 60000 tokens 235 -> 194 us (390 -> 244).  Head sizes past 144 have no registers for it.
+    p.NB = p.G > kHQ && c->dim <= 144 ? 2 : 1;
     p.UG = (p.G + p.NB * kHQ - 1) / (p.NB * kHQ);
     p.UH = pg.Hkv * p.UG;
     p.dim = c->dim;
@@ -1042,12 +1042,15 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
 
 // fp32 results get the tiles' sums added in rounded fp32 (about an eighth more time); for 16-bit results the
 // truncation of the running sums (a few 1e-6 relative) is far below their own rounding.
+// Warps by what a lane holds: 16 of 128 registers for up to 32 triplets (14 take 10 % longer, 10 take 20 %), 12 of 168
+// up to 48 (16 spill: + 9 %; 10: + 12 %), 8 of 255 up to 64 (12: + 7 %).
 template <int MODE, bool EX>
 static int launch_paged_mode(const PagedParams& p, cudaStream_t st) {
     if (p.m <= 32)
         return p.NB == 2 ? launch_paged_as<PA<MODE, 8, 2, 8, 2, EX>>(p, st) : launch_paged_as<PA<MODE, 8, 2, 16, 1, EX>>(p, st);
-    if (p.m <= 48) return launch_paged_as<PA<MODE, 12, 1, 12, 1, EX>>(p, st);
-    return launch_paged_as<PA<MODE, 16, 1, 12, 1, EX>>(p, st);
+    if (p.m <= 48)
+        return p.NB == 2 ? launch_paged_as<PA<MODE, 12, 1, 8, 2, EX>>(p, st) : launch_paged_as<PA<MODE, 12, 1, 12, 1, EX>>(p, st);
+    return launch_paged_as<PA<MODE, 16, 1, 8, 1, EX>>(p, st);
 }
 
 template <bool EX>

@@ -165,6 +165,14 @@ CASES = [
     ([9000, 4000, 100, 1], 4, 1, 96, "v1", (4, 4, 4), BF, 16, "hnd"),     # ragged
     ([40] * 70, 4, 1, 96, "v1", (4, 4, 4), F32, 16, "hnd"),               # more sequences than a warp's lanes
     ([20000], 4, 1, 96, "v1", (4, 4, 4), F32, 16, "hnd"),
+    # more than four query heads per KV head: two blocks of heads to a unit (up to head size 144)
+    ([700, 33, 0], 64, 8, 129, "v1", (4, 4, 4), BF, 16, "hnd"),
+    ([300], 12, 2, 129, "learned_bias", (4, 4, 4), F32, 32, "nhd"),
+    ([300, 65], 16, 2, 96, "learned", (3, 3, 2), BF, 16, "hnd"),
+    ([300, 1], 10, 1, 66, "v1", (3, 3, 2), F16, 16, "hnd"),
+    ([513], 18, 2, 96, "lloyd_bias", (4, 4, 4), BF, 64, "hnd"),           # group 9: three blocks, the last one alone
+    ([200], 14, 2, 192, "v1", (4, 4, 4), F32, 16, "hnd"),                 # one block to a unit
+    ([200, 90], 16, 1, 144, "learned", (3, 3, 2), F32, 16, "nhd"),
 ]
 
 
