@@ -131,9 +131,9 @@ int pkv_pages_store(const pkv_pages* pages, int32_t m, void* dst, const void* co
     if (n < 0) return PKV_ERR_INVALID;
     if (n == 0 || pages->batch == 0) return PKV_OK;
     if (!dst || !codes || !start) return PKV_ERR_INVALID;
-    if (reinterpret_cast<uintptr_t>(dst) % 16) return PKV_ERR_ALIGNMENT;
+    if (reinterpret_cast<uintptr_t>(dst) % 16 || reinterpret_cast<uintptr_t>(codes) % pages->code_bytes) return PKV_ERR_ALIGNMENT;
     return pkv::launch_pages_store(device_pages(pages), static_cast<uint8_t*>(dst), static_cast<const uint8_t*>(codes),
-                                   m * pages->code_bytes, n, start, counts, static_cast<cudaStream_t>(stream));
+                                   m * pages->code_bytes, pages->code_bytes, n, start, counts, static_cast<cudaStream_t>(stream));
 }
 
 int pkv_pages_summarize(const pkv_codec* c, const pkv_pages* pages, const int32_t* seq_lens, const int32_t* start,

@@ -918,11 +918,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
         return;
     }
     cudaGridDependencySynchronize();
-    // ---- weights -----------------------------------------------------------------------------
-    const int w = blockIdx.x - blocks, chunk = w % chunks, bh = w / chunks, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
+    // ---- weights: chunks of all rows in turn (a wide table names many that are empty) ------------------
+    for (int w = blockIdx.x - blocks; w < p.pg.B * p.pg.Hkv * chunks; w += gridDim.x - blocks) {
+    const int chunk = w % chunks, bh = w / chunks, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
     const int L = clamp_len(p.pg, input(p.seq_lens + b));
     const int nv = p.selected ? p.n_sel << p.pg.ps_log2 : L;   // listed or dense tokens
-    if (chunk * kWeighTokens >= nv) return;
+    if (chunk * kWeighTokens >= nv) continue;
+    __syncthreads();                           // (the last chunk's offsets are read)
     float* sOff = jsm;                         // [G] m + log2 l
     for (int h = warp; h < p.G; h += kJoinThreads / 32) {
         int r0, r1;
@@ -977,6 +979,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
                 sum += exp2f(__ldcg(raw + h / kHQ * p.raw_us + (int64_t)(i0 + u * kJoinThreads) * p.raw_h + h % kHQ) - sOff[h]);
             p.w_out[row + t[u]] = w0[u] + sum;
         }
+    }
     }
 }
 
@@ -1071,8 +1074,9 @@ int launch_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg
     const int rc = a->out_dtype == PKV_F32 ? launch_paged_any<true>(c, p, st) : launch_paged_any<false>(c, p, st);
     if (rc) return rc;
     const int chunks = a->weights ? (int)((p.raw_us / p.raw_h + kWeighTokens - 1) / kWeighTokens) : 0;
-    const int64_t ctas = (int64_t)p.units * p.NB + (int64_t)pg.B * pg.Hkv * chunks;
-    if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
+    const int64_t all = (int64_t)pg.B * pg.Hkv * chunks;
+    if (all > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
+    const int64_t ctas = (int64_t)p.units * p.NB + (all < 16 * (int64_t)sms ? all : 16 * (int64_t)sms);
     const size_t smem = (size_t)(kHQ * p.dim + kHQ * p.grid + kJoinThreads / ((p.dim + 31) / 32 * 32) * kHQ * p.dim) * 4;
     return launch_behind(paged_join_kernel, (unsigned)ctas, kJoinThreads, smem, 0, st, p, chunks);
 }

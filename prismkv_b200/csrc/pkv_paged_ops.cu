@@ -36,25 +36,27 @@ __device__ __forceinline__ void store_piece(uint8_t* row, int bytes, int i, uint
         if (at + x < bytes) row[at + x] = (uint8_t)(w[x >> 2] >> (8 * (x & 3)));
 }
 
-// Rows (b, hk, i) of contiguous codes (any alignment of two bytes) into slots start[b] + i.
-__global__ void pages_store_kernel(Pages g, uint8_t* dst, const uint8_t* codes, int bytes, int n,
-                                   const int32_t* start, const int32_t* counts) {
+// Rows (b, hk, i) of contiguous codes into slots start[b] + i, eight threads a row.  Unit: what a thread copies at a
+// time -- 16 bytes where rows are whole pieces of that, else a code.
+template <class Unit>
+__global__ void __launch_bounds__(256) pages_store_kernel(Pages g, uint8_t* dst, const uint8_t* codes, int bytes, int n,
+                                                          const int32_t* start, const int32_t* counts) {
     cudaGridDependencySynchronize();
     const int64_t rows = (int64_t)g.B * g.Hkv * n;
-    const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;   // eight threads a row
+    const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
     if (row >= rows) return;
     const int i = (int)(row % n), hk = (int)(row / n % g.Hkv), b = (int)(row / n / g.Hkv);
-    if (counts && i >= counts[b]) return;
-    const int64_t t = (int64_t)start[b] + i;
+    if (counts && i >= input(counts + b)) return;
+    const int64_t t = (int64_t)input(start + b) + i;
     if (t < 0 || t >= ((int64_t)g.max_pages << g.ps_log2)) {
         flag_error(kErrPage);
         return;
     }
     const int page = page_of(g, b, (int)(t >> g.ps_log2));
     if (page < 0) return;
-    uint8_t* d = dst + slot_offset(g, page, hk, (int)(t & ((1 << g.ps_log2) - 1)));
-    const uint8_t* s = codes + row * bytes;
-    for (int x = threadIdx.x & 7; x < bytes; x += 8) d[x] = s[x];
+    Unit* d = reinterpret_cast<Unit*>(dst + slot_offset(g, page, hk, (int)(t & ((1 << g.ps_log2) - 1))));
+    const Unit* s = reinterpret_cast<const Unit*>(codes + row * bytes);
+    for (int x = threadIdx.x & 7; x < bytes / (int)sizeof(Unit); x += 8) d[x] = s[x];
 }
 
 // Slots kept[b, hk, i] of the source pages into slots i of the destination's, K and V.  A CTA takes kGatherRows
@@ -724,11 +726,15 @@ int launch_pages_summarize(const pkv_codec* c, Pages pg, int cb, const int32_t* 
     return words <= 16 ? launch_summaries<2, 16>(p, st) : launch_summaries<2, 32>(p, st);
 }
 
-int launch_pages_store(Pages pg, uint8_t* dst, const uint8_t* codes, int bytes, int n, const int32_t* start,
+int launch_pages_store(Pages pg, uint8_t* dst, const uint8_t* codes, int bytes, int code_bytes, int n, const int32_t* start,
                        const int32_t* counts, cudaStream_t st) {
     const int64_t threads = (int64_t)pg.B * pg.Hkv * n * 8, ctas = (threads + 255) / 256;
     if (ctas > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-    return launch_behind(pages_store_kernel, (unsigned)ctas, 256, 0, 0, st, pg, dst, codes, bytes, n, start, counts);
+    const unsigned grid = (unsigned)ctas;
+    if (bytes % 16 == 0 && reinterpret_cast<uintptr_t>(codes) % 16 == 0)
+        return launch_behind(pages_store_kernel<uint4>, grid, 256, 0, 0, st, pg, dst, codes, bytes, n, start, counts);
+    if (code_bytes == 2) return launch_behind(pages_store_kernel<uint16_t>, grid, 256, 0, 0, st, pg, dst, codes, bytes, n, start, counts);
+    return launch_behind(pages_store_kernel<uint8_t>, grid, 256, 0, 0, st, pg, dst, codes, bytes, n, start, counts);
 }
 
 int launch_tokens_gather(Pages s, Pages d, uint8_t* dk, uint8_t* dv, int bytes, const int32_t* kept, int keep,

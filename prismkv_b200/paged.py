@@ -9,9 +9,10 @@ the last token are never read.  ``page_size`` is a power of two, 16 to 1024.
 Any strides serve whose rows start on 16-byte boundaries with unit code stride,
 so (num_pages, page_size, kv_heads, m) pools pass as transposed views.
 
-Nothing here synchronises, keeps state between calls or allocates beyond its
+Nothing here synchronises, keeps results between calls or allocates beyond its
 outputs and a workspace from torch's allocator, so every call can be captured
-into a CUDA graph.  A page id outside the pool, a token past the table or a
+into a CUDA graph (``empty_summaries`` or a first ``summarize_pages`` uploads the
+summaries' grid: make one of them before a capture).  A page id outside the pool, a token past the table or a
 page list out of order is skipped on the device and shows in
 ``_lib.device_error()`` as 6.
 """
@@ -61,6 +62,7 @@ class PagedOps:
 
     def empty_summaries(self, num_pages: int, kv_heads: int) -> torch.Tensor:
         """Uninitialised (num_pages, kv_heads, 2, summary_pitch) int8 page summaries."""
+        self._grid()                                      # uploaded here, so that a capture need not
         return torch.empty((num_pages, kv_heads, 2, self.summary_pitch), dtype=torch.int8, device=self.device)
 
     # ------------------------------------------------------------------
