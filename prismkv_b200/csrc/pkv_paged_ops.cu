@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256) pages_store_kernel(Pages g, uint8_t* dst,
 // Slots kept[b, hk, i] of the source pages into slots i of the destination's, K and V.  A CTA takes kGatherRows
 // x (256 / pieces) neighbouring rows of one (sequence, KV head), a thread the same 16-byte piece of kGatherRows
 // of them: the three dependent steps (slot, pages, codes) of its rows overlap.  The copies' bytes bound it.
-constexpr int kGatherRows = 4;
+constexpr int kGatherRows = 2;
 __global__ void __launch_bounds__(256) tokens_gather_kernel(Pages s, Pages d, uint8_t* dk, uint8_t* dv, int bytes,
                                                             const int32_t* kept, int keep, int chunks) {
     constexpr int U = kGatherRows;
@@ -277,15 +277,16 @@ __device__ void top_row(TopShared<THREADS, DIGIT>& s, int lo, int hi, int n, int
         for (int pass = 0; pass < PASSES; ++pass) {
             const int bits = min(DIGIT, shift), low = shift - bits;
             uint32_t* hist = s.hist[pass & 1];
-            for (int i0 = lo + tid; i0 < hi; i0 += 4 * THREADS) {
-                uint32_t x[4];
-                #pragma unroll
-                for (int u = 0; u < 4; ++u) x[u] = i0 + u * THREADS < hi ? key(i0 + u * THREADS) : 0u;
-                #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (i0 + u * THREADS < hi && (shift == BITS || (x[u] >> shift) == (prefix >> shift)))
-                        atomicAdd(&hist[(x[u] >> low) & ((1u << bits) - 1u)], 1u);
+            const uint32_t field = (1u << bits) - 1u, want = shift < 32 ? prefix >> shift : 0u;
+            auto note = [&](uint32_t x) {
+                if (shift == BITS || (x >> shift) == want) atomicAdd(&hist[(x >> low) & field], 1u);
+            };
+            int i = lo + tid;
+            for (; i + 3 * THREADS < hi; i += 4 * THREADS) {
+                const uint32_t x0 = key(i), x1 = key(i + THREADS), x2 = key(i + 2 * THREADS), x3 = key(i + 3 * THREADS);
+                note(x0); note(x1); note(x2); note(x3);
             }
+            for (; i < hi; i += THREADS) note(key(i));
             cl.sync();
             if (pass + 2 < PASSES + 1 && pass > 0)          // the other one was read before this barrier
                 for (int i = tid; i < BINS; i += THREADS) s.hist[(pass + 1) & 1][i] = 0;
@@ -337,16 +338,21 @@ __device__ void top_row(TopShared<THREADS, DIGIT>& s, int lo, int hi, int n, int
     const int part = (hi - lo + (THREADS / 32) - 1) / (THREADS / 32);
     const int w0 = min(hi, lo + warp * part), w1 = min(hi, w0 + part);
     uint32_t above = 0, equal = 0;
-    for (int i0 = w0 + lane; i0 < w1; i0 += 128) {
-        uint32_t x[4];
-        #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = i0 + 32 * u < w1 ? key(i0 + 32 * u) : 0u;
-        #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (i0 + 32 * u < w1) {
-                above += all || x[u] > prefix;
-                equal += !all && x[u] == prefix;
+    {
+        auto note = [&](uint32_t x) {
+            above += x > prefix;
+            equal += x == prefix;
+        };
+        int i = w0 + lane;
+        if (all) {
+            above = i < w1 ? (uint32_t)(w1 - i + 31) / 32 : 0u;
+        } else {
+            for (; i + 96 < w1; i += 128) {
+                const uint32_t x0 = key(i), x1 = key(i + 32), x2 = key(i + 64), x3 = key(i + 96);
+                note(x0); note(x1); note(x2); note(x3);
             }
+            for (; i < w1; i += 32) note(key(i));
+        }
     }
     above = __reduce_add_sync(0xffffffffu, above);
     equal = __reduce_add_sync(0xffffffffu, equal);
@@ -371,12 +377,11 @@ __device__ void top_row(TopShared<THREADS, DIGIT>& s, int lo, int hi, int n, int
         const int i = i0 + 4 * lane;
         uint32_t take = 0, same = 0;                         // keys above the threshold, and equal to it
         #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (i + u < w1) {
-                const uint32_t x = key(i + u);
-                take |= (uint32_t)(all || x > prefix) << u;
-                same |= (uint32_t)(!all && x == prefix) << u;
-            }
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t x = i + u < w1 ? key(i + u) : 0u;
+            take |= (uint32_t)(i + u < w1 && (all || x > prefix)) << u;
+            same |= (uint32_t)(i + u < w1 && !all && x == prefix) << u;
+        }
         if (__any_sync(0xffffffffu, same)) {                 // of the equal ones the first `need` of the row
             const uint32_t ce = __popc(same);
             const unsigned e0 = __ballot_sync(0xffffffffu, ce & 1), e1 = __ballot_sync(0xffffffffu, ce & 2),
