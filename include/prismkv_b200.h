@@ -316,7 +316,9 @@ PKV_API int pkv_polar_scores(const float *q_rot, const void *k_codes, int32_t co
  * table names sequence b's pages: token t sits in slot t % page_size of page
  * table[b*table_stride + t / page_size].  page_size is a power of two, 16 to
  * 1024; k, v and the three strides are multiples of 16 bytes; a page_stride of
- * 2 GiB or a token_stride of 2 MiB and more is PKV_ERR_UNSUPPORTED.
+ * 2 GiB or a token_stride of 2 MiB and more is PKV_ERR_UNSUPPORTED, and so are
+ * more than 2^31 - 2^16 slots of a sequence (kept tokens, listed pages).  Rows are
+ * read in whole pieces of 16 bytes: the last row's last piece must be readable.
  * Page ids outside [0, num_pages) are never followed: their tokens count as
  * masked and the device error word is set to 6.  Sequence lengths are read on
  * the device, clamped to [0, max_pages * page_size].                        */
@@ -337,9 +339,10 @@ typedef struct pkv_pages {
  * weights / weights_out (both or neither): (batch, kv_heads, slots) f32 rows of
  * weights_row_stride floats; every attended token t gets
  *     weights_out[b, hk, t] = weights[b, hk, t] + sum over hk's query heads of p(t)
- * (the two may be the same buffer); other entries are not touched.  A row with
- * no attended token gives zeros.  The workspace needs no initialisation and
- * belongs to one call until that call's kernels are done.                    */
+ * (the two may be the same buffer); other entries are not touched, and tokens
+ * past `slots` are not recorded.  A row with no attended token gives zeros.  The
+ * workspace needs no initialisation and belongs to one call until that call's
+ * kernels are done.                                                          */
 typedef struct pkv_paged_attn_args {
     pkv_pages pages;
     int32_t q_heads, q_dtype;

@@ -14,7 +14,8 @@ On top of the pool:
 
 The reference has no paged cache; its RawKVCache (cache/raw_cache.py:57-292) is
 the nearest relative.  Tensors and pages belong to one CUDA stream at a time:
-a page is reused as soon as it is free, in stream order.
+a page is reused as soon as it is free, in stream order.  Threads that share
+the stream may share the cache.
 """
 
 from __future__ import annotations
@@ -109,9 +110,11 @@ class PagedKVCache:
         counts = [s] * B if lengths is None else [int(n) for n in lengths]
         if len(counts) != B or any(n < 0 or n > s for n in counts):
             raise ValueError(f"lengths must be {B} numbers from 0 to {s}, got {counts}")
-        dev = self._device if self._device is not None else _cuda_device(k)
+        st = self._layers.get(layer_idx)
+        dev = st.lens.device if st is not None else self._device if self._device is not None else _cuda_device(k)
         codec = backend.codec(dev)
-        codes = [codec.encode(backend.aligner.pad(x.to(dev).reshape(B * H * s, -1))).view(B, H, s, codec.m) for x in (k, v)]
+        codes = [codec.encode(backend.aligner.pad(x.to(dev).reshape(B * H * s, x.shape[3]))).view(B, H, s, codec.m)
+                 for x in (k, v)]
         with self._lock:
             st = self._layers.get(layer_idx)
             if st is None:
@@ -145,36 +148,42 @@ class PagedKVCache:
         ``top_pages``: attend to that many pages per KV head at most, the first
         ``sinks`` and last ``recent`` among them.
         """
-        st, backend = self._layer(layer_idx), self._backend(layer_idx)
-        codec = backend.codec(st.lens.device)
+        backend = self._backend(layer_idx)
         if q.dim() != 3 or q.shape[2] != backend.head_dim:
             raise ValueError(f"q must be ({self.batch}, q_heads, {backend.head_dim}), got {tuple(q.shape)}")
-        qp = backend.aligner.pad(q.to(st.lens.device))
         if scale is None:
             scale = backend.head_dim ** -0.5
-        pages = None
-        if top_pages is not None:
-            if st.summaries is None:
-                raise RuntimeError("top_pages needs a cache made with page_summaries=True")
-            if max(len(r) for r in st.rows) > top_pages:
-                pages = codec.select_pages(qp, st.summaries, st.table, st.lens, self.page_size, top_pages, sinks=sinks,
-                                           recent=recent)
-        out = codec.paged_attention(qp, st.k, st.v, st.table, st.lens, scale=scale, pages=pages, weights=st.weights,
-                                    out_dtype=out_dtype)
+        with self._lock:
+            st = self._layer(layer_idx)
+            codec = backend.codec(st.lens.device)
+            qp = backend.aligner.pad(q.to(st.lens.device))
+            pages = None
+            if top_pages is not None:
+                if not self.page_summaries:
+                    raise RuntimeError("top_pages needs a cache made with page_summaries=True")
+                if top_pages < 1 or sinks < 0 or recent < 0 or sinks + recent > top_pages:
+                    raise ValueError("need 0 <= sinks + recent <= top_pages and top_pages >= 1, "
+                                     f"got {sinks}, {recent}, {top_pages}")
+                if max(len(r) for r in st.rows) > top_pages:
+                    pages = codec.select_pages(qp, st.summaries, st.table, st.lens, self.page_size, top_pages, sinks=sinks,
+                                               recent=recent)
+            out = codec.paged_attention(qp, st.k, st.v, st.table, st.lens, scale=scale, pages=pages, weights=st.weights,
+                                        out_dtype=out_dtype)
         return backend.aligner.unpad(out)
 
     def evict(self, layer_idx: int, keep: int, sinks: int = 4, recent: int = 32) -> List[int]:
         """Cut every sequence of more than ``keep`` tokens to ``keep``: its first ``sinks``, its last ``recent`` and
         the most attended others of each KV head, in their order.  Returns the new lengths.  The kept tokens move
         to free pages (ceil(keep / page_size) per sequence, needed for the move) and the old ones come free."""
-        st, backend = self._layer(layer_idx), self._backend(layer_idx)
-        if st.weights is None:
+        backend = self._backend(layer_idx)
+        if not self.track_weights:
             raise RuntimeError("evict needs a cache made with track_weights=True")
         if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
             raise ValueError(f"need 0 <= sinks + recent <= keep and keep >= 1, got {sinks}, {recent}, {keep}")
-        dev = st.lens.device
-        codec = backend.codec(dev)
         with self._lock:
+            st = self._layer(layer_idx)
+            dev = st.lens.device
+            codec = backend.codec(dev)
             cut = [b for b in range(self.batch) if st.lengths[b] > keep]
             if not cut:
                 return list(st.lengths)
@@ -202,10 +211,10 @@ class PagedKVCache:
     # ------------------------------------------------------------------
     def release(self, layer_idx: int, sequence: int) -> None:
         """Forget one sequence of a layer; its pages come free."""
-        st = self._layer(layer_idx)
         if not 0 <= sequence < self.batch:
             raise IndexError(f"sequence {sequence} outside a batch of {self.batch}")
         with self._lock:
+            st = self._layer(layer_idx)
             st.free.extend(reversed(st.rows[sequence]))
             st.rows[sequence], st.lengths[sequence] = [], 0
             st.lens[sequence] = 0

@@ -58,6 +58,8 @@ class DeviceCodec(PagedOps):
     def __init__(self, host: HostTables, device: torch.device):
         self.host = host
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:     # where the tables below go, for good
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.dim = host.dim
         self.m = host.dim // 3
         self.bits = host.bits

@@ -20,6 +20,9 @@ int paged_device_error(int32_t* flag_out, int32_t clear) {
 
 namespace {
 
+// Token and list indexes are 32-bit, with room above them for what the kernels' loops add before they stop.
+constexpr int64_t kMaxIndex = 0x7fff0000;
+
 bool paged_dtype(int dt) { return dt == PKV_F32 || dt == PKV_BF16 || dt == PKV_F16; }
 
 int check_paged_codec(const pkv_codec* c, bool tables) {
@@ -39,7 +42,7 @@ int check_pages(const pkv_pages* g, int m, bool need_codes) {
     if (g->code_bytes != 1 && g->code_bytes != 2) return PKV_ERR_INVALID;
     const int ps = g->page_size;
     if (ps < 16 || ps > 1024 || (ps & (ps - 1))) return PKV_ERR_INVALID;
-    if ((int64_t)g->max_pages * ps > 0x7fffff00) return PKV_ERR_UNSUPPORTED;       // token indexes are 32-bit
+    if ((int64_t)g->max_pages * ps > kMaxIndex) return PKV_ERR_UNSUPPORTED;
     if (g->token_stride < m || g->head_stride < 0 || g->page_stride < 0) return PKV_ERR_INVALID;
     if (g->batch > 0 && g->max_pages > 0 && (!g->table || g->table_stride < g->max_pages)) return PKV_ERR_INVALID;
     if (need_codes && g->num_pages > 0 && !g->k) return PKV_ERR_INVALID;
@@ -80,7 +83,7 @@ int check_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a) {
     if (a->q_heads / g.kv_heads > 16) return PKV_ERR_UNSUPPORTED;
     if (!paged_dtype(a->q_dtype) || !paged_dtype(a->out_dtype) || !std::isfinite(a->scale)) return PKV_ERR_INVALID;
     if (a->n_selected < 0 || (a->n_selected > 0 && !a->selected)) return PKV_ERR_INVALID;
-    if ((int64_t)a->n_selected * g.page_size > 0x7fffff00) return PKV_ERR_UNSUPPORTED;
+    if ((int64_t)a->n_selected * g.page_size > kMaxIndex) return PKV_ERR_UNSUPPORTED;
     if ((a->weights == nullptr) != (a->weights_out == nullptr)) return PKV_ERR_INVALID;
     if (a->weights && (a->weights_slots < 0 || a->weights_row_stride < a->weights_slots)) return PKV_ERR_INVALID;
     if (g.batch == 0) return PKV_OK;
@@ -162,6 +165,7 @@ int pkv_pages_select(const pkv_codec* c, const pkv_pages* pages, const void* q, 
     if (q_heads < 1 || q_heads % pages->kv_heads != 0 || !paged_dtype(q_dtype)) return PKV_ERR_INVALID;
     if (q_heads / pages->kv_heads > 16) return PKV_ERR_UNSUPPORTED;
     if (top < 1 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > top) return PKV_ERR_INVALID;
+    if (top > kMaxIndex) return PKV_ERR_UNSUPPORTED;
     if (pages->batch == 0) return PKV_OK;
     if (!q || !seq_lens || !out || (pages->num_pages > 0 && !summaries)) return PKV_ERR_INVALID;
     if (reinterpret_cast<uintptr_t>(summaries) % 16) return PKV_ERR_ALIGNMENT;
@@ -176,6 +180,7 @@ int pkv_tokens_select(const float* weights, int32_t batch, int32_t kv_heads, int
                       float* kept_weights, void* stream) {
     if (batch < 0 || kv_heads < 1 || slots < 0 || row_stride < slots) return PKV_ERR_INVALID;
     if (keep < 1 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > keep) return PKV_ERR_INVALID;
+    if (slots > kMaxIndex || keep > kMaxIndex) return PKV_ERR_UNSUPPORTED;
     if (batch == 0) return PKV_OK;
     if (!seq_lens || !kept || !kept_weights || (slots > 0 && !weights)) return PKV_ERR_INVALID;
     int sms = 0;

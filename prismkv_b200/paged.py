@@ -70,8 +70,7 @@ class PagedOps:
     # tensor is read once, and the device is compared as an index (-1 for CPU tensors).
     def _index(self) -> int:
         """The codec's CUDA device index."""
-        i = self.device.index
-        return torch.cuda.current_device() if i is None else i
+        return self.device.index
 
     def _elsewhere(self, t: torch.Tensor, name: str) -> Exception:
         if not t.is_cuda:

@@ -1,6 +1,8 @@
 """PagedKVCache against RawKVCache (the same codes, so the same attention to rounding) and against itself
 after eviction, release and reuse of pages."""
 
+import threading
+
 import pytest
 import torch
 
@@ -114,3 +116,51 @@ def test_eviction_keeps_what_was_attended_to(cuda_ready):
     assert (cache.attention(0, q, top_pages=5) - full).abs().max() <= TOL
     assert torch.isfinite(cache.attention(0, q, top_pages=3)).all()
     assert _lib.device_error() == 0
+
+
+def test_calls_at_the_edges(cuda_ready):
+    d = 96
+    backend = PrismKVBackend(PrismKVConfig(), head_dim=d)
+    cache = PagedKVCache(backend, 2, 2, num_pages=8, page_size=16, page_summaries=True, track_weights=True)
+    k, v = _kv(2, 2, 5, d, 0)
+    assert cache.append(0, k[:, :, :0], v[:, :, :0]) == [0, 0]            # no token yet
+    q = torch.randn(2, 4, d, generator=torch.Generator().manual_seed(1)).to(DEV)
+    assert (cache.attention(0, q) == 0).all()
+    # a page count that cannot hold the first and last pages is refused at every length
+    for top in (0, 1, -1):
+        with pytest.raises(ValueError, match="top_pages"):
+            cache.attention(0, q, top_pages=top)
+    assert cache.append(0, k.cpu(), v.cpu()) == [5, 5]
+    out = cache.attention(0, q)
+    assert cache.append(0, k[:, :, :0], v[:, :, :0]) == [5, 5]
+    assert torch.equal(cache.attention(0, q.cpu()), out)
+    assert cache.evict(0, 5, sinks=0, recent=0) == [5, 5]
+    assert cache.evict(0, 1, sinks=0, recent=1) == [1, 1]
+    raw = RawKVCache(backend)
+    raw.append(0, k[:, :, 4:], v[:, :, 4:])
+    assert (cache.attention(0, q) - raw.attention(0, q)).abs().max() <= TOL
+    assert _lib.device_error() == 0
+
+
+def test_threads_share_a_cache(cuda_ready):
+    """Attention waits while another thread moves the tokens (an eviction changes table, lengths and weights)."""
+    d = 96
+    backend = PrismKVBackend(PrismKVConfig(), head_dim=d)
+    cache = PagedKVCache(backend, 1, 2, num_pages=8, page_size=16, track_weights=True)
+    cache.append(0, *_kv(1, 2, 40, d, 0))
+    q = torch.randn(1, 2, d, generator=torch.Generator().manual_seed(1)).to(DEV)
+    want, got = cache.attention(0, q), []
+    t = threading.Thread(target=lambda: got.append(cache.attention(0, q)))
+    with cache._lock:
+        t.start()
+        t.join(0.5)
+        assert t.is_alive()
+    t.join(60)
+    assert not t.is_alive() and torch.equal(got[0], want)
+
+
+def test_a_codec_stays_on_its_device(cuda_ready):
+    from prismkv_b200.codec import DeviceCodec
+
+    codec = PrismKVBackend(PrismKVConfig(), head_dim=96).codec(torch.device(DEV))
+    assert DeviceCodec(codec.host, torch.device("cuda")).device == codec._R.device

@@ -162,3 +162,17 @@ def test_summary_grid():
     assert np.abs(gz / 128.0 * (6 / 127) - z).max() <= 6 / 127 / 256 + 1e-7
     gz, gxy = _summary_grid(np.zeros(2, np.float32), np.zeros((4, 2), np.float32), 8)     # a table of zeros
     assert not gz.any() and not gxy.any()
+
+
+def test_indexes_that_pass_32_bits_are_refused():
+    lib = _lib.load()
+    c, big = _codec(), 0x7fffffff
+    keep = lambda slots, keep: lib.pkv_tokens_select(256, 1, 1, slots, big, 256, keep, 0, 0, 256, 256, None)  # noqa: E731
+    assert keep(big, 8) == UNSUPPORTED and keep(0x7fff0001, 8) == UNSUPPORTED and keep(64, big) == UNSUPPORTED
+    assert lib.pkv_pages_select(ctypes.byref(c), ctypes.byref(_pages()), 256, 0, 8, 96, 96, 256, 256, big, 1, 1, 256,
+                                None) == UNSUPPORTED
+    wide = _pages(max_pages=0x7ffffff, table_stride=0x7ffffff)           # 2^31 - 16 tokens
+    assert lib.pkv_paged_attn(ctypes.byref(c), ctypes.byref(_args(wide)), 256, 1 << 30, None) == UNSUPPORTED
+    assert lib.pkv_tokens_gather(ctypes.byref(_pages()), 32, 256, 8, ctypes.byref(wide), 256, 256, None) == UNSUPPORTED
+    assert lib.pkv_paged_attn(ctypes.byref(c), ctypes.byref(_args(selected=256, n_selected=0x7ffffff)), 256, 1 << 30,
+                              None) == UNSUPPORTED
