@@ -1,5 +1,5 @@
-// pkv_lib.cu -- single translation unit of libprismkv_b200.so (the kernels
-// share the device error word without relocatable device code).
+// pkv_lib.cu -- one translation unit for everything but the paged cache (its kernels share
+// a device error word without relocatable device code).
 #include "pkv_codec.cu"
 #include "pkv_encode_tc.cu"
 #include "pkv_attn.cu"

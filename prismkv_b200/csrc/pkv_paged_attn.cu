@@ -8,7 +8,9 @@
 // paged_query_kernel rotates the queries into operand fragments, paged_attn_kernel leaves one partial
 // state per (CTA, unit) range, paged_join_kernel joins a unit's ranges, normalises and rotates back (and,
 // in further CTAs, adds the weights from the scores that the second launch kept).  Small calls are bound by
-// the chain of memory round trips through the three, large ones by the issue slots of the decode.
+// the chain of memory round trips through the three (16 us for 37 tokens of 8 heads), large ones by the issue
+// slots of the decode (4 x 131072 tokens, 32 query over 8 KV heads, head size 96, two-byte codes: 162 us, 3.3 TB/s,
+// half of the copy rate; 395 instructions per 16 tokens, 56 % of the slots used, tensor pipe 23 %).
 
 #include "pkv_paged.cuh"
 
@@ -1043,7 +1045,7 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
     return launch_behind(paged_attn_kernel<T>, (unsigned)p.grid, T::THREADS, (size_t)smem, 0, st, p);
 }
 
-// fp32 results get the tiles' sums added in rounded fp32 (about an eighth more time); for 16-bit results the
+// fp32 results get the tiles' sums added in rounded fp32 (4 x 131072 tokens: 180 us against 163); for 16-bit results the
 // truncation of the running sums (a few 1e-6 relative) is far below their own rounding.
 // Warps by what a lane holds: 16 of 128 registers for up to 32 triplets (14 take 10 % longer, 10 take 20 %), 12 of 168
 // up to 48 (16 spill: + 9 %; 10: + 12 %), 8 of 255 up to 64 (12: + 7 %).
