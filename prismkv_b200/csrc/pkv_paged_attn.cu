@@ -824,14 +824,14 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
 
 constexpr int kJoinThreads = 384;
 constexpr int kMaxGrid = 160;                  // CTAs of the attention launch, at most
-constexpr int kWeighBatch = 4;
-constexpr int kWeighTokens = kWeighBatch * kJoinThreads;   // tokens per CTA of the weight pass
 
 // CTAs [0, blocks): one block each -- join its ranges, normalise, rotate back.  CTAs behind them (with
-// weights): kWeighTokens tokens of one (sequence, KV head) each, p = exp2(score - m) / l summed over its heads.
+// weights): BATCH tokens a thread of one (sequence, KV head) each, p = exp2(score - m) / l summed over its heads.
 // A unit is three round trips to memory: the ranges' (m, l), their sums, and R -- whose first rows are asked
 // for before the grid dependency, thread (group kg, column d) holding rows kg, kg + groups, ... of column d.
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p, int chunks) {
+// CTAS a multiprocessor; RB rows of R a thread asks for at a time; BATCH 0: no weights.
+template <int CTAS, int RB, int BATCH>
+__global__ void __launch_bounds__(kJoinThreads, CTAS) paged_join_kernel(PagedParams p, int chunks) {
     extern __shared__ float jsm[];
     const int tid = threadIdx.x, dim = p.dim, rs = dim + 2, warp = tid >> 5, lane = tid & 31;
     const int blocks = p.units * p.NB;
@@ -840,7 +840,6 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
         float* sF = sO + kHQ * dim;            // [ranges][4] exp2(m_r - m), at most grid ranges
         float* sP = sF + kHQ * p.grid;         // [groups][4][dim] partial rotations
         __shared__ float sInv[kHQ];
-        constexpr int RB = 24;
         const int cols = (dim + 31) / 32 * 32, groups = kJoinThreads / cols;
         const int kg = tid / cols, d = tid - kg * cols;
         const bool mine = kg < groups && d < dim;
@@ -919,13 +918,35 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
         }
         return;
     }
+    if constexpr (BATCH > 0) {
     cudaGridDependencySynchronize();
     // ---- weights: chunks of all rows in turn (a wide table names many that are empty) ------------------
     for (int w = blockIdx.x - blocks; w < p.pg.B * p.pg.Hkv * chunks; w += gridDim.x - blocks) {
+    constexpr int TOKENS = BATCH * kJoinThreads;
     const int chunk = w % chunks, bh = w / chunks, b = bh / p.pg.Hkv, hk = bh % p.pg.Hkv;
     const int L = clamp_len(p.pg, input(p.seq_lens + b));
     const int nv = p.selected ? p.n_sel << p.pg.ps_log2 : L;   // listed or dense tokens
-    if (chunk * kWeighTokens >= nv) continue;
+    if (chunk * TOKENS >= nv) continue;
+    // a thread's tokens: their pages, scores and weights are on their way while the heads' offsets are made
+    const int end = min(nv, (chunk + 1) * TOKENS), i0 = chunk * TOKENS + tid;
+    const float* raw = p.raw + ((int64_t)b * p.UH + hk * p.UG) * p.NB * p.raw_us;
+    const int64_t row = ((int64_t)b * p.pg.Hkv + hk) * p.w_rs;
+    int t[BATCH];
+    float s[BATCH], w0[BATCH];
+    #pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+        const int i = i0 + u * kJoinThreads;
+        t[u] = -1;
+        if (i >= end) continue;
+        const RangePage r = range_page(p, b, hk, i >> p.pg.ps_log2);
+        const int tok = (r.logical << p.pg.ps_log2) + (i & ((1 << p.pg.ps_log2) - 1));
+        if (r.page >= 0 && tok < min(L, p.w_slots)) t[u] = tok;
+    }
+    #pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+        s[u] = t[u] >= 0 ? __ldcg(raw + (int64_t)(i0 + u * kJoinThreads) * p.raw_h) : 0.f;
+        w0[u] = t[u] >= 0 ? __ldcg(p.w_in + row + t[u]) : 0.f;
+    }
     __syncthreads();                           // (the last chunk's offsets are read)
     float* sOff = jsm;                         // [G] m + log2 l
     for (int h = warp; h < p.G; h += kJoinThreads / 32) {
@@ -951,36 +972,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
         if (lane == 0) sOff[h] = mx + log2f(l);
     }
     __syncthreads();
-    // a thread's tokens kWeighBatch at a time: their pages, scores and weights are all on their way before the first
-    // is used
-    const int end = min(nv, (chunk + 1) * kWeighTokens);
-    const float* raw = p.raw + ((int64_t)b * p.UH + hk * p.UG) * p.NB * p.raw_us;
-    const int64_t row = ((int64_t)b * p.pg.Hkv + hk) * p.w_rs;
-    for (int i0 = chunk * kWeighTokens + tid; i0 < end; i0 += kWeighBatch * kJoinThreads) {
-        int t[kWeighBatch];
-        float s[kWeighBatch], w0[kWeighBatch];
-        #pragma unroll
-        for (int u = 0; u < kWeighBatch; ++u) {
-            const int i = i0 + u * kJoinThreads;
-            t[u] = -1;
-            if (i >= end) continue;
-            const RangePage r = range_page(p, b, hk, i >> p.pg.ps_log2);
-            const int tok = (r.logical << p.pg.ps_log2) + (i & ((1 << p.pg.ps_log2) - 1));
-            if (r.page >= 0 && tok < min(L, p.w_slots)) t[u] = tok;
-        }
-        #pragma unroll
-        for (int u = 0; u < kWeighBatch; ++u) {
-            s[u] = t[u] >= 0 ? __ldcg(raw + (int64_t)(i0 + u * kJoinThreads) * p.raw_h) : 0.f;
-            w0[u] = t[u] >= 0 ? __ldcg(p.w_in + row + t[u]) : 0.f;
-        }
-        #pragma unroll
-        for (int u = 0; u < kWeighBatch; ++u) {
-            if (t[u] < 0) continue;
-            float sum = exp2f(s[u] - sOff[0]);
-            for (int h = 1; h < p.G; ++h)
-                sum += exp2f(__ldcg(raw + h / kHQ * p.raw_us + (int64_t)(i0 + u * kJoinThreads) * p.raw_h + h % kHQ) - sOff[h]);
-            p.w_out[row + t[u]] = w0[u] + sum;
-        }
+    #pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+        if (t[u] < 0) continue;
+        float sum = exp2f(s[u] - sOff[0]);
+        for (int h = 1; h < p.G; ++h)
+            sum += exp2f(__ldcg(raw + h / kHQ * p.raw_us + (int64_t)(i0 + u * kJoinThreads) * p.raw_h + h % kHQ) - sOff[h]);
+        p.w_out[row + t[u]] = w0[u] + sum;
+    }
     }
     }
 }
@@ -1066,6 +1065,24 @@ static int launch_paged_any(const pkv_codec* c, const PagedParams& p, cudaStream
     return launch_paged_mode<2, EX>(p, st);
 }
 
+template <int CTAS, int RB, int BATCH>
+static int launch_join(const PagedParams& p, int64_t tokens, int sms, cudaStream_t st) {
+    const int64_t per = BATCH * kJoinThreads, chunks = BATCH ? (tokens + per - 1) / per : 0, all = p.pg.B * p.pg.Hkv * chunks;
+    if (all > 0x7fff0000) return PKV_ERR_UNSUPPORTED;
+    const int64_t ctas = (int64_t)p.units * p.NB + (all < 16 * (int64_t)sms ? all : 16 * (int64_t)sms);
+    const size_t smem = (size_t)(kHQ * p.dim + kHQ * p.grid + kJoinThreads / ((p.dim + 31) / 32 * 32) * kHQ * p.dim) * 4;
+    return launch_behind(paged_join_kernel<CTAS, RB, BATCH>, (unsigned)ctas, kJoinThreads, smem, 0, st, p, (int)chunks);
+}
+
+// With weights: a third CTA per multiprocessor in place of registers where two leave more than three waves of 1536
+// tokens: 128 rows of 16384 tokens 126 -> 120 us in all.  With fewer the join's rows of R count for more: 32 rows of
+// 11469 to 16384 tokens (head size 129) 61.5 us with two, 65.5 with three.
+static int launch_weigh(const PagedParams& p, int sms, cudaStream_t st) {
+    const int64_t tokens = p.raw_us / p.raw_h;              // room for every slot that the table (or the list) can name
+    const int64_t tiles = (int64_t)p.pg.B * p.pg.Hkv * ((tokens + 1535) / 1536);
+    return tiles > 6 * (int64_t)sms ? launch_join<3, 8, 4>(p, tokens, sms, st) : launch_join<2, 24, 6>(p, tokens, sms, st);
+}
+
 int launch_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg, int sms, void* ws, cudaStream_t st) {
     PagedParams p = paged_params(c, a, pg, sms);
     uint8_t* w = static_cast<uint8_t*>(ws);
@@ -1075,12 +1092,7 @@ int launch_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg
     if (a->weights) p.raw = reinterpret_cast<float*>(w + paged_head_bytes(p));
     const int rc = a->out_dtype == PKV_F32 ? launch_paged_any<true>(c, p, st) : launch_paged_any<false>(c, p, st);
     if (rc) return rc;
-    const int chunks = a->weights ? (int)((p.raw_us / p.raw_h + kWeighTokens - 1) / kWeighTokens) : 0;
-    const int64_t all = (int64_t)pg.B * pg.Hkv * chunks;
-    if (all > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-    const int64_t ctas = (int64_t)p.units * p.NB + (all < 16 * (int64_t)sms ? all : 16 * (int64_t)sms);
-    const size_t smem = (size_t)(kHQ * p.dim + kHQ * p.grid + kJoinThreads / ((p.dim + 31) / 32 * 32) * kHQ * p.dim) * 4;
-    return launch_behind(paged_join_kernel, (unsigned)ctas, kJoinThreads, smem, 0, st, p, chunks);
+    return a->weights ? launch_weigh(p, sms, st) : launch_join<2, 24, 0>(p, 0, sms, st);
 }
 
 }  // namespace pkv

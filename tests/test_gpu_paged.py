@@ -202,6 +202,29 @@ def test_attention_and_weights(cuda_ready, lens, Hq, Hkv, dim, variant, bits, qd
     _no_error()
 
 
+@pytest.mark.parametrize("lens,Hq,Hkv,dim", [([3100, 0, 1, 40], 8, 8, 96), ([1700, 20], 18, 2, 96), ([900, 33], 8, 2, 192)])
+def test_weights_under_a_wide_table(cuda_ready, lens, Hq, Hkv, dim):
+    """Room for many more tokens than there are: the same results, whichever form of the weight pass that takes."""
+    c = Cache(_quantizer("v1", (4, 4, 4), dim), lens, Hkv, 16, seed=dim)
+    q = _query(len(lens), Hq, dim)
+    T = c.table.shape[1] * 16
+    w = torch.rand((len(lens), Hkv, T), generator=torch.Generator().manual_seed(3)).to(DEV)
+    want_w = w.clone()
+    want = c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=want_w)
+    ref, tol, _, _ = c.reference(q)
+    _close(want, ref, tol, "out")
+    rows = len(lens) * Hkv
+    for tokens in (T + 1536, 1536 * (1200 // rows + 1)):             # one beside it, and past a thousand tiles of 1536
+        n = -(-tokens // 16)
+        table = torch.full((len(lens), n), -1, dtype=torch.int32, device=DEV)
+        table[:, :c.table.shape[1]] = c.table
+        wide = torch.full((len(lens), Hkv, n * 16), -5.0, device=DEV)
+        wide[..., :T] = w
+        got = c.codec.paged_attention(q, c.k, c.v, table, c.lens, weights=wide)
+        assert torch.equal(got, want) and torch.equal(wide[..., :T], want_w) and (wide[..., T:] == -5.0).all()
+    _no_error()
+
+
 @pytest.mark.parametrize("spread,scale", [(6.0, None), (1.0, 0.0), (1.0, -0.3), (20.0, 1.0)])
 def test_attention_scales(cuda_ready, spread, scale):
     """Peaked, flat, negated and one-token softmaxes; values at the ends of the grid."""
