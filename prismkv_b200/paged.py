@@ -12,9 +12,9 @@ so (num_pages, page_size, kv_heads, m) pools pass as transposed views.
 Nothing here synchronises, keeps results between calls or allocates beyond its
 outputs and a workspace from torch's allocator, so every call can be captured
 into a CUDA graph (``empty_summaries`` or a first ``summarize_pages`` uploads the
-summaries' grid: make one of them before a capture).  A page id outside the pool, a token past the table or a
-page list out of order is skipped on the device and shows in
-``_lib.device_error()`` as 6.
+summaries' grid: make one of them before a capture).  A page id outside the
+pool, a token past the table or a listed page not above the one before it is
+skipped on the device and shows in ``_lib.device_error()`` as 6.
 """
 
 from __future__ import annotations
