@@ -1044,8 +1044,9 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
     return launch_behind(paged_attn_kernel<T>, (unsigned)p.grid, T::THREADS, (size_t)smem, 0, st, p);
 }
 
-// fp32 results get the tiles' sums added in rounded fp32 (4 x 131072 tokens: 180 us against 163); for 16-bit results the
-// truncation of the running sums (a few 1e-6 relative) is far below their own rounding.
+// EX: fp32 results -- outputs, or the running weights whatever type the outputs have -- get z from the middle bin and the
+// tiles' sums added in rounded fp32 (4 x 131072 tokens: 180 us against 163; the weights' error 6e-7 relative against 2e-6
+// to 6e-6). For 16-bit outputs alone the truncation of the running sums (a few 1e-6) is far below their own rounding.
 // Warps by what a lane holds: 16 of 128 registers for up to 32 triplets (14 take 10 % longer, 10 take 20 %), 12 of 168
 // up to 48 (16 spill: + 9 %; 10: + 12 %), 8 of 255 up to 64 (12: + 7 %).
 template <int MODE, bool EX>
@@ -1090,7 +1091,7 @@ int launch_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg
     p.frag = reinterpret_cast<uint32_t*>(w += paged_part_bytes(p));
     p.head = reinterpret_cast<float*>(w += paged_frag_bytes(p));
     if (a->weights) p.raw = reinterpret_cast<float*>(w + paged_head_bytes(p));
-    const int rc = a->out_dtype == PKV_F32 ? launch_paged_any<true>(c, p, st) : launch_paged_any<false>(c, p, st);
+    const int rc = a->out_dtype == PKV_F32 || a->weights ? launch_paged_any<true>(c, p, st) : launch_paged_any<false>(c, p, st);
     if (rc) return rc;
     return a->weights ? launch_weigh(p, sms, st) : launch_join<2, 24, 0>(p, 0, sms, st);
 }

@@ -1,0 +1,27 @@
+"""Paged calls beside the tables of test_gpu_paged.py: what one output's type, an earlier call or a value's size must
+not change.  Tolerances are that file's."""
+
+import pytest
+import torch
+
+from prismkv_b200 import StackedPlaneQuantizer, _lib
+from test_gpu_paged import BF, DEV, F16, F32, U, Cache, _close, _no_error, _quantizer, _query
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("odt", [BF, F16])
+@pytest.mark.parametrize("bits,dim,Hq,Hkv,variant", [
+    ((4, 4, 4), 96, 8, 2, "v1"), ((3, 3, 2), 96, 4, 4, "v1"), ((4, 4, 4), 129, 8, 2, "v1"), ((4, 4, 4), 96, 16, 2, "v1"),
+    ((4, 4, 4), 96, 4, 1, "learned_bias"), ((3, 3, 2), 192, 4, 2, "lloyd")])
+def test_weights_do_not_depend_on_the_output_type(cuda_ready, bits, dim, Hq, Hkv, variant, odt):
+    """The running weights are float32 whatever the outputs are; a 16-bit output is the float32 one, rounded."""
+    c = Cache(_quantizer(variant, bits, dim), [900, 77], Hkv, 16, seed=dim)
+    q = _query(2, Hq, dim)
+    _, _, w, wt = c.reference(q)
+    w32, w16 = (torch.zeros(w.shape, device=DEV) for _ in range(2))
+    out32 = c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=w32)
+    out16 = c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=w16, out_dtype=odt)
+    assert torch.equal(w16, w32) and torch.equal(out16, out32.to(odt))
+    assert ((w16.double() - w).abs() <= wt + Hq // Hkv * w * 2 * U).all()
+    _no_error()
