@@ -226,10 +226,11 @@ class PagedOps:
         need = sizes.get(key)
         if need is None:
             with torch.cuda.device(dev):
-                need = max(int(lib.pkv_paged_attn_workspace_size(self._struct_ref(), args)), 256)
-            if len(sizes) > 256:
-                sizes.clear()
-            sizes[key] = need
+                need = int(lib.pkv_paged_attn_workspace_size(self._struct_ref(), args))
+            if need:                                      # 0: nothing to do, or arguments that the call refuses
+                if len(sizes) > 256:
+                    sizes.clear()
+                sizes[key] = need
         ws = q.new_empty(need, dtype=torch.uint8)
         self._call(lib.pkv_paged_attn, "pkv_paged_attn", dev, self._struct_ref(), args, ws.data_ptr(), need)
         return out

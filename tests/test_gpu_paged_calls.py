@@ -25,3 +25,14 @@ def test_weights_do_not_depend_on_the_output_type(cuda_ready, bits, dim, Hq, Hkv
     assert torch.equal(w16, w32) and torch.equal(out16, out32.to(odt))
     assert ((w16.double() - w).abs() <= wt + Hq // Hkv * w * 2 * U).all()
     _no_error()
+
+
+def test_a_refused_call_does_not_spoil_the_next_one(cuda_ready):
+    """The workspace's size is kept by the shapes; a call that is refused has none to keep."""
+    c = Cache(_quantizer(), [100, 50], 2, 16)
+    q = _query(2, 8, 96)
+    with pytest.raises(RuntimeError, match="invalid"):
+        c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, scale=float("nan"))
+    ref, tol, _, _ = c.reference(q)
+    _close(c.codec.paged_attention(q, c.k, c.v, c.table, c.lens), ref, tol)
+    _no_error()
