@@ -148,7 +148,9 @@ PKV_API int pkv_abi_version(void);
 PKV_API const char *pkv_strerror(int status);
 
 /* Reads (and optionally clears) the device error word set by a kernel whose
- * bounded wait expired.  Synchronous on the current device.                */
+ * bounded wait expired, or (6) that met a page outside the cache.  Of several
+ * errors one is read, and cleared, per call: read until 0.  Synchronous on the
+ * current device.                                                            */
 PKV_API int pkv_device_error(int32_t *flag_out, int32_t clear);
 
 /* codes[n, j] for n < N, j < m.  x: (N, dim) rows of x_dtype, row stride

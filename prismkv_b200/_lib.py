@@ -213,6 +213,7 @@ def raw_stream(index: int) -> int:
 
 
 def device_error(clear: bool = True) -> int:
+    """The current device's error word, 0 for none; of several errors one a call (see pkv_device_error)."""
     flag = c_int32(0)
     check(load().pkv_device_error(ctypes.byref(flag), int(clear)), "pkv_device_error")
     return int(flag.value)

@@ -86,14 +86,12 @@ const char* pkv_strerror(int status) {
 int pkv_device_error(int32_t* flag_out, int32_t clear) {
     if (!flag_out) return PKV_ERR_INVALID;
     if (cudaMemcpyFromSymbol(flag_out, pkv::g_device_error, sizeof(int32_t)) != cudaSuccess) return PKV_ERR_CUDA;
+    if (*flag_out == 0) return pkv::paged_device_error(flag_out, clear);      // the other word waits its turn
     if (clear) {
         const int32_t zero = 0;
         if (cudaMemcpyToSymbol(pkv::g_device_error, &zero, sizeof(int32_t)) != cudaSuccess) return PKV_ERR_CUDA;
     }
-    int32_t paged = 0;
-    const int rc = pkv::paged_device_error(&paged, clear);
-    if (*flag_out == 0) *flag_out = paged;
-    return rc;
+    return PKV_OK;
 }
 
 int pkv_encode(const pkv_codec* c, const void* x, int32_t x_dtype, int64_t n, int64_t x_stride, void* codes,

@@ -15,7 +15,7 @@
 namespace pkv {
 
 // Device error word, one per translation unit: set when a bounded wait expires or a page index is
-// out of range; pkv_device_error reads them all.
+// out of range; pkv_device_error reads them one after the other.
 static __device__ int32_t g_device_error = 0;
 
 // 4: a split-sequence exchange waited past its bound for the other ranks' outputs

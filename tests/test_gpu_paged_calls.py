@@ -36,3 +36,37 @@ def test_a_refused_call_does_not_spoil_the_next_one(cuda_ready):
     ref, tol, _, _ = c.reference(q)
     _close(c.codec.paged_attention(q, c.k, c.v, c.table, c.lens), ref, tol)
     _no_error()
+
+
+def _expired_wait(q):
+    """A split-sequence exchange whose second rank does not exist: the wait runs out after 20 ms and sets error 4."""
+    from prismkv_b200.dist import SequenceExchange
+
+    g = torch.Generator(device=DEV).manual_seed(7)
+    kc, vc = (q.encode_compact(torch.randn(2 * 4 * 3000, 96, generator=g, device=DEV)).view(2, 4, 3000, 32) for _ in range(2))
+    ex = SequenceExchange.single_process(q, _query(2, 16, 96, BF), kc, world=2, wait_ms=20)
+    ex.run(_query(2, 16, 96, BF), kc, vc)
+    torch.cuda.synchronize()
+    return ex
+
+
+def _bad_page():
+    c = Cache(_quantizer(), [100], 2, 16)
+    c.table[0, 1] = c.k.shape[0]
+    c.codec.paged_attention(_query(1, 4, 96), c.k, c.v, c.table, c.lens)
+    torch.cuda.synchronize()
+
+
+def test_no_device_error_hides_another(cuda_ready):
+    """An expired wait and a page outside the pool are both reported, one reading after the other."""
+    _no_error()
+    ex = _expired_wait(_quantizer())
+    try:
+        _bad_page()
+        assert _lib.device_error(clear=False) == 4
+        assert _lib.device_error(clear=True) == 4
+        assert _lib.device_error(clear=False) == 6
+        assert _lib.device_error(clear=True) == 6
+        assert _lib.device_error(clear=True) == 0
+    finally:
+        ex.close()
