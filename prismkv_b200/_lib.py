@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(HERE, "libprismkv_b200.so")
 
 PKV_OK = 0
 PKV_F32, PKV_BF16, PKV_F16 = 0, 1, 2
+PKV_DEVICE_ERR_PAGE = 6                     # pkv_device_error: a page outside the cache
 PKV_CODEC_Z_UNIFORM = 1
 PKV_CODEC_FP32_ATTN = 2
 DTYPE_CODES = {torch.float32: PKV_F32, torch.bfloat16: PKV_BF16, torch.float16: PKV_F16}

@@ -174,7 +174,11 @@ class SequenceExchange:
         """Raise if a bounded wait ran out (synchronises the device)."""
         from . import _lib
         with torch.cuda.device(self.device):
-            err = _lib.device_error(clear=True)
+            err = _lib.device_error(clear=False)
+            if err == _lib.PKV_DEVICE_ERR_PAGE:           # some paged call's, and its caller's to read
+                return
+            if err:
+                _lib.device_error(clear=True)
         if err:
             raise RuntimeError(f"split-sequence exchange: device error {err} (a rank's wait ran out); "
                                "every rank must reset() the exchange before the next step")

@@ -70,3 +70,18 @@ def test_no_device_error_hides_another(cuda_ready):
         assert _lib.device_error(clear=True) == 0
     finally:
         ex.close()
+
+
+def test_exchange_check_leaves_page_errors_to_their_reader(cuda_ready):
+    """A page error is not an expired wait: the exchange's check neither raises for it nor clears it."""
+    _no_error()
+    _bad_page()
+    ex = _expired_wait(_quantizer())
+    try:
+        with pytest.raises(RuntimeError, match="device error 4"):
+            ex.check()
+        ex.check()
+        assert _lib.device_error(clear=True) == 6
+        ex.check()
+    finally:
+        ex.close()
