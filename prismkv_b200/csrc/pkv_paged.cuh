@@ -24,9 +24,9 @@ __device__ __forceinline__ int clamp_len(const Pages& g, int len) {
     return (int)min((int64_t)max(len, 0), cap);
 }
 
-// What a call reads was written by earlier kernels of its stream, whose last one may still run when this one's
-// CTAs come up (launch_behind): such inputs are read by ordinary loads, which stay behind the grid dependency. The
-// read-only path (__ldg), which need not, is for the codec's constant tables.
+// What a call reads -- its inputs and its codec's tables -- was written by earlier kernels of its stream, whose last one
+// may still run when the call's first CTAs come up (launch_behind). A call's first kernel reads it by ordinary loads,
+// which stay behind the grid dependency; the read-only path (__ldg) need not, and is for the tables in later kernels.
 template <class T> __device__ __forceinline__ T input(const T* p) { return *p; }
 
 // Physical page of logical page j of sequence b, or -1 (and the error word) when the table names none.
@@ -63,8 +63,12 @@ static int allow_smem(K kernel, int bytes, std::atomic<int> (&seen)[64]) {
     return PKV_OK;
 }
 
-// A launch whose CTAs may come up while the launch before it in the stream drains: every kernel started this way
-// waits for the grid dependency before it touches anything but its codec's constant tables.
+// A launch whose CTAs may come up while the launch before it in the stream drains (programmatic dependent launch).
+//  * The first kernel of a call waits for the grid dependency before it reads anything, and lets the next kernel come up
+//    (triggers) only after that wait. So whatever ran before the call is complete when a later kernel of the call starts.
+//  * A later kernel may therefore read the call's inputs and tables ahead of its own wait, but what the call's earlier
+//    kernels write only behind it.
+//  * No kernel writes outputs or workspace ahead of its wait, and every CTA waits before it ends.
 template <class... A, class... B>
 static int launch_behind(void (*kernel)(A...), unsigned ctas, int threads, size_t smem, int cluster, cudaStream_t st, B... args) {
     cudaLaunchConfig_t cfg{};

@@ -4,7 +4,7 @@
 //
 // over the sequence's tokens or those of listed pages; optionally weights_out[t] = weights[t] +
 // sum_h p_t / sum p.  Three launches, each started while the one before still runs (programmatic
-// dependent launches; what does not depend on it is read ahead, the rest behind the grid dependency):
+// dependent launches; launch_behind says what each may read ahead of its grid dependency):
 // paged_query_kernel rotates the queries into operand fragments, paged_attn_kernel leaves one partial
 // state per (CTA, unit) range, paged_join_kernel joins a unit's ranges, normalises and rotates back (and,
 // in further CTAs, adds the weights from the scores that the second launch kept).  Small calls are bound by
@@ -98,7 +98,7 @@ __host__ __device__ inline PASmem pa_smem(int dim) {
 struct AffineZ { int c; float zc, dz; };
 __device__ __forceinline__ AffineZ affine_z(const PagedParams& p) {
     const int n = 1 << p.bits_z, c = n >> 1;
-    return {c, __ldg(p.dec_z + c), (__ldg(p.dec_z + n - 1) - __ldg(p.dec_z)) / (float)(n - 1)};
+    return {c, input(p.dec_z + c), (input(p.dec_z + n - 1) - input(p.dec_z)) / (float)(n - 1)};
 }
 
 // triplet j of lane c (scores), triplet i of lane g (values)
@@ -180,6 +180,10 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
     __shared__ int sk[kHQ];
     const int per = p.UG * p.NB;                             // blocks per KV head
     const int b = unit / (p.pg.Hkv * per), u = unit % (p.pg.Hkv * per), hk = u / per, hg = u % per;
+    // What the call reads is there from here on -- for the attention launch too, which comes up once every CTA of
+    // this one is past this point, and reads pages and lengths before it waits for this one's results.
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
     const AffineZ az = affine_z(p);
     const float dz = az.dz;
     float rr[6][6];                                          // rows warp, warp + NW, ... of R, six at a time
@@ -189,14 +193,10 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
             #pragma unroll
             for (int x = 0; x < 6; ++x) {
                 const int k = k0 + i * NW, d = lane + 32 * x;
-                rr[i][x] = (k < dim && d < dim) ? __ldg(p.R + k * dim + d) : 0.f;
+                rr[i][x] = (k < dim && d < dim) ? input(p.R + k * dim + d) : 0.f;
             }
     };
     load_rows(warp);
-    // What the call reads is there from here on -- for the attention launch too, which comes up once every CTA of
-    // this one is past this point, and reads pages and lengths before it waits for this one's results.
-    cudaGridDependencySynchronize();
-    cudaTriggerProgrammaticLaunchCompletion();
     for (int i = tid; i < kHQ * dim; i += kQueryThreads) {
         const int h = hg * kHQ + i / dim;
         sRaw[i] = h < p.G ? load_any(p.q, p.qdt, b * p.q_bs + (int64_t)(hk * p.G + h) * p.q_hs + i % dim) : 0.f;

@@ -137,15 +137,15 @@ __global__ void __launch_bounds__(256) pages_summarize_kernel(SummaryParams p) {
     if (j0 >= j1 || start >= L) return;
     const uint32_t* xy = reinterpret_cast<const uint32_t*>(p.grid_xy);
     int next = j0 + warp < j1 ? page_of(p.pg, b, j0 + warp) : -1;
-    for (int i = tid; i < 1 << p.bits_z; i += 256) gz[i] = __ldg(p.grid_z + i);
+    for (int i = tid; i < 1 << p.bits_z; i += 256) gz[i] = input(p.grid_z + i);
     if constexpr (COPIES) {                                  // 16-byte pieces of four copies, spread over the banks
         for (int e = tid; e < p.entries; e += 256) {
-            const uint32_t v = __ldg(xy + e);
+            const uint32_t v = input(xy + e);
             #pragma unroll
             for (int k = 0; k < 8; ++k) reinterpret_cast<uint4*>(lut)[e * 8 + ((k + e) & 7)] = make_uint4(v, v, v, v);
         }
     } else {
-        for (int i = tid; i < p.entries; i += 256) lut[i] = __ldg(xy + i);
+        for (int i = tid; i < p.entries; i += 256) lut[i] = input(xy + i);
     }
     __syncthreads();
     const int word = lane % LPT, tok = lane / LPT;
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kPageThreads) pages_select_kernel(SelectParams
     for (int k = rank * kPageWarps + warp; k < dim; k += C * kPageWarps) {
         float r[6];
         #pragma unroll
-        for (int x = 0; x < 6; ++x) r[x] = lane + 32 * x < dim ? __ldg(p.R + k * dim + lane + 32 * x) : 0.f;
+        for (int x = 0; x < 6; ++x) r[x] = lane + 32 * x < dim ? input(p.R + k * dim + lane + 32 * x) : 0.f;
         for (int h0 = 0; h0 < p.G; h0 += 4) {
             double a[4] = {0.0, 0.0, 0.0, 0.0};
             #pragma unroll

@@ -85,3 +85,42 @@ def test_exchange_check_leaves_page_errors_to_their_reader(cuda_ready):
         ex.check()
     finally:
         ex.close()
+
+
+def test_codec_tables_written_just_before_the_call(cuda_ready):
+    """The codec's tables are inputs like any other: a kernel right before the call, of the same library or not, may
+    write them."""
+    c = Cache(_quantizer(), [900, 700, 64], 2, 16, seed=5)
+    q, w = _query(3, 8, 96), torch.rand(3, 2, 960, generator=torch.Generator().manual_seed(3)).to(DEV)
+    names = ("_R", "_dz", "_dxy", "_grid_z", "_grid_xy")
+    sums = c.codec.empty_summaries(c.k.shape[0], 2).zero_()
+    first = [getattr(c.codec, n).clone() for n in names]
+    turned = [first[0].view(96, 96).flip(0).reshape(first[0].shape).contiguous(), first[1] * 0.5, first[2] * 0.25, first[3] // 2,
+              first[4] // 4]
+
+    def use(tables, settle):
+        wait = torch.cuda.synchronize if settle else (lambda: None)
+
+        def put():
+            for n, t in zip(names, tables):
+                getattr(c.codec, n).copy_(t)
+            wait()
+
+        put()
+        s = c.codec.summarize_pages(c.k, c.table, c.lens, sums).clone()
+        put()
+        pages = c.codec.select_pages(q, s, c.table, c.lens, 16, 9)
+        put()
+        a = c.codec.paged_attention(q, c.k, c.v, c.table, c.lens)
+        put()
+        w2 = w.clone()
+        b = c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, pages=pages, weights=w2, out_dtype=BF)
+        return s, pages, a, b, w2
+
+    want = [use(t, True) for t in (first, turned)]
+    assert not torch.equal(want[0][2], want[1][2]) and not torch.equal(want[0][0], want[1][0])
+    for i in (1, 0) * 5:
+        got = use((first, turned)[i], False)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want[i]))
+    _no_error()
