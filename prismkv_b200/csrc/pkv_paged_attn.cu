@@ -30,9 +30,9 @@ constexpr int kHQ = 4;                         // query heads per block: with th
 //  * a decoded x, y (and z from a table) is a pair along the contraction: k-pair = (hi, lo);
 //  * queries and softmax weights are pairs across the eight columns: column h < 4 is head h's hi part,
 //    column h + 4 its lo part; both columns are added afterwards.  So all four cross products count.
-//  * table values are scaled by a power of two that puts the largest in [2^9, 2^10), the queries per head by
-//    one that puts theirs in [2^13, 2^14): pairs of normal fp16 whatever the ranges of the codec and the
-//    data.  Weights are 2^12 exp2(score - running max).
+//  * table values are scaled by a power of two that puts the largest in [2^9, 2^10), a bin width dz (MODE 0, 3) by
+//    one that puts it in [1, 2), the queries per head -- z channels times that width -- by one that puts theirs in
+//    [2^13, 2^14): pairs of normal fp16 whatever the ranges of the codec and the data.  Weights are 2^12 exp2(score - running max).
 //  * MODE 0 (two-byte codes, 8 bits of (r, theta)) and 3 (one-byte codes), both with uniform z of up to 4 bits and
 //    one polar grid: z = zc + (i - c) dz, c the middle bin, enters by its index -- for the scores as the exact fp16
 //    subnormal i 2^-24 (EX: as i - c), for the values as the exact i - c; what does not depend on i is added outside.
@@ -161,6 +161,7 @@ template <class T> __device__ __forceinline__ uint32_t look_z(const Lookup& l, c
 }
 
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
+constexpr int kTabLim = 100;                   // tables' and bin widths' powers of two, at most
 // k with |v| 2^k in [2^top, 2^(top + 1)), held in [-lim, lim]; 0 for zero and non-finite v
 __device__ __forceinline__ int pow2_to(float v, int top, int lim) {
     if (!(v > 0.f) || v > 3.0e38f) return 0;
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
     cudaGridDependencySynchronize();
     cudaTriggerProgrammaticLaunchCompletion();
     const AffineZ az = affine_z(p);
-    const float dz = az.dz;
+    const float dz = az.dz * pow2(pow2_to(fabsf(az.dz), 0, kTabLim));
     float rr[6][6];                                          // rows warp, warp + NW, ... of R, six at a time
     auto load_rows = [&](int k0) {
         #pragma unroll
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
             const int k = pow2_to(am, 13, 90);
             sk[warp] = k;
             p.head[unit * 8 + warp] = __int_as_float(k);
-            p.head[unit * 8 + 4 + warp] = affine ? cz * (ex ? az.zc : fmaf(-(float)az.c, dz, az.zc)) : 0.f;
+            p.head[unit * 8 + 4 + warp] = affine ? cz * (ex ? az.zc : fmaf(-(float)az.c, az.dz, az.zc)) : 0.f;
         }
     }
     __syncthreads();
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
         uint32_t v;
         if (r < nxy) {
             v = h2_dup_part(qv(k_triplet_of(cpl, c, r >> 1), 1 + (r & 1)), lo);
-        } else if (affine) {                              // two triplets' z, times the bin width
+        } else if (affine) {                              // two triplets' z, times the scaled bin width
             const int j = 2 * (r - nxy);
             v = h2_pair_part(qv(k_triplet_of(cpl, c, j), 0) * dz, qv(k_triplet_of(cpl, c, j + 1), 0) * dz, lo);
         } else {
@@ -534,7 +535,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
                 bz[x][j][1] = __ldcg(fr + 64 * (CPL + j) + 32);
             }
             const float* hd = p.head + block * 8 + 2 * hp;
-            uu[x] = f2_pack(pow2(-__float_as_int(__ldcg(hd)) - tk), pow2(-__float_as_int(__ldcg(hd + 1)) - tk));
+            uu[x] = f2_pack(pow2(-__float_as_int(__ldcg(hd))) * pow2(-tk), pow2(-__float_as_int(__ldcg(hd + 1))) * pow2(-tk));
             czz[x] = f2_pack(__ldcg(hd + 4), __ldcg(hd + 5));
         }
     };
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
     if (more) start_item();
     #pragma unroll
     for (int w = 0; w < W; ++w) am = fmaxf(am, sRed[w]);
-    tk = pow2_to(am, 9, 30);
+    tk = pow2_to(am, 9, kTabLim);
     fill_tables();                                            // while the first codes are on their way
     __syncthreads();
     cudaGridDependencySynchronize();                          // the queries' fragments
@@ -560,7 +561,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) paged_attn_kernel(PagedParams p
             list_load(nx, nx.g0, sList + (lbuf ^ 1) * T::CHUNK);
             if (tid == 0) *sNext = nx;
         }
-        const float zs = pow2((T::EX ? 0 : 24) + tk);         // AFF: z sums onto the (x, y) sums' scale
+        // AFF: z sums onto the (x, y) sums' scale
+        const float zs = pow2(max(-126, min(127, (T::EX ? 0 : 24) + tk - pow2_to(fabsf(az.dz), 0, kTabLim))));
         float M0[NB], M1[NB], l0[NB], l1[NB];
         float acc[NB][CPV + CPV / 2][4];
         #pragma unroll

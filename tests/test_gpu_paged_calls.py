@@ -124,3 +124,18 @@ def test_codec_tables_written_just_before_the_call(cuda_ready):
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want[i]))
     _no_error()
+
+
+@pytest.mark.parametrize("size", [2.0 ** -40, 2.0 ** -30, 2.0 ** 40])
+@pytest.mark.parametrize("bits", [(4, 4, 4), (3, 3, 2), (2, 5, 5)])
+def test_codecs_of_any_size(cuda_ready, size, bits):
+    """Codecs calibrated to values far from one, queries the other way round: the same softmax, outputs in proportion."""
+    quant = StackedPlaneQuantizer(96, *bits, seed=42, z_min=-7.0 * size, z_max=9.0 * size, r_max=8.0 * size)
+    c = Cache(quant, [300, 21], 2, 16, seed=2, spread=size)
+    q = _query(2, 8, 96) / size
+    ref, tol, w, wt = c.reference(q)
+    for odt in (F32, BF):
+        _close(c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, out_dtype=odt), ref, tol)
+    got = torch.zeros(w.shape, device=DEV)
+    c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=got)
+    assert ((got.double() - w).abs() <= wt + 8 * U * w).all()
