@@ -161,10 +161,10 @@ template <class T> __device__ __forceinline__ uint32_t look_z(const Lookup& l, c
 }
 
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
-constexpr int kTabLim = 100;                   // tables' and bin widths' powers of two, at most
+constexpr int kTabLim = 100, kQueryLim = 126;  // powers of two of tables and bin widths, and of queries, at most
 // k with |v| 2^k in [2^top, 2^(top + 1)), held in [-lim, lim]; 0 for zero and non-finite v
 __device__ __forceinline__ int pow2_to(float v, int top, int lim) {
-    if (!(v > 0.f) || v > 3.0e38f) return 0;
+    if (!(v > 0.f) || v > 3.402823466e38f) return 0;
     const int e = max((int)((__float_as_uint(v) >> 23) & 0xFF) - 127, -126);
     return max(-lim, min(lim, top - e));
 }
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kQueryThreads) paged_query_kernel(PagedParams 
             cz += __shfl_xor_sync(0xffffffffu, cz, off);
         }
         if (lane == 0) {
-            const int k = pow2_to(am, 13, 90);
+            const int k = pow2_to(am, 13, kQueryLim);
             sk[warp] = k;
             p.head[unit * 8 + warp] = __int_as_float(k);
             p.head[unit * 8 + 4 + warp] = affine ? cz * (ex ? az.zc : fmaf(-(float)az.c, az.dz, az.zc)) : 0.f;

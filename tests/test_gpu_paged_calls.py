@@ -139,3 +139,24 @@ def test_codecs_of_any_size(cuda_ready, size, bits):
     got = torch.zeros(w.shape, device=DEV)
     c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=got)
     assert ((got.double() - w).abs() <= wt + 8 * U * w).all()
+
+
+@pytest.mark.parametrize("size", [2.0 ** 100, 2.0 ** 112])
+@pytest.mark.parametrize("bits", [(4, 4, 4), (3, 3, 2), (2, 5, 5)])
+def test_queries_as_large_as_float32_holds(cuda_ready, size, bits):
+    """Scores of 2^100 and more are finite: the largest takes all the weight."""
+    c = Cache(_quantizer(bits=bits), [300, 21], 2, 16, seed=2)
+    q = _query(2, 8, 96) * size
+    out = c.codec.paged_attention(q, c.k, c.v, c.table, c.lens)
+    for b in range(2):
+        for h in range(8):
+            _, k, v = c.slots(b, h // 4)
+            s = (q[b, h].double() @ c.R.T) @ k.T
+            best = s.topk(2)
+            # only where the two best are further apart than the operands' 2^-22 can bring them together
+            if best.values[0] - best.values[1] > 2.0 ** -16 * ((q[b, h].double() @ c.R.T).abs() @ k.abs().T).max():
+                want = v[best.indices[0]] @ c.R
+                assert (out[b, h].double() - want).abs().max() <= 2.0 ** -18 * v[best.indices[0]].norm()
+            else:
+                assert torch.isfinite(out[b, h]).all()
+    _no_error()
