@@ -64,7 +64,8 @@ enum {
 /* ---- codec flags -------------------------------------------------------- */
 #define PKV_CODEC_Z_UNIFORM 1   /* uniform z bins without BiasTable (dec_z affine in i_z) */
 #define PKV_CODEC_FP32_ATTN 2   /* attention arithmetic in fp32 throughout: no fp16-pair
-                                   tensor-core tiles (attn_gqa12_mma_kernel is not planned) */
+                                   tensor-core tiles (attn_gqa12_mma_kernel is not planned,
+                                   pkv_paged_attn returns PKV_ERR_UNSUPPORTED) */
 
 /* ---- element types ----------------------------------------------------- */
 enum { PKV_F32 = 0, PKV_BF16 = 1, PKV_F16 = 2 };
@@ -334,7 +335,9 @@ typedef struct pkv_pages {
     int32_t batch, max_pages;
 } pkv_pages;
 
-/* Decode attention over a paged cache (the mathematics of pkv_attn_decode).
+/* Decode attention over a paged cache (the mathematics of pkv_attn_decode;
+ * operands as fp16 (hi, lo) pairs, 2^-22, sums in fp32: codecs that ask for
+ * PKV_CODEC_FP32_ATTN are PKV_ERR_UNSUPPORTED).
  * selected: optional device (batch, kv_heads, n_selected) logical page indexes,
  * strictly ascending and padded with -1; only their tokens are attended (an
  * entry not above the one before it is skipped and sets the device error word

@@ -114,7 +114,8 @@ class DeviceCodec(PagedOps):
     @property
     def fp32_attention(self) -> bool:
         """Attention arithmetic in fp32 throughout: the grouped 12-bit decode then runs on the fp32
-        kernel instead of the fp16-pair tensor-core one (both are within 1e-5 of fp64)."""
+        kernel instead of the fp16-pair tensor-core one (both are within 1e-5 of fp64).  Paged attention
+        has the fp16-pair form alone and refuses such a codec."""
         return bool(self.struct.flags & _lib.PKV_CODEC_FP32_ATTN)
 
     @fp32_attention.setter

@@ -79,6 +79,7 @@ int check_paged_attn(const pkv_codec* c, const pkv_paged_attn_args* a) {
     if (rc) return rc;
     const pkv_pages& g = a->pages;
     if (g.code_bytes == 1 && c->bits_z + c->bits_r + c->bits_theta > 8) return PKV_ERR_INVALID;
+    if (c->flags & PKV_CODEC_FP32_ATTN) return PKV_ERR_UNSUPPORTED;                // fp16 pairs are all there is
     if (a->q_heads < 1 || a->q_heads % g.kv_heads != 0) return PKV_ERR_INVALID;
     if (a->q_heads / g.kv_heads > 16) return PKV_ERR_UNSUPPORTED;
     if (!paged_dtype(a->q_dtype) || !paged_dtype(a->out_dtype) || !std::isfinite(a->scale)) return PKV_ERR_INVALID;

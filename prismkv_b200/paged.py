@@ -173,7 +173,8 @@ class PagedOps:
         softmax weights, summed over the KV head's query heads, are added --
         in place, or into ``weights_out`` of the same shape, whose other entries
         are not touched; slots must cover every token.  A sequence without
-        tokens gives zeros.
+        tokens gives zeros.  Operands are fp16 (hi, lo) pairs, so a codec with
+        ``fp32_attention`` set is refused.
         """
         dev = self._index()
         g = self._pages(k_pages, v_pages, page_table, dev)
