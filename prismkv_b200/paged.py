@@ -115,7 +115,9 @@ class PagedOps:
         if v is not None:
             if v.get_device() != dev:
                 raise self._elsewhere(v, "v_pages")
-            if v.shape != shape or v.dtype is not dtype or v.stride() != strides:
+            # (a dimension of one element has no stride of its own)
+            if v.shape != shape or v.dtype is not dtype or (v.stride() != strides and any(
+                    n > 1 and a != b for n, a, b in zip(shape, strides, v.stride()))):
                 raise ValueError("k_pages and v_pages must have the same shape, dtype and strides")
             vp = v.data_ptr()
         if strides[3] != 1:
@@ -123,7 +125,6 @@ class PagedOps:
         if ps < 16 or ps > 1024 or ps & (ps - 1):
             raise ValueError(f"page_size must be a power of two from 16 to 1024, got {ps}")
         table, table_stride, B, max_pages = self._check_table(page_table, dev)
-        # (a dimension of one element has no stride of its own)
         return _lib.PkvPages(k.data_ptr(), vp, code_bytes, P, H, ps, strides[0] if P > 1 else 0,
                              strides[1] if H > 1 else 0, strides[2], table, table_stride, B, max_pages)
 

@@ -160,3 +160,19 @@ def test_queries_as_large_as_float32_holds(cuda_ready, size, bits):
             else:
                 assert torch.isfinite(out[b, h]).all()
     _no_error()
+
+
+def test_strides_of_single_pages_and_heads_do_not_count(cuda_ready):
+    """A dimension of one element has no stride of its own: pools that differ there alone are the same."""
+    c = Cache(_quantizer(), [14], 1, 16, seed=4)
+    page = int(c.table[0, 0])
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    k = c.k[page:page + 1].clone(memory_format=torch.contiguous_format)
+    wide = torch.zeros(3, 5, 16, 32, dtype=c.v.dtype, device=DEV)
+    wide[1, 2] = c.v[page, 0]
+    v = wide[1:2, 2:3]
+    assert v.stride() != k.stride()
+    q = _query(1, 4, 96)
+    ref, tol, _, _ = c.reference(q)
+    _close(c.codec.paged_attention(q, k, v, table, c.lens), ref, tol)
+    _no_error()
