@@ -397,7 +397,10 @@ PKV_API int pkv_pages_summarize(const pkv_codec *c, const pkv_pages *pages, cons
  * an upper bound of its tokens' scores.  The first `sinks` and the last
  * `recent` pages of a sequence are always taken; the others by score, ties by
  * the lower index.  out (batch, kv_heads, top): logical page indexes,
- * ascending, -1 behind the last.  sinks + recent <= top.                     */
+ * ascending, -1 behind the last.  sinks + recent <= top.  With G query heads per
+ * KV head, max_pages is at most 8 floor((194560 - G (12 dim + 2 pitch)) / 4) --
+ * 303104 for 16 heads of size 192, 386432 for one of 96 -- else
+ * PKV_ERR_UNSUPPORTED: a longer table passes as its first columns.           */
 PKV_API int pkv_pages_select(const pkv_codec *c, const pkv_pages *pages, const void *q, int32_t q_dtype,
                              int32_t q_heads, int64_t q_batch_stride, int64_t q_head_stride,
                              const int32_t *seq_lens, const int8_t *summaries, int32_t top, int32_t sinks,

@@ -166,7 +166,7 @@ int pkv_pages_select(const pkv_codec* c, const pkv_pages* pages, const void* q, 
     if (q_heads < 1 || q_heads % pages->kv_heads != 0 || !paged_dtype(q_dtype)) return PKV_ERR_INVALID;
     if (q_heads / pages->kv_heads > 16) return PKV_ERR_UNSUPPORTED;
     if (top < 1 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > top) return PKV_ERR_INVALID;
-    if (top > kMaxIndex) return PKV_ERR_UNSUPPORTED;
+    if (top > kMaxIndex || !pkv::pages_select_fits(c->dim, q_heads / pages->kv_heads, pages->max_pages)) return PKV_ERR_UNSUPPORTED;
     if (pages->batch == 0) return PKV_OK;
     if (!q || !seq_lens || !out || (pages->num_pages > 0 && !summaries)) return PKV_ERR_INVALID;
     if (reinterpret_cast<uintptr_t>(summaries) % 16) return PKV_ERR_ALIGNMENT;

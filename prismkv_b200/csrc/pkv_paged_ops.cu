@@ -679,7 +679,12 @@ int launch_tokens_select(const float* w, int B, int Hkv, int slots, int64_t rs, 
     return launch_cluster(tokens_select_kernel<1024, 11>, p, rows, c, 1024, smem, st, seen_long);
 }
 
-// Shared memory of the selection without its keys; keys of a slice take what is left of 190 KB.
+// Shared memory of the selection without its keys; keys of a slice take what is left of 190 KB, so that a cluster of
+// eight holds those of a row of 303104 pages (16 heads of size 192) and more.
+static int64_t select_fixed(int dim, int G) { return (int64_t)G * dim * 12 + 2 * (int64_t)G * ((dim + 15) / 16 * 16); }
+static int64_t select_cap(int dim, int G) { return (190 * 1024 - select_fixed(dim, G)) / 4; }
+bool pages_select_fits(int dim, int G, int max_pages) { return ((int64_t)max_pages + 7) / 8 <= select_cap(dim, G); }
+
 int launch_pages_select(const pkv_codec* c, Pages pg, const void* q, int qdt, int q_heads, int64_t q_bs, int64_t q_hs,
                         const int32_t* lens, const int8_t* sums, int top, int sinks, int recent, int32_t* out, int sms,
                         cudaStream_t st) {
@@ -694,11 +699,9 @@ int launch_pages_select(const pkv_codec* c, Pages pg, const void* q, int qdt, in
     p.sums = sums;
     p.top = top; p.sinks = sinks; p.recent = recent;
     p.out = out;
-    const int64_t fixed = (int64_t)p.G * p.dim * 12 + 2 * (int64_t)p.G * p.pitch;
-    const int64_t cap = (190 * 1024 - fixed) / 4, rows = (int64_t)pg.B * pg.Hkv;
+    const int64_t fixed = select_fixed(p.dim, p.G), cap = select_cap(p.dim, p.G), rows = (int64_t)pg.B * pg.Hkv;
     const int cl = top_cluster(rows, pg.max_pages, sms, cap, 32);
-    const int64_t per = ((int64_t)pg.max_pages + cl - 1) / cl;
-    if (per > cap) return PKV_ERR_UNSUPPORTED;
+    const int64_t per = ((int64_t)pg.max_pages + cl - 1) / cl;   // at most cap: pages_select_fits
     static std::atomic<int> seen3[64], seen6[64];
     const size_t smem = (size_t)(fixed + per * 4);
     if (2 * p.pitch <= 16 * 4 * 3) return launch_cluster(pages_select_kernel<3>, p, rows, cl, kPageThreads, smem, st, seen3);

@@ -305,7 +305,9 @@ class PagedOps:
         taken, the others by an upper bound of their tokens' scores: the KV
         head's queries, rotated and rounded to int8 on a common scale, against
         the summaries' greatest (positive) and least (negative) values; the
-        largest over the heads counts, ties go to the lower page.
+        largest over the heads counts, ties go to the lower page.  A page table
+        of more than about 300000 columns is refused (``pkv_pages_select`` gives
+        the limit): pass the columns that the sequences use.
         """
         if summaries.dim() != 4:
             raise ValueError("summaries must be (num_pages, kv_heads, 2, summary_pitch)")

@@ -176,3 +176,23 @@ def test_strides_of_single_pages_and_heads_do_not_count(cuda_ready):
     ref, tol, _, _ = c.reference(q)
     _close(c.codec.paged_attention(q, k, v, table, c.lens), ref, tol)
     _no_error()
+
+
+def test_page_selection_at_the_widest_table(cuda_ready):
+    """The limit itself is served: the keys of a row's slices fill the shared memory that the cluster has."""
+    c = Cache(_quantizer(dim=192), [900, 30], 1, 16, seed=6)
+    sums = c.codec.summarize_pages(c.k, c.table, c.lens, c.codec.empty_summaries(c.k.shape[0], 1))
+    q = _query(2, 16, 192)
+    want = c.codec.select_pages(q, sums, c.table, c.lens, 16, 9)
+    table = torch.full((2, 303104), -1, dtype=torch.int32, device=DEV)
+    table[:, :c.table.shape[1]] = c.table
+    assert torch.equal(c.codec.select_pages(q, sums, table, c.lens, 16, 9), want)
+    # every page of the row in use: the first sequence's pages over and over
+    long = c.table[:1, :56].repeat(1, 303104 // 56 + 1)[:, :303104].contiguous()
+    lens = torch.full((1,), 303104 * 16, dtype=torch.int32, device=DEV)
+    got = c.codec.select_pages(q[:1], sums, long, lens, 16, 40, sinks=0, recent=0)
+    one = c.codec.select_pages(q[:1], sums, c.table[:1, :56].contiguous(), c.lens[:1] * 0 + 56 * 16, 16, 1, sinks=0, recent=0)
+    assert torch.equal(got[0, 0], one[0, 0] + 56 * torch.arange(40, dtype=torch.int32, device=DEV))
+    with pytest.raises(RuntimeError, match="unsupported"):
+        c.codec.select_pages(q, sums, torch.full((2, 303105), -1, dtype=torch.int32, device=DEV), c.lens, 16, 9)
+    _no_error()
