@@ -94,11 +94,13 @@ class PagedKVCache:
     def _ints(self, values: Sequence[int], dev: torch.device) -> torch.Tensor:
         return torch.tensor(list(values), dtype=torch.int32, device=dev)
 
-    def _push_table(self, st: _PagedLayer) -> None:
-        rows = [r + [-1] * (self.max_pages - len(r)) for r in st.rows]
-        st.table.copy_(torch.tensor(rows, dtype=torch.int32))
+    def _table_of(self, rows: List[List[int]]) -> torch.Tensor:
+        """The page table of these rows, on the host."""
+        return torch.tensor([r + [-1] * (self.max_pages - len(r)) for r in rows], dtype=torch.int32)
 
     # ------------------------------------------------------------------
+    # A change is made on copies, or behind a sequence's end where nothing reads, and becomes the layer's state after
+    # its last launch: a call that raises leaves the layer as it was.
     def append(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, lengths: Optional[Sequence[int]] = None) -> List[int]:
         """Compress and append (batch, kv_heads, s, head_dim) tokens; ``lengths`` (host integers) takes only the
         first lengths[b] of a padded row.  Returns the sequences' new lengths."""
@@ -125,20 +127,22 @@ class PagedKVCache:
                 raise ValueError(f"sequences of {new} tokens exceed {self.max_pages} pages of {ps}")
             if sum(need) > len(st.free):
                 raise RuntimeError(f"layer {layer_idx}: {sum(need)} pages needed, {len(st.free)} free")
-            self._layers[layer_idx] = st
-            for r, n in zip(st.rows, need):
-                for _ in range(n):
-                    r.append(st.free.pop())
-            if any(need):
-                self._push_table(st)
+            total = sum(need)
+            fresh = iter(st.free[len(st.free) - total:][::-1])
+            rows = [r + [next(fresh) for _ in range(n)] if n else r for r, n in zip(st.rows, need)]
+            if total:
+                st.table.copy_(self._table_of(rows))
             start = st.lens.clone()
             cnt = None if lengths is None else self._ints(counts, st.lens.device)
+            lens = start + (s if cnt is None else cnt)
             codec.store_pages(codes[0], st.k, st.table, start, cnt)
             codec.store_pages(codes[1], st.v, st.table, start, cnt)
-            st.lens += s if cnt is None else cnt
-            st.lengths = new
             if st.summaries is not None:
-                codec.summarize_pages(st.k, st.table, st.lens, st.summaries, start=start)
+                codec.summarize_pages(st.k, st.table, lens, st.summaries, start=start)
+            st.lens.copy_(lens)
+            st.rows, st.lengths = rows, new
+            del st.free[len(st.free) - total:]
+            self._layers[layer_idx] = st
             return list(new)
 
     def attention(self, layer_idx: int, q: torch.Tensor, scale: Optional[float] = None, top_pages: Optional[int] = None,
@@ -190,23 +194,28 @@ class PagedKVCache:
             per = -(-keep // self.page_size)
             if per * len(cut) > len(st.free):
                 raise RuntimeError(f"layer {layer_idx}: {per * len(cut)} pages needed, {len(st.free)} free")
-            fresh = {b: [st.free.pop() for _ in range(per)] for b in cut}
+            pages = iter(st.free[len(st.free) - per * len(cut):][::-1])
+            fresh = {b: [next(pages) for _ in range(per)] for b in cut}
             lens = self._ints([st.lengths[b] if b in fresh else 0 for b in range(self.batch)], dev)
             table2 = torch.tensor([fresh.get(b, [-1] * per) for b in range(self.batch)], dtype=torch.int32, device=dev)
             kept, kw = codec.select_tokens(st.weights, lens, keep, sinks=sinks, recent=recent)
             codec.gather_tokens(st.k, st.v, st.table, kept, st.k, st.v, table2)
+            rows = [fresh.get(b, r) for b, r in enumerate(st.rows)]
+            lengths = [keep if b in fresh else n for b, n in enumerate(st.lengths)]
+            table, lens = self._table_of(rows).to(dev), self._ints(lengths, dev)
+            if st.summaries is not None:
+                start = self._ints([0 if b in fresh else n for b, n in enumerate(lengths)], dev)
+                codec.summarize_pages(st.k, table, lens, st.summaries, start=start)
             for b in cut:
-                st.free.extend(reversed(st.rows[b]))
-                st.rows[b] = fresh[b]
-                st.lengths[b] = keep
                 st.weights[b] = 0
                 st.weights[b, :, :keep] = kw[b]
-            self._push_table(st)
-            st.lens.copy_(torch.tensor(st.lengths, dtype=torch.int32))
-            if st.summaries is not None:
-                start = self._ints([0 if b in fresh else n for b, n in enumerate(st.lengths)], dev)
-                codec.summarize_pages(st.k, st.table, st.lens, st.summaries, start=start)
-            return list(st.lengths)
+            st.table.copy_(table)
+            st.lens.copy_(lens)
+            old, st.rows, st.lengths = st.rows, rows, lengths
+            del st.free[len(st.free) - per * len(cut):]
+            for b in cut:
+                st.free.extend(reversed(old[b]))
+            return list(lengths)
 
     # ------------------------------------------------------------------
     def release(self, layer_idx: int, sequence: int) -> None:
@@ -215,12 +224,12 @@ class PagedKVCache:
             raise IndexError(f"sequence {sequence} outside a batch of {self.batch}")
         with self._lock:
             st = self._layer(layer_idx)
-            st.free.extend(reversed(st.rows[sequence]))
-            st.rows[sequence], st.lengths[sequence] = [], 0
+            st.table.copy_(self._table_of([[] if b == sequence else r for b, r in enumerate(st.rows)]))
             st.lens[sequence] = 0
-            self._push_table(st)
             if st.weights is not None:
                 st.weights[sequence] = 0
+            st.free.extend(reversed(st.rows[sequence]))
+            st.rows[sequence], st.lengths[sequence] = [], 0
 
     def clear(self, layer_idx: Optional[int] = None) -> None:
         with self._lock:
