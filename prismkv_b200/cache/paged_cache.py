@@ -177,8 +177,10 @@ class PagedKVCache:
 
     def evict(self, layer_idx: int, keep: int, sinks: int = 4, recent: int = 32) -> List[int]:
         """Cut every sequence of more than ``keep`` tokens to ``keep``: its first ``sinks``, its last ``recent`` and
-        the most attended others of each KV head, in their order.  Returns the new lengths.  The kept tokens move
-        to free pages (ceil(keep / page_size) per sequence, needed for the move) and the old ones come free."""
+        the most attended others of each KV head, in their order.  Returns the new lengths.  The kept tokens move to
+        free pages and the old ones come free, as many sequences at a time as the free pages take
+        (ceil(keep / page_size) each); one that finds no room moves through a buffer of that size into its own first
+        pages, so a full pool can be cut too.  A call that raises leaves sequences as they were or cut."""
         backend = self._backend(layer_idx)
         if not self.track_weights:
             raise RuntimeError("evict needs a cache made with track_weights=True")
@@ -192,30 +194,54 @@ class PagedKVCache:
             if not cut:
                 return list(st.lengths)
             per = -(-keep // self.page_size)
-            if per * len(cut) > len(st.free):
-                raise RuntimeError(f"layer {layer_idx}: {per * len(cut)} pages needed, {len(st.free)} free")
-            pages = iter(st.free[len(st.free) - per * len(cut):][::-1])
-            fresh = {b: [next(pages) for _ in range(per)] for b in cut}
-            lens = self._ints([st.lengths[b] if b in fresh else 0 for b in range(self.batch)], dev)
-            table2 = torch.tensor([fresh.get(b, [-1] * per) for b in range(self.batch)], dtype=torch.int32, device=dev)
+            lens = self._ints([n if n > keep else 0 for n in st.lengths], dev)
             kept, kw = codec.select_tokens(st.weights, lens, keep, sinks=sinks, recent=recent)
-            codec.gather_tokens(st.k, st.v, st.table, kept, st.k, st.v, table2)
-            rows = [fresh.get(b, r) for b, r in enumerate(st.rows)]
-            lengths = [keep if b in fresh else n for b, n in enumerate(st.lengths)]
-            table, lens = self._table_of(rows).to(dev), self._ints(lengths, dev)
+            while cut:
+                n = max(1, min(len(cut), len(st.free) // per))
+                self._move(st, codec, cut[:n], kept, kw)
+                cut = cut[n:]
+            return list(st.lengths)
+
+    def _move(self, st: _PagedLayer, codec, group: List[int], kept: torch.Tensor, kw: torch.Tensor) -> None:
+        """Cut the group's sequences to their kept slots: into free pages or, one without room, its own first ones."""
+        dev, keep = st.lens.device, kept.shape[2]
+        per = -(-keep // self.page_size)
+        room = per * len(group) <= len(st.free)
+        taken = per * len(group) if room else 0
+        fresh = iter(st.free[len(st.free) - taken:][::-1])
+        to = {b: [next(fresh) for _ in range(per)] if room else st.rows[b][:per] for b in group}
+        table2 = torch.tensor([to.get(b, [-1] * per) for b in range(self.batch)], dtype=torch.int32, device=dev)
+        others = torch.tensor([b not in to for b in range(self.batch)], device=dev).view(-1, 1, 1)
+        picks = kept.masked_fill(others, -1)
+        rows = [to.get(b, r) for b, r in enumerate(st.rows)]
+        lengths = [keep if b in to else n for b, n in enumerate(st.lengths)]
+        table, lens = self._table_of(rows).to(dev), self._ints(lengths, dev)
+        start = self._ints([0 if b in to else n for b, n in enumerate(lengths)], dev)
+        if room:
+            codec.gather_tokens(st.k, st.v, st.table, picks, st.k, st.v, table2)
             if st.summaries is not None:
-                start = self._ints([0 if b in fresh else n for b, n in enumerate(lengths)], dev)
                 codec.summarize_pages(st.k, table, lens, st.summaries, start=start)
-            for b in cut:
-                st.weights[b] = 0
-                st.weights[b, :, :keep] = kw[b]
-            st.table.copy_(table)
-            st.lens.copy_(lens)
-            old, st.rows, st.lengths = st.rows, rows, lengths
-            del st.free[len(st.free) - per * len(cut):]
-            for b in cut:
-                st.free.extend(reversed(old[b]))
-            return list(lengths)
+        else:                                             # all that can fail comes before the pages are written over
+            k, v = (codec.empty_pages(per, self.kv_heads, self.page_size, st.k.dtype) for _ in range(2))
+            side = torch.tensor([list(range(per)) if b in to else [-1] * per for b in range(self.batch)], dtype=torch.int32,
+                                device=dev)
+            order = torch.arange(keep, dtype=torch.int32, device=dev).expand(kept.shape).masked_fill(others, -1)
+            codec.gather_tokens(st.k, st.v, st.table, picks, k, v, side)
+            if st.summaries is not None:
+                sums = codec.summarize_pages(k, side, lens.masked_fill(others.view(-1), 0),
+                                             codec.empty_summaries(per, self.kv_heads))
+            codec.gather_tokens(k, v, side, order, st.k, st.v, table2)
+            if st.summaries is not None:
+                st.summaries[table2[group[0]].long()] = sums
+        for b in group:
+            st.weights[b] = 0
+            st.weights[b, :, :keep] = kw[b]
+        st.table.copy_(table)
+        st.lens.copy_(lens)
+        old, st.rows, st.lengths = st.rows, rows, lengths
+        del st.free[len(st.free) - taken:]
+        for b in group:
+            st.free.extend(reversed(old[b] if room else old[b][per:]))
 
     # ------------------------------------------------------------------
     def release(self, layer_idx: int, sequence: int) -> None:

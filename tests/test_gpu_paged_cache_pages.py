@@ -1,0 +1,57 @@
+"""PagedKVCache's pages and buffers on the GPU: eviction with few or no free pages, buffers in proportion to the
+tokens, attention captured into a graph."""
+
+import pytest
+import torch
+
+from prismkv_b200 import _lib
+from prismkv_b200.cache import PagedKVCache, PrismKVBackend, PrismKVConfig, RawKVCache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _kv(B, H, s, d, seed):
+    g = torch.Generator().manual_seed(seed)
+    return tuple(torch.randn(B, H, s, d, generator=g).to(DEV) for _ in range(2))
+
+
+def _q(B, H, d, seed=1):
+    return torch.randn(B, H, d, generator=torch.Generator().manual_seed(seed)).to(DEV)
+
+
+def _filled(num_pages, lengths, seed=3):
+    """A cache of 2 KV heads that has attended once, and what it holds."""
+    backend = PrismKVBackend(PrismKVConfig(), head_dim=96)
+    cache = PagedKVCache(backend, len(lengths), 2, num_pages=num_pages, page_size=16, page_summaries=True, track_weights=True)
+    k, v = _kv(len(lengths), 2, max(lengths), 96, seed)
+    q = _q(len(lengths), 4, 96)
+    cache.append(0, k, v, lengths=lengths)
+    cache.attention(0, q)
+    return cache, q
+
+
+@pytest.mark.parametrize("lengths,keep", [([100, 90, 20], 40), ([64, 64, 64], 48), ([33, 64, 17], 32), ([40, 40, 1], 1)])
+def test_eviction_needs_no_free_pages(cuda_ready, lengths, keep):
+    """The same tokens stay whether the pool has room for every move, for some or for none."""
+    used = sum(-(-n // 16) for n in lengths)
+    per = -(-keep // 16)
+    roomy, q = _filled(used + 100, lengths)
+    want_n = roomy.evict(0, keep, sinks=0, recent=1)
+    want = roomy.attention(0, q)
+    for spare in (0, 1, per, 2 * per):
+        cache, _ = _filled(used + spare, lengths)
+        assert cache.free_pages(0) == spare
+        assert cache.evict(0, keep, sinks=0, recent=1) == want_n == [min(n, keep) for n in lengths]
+        left = used + spare - sum(-(-n // 16) for n in want_n)
+        assert cache.free_pages(0) == left
+        owned = [p for row in cache._layers[0].rows for p in row]
+        assert sorted(owned + cache._layers[0].free) == list(range(used + spare))
+        assert torch.equal(cache.attention(0, q), want)
+        n = max(want_n)
+        assert torch.equal(cache.get_weights(0)[..., :n], roomy.get_weights(0)[..., :n])
+        assert (cache.attention(0, q, top_pages=max(2, per)) - cache.attention(0, q)).abs().max() <= 1e-4
+        if left:                                        # the freed pages serve again
+            more = [1 if n % 16 else 0 for n in want_n]
+            cache.append(0, *_kv(3, 2, 1, 96, 5), lengths=more)
+    assert _lib.device_error() == 0

@@ -187,3 +187,93 @@ def test_a_failed_eviction_changes_nothing(monkeypatch, call):
     assert (cache.free_pages(0), cache.get_seq_lengths(0), [_content(cache, b) for b in range(3)]) == state
     assert cache.evict(0, 20, sinks=1, recent=2) == [20, 10, 20]
     _whole(cache)
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_appends_evictions_and_releases_against_lists(seed):
+    """A run of calls on a pool that is nearly always full: tokens, weights and pages as plain lists have them."""
+    rng = random.Random(seed)
+    batch, num_pages = rng.choice([1, 2, 3, 5]), rng.randint(4, 14)
+    cache = _cache(batch, num_pages, max_tokens=rng.choice([None, num_pages * 16]))
+    model = [[([], [], []) for _ in range(2)] for _ in range(batch)]     # per sequence and head: K, V, weights
+    at = 0
+    for _ in range(25):
+        act = rng.choice(["append", "append", "append", "evict", "attend", "release"])
+        used = lambda: sum(-(-len(m[0][0]) // 16) for m in model)  # noqa: E731
+        if act == "append":
+            s = rng.choice([1, 5, 16, 33])
+            n = [rng.randint(0, s) for _ in range(batch)]
+            k, v = _tokens(batch, s, at % 800)
+            at += s
+            fits = sum(-(-(len(m[0][0]) + x) // 16) for m, x in zip(model, n)) <= num_pages
+            if not fits:
+                with pytest.raises((RuntimeError, ValueError)):
+                    cache.append(0, k, v, lengths=n)
+                continue
+            cache.append(0, k, v, lengths=n)
+            for b in range(batch):
+                for h in range(2):
+                    for x, src in ((0, k), (1, v)):
+                        model[b][h][x].extend(src[b, h, :n[b], 0].int().tolist())
+                    model[b][h][2].extend([0.0] * n[b])
+        elif 0 not in cache.cached_layers:
+            continue
+        elif act == "attend":
+            cache.attention(0, torch.zeros(batch, 2, 3))
+            for m in model:
+                for kk, _, ww in m:
+                    ww[:] = [w + x + 1 for w, x in zip(ww, kk)]
+        elif act == "release":
+            b = rng.randrange(batch)
+            cache.release(0, b)
+            model[b] = [([], [], []) for _ in range(2)]
+        else:
+            keep = rng.choice([1, 7, 16, 30])
+            sinks, recent = rng.choice([(0, 0), (0, 1), (min(2, keep - 1), 1), (0, keep)])
+            cache.evict(0, keep, sinks=sinks, recent=recent)             # never refused, however full the pool
+            for m in model:
+                n = len(m[0][0])
+                if n > keep:
+                    for h in range(2):
+                        w = m[h][2]
+                        order = sorted(range(n), key=lambda i: (not (i < sinks or i >= n - recent), -w[i], i))
+                        ids = sorted(order[:keep])
+                        m[h] = tuple([x[i] for i in ids] for x in m[h])
+        if 0 in cache.cached_layers:
+            _whole(cache)
+            assert cache.free_pages(0) == num_pages - used()
+            for b in range(batch):
+                assert _content(cache, b) == [tuple(x) for x in model[b]], (act, b)
+
+
+@pytest.mark.parametrize("call,nth", [("select_tokens", 1), ("gather_tokens", 1), ("gather_tokens", 2), ("summarize_pages", 1),
+                                      ("empty_pages", 1), ("empty_pages", 2), ("empty_summaries", 1)])
+def test_a_failed_eviction_of_a_full_pool_changes_nothing(monkeypatch, call, nth):
+    cache = _cache(num_pages=8)
+    codec = cache._backend(0)._codec
+    cache.append(0, *_tokens(3, 60, 0), lengths=[60, 10, 45])
+    assert cache.free_pages(0) == 0
+    cache.attention(0, torch.zeros(3, 2, 3))
+    state = cache.get_seq_lengths(0), [_content(cache, b) for b in range(3)], cache._layers[0].summaries.clone()
+    real, count = getattr(codec, call), [0]
+
+    def fail(*a, **k):
+        count[0] += 1
+        if count[0] == nth:
+            raise RuntimeError("broken")
+        return real(*a, **k)
+
+    with monkeypatch.context() as mp:
+        mp.setattr(codec, call, fail)
+        with pytest.raises(RuntimeError, match="broken"):
+            cache.evict(0, 20, sinks=1, recent=2)
+    _whole(cache)
+    assert (cache.get_seq_lengths(0), [_content(cache, b) for b in range(3)]) == state[:2]
+    assert torch.equal(cache._layers[0].summaries, state[2])
+    assert cache.evict(0, 20, sinks=1, recent=2) == [20, 10, 20]
+    _whole(cache)
+    # the summaries are those of the pages as they are
+    k, _, table, lens = cache.get_pages(0)
+    want = codec.summarize_pages(k, table, lens, codec.empty_summaries(8, 2))
+    for r in cache._layers[0].rows:
+        assert torch.equal(cache._layers[0].summaries[r], want[r])
