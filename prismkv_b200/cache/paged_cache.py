@@ -43,6 +43,14 @@ class _PagedLayer:
     weights: Optional[torch.Tensor] = None
 
 
+def _capturing(dev: torch.device) -> bool:
+    """Whether the device's current stream records a CUDA graph, to be replayed when the sequences are longer."""
+    if dev.type != "cuda":
+        return False
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class PagedKVCache:
     """backend: one CacheBackend for every layer, or a dict keyed by layer index; batch sequences of kv_heads
     heads share num_pages pages (per layer) of page_size tokens.  max_tokens: the longest sequence (default: all
@@ -150,7 +158,8 @@ class PagedKVCache:
         """Decode attention of q (batch, q_heads, head_dim) -> the same shape.
 
         ``top_pages``: attend to that many pages per KV head at most, the first
-        ``sinks`` and last ``recent`` among them.
+        ``sinks`` and last ``recent`` among them.  Captured into a CUDA graph,
+        the call follows the cache's later changes when it is replayed.
         """
         backend = self._backend(layer_idx)
         if q.dim() != 3 or q.shape[2] != backend.head_dim:
@@ -168,7 +177,7 @@ class PagedKVCache:
                 if top_pages < 1 or sinks < 0 or recent < 0 or sinks + recent > top_pages:
                     raise ValueError("need 0 <= sinks + recent <= top_pages and top_pages >= 1, "
                                      f"got {sinks}, {recent}, {top_pages}")
-                if max(len(r) for r in st.rows) > top_pages:
+                if max(len(r) for r in st.rows) > top_pages or _capturing(st.lens.device):
                     pages = codec.select_pages(qp, st.summaries, st.table, st.lens, self.page_size, top_pages, sinks=sinks,
                                                recent=recent)
             out = codec.paged_attention(qp, st.k, st.v, st.table, st.lens, scale=scale, pages=pages, weights=st.weights,

@@ -55,3 +55,34 @@ def test_eviction_needs_no_free_pages(cuda_ready, lengths, keep):
             more = [1 if n % 16 else 0 for n in want_n]
             cache.append(0, *_kv(3, 2, 1, 96, 5), lengths=more)
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("track", [False, True])
+def test_captured_attention_follows_the_cache(cuda_ready, track):
+    """Attention captured while the sequences are short, replayed as they grow and after an eviction."""
+    backend = PrismKVBackend(PrismKVConfig(), head_dim=96)
+    make = lambda: PagedKVCache(backend, 2, 2, num_pages=40, page_size=16, max_tokens=320, page_summaries=True,  # noqa: E731
+                                track_weights=track)
+    caches, q = [make(), make()], _q(2, 4, 96)
+    for c in caches:
+        c.append(0, *_kv(2, 2, 20, 96, 0))
+        c.attention(0, q), c.attention(0, q, top_pages=3)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        held = caches[0].attention(0, q), caches[0].attention(0, q, top_pages=3)
+    for step in range(3):
+        g.replay()
+        want = caches[1].attention(0, q), caches[1].attention(0, q, top_pages=3)
+        torch.cuda.synchronize()
+        assert torch.equal(held[0], want[0]) and torch.equal(held[1], want[1]), step
+        if track:
+            w = [c.get_weights(0) for c in caches]
+            assert torch.equal(*w)
+        for c in caches:
+            if step == 0:
+                c.append(0, *_kv(2, 2, 150, 96, 1), lengths=[150, 60])
+            elif track:
+                c.evict(0, 50)
+    assert _lib.device_error() == 0
+
