@@ -47,6 +47,8 @@ def _capturing(dev: torch.device) -> bool:
     """Whether the device's current stream records a CUDA graph, to be replayed when the sequences are longer."""
     if dev.type != "cuda":
         return False
+    if torch.cuda.current_device() == dev.index:
+        return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(dev):
         return torch.cuda.is_current_stream_capturing()
 
@@ -54,7 +56,11 @@ def _capturing(dev: torch.device) -> bool:
 class PagedKVCache:
     """backend: one CacheBackend for every layer, or a dict keyed by layer index; batch sequences of kv_heads
     heads share num_pages pages (per layer) of page_size tokens.  max_tokens: the longest sequence (default: all
-    pages in one).  page_summaries: keep what ``top_pages`` needs; track_weights: keep what ``evict`` needs."""
+    pages in one).  page_summaries: keep what ``top_pages`` needs; track_weights: keep what ``evict`` needs.
+
+    Attention weights are a buffer of (batch, kv_heads, slots) floats.  With ``max_tokens``, and wherever slots for
+    the whole pool take at most a quarter of what the codes take, it is made once; otherwise it is replaced by a wider
+    one when the longest sequence outgrows it, and attention cannot be captured into a CUDA graph."""
 
     def __init__(self, backend: Union[CacheBackend, Dict[int, CacheBackend]], batch: int, kv_heads: int, num_pages: int,
                  page_size: int = 16, max_tokens: Optional[int] = None, page_summaries: bool = False,
@@ -70,6 +76,7 @@ class PagedKVCache:
         if self.max_pages < 1:
             raise ValueError(f"max_tokens must be positive, got {max_tokens}")
         self.page_summaries, self.track_weights = page_summaries, track_weights
+        self._whole = max_tokens is not None                  # weights for the longest possible sequence at once
         self._device = device
         self._layers: Dict[int, _PagedLayer] = {}
         self._lock = threading.Lock()
@@ -96,8 +103,20 @@ class PagedKVCache:
         if self.page_summaries:
             st.summaries = codec.empty_summaries(self.num_pages, self.kv_heads)
         if self.track_weights:
-            st.weights = torch.zeros((self.batch, self.kv_heads, self.max_pages * self.page_size), device=dev)
+            slots = self.max_pages * self.page_size
+            codes = 2 * self.num_pages * self.page_size * k.stride(2) * k.element_size()
+            whole = self._whole or 4 * (4 * self.batch * slots) <= codes
+            st.weights = torch.zeros((self.batch, self.kv_heads, slots if whole else 0), device=dev)
         return st
+
+    def _wide_enough(self, st: _PagedLayer, pages: int) -> Optional[torch.Tensor]:
+        """The layer's weights, in a wider buffer where sequences of so many pages need it."""
+        w, ps = st.weights, self.page_size
+        if w is None or w.shape[2] >= pages * ps:
+            return w
+        wide = w.new_zeros((self.batch, self.kv_heads, min(self.max_pages, max(pages, w.shape[2] // ps * 3 // 2)) * ps))
+        wide[..., :w.shape[2]] = w
+        return wide
 
     def _ints(self, values: Sequence[int], dev: torch.device) -> torch.Tensor:
         return torch.tensor(list(values), dtype=torch.int32, device=dev)
@@ -138,6 +157,7 @@ class PagedKVCache:
             total = sum(need)
             fresh = iter(st.free[len(st.free) - total:][::-1])
             rows = [r + [next(fresh) for _ in range(n)] if n else r for r, n in zip(st.rows, need)]
+            weights = self._wide_enough(st, max(map(len, rows)))
             if total:
                 st.table.copy_(self._table_of(rows))
             start = st.lens.clone()
@@ -148,7 +168,7 @@ class PagedKVCache:
             if st.summaries is not None:
                 codec.summarize_pages(st.k, st.table, lens, st.summaries, start=start)
             st.lens.copy_(lens)
-            st.rows, st.lengths = rows, new
+            st.rows, st.lengths, st.weights = rows, new, weights
             del st.free[len(st.free) - total:]
             self._layers[layer_idx] = st
             return list(new)
@@ -170,6 +190,16 @@ class PagedKVCache:
             st = self._layer(layer_idx)
             codec = backend.codec(st.lens.device)
             qp = backend.aligner.pad(q.to(st.lens.device))
+            longest, capturing = max(map(len, st.rows)), _capturing(st.lens.device)
+            # tables and weights as far as the longest sequence goes: scratch and grids go by their width. A graph will
+            # be replayed over longer ones.
+            width = self.max_pages if capturing else max(longest, 1)
+            table, weights = st.table[:, :width], st.weights
+            if weights is not None:
+                if capturing and weights.shape[2] < width * self.page_size:
+                    raise RuntimeError("attention captured into a graph needs weights that are not replaced as sequences "
+                                       "grow: make the cache with max_tokens")
+                weights = weights[..., :width * self.page_size]
             pages = None
             if top_pages is not None:
                 if not self.page_summaries:
@@ -177,10 +207,10 @@ class PagedKVCache:
                 if top_pages < 1 or sinks < 0 or recent < 0 or sinks + recent > top_pages:
                     raise ValueError("need 0 <= sinks + recent <= top_pages and top_pages >= 1, "
                                      f"got {sinks}, {recent}, {top_pages}")
-                if max(len(r) for r in st.rows) > top_pages or _capturing(st.lens.device):
-                    pages = codec.select_pages(qp, st.summaries, st.table, st.lens, self.page_size, top_pages, sinks=sinks,
+                if longest > top_pages or capturing:
+                    pages = codec.select_pages(qp, st.summaries, table, st.lens, self.page_size, top_pages, sinks=sinks,
                                                recent=recent)
-            out = codec.paged_attention(qp, st.k, st.v, st.table, st.lens, scale=scale, pages=pages, weights=st.weights,
+            out = codec.paged_attention(qp, st.k, st.v, table, st.lens, scale=scale, pages=pages, weights=weights,
                                         out_dtype=out_dtype)
         return backend.aligner.unpad(out)
 
@@ -204,7 +234,8 @@ class PagedKVCache:
                 return list(st.lengths)
             per = -(-keep // self.page_size)
             lens = self._ints([n if n > keep else 0 for n in st.lengths], dev)
-            kept, kw = codec.select_tokens(st.weights, lens, keep, sinks=sinks, recent=recent)
+            longest = max(map(len, st.rows)) * self.page_size
+            kept, kw = codec.select_tokens(st.weights[..., :longest], lens, keep, sinks=sinks, recent=recent)
             while cut:
                 n = max(1, min(len(cut), len(st.free) // per))
                 self._move(st, codec, cut[:n], kept, kw)
@@ -282,7 +313,8 @@ class PagedKVCache:
         return self.num_pages if st is None else len(st.free)
 
     def get_weights(self, layer_idx: int) -> Optional[torch.Tensor]:
-        """(batch, kv_heads, slots) accumulated attention weights; a sequence's tokens come first."""
+        """(batch, kv_heads, slots) accumulated attention weights, slots for the longest sequence at least; a
+        sequence's tokens come first."""
         return self._layer(layer_idx).weights
 
     def get_pages(self, layer_idx: int):

@@ -150,6 +150,20 @@ class PagedOps:
             strides = q.stride()
         return q, shape, strides, code
 
+    def _weight_rows(self, t: torch.Tensor, name: str, B: int, H: int, dev: int) -> int:
+        """Floats from one (sequence, KV head) row of weights to the next."""
+        if t.get_device() != dev:
+            raise self._elsewhere(t, name)
+        if t.dtype is torch.float32 and t.dim() == 3 and t.shape[:2] == (B, H):
+            n = t.shape[2]
+            if t.is_contiguous():
+                return n
+            s0, s1, s2 = t.stride()
+            row = s1 if H > 1 else s0 if B > 1 else n
+            if (n <= 1 or s2 == 1) and (B <= 1 or H <= 1 or s0 == H * s1) and row >= n:
+                return row
+        raise ValueError(f"{name} must be a float32 ({B}, {H}, slots) tensor, contiguous or the first slots of one")
+
     def _call(self, fn, what: str, dev: int, *args) -> None:
         """fn(*args, stream) with CUDA device ``dev`` current; a non-zero status raises."""
         if torch.cuda.current_device() == dev:
@@ -168,6 +182,9 @@ class PagedOps:
                         out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """Decode attention over a paged cache: q (B, Hq, dim) [or (B, Hq, 1, dim)] -> (B, Hq, dim) of out_dtype.
 
+        The workspace holds a float per query head and slot of the page table
+        when there are ``weights``: pass the table's first columns, as far as
+        the longest sequence goes, and the weights' first slots.
         ``pages`` (B, Hkv, n) int32 restricts each KV head to the listed logical
         pages (``select_pages`` makes such lists): strictly ascending, -1 behind
         the last.  ``weights`` (B, Hkv, slots) fp32: every attended token's
@@ -204,22 +221,19 @@ class PagedOps:
             if n_selected == 0:
                 raise ValueError("pages lists no page; leave it out to attend to every token")
         w_in = w_out = None
-        slots = 0
+        slots = row = 0
         if weights_out is not None and weights is None:
             raise ValueError("weights_out needs weights")
         if weights is not None:
             to = weights if weights_out is None else weights_out
-            for t, n in ((weights, "weights"), (to, "weights_out")):
-                if t.get_device() != dev:
-                    raise self._elsewhere(t, n)
-                if t.dtype is not torch.float32 or t.dim() != 3 or t.shape[:2] != (B, kv_heads) or not t.is_contiguous():
-                    raise ValueError(f"{n} must be a contiguous float32 ({B}, {kv_heads}, slots) tensor")
-            if to.shape != weights.shape:
-                raise ValueError("weights and weights_out must have the same shape")
+            row = self._weight_rows(weights, "weights", B, kv_heads, dev)
+            if to is not weights:
+                if self._weight_rows(to, "weights_out", B, kv_heads, dev) != row or to.shape != weights.shape:
+                    raise ValueError("weights and weights_out must have the same shape and strides")
             w_in, w_out, slots = weights.data_ptr(), to.data_ptr(), weights.shape[2]
         args = ctypes.byref(_lib.PkvPagedAttnArgs(
             g, Hq, q_code, q.data_ptr(), qs[0], qs[1], lens, selected, n_selected,
-            self.dim ** -0.5 if scale is None else float(scale), out.data_ptr(), out_code, os[0], os[1], w_in, w_out, slots,
+            self.dim ** -0.5 if scale is None else float(scale), out.data_ptr(), out_code, os[0], os[1], w_in, w_out, row,
             slots))
         lib = _lib.load()
         # the workspace's size follows from the shapes alone
@@ -341,17 +355,16 @@ class PagedOps:
         NaN last), ascending; -1 and 0 behind the last.
         """
         dev = self._index()
-        if weights.get_device() != dev:
-            raise self._elsewhere(weights, "weights")
-        if weights.dim() != 3 or weights.dtype is not torch.float32 or not weights.is_contiguous():
-            raise ValueError("weights must be a contiguous float32 (batch, kv_heads, slots) tensor")
+        if weights.dim() != 3:
+            raise ValueError("weights must be a float32 (batch, kv_heads, slots) tensor")
+        row = self._weight_rows(weights, "weights", weights.shape[0], weights.shape[1], dev)
         if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
             raise ValueError(f"need 0 <= sinks + recent <= keep and keep >= 1, got {sinks}, {recent}, {keep}")
         B, H, T = weights.shape
         lens = self._check_ints(seq_lens, "seq_lens", (B,), dev)
         kept = weights.new_empty((B, H, keep), dtype=torch.int32)
         kw = weights.new_empty((B, H, keep))
-        self._call(_lib.load().pkv_tokens_select, "pkv_tokens_select", dev, weights.data_ptr(), B, H, T, T, lens, keep,
+        self._call(_lib.load().pkv_tokens_select, "pkv_tokens_select", dev, weights.data_ptr(), B, H, T, row, lens, keep,
                    sinks, recent, kept.data_ptr(), kw.data_ptr())
         return kept, kw
 

@@ -86,3 +86,55 @@ def test_captured_attention_follows_the_cache(cuda_ready, track):
                 c.evict(0, 50)
     assert _lib.device_error() == 0
 
+
+
+def test_buffers_follow_the_tokens_not_the_pool(cuda_ready):
+    """Running weights and an attention call's scratch grow with the longest sequence, not with the pool."""
+    B, H, Hq, d = 16, 2, 8, 96
+    backend = PrismKVBackend(PrismKVConfig(), head_dim=d)
+    cache = PagedKVCache(backend, B, H, num_pages=B * 256, page_size=16, page_summaries=True, track_weights=True)
+    q = _q(B, Hq, d)
+    k, v = _kv(B, H, 40, d, 0)
+    cache.append(0, k, v)
+    slots = 48
+    cache.attention(0, q)
+    assert cache.get_weights(0).shape[:2] == (B, H) and slots <= cache.get_weights(0).shape[2] <= 4 * slots
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = cache.attention(0, q)
+    used = torch.cuda.max_memory_allocated() - before
+    # scores of 48 slots (16 x 8 rows), and what does not depend on lengths: partial states and query fragments
+    fixed = 4 * (160 + B * H) * 2 * 4 * (d + 2) + 4 * B * H * 2 * (48 * 32 + 8) + out.numel() * 4
+    assert used <= 4 * B * Hq * slots + fixed + (1 << 16)
+    # growth keeps what was there
+    before = cache.get_weights(0)[..., :slots].clone()
+    cache.append(0, *_kv(B, H, 300, d, 1))
+    assert torch.equal(cache.get_weights(0)[..., :slots], before) and not cache.get_weights(0)[..., slots:].any()
+    wide = PagedKVCache(backend, B, H, num_pages=B * 256, page_size=16, max_tokens=4096, track_weights=True)
+    for s, seed in ((40, 0), (300, 1)):
+        wide.append(0, *_kv(B, H, s, d, seed))
+        if s == 40:
+            wide.attention(0, q), wide.attention(0, q)
+    assert wide.get_weights(0).shape == (B, H, 4096)
+    assert torch.equal(wide.attention(0, q), cache.attention(0, q))
+    n = cache.get_weights(0).shape[2]
+    assert torch.equal(wide.get_weights(0)[..., :n], cache.get_weights(0)) and not wide.get_weights(0)[..., n:].any()
+    assert cache.evict(0, 64) == wide.evict(0, 64) == [64] * B
+    assert torch.equal(wide.attention(0, q), cache.attention(0, q))
+    assert _lib.device_error() == 0
+
+
+def test_capture_with_buffers_that_may_grow_is_refused(cuda_ready):
+    """Without max_tokens the weights' buffer is replaced when a sequence outgrows it; a graph would hold the old one."""
+    backend = PrismKVBackend(PrismKVConfig(), head_dim=96)
+    cache = PagedKVCache(backend, 12, 2, num_pages=240, page_size=16, track_weights=True)
+    cache.append(0, *_kv(12, 2, 20, 96, 0))
+    q = _q(12, 4, 96)
+    want = cache.attention(0, q)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="max_tokens"):
+        with torch.cuda.graph(g):
+            cache.attention(0, q)
+    assert torch.equal(cache.attention(0, q), want)

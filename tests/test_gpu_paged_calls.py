@@ -196,3 +196,49 @@ def test_page_selection_at_the_widest_table(cuda_ready):
     with pytest.raises(RuntimeError, match="unsupported"):
         c.codec.select_pages(q, sums, torch.full((2, 303105), -1, dtype=torch.int32, device=DEV), c.lens, 16, 9)
     _no_error()
+
+
+@pytest.mark.parametrize("lens,Hq,Hkv", [([100, 50], 8, 2), ([90], 4, 4), ([70, 33, 5], 4, 1), ([60], 2, 1)])
+def test_weights_may_be_the_first_slots_of_wider_rows(cuda_ready, lens, Hq, Hkv):
+    """The columns of a table and the slots of the weights as far as the tokens go: the same, and nothing behind them."""
+    c = Cache(_quantizer(), lens, Hkv, 16, seed=8)
+    B, n = len(lens), -(-max(lens) // 16)
+    q = _query(B, Hq, 96)
+    w = torch.rand(B, Hkv, c.table.shape[1] * 16, generator=torch.Generator().manual_seed(3)).to(DEV)
+    want_w = w.clone()
+    want = c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=want_w)
+    kept, kw = c.codec.select_tokens(want_w, c.lens, 30, recent=2)
+    wide = torch.full((B, Hkv, w.shape[2] + 7), -5.0, device=DEV)
+    wide[..., :w.shape[2]] = w
+    view = wide[..., :n * 16]
+    assert torch.equal(c.codec.paged_attention(q, c.k, c.v, c.table[:, :n], c.lens, weights=view), want)
+    assert torch.equal(wide[..., :w.shape[2]], want_w) and (wide[..., w.shape[2]:] == -5.0).all()
+    got = c.codec.select_tokens(view, c.lens, 30, recent=2)
+    assert torch.equal(got[0], kept) and torch.equal(got[1], kw)
+    to = torch.full_like(wide, -6.0)[..., :n * 16]
+    wide[..., :w.shape[2]] = w
+    c.codec.paged_attention(q, c.k, c.v, c.table[:, :n], c.lens, weights=view, weights_out=to)
+    for b, t in enumerate(lens):
+        assert torch.equal(to[b, :, :t], want_w[b, :, :t]) and (to[b, :, t:] == -6.0).all()
+    _no_error()
+
+
+def test_weights_in_other_strides_are_refused(cuda_ready):
+    c = Cache(_quantizer(), [100, 50], 2, 16)
+    q, full = _query(2, 8, 96), torch.zeros(2, 2, 256, device=DEV)
+    good = full[..., :128]
+    for bad in (full[..., ::2], torch.zeros(1, 1, 128, device=DEV).expand(2, 2, 128), torch.zeros(2, 128, 2, device=DEV).transpose(1, 2),
+                torch.zeros(2, 3, 128, device=DEV)[:, :2], torch.zeros(2, 2, 128, device=DEV).transpose(0, 1), good.double(), good[0],
+                good[:, :1]):
+        with pytest.raises(ValueError, match="weights"):
+            c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=bad)
+        if bad.dim() == 3 and bad.shape[1] == 2 and bad.dtype == F32:
+            with pytest.raises(ValueError, match="weights"):
+                c.codec.select_tokens(bad, c.lens, 8)
+    for bad in (torch.zeros(2, 2, 128, device=DEV), full[..., :127]):
+        with pytest.raises(ValueError, match="weights"):
+            c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=good, weights_out=bad)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=good.cpu())
+    assert not full.any()
+    _no_error()

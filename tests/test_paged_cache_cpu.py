@@ -277,3 +277,28 @@ def test_a_failed_eviction_of_a_full_pool_changes_nothing(monkeypatch, call, nth
     want = codec.summarize_pages(k, table, lens, codec.empty_summaries(8, 2))
     for r in cache._layers[0].rows:
         assert torch.equal(cache._layers[0].summaries[r], want[r])
+
+
+def test_buffers_and_tables_follow_the_tokens():
+    cache = _cache(batch=8, num_pages=8 * 64)
+    codec = cache._backend(0)._codec
+    cache.append(0, *_tokens(8, 20, 0))
+    assert cache.get_weights(0).shape == (8, 2, 32)
+    cache.attention(0, torch.zeros(8, 2, 3))
+    assert codec.seen == ((8, 2), (8, 2, 32), False)
+    cache.attention(0, torch.zeros(8, 2, 3), top_pages=2)
+    assert codec.seen == ((8, 2), (8, 2, 32), False)                     # no sequence has more than two pages
+    seen = [_content(cache, b) for b in range(8)]
+    cache.append(0, *_tokens(8, 30, 100), lengths=[30] + [0] * 7)
+    assert 64 <= cache.get_weights(0).shape[2] <= 96
+    assert [_content(cache, b) for b in range(1, 8)] == seen[1:]
+    cache.attention(0, torch.zeros(8, 2, 3), top_pages=2)
+    assert codec.seen[0] == (8, 4) and codec.seen[2]
+    _whole(cache)
+    # given a longest sequence, or where whole rows cost little beside the codes, there is one buffer for good
+    fixed = _cache(batch=8, num_pages=8 * 64, max_tokens=200)
+    fixed.append(0, *_tokens(8, 20, 0))
+    assert fixed.get_weights(0).shape == (8, 2, 13 * 16)
+    few = _cache(batch=2, num_pages=30)
+    few.append(0, *_tokens(2, 20, 0))
+    assert few.get_weights(0).shape == (2, 2, 480)
