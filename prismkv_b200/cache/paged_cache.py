@@ -305,37 +305,44 @@ class PagedKVCache:
                 self._layers.pop(layer_idx, None)
 
     def get_seq_lengths(self, layer_idx: int = 0) -> List[int]:
-        st = self._layers.get(layer_idx)
-        return [0] * self.batch if st is None else list(st.lengths)
+        with self._lock:
+            st = self._layers.get(layer_idx)
+            return [0] * self.batch if st is None else list(st.lengths)
 
     def free_pages(self, layer_idx: int = 0) -> int:
-        st = self._layers.get(layer_idx)
-        return self.num_pages if st is None else len(st.free)
+        with self._lock:
+            st = self._layers.get(layer_idx)
+            return self.num_pages if st is None else len(st.free)
 
     def get_weights(self, layer_idx: int) -> Optional[torch.Tensor]:
         """(batch, kv_heads, slots) accumulated attention weights, slots for the longest sequence at least; a
         sequence's tokens come first."""
-        return self._layer(layer_idx).weights
+        with self._lock:
+            return self._layer(layer_idx).weights
 
     def get_pages(self, layer_idx: int):
         """The device buffers: K and V pools, page table and lengths."""
-        st = self._layer(layer_idx)
-        return st.k, st.v, st.table, st.lens
+        with self._lock:
+            st = self._layer(layer_idx)
+            return st.k, st.v, st.table, st.lens
 
     @property
     def cached_layers(self) -> list:
-        return sorted(self._layers)
+        with self._lock:
+            return sorted(self._layers)
 
     def memory_footprint(self) -> dict:
         """codes_bytes (K + V codes of cached tokens), fp16_bytes (the same in FP16), compression, pool_bytes, n_layers."""
         codes = fp16 = pool = 0
-        for layer_idx, st in self._layers.items():
-            n = sum(st.lengths) * self.kv_heads
-            codes += 2 * n * st.k.shape[3] * st.k.element_size()
-            fp16 += 4 * n * self._backend(layer_idx).head_dim
-            pool += 2 * st.k.shape[0] * self.kv_heads * self.page_size * st.k.stride(2) * st.k.element_size()
+        with self._lock:
+            for layer_idx, st in self._layers.items():
+                n = sum(st.lengths) * self.kv_heads
+                codes += 2 * n * st.k.shape[3] * st.k.element_size()
+                fp16 += 4 * n * self._backend(layer_idx).head_dim
+                pool += 2 * st.k.shape[0] * self.kv_heads * self.page_size * st.k.stride(2) * st.k.element_size()
+            layers = len(self._layers)
         return {"codes_bytes": codes, "fp16_bytes": fp16, "compression": fp16 / codes if codes else float("nan"),
-                "pool_bytes": pool, "n_layers": len(self._layers)}
+                "pool_bytes": pool, "n_layers": layers}
 
     def __repr__(self) -> str:
         return (f"PagedKVCache(batch={self.batch}, kv_heads={self.kv_heads}, pages={self.num_pages}x{self.page_size}, "

@@ -302,3 +302,19 @@ def test_buffers_and_tables_follow_the_tokens():
     few = _cache(batch=2, num_pages=30)
     few.append(0, *_tokens(2, 20, 0))
     assert few.get_weights(0).shape == (2, 2, 480)
+
+
+@pytest.mark.parametrize("read", [lambda c: c.get_weights(0), lambda c: c.get_pages(0), lambda c: c.memory_footprint(),
+                                  lambda c: c.get_seq_lengths(0), lambda c: c.free_pages(0), lambda c: c.cached_layers])
+def test_readers_wait_for_a_change_in_another_thread(read):
+    """What a reader gets belongs together: not a table from before an eviction beside lengths from after it."""
+    cache = _cache()
+    cache.append(0, *_tokens(3, 5, 0))
+    got = []
+    t = threading.Thread(target=lambda: got.append(read(cache)))
+    with cache._lock:
+        t.start()
+        t.join(0.2)
+        assert t.is_alive()
+    t.join(60)
+    assert not t.is_alive() and len(got) == 1
