@@ -394,7 +394,10 @@ PKV_API int pkv_pages_summarize(const pkv_codec *c, const pkv_pages *pages, cons
  * rounded to int8 on the group's common scale (largest magnitude of the KV
  * head's query heads at 127), scores a page by
  *     max over the group's heads of sum_d (q_d > 0 ? q_d greatest_d : q_d least_d),
- * an upper bound of its tokens' scores.  The first `sinks` and the last
+ * an upper bound of the rounded query's scores with the page's tokens, in grid
+ * steps and but for the 1/256 of a step that a summary leaves out per channel
+ * (the query is rounded to nearest, so not of the query's own scores).  The
+ * first `sinks` and the last
  * `recent` pages of a sequence are always taken; the others by score, ties by
  * the lower index.  out (batch, kv_heads, top): logical page indexes,
  * ascending, -1 behind the last.  sinks + recent <= top.  With G query heads per

@@ -316,10 +316,12 @@ class PagedOps:
         """The pages worth attending to: (B, Hkv, top) int32 logical pages, ascending, -1 behind the last.
 
         The first ``sinks`` and last ``recent`` pages of a sequence are always
-        taken, the others by an upper bound of their tokens' scores: the KV
-        head's queries, rotated and rounded to int8 on a common scale, against
-        the summaries' greatest (positive) and least (negative) values; the
-        largest over the heads counts, ties go to the lower page.  A page table
+        taken, the others by the greatest score that a token within the page's
+        bounds could have: the KV head's queries, rotated and rounded to int8
+        on a common scale, against the summaries' greatest (positive) and least
+        (negative) values (an upper bound for the rounded queries, not for the
+        queries themselves); the largest over the heads counts, ties go to the
+        lower page.  A page table
         of more than about 300000 columns is refused (``pkv_pages_select`` gives
         the limit): pass the columns that the sequences use.
         """

@@ -242,3 +242,26 @@ def test_weights_in_other_strides_are_refused(cuda_ready):
         c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=good.cpu())
     assert not full.any()
     _no_error()
+
+
+@pytest.mark.parametrize("dim,bits,ps", [(96, (4, 4, 4), 16), (129, (3, 3, 2), 32), (66, (2, 5, 5), 64)])
+def test_page_score_bounds_the_rounded_query_with_every_token(cuda_ready, dim, bits, ps):
+    """A page's score is at least every token's product with the int8 query, in grid steps, but for the 1/256 of a step
+    per channel that a summary may leave out -- and the pages chosen are those of the largest scores."""
+    c = Cache(_quantizer(bits=bits, dim=dim), [700], 2, ps, seed=8)
+    sums = c.codec.summarize_pages(c.k, c.table, c.lens, c.codec.empty_summaries(c.k.shape[0], 2))
+    q = _query(1, 8, dim)
+    grid = 127 / max(c.dz.abs().max().item(), c.dxy.abs().max().item())
+    n = -(-700 // ps)
+    got = c.codec.select_pages(q, sums, c.table, c.lens, ps, 3, sinks=0, recent=0)
+    for h in range(2):
+        qr = q[0, 4 * h:4 * h + 4].double() @ c.R.T
+        qi = torch.round(qr * 127 / qr.abs().max())
+        s = sums[c.table[0, :n].long(), h].double()[..., :dim]
+        score = qi.clamp(min=0) @ s[:, 1].T + qi.clamp(max=0) @ s[:, 0].T            # (heads, pages)
+        t, k, _ = c.slots(0, h)
+        own = qi @ (k * grid).T                                                      # (heads, tokens)
+        assert (own <= score[:, t // ps] + qi.abs().sum(1, keepdim=True) / 256 * (1 + 1e-9)).all()
+        best = score.amax(0)
+        assert best[got[0, h].long()].min() == best.topk(3).values.min()
+    _no_error()
