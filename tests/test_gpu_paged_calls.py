@@ -265,3 +265,16 @@ def test_page_score_bounds_the_rounded_query_with_every_token(cuda_ready, dim, b
         best = score.amax(0)
         assert best[got[0, h].long()].min() == best.topk(3).values.min()
     _no_error()
+
+
+def test_workspace_size_is_checked(cuda_ready):
+    import ctypes
+
+    from test_paged_cpu import ALIGNMENT, WORKSPACE, _args, _codec
+
+    lib, a, c = _lib.load(), _args(), _codec()
+    need = lib.pkv_paged_attn_workspace_size(ctypes.byref(c), ctypes.byref(a))
+    assert need > 0
+    call = lambda ws, n: lib.pkv_paged_attn(ctypes.byref(c), ctypes.byref(a), ws, n, None)  # noqa: E731
+    assert call(None, 0) == WORKSPACE and call(None, need) == WORKSPACE and call(256, need - 1) == WORKSPACE
+    assert call(256 + 16, need) == ALIGNMENT
