@@ -341,7 +341,8 @@ typedef struct pkv_pages {
  * selected: optional device (batch, kv_heads, n_selected) logical page indexes,
  * strictly ascending and padded with -1; only their tokens are attended (an
  * entry not above the one before it is skipped and sets the device error word
- * to 6; a page that such a list names again further on counts again).
+ * to 6; a page that such a list names again further on counts again, and its
+ * weights are added once or as often).
  * weights / weights_out (both or neither): (batch, kv_heads, slots) f32 rows of
  * weights_row_stride floats; every attended token t gets
  *     weights_out[b, hk, t] = weights[b, hk, t] + sum over hk's query heads of p(t)

@@ -103,7 +103,7 @@ constexpr int kUnitShare = 4096;
 
 struct PagedParams {
     Pages pg;
-    int Hq, G, NB, UG, UH, dim, m, cb, gran_log2;   // NB blocks of four heads to a unit, UG units per KV head, UH = Hkv UG
+    int G, NB, UG, UH, dim, m, cb, gran_log2;   // NB blocks of four heads to a unit, UG units per KV head, UH = Hkv UG
     const void* q; int qdt; int64_t q_bs, q_hs;
     const int32_t* seq_lens;
     const int32_t* selected; int n_sel;
@@ -147,7 +147,7 @@ __device__ inline void granule_line(const PagedParams& p, int b, int64_t& before
     total = st * p.UH;
 }
 
-struct PagedItem { int b, hk, hg, unit, g0, g1, row; };     // granules [g0, g1) of the unit, partial row
+struct PagedItem { int b, hk, unit, g0, g1, row; };     // granules [g0, g1) of the unit, partial row
 
 struct PagedCut { int64_t total; int gd; bool by_unit; };
 
@@ -223,7 +223,6 @@ __device__ inline bool paged_next(const PagedParams& p, PagedCursor& c, PagedIte
         const int u = (int)(off / n);
         it.b = c.b;
         it.hk = u / p.UG;
-        it.hg = u % p.UG;
         it.unit = c.b * p.UH + u;
         it.row = x + it.unit;
         if (c.cut.by_unit) {

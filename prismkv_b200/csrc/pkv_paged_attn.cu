@@ -26,7 +26,9 @@ constexpr int kHQ = 4;                         // query heads per block: with th
 // table lookup in registers; tcgen05 wants M >= 64 and operands in shared or tensor memory, and writing the
 // decoded tiles there costs more shared-memory bandwidth than the lookups themselves.
 //
-// Numbers: every operand is an fp16 pair (hi, lo) equal to its fp32 value to 2^-22; sums are fp32.
+// Numbers: every operand is an fp16 pair (hi, lo) equal to its fp32 value to 2^-22 (weights below 2^-15 of the running
+// maximum's: to 2^-37 of that, half a step of a subnormal fp16 under the 2^12; one that rounds to zero still counts in
+// the fp32 sum of the weights); sums are fp32.
 //  * a decoded x, y (and z from a table) is a pair along the contraction: k-pair = (hi, lo);
 //  * queries and softmax weights are pairs across the eight columns: column h < 4 is head h's hi part,
 //    column h + 4 its lo part; both columns are added afterwards.  So all four cross products count.
@@ -990,7 +992,6 @@ __global__ void __launch_bounds__(kJoinThreads, CTAS) paged_join_kernel(PagedPar
 static PagedParams paged_params(const pkv_codec* c, const pkv_paged_attn_args* a, Pages pg, int sms) {
     PagedParams p{};
     p.pg = pg;
-    p.Hq = a->q_heads;
     p.G = a->q_heads / pg.Hkv;
     // Two blocks to a unit decode each code once for eight heads, on 8 warps of 255 registers.  64 query heads over 8 KV
     // heads, one block against two: head size 96, 4 x 131072 tokens 295 -> 255 us (learned codebooks 542 -> 342); head
