@@ -237,7 +237,7 @@ class PagedOps:
             slots))
         lib = _lib.load()
         # the workspace's size follows from the shapes alone
-        key = (B, Hq, kv_heads, g.page_size, g.max_pages, n_selected, w_in is None)
+        key = (B, Hq, kv_heads, g.page_size, g.max_pages, n_selected, not w_in)    # (no slots: a null pointer)
         sizes = self.__dict__.setdefault("_paged_sizes", {})
         need = sizes.get(key)
         if need is None:

@@ -279,3 +279,14 @@ def test_workspace_size_is_checked(cuda_ready):
     call = lambda ws, n: lib.pkv_paged_attn(ctypes.byref(c), ctypes.byref(a), ws, n, None)  # noqa: E731
     assert call(None, 0) == WORKSPACE and call(None, need) == WORKSPACE and call(256, need - 1) == WORKSPACE
     assert call(256 + 16, need) == ALIGNMENT
+
+
+def test_weights_of_no_slots_do_not_size_the_next_workspace(cuda_ready):
+    c = Cache(_quantizer(), [9, 0], 2, 16)
+    q = _query(2, 8, 96)
+    want = c.codec.paged_attention(q, c.k, c.v, c.table, c.lens)
+    assert torch.equal(c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=torch.empty(2, 2, 0, device=DEV)), want)
+    w = torch.zeros(2, 2, 48, device=DEV)
+    assert torch.equal(c.codec.paged_attention(q, c.k, c.v, c.table, c.lens, weights=w), want)
+    assert (w.sum(-1) - torch.tensor([[4.0], [0.0]], device=DEV)).abs().max() <= 1e-5
+    _no_error()
