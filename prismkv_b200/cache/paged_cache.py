@@ -155,19 +155,20 @@ class PagedKVCache:
             if sum(need) > len(st.free):
                 raise RuntimeError(f"layer {layer_idx}: {sum(need)} pages needed, {len(st.free)} free")
             total = sum(need)
-            fresh = iter(st.free[len(st.free) - total:][::-1])
-            rows = [r + [next(fresh) for _ in range(n)] if n else r for r, n in zip(st.rows, need)]
-            weights = self._wide_enough(st, max(map(len, rows)))
+            rows, weights = st.rows, st.weights
             if total:
+                fresh = iter(st.free[len(st.free) - total:][::-1])
+                rows = [r + [next(fresh) for _ in range(n)] for r, n in zip(rows, need)]
+                weights = self._wide_enough(st, max(map(len, rows)))
                 st.table.copy_(self._table_of(rows))
             start = st.lens.clone()
             cnt = None if lengths is None else self._ints(counts, st.lens.device)
-            lens = start + (s if cnt is None else cnt)
+            more = s if cnt is None else cnt
             codec.store_pages(codes[0], st.k, st.table, start, cnt)
             codec.store_pages(codes[1], st.v, st.table, start, cnt)
             if st.summaries is not None:
-                codec.summarize_pages(st.k, st.table, lens, st.summaries, start=start)
-            st.lens.copy_(lens)
+                codec.summarize_pages(st.k, st.table, start + more, st.summaries, start=start)
+            st.lens += more
             st.rows, st.lengths, st.weights = rows, new, weights
             del st.free[len(st.free) - total:]
             self._layers[layer_idx] = st
@@ -191,15 +192,21 @@ class PagedKVCache:
             codec = backend.codec(st.lens.device)
             qp = backend.aligner.pad(q.to(st.lens.device))
             longest, capturing = max(map(len, st.rows)), _capturing(st.lens.device)
-            # tables and weights as far as the longest sequence goes: scratch and grids go by their width. A graph will
-            # be replayed over longer ones.
-            width = self.max_pages if capturing else max(longest, 1)
-            table, weights = st.table[:, :width], st.weights
+            # Scratch and grids go by the width of the table and the weights: where that is more than twice the longest
+            # sequence, only the first columns are passed. A graph will be replayed over longer sequences.
+            width = self.max_pages if capturing or 2 * longest > self.max_pages else max(longest, 1)
+            table, weights = st.table, st.weights
             if weights is not None:
-                if capturing and weights.shape[2] < width * self.page_size:
-                    raise RuntimeError("attention captured into a graph needs weights that are not replaced as sequences "
-                                       "grow: make the cache with max_tokens")
-                weights = weights[..., :width * self.page_size]
+                slots = weights.shape[2]
+                if slots < width * self.page_size:
+                    if capturing:
+                        raise RuntimeError("attention captured into a graph needs weights that are not replaced as "
+                                           "sequences grow: make the cache with max_tokens")
+                    width = max(1, slots // self.page_size)
+                elif slots > width * self.page_size:
+                    weights = weights[..., :width * self.page_size]
+            if width < self.max_pages:
+                table = table[:, :width]
             pages = None
             if top_pages is not None:
                 if not self.page_summaries:
@@ -236,14 +243,16 @@ class PagedKVCache:
             lens = self._ints([n if n > keep else 0 for n in st.lengths], dev)
             longest = max(map(len, st.rows)) * self.page_size
             kept, kw = codec.select_tokens(st.weights[..., :longest], lens, keep, sinks=sinks, recent=recent)
-            while cut:
-                n = max(1, min(len(cut), len(st.free) // per))
-                self._move(st, codec, cut[:n], kept, kw)
-                cut = cut[n:]
+            at = 0
+            while at < len(cut):
+                n = max(1, min(len(cut) - at, len(st.free) // per))
+                self._move(st, codec, cut[at:at + n], kept, kw, n < len(cut))
+                at += n
             return list(st.lengths)
 
-    def _move(self, st: _PagedLayer, codec, group: List[int], kept: torch.Tensor, kw: torch.Tensor) -> None:
-        """Cut the group's sequences to their kept slots: into free pages or, one without room, its own first ones."""
+    def _move(self, st: _PagedLayer, codec, group: List[int], kept: torch.Tensor, kw: torch.Tensor, some: bool) -> None:
+        """Cut the group's sequences to their kept slots: into free pages or, one without room, its own first ones.
+        some: kept has slots of other sequences too."""
         dev, keep = st.lens.device, kept.shape[2]
         per = -(-keep // self.page_size)
         room = per * len(group) <= len(st.free)
@@ -251,24 +260,23 @@ class PagedKVCache:
         fresh = iter(st.free[len(st.free) - taken:][::-1])
         to = {b: [next(fresh) for _ in range(per)] if room else st.rows[b][:per] for b in group}
         table2 = torch.tensor([to.get(b, [-1] * per) for b in range(self.batch)], dtype=torch.int32, device=dev)
-        others = torch.tensor([b not in to for b in range(self.batch)], device=dev).view(-1, 1, 1)
-        picks = kept.masked_fill(others, -1)
+        picks = kept.masked_fill(table2[:, :1, None] < 0, -1) if some else kept
         rows = [to.get(b, r) for b, r in enumerate(st.rows)]
         lengths = [keep if b in to else n for b, n in enumerate(st.lengths)]
         table, lens = self._table_of(rows).to(dev), self._ints(lengths, dev)
-        start = self._ints([0 if b in to else n for b, n in enumerate(lengths)], dev)
         if room:
             codec.gather_tokens(st.k, st.v, st.table, picks, st.k, st.v, table2)
             if st.summaries is not None:
+                start = self._ints([0 if b in to else n for b, n in enumerate(lengths)], dev)
                 codec.summarize_pages(st.k, table, lens, st.summaries, start=start)
         else:                                             # all that can fail comes before the pages are written over
             k, v = (codec.empty_pages(per, self.kv_heads, self.page_size, st.k.dtype) for _ in range(2))
             side = torch.tensor([list(range(per)) if b in to else [-1] * per for b in range(self.batch)], dtype=torch.int32,
                                 device=dev)
-            order = torch.arange(keep, dtype=torch.int32, device=dev).expand(kept.shape).masked_fill(others, -1)
+            order = torch.arange(keep, dtype=torch.int32, device=dev).expand(kept.shape).masked_fill(picks < 0, -1)
             codec.gather_tokens(st.k, st.v, st.table, picks, k, v, side)
             if st.summaries is not None:
-                sums = codec.summarize_pages(k, side, lens.masked_fill(others.view(-1), 0),
+                sums = codec.summarize_pages(k, side, lens.masked_fill(table2[:, 0] < 0, 0),
                                              codec.empty_summaries(per, self.kv_heads))
             codec.gather_tokens(k, v, side, order, st.k, st.v, table2)
             if st.summaries is not None:

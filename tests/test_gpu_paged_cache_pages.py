@@ -138,3 +138,21 @@ def test_capture_with_buffers_that_may_grow_is_refused(cuda_ready):
         with torch.cuda.graph(g):
             cache.attention(0, q)
     assert torch.equal(cache.attention(0, q), want)
+
+
+def test_a_growing_cache_without_tokens(cuda_ready):
+    backend = PrismKVBackend(PrismKVConfig(), head_dim=96)
+    cache = PagedKVCache(backend, 12, 2, num_pages=240, page_size=16, page_summaries=True, track_weights=True)
+    none = torch.empty(12, 2, 0, 96, device=DEV)
+    assert cache.append(0, none, none) == [0] * 12
+    q = _q(12, 4, 96)
+    assert not cache.attention(0, q).any() and not cache.attention(0, q, top_pages=2).any()
+    assert cache.evict(0, 1, sinks=0, recent=0) == [0] * 12
+    k, v = _kv(12, 2, 3, 96, 0)
+    assert cache.append(0, k, v, lengths=[3] + [0] * 11) == [3] + [0] * 11
+    raw = RawKVCache(backend)
+    raw.append(0, k[:1], v[:1])
+    out = cache.attention(0, q)
+    assert (out[0] - raw.attention(0, q[:1])[0]).abs().max() <= 1e-4 and not out[1:].any()
+    assert (cache.get_weights(0)[0, :, :3].sum(-1) - 2).abs().max() <= 1e-5 and not cache.get_weights(0)[1:].any()
+    assert _lib.device_error() == 0
