@@ -8,9 +8,10 @@
 // paged_query_kernel rotates the queries into operand fragments, paged_attn_kernel leaves one partial
 // state per (CTA, unit) range, paged_join_kernel joins a unit's ranges, normalises and rotates back (and,
 // in further CTAs, adds the weights from the scores that the second launch kept).  Small calls are bound by
-// the chain of memory round trips through the three (16 us for 37 tokens of 8 heads), large ones by the issue
-// slots of the decode (4 x 131072 tokens, 32 query over 8 KV heads, head size 96, two-byte codes: 162 us, 3.3 TB/s,
-// half of the copy rate; 395 instructions per 16 tokens, 56 % of the slots used, tensor pipe 23 %).
+// the chain of memory round trips through the three (16 us for 37 tokens of 8 heads), large ones by the decode's
+// dependent chain at four warps per scheduler (4 x 131072 tokens, 32 query over 8 KV heads, head size 96, two-byte codes:
+// 163 us, 3.3 TB/s, half of the copy rate; 398 instructions per 16 tokens, issue slots 56 % used, shared-memory pipe 61 %,
+// tensor pipe 22 %).
 
 #include "pkv_paged.cuh"
 
@@ -1048,10 +1049,12 @@ static int launch_paged_as(const PagedParams& p, cudaStream_t st) {
 }
 
 // EX: fp32 results -- outputs, or the running weights whatever type the outputs have -- get z from the middle bin and the
-// tiles' sums added in rounded fp32 (4 x 131072 tokens: 180 us against 163; the weights' error 6e-7 relative against 2e-6
+// tiles' sums added in rounded fp32 (4 x 131072 tokens: 178 us against 163; the weights' error 6e-7 relative against 2e-6
 // to 6e-6). For 16-bit outputs alone the truncation of the running sums (a few 1e-6) is far below their own rounding.
 // Warps by what a lane holds: 16 of 128 registers for up to 32 triplets (14 take 10 % longer, 10 take 20 %), 12 of 168
-// up to 48 (16 spill: + 9 %; 10: + 12 %), 8 of 255 up to 64 (12: + 7 %).
+// up to 48 (16: + 9 %; 10: + 12 %), 8 of 255 up to 64 (12: + 7 %). They are what measured best, spills and all: bytes
+// of spill stores with 16-bit outputs 12 to 76 (16 warps), 0 to 20 (12) and 0 (8); with EX 92 to 180, 40 to 56 and 0;
+// of the two-block forms 0 to 24 and, with EX, 0 to 296.
 template <int MODE, bool EX>
 static int launch_paged_mode(const PagedParams& p, cudaStream_t st) {
     if (p.m <= 32)
@@ -1079,8 +1082,8 @@ static int launch_join(const PagedParams& p, int64_t tokens, int sms, cudaStream
 }
 
 // With weights: a third CTA per multiprocessor in place of registers where two leave more than three waves of 1536
-// tokens: 128 rows of 16384 tokens 126 -> 120 us in all.  With fewer the join's rows of R count for more: 32 rows of
-// 11469 to 16384 tokens (head size 129) 61.5 us with two, 65.5 with three.
+// tokens: 128 rows of 16384 tokens 136 -> 129 us in all.  With fewer the join's rows of R count for more: 32 rows of
+// 11469 to 16384 tokens (head size 129) 64.9 us with two, 68.6 with three.
 static int launch_weigh(const PagedParams& p, int sms, cudaStream_t st) {
     const int64_t tokens = p.raw_us / p.raw_h;              // room for every slot that the table (or the list) can name
     const int64_t tiles = (int64_t)p.pg.B * p.pg.Hkv * ((tokens + 1535) / 1536);

@@ -112,8 +112,9 @@ __global__ void __launch_bounds__(256) tokens_gather_kernel(Pages s, Pages d, ui
 // load covers 32 / LPT tokens; a lane keeps, per code, the least and greatest (x, y) as packed 16-bit pairs and
 // of z the least and greatest bin (grid values rise with the bin).  (x, y) come from shared memory: up to 256
 // entries in 32 copies, one per lane, so that lookups never collide; more entries in one copy, with conflicts.
-// Issue slots bound it (7 instructions a code, and 160 a page for the reduction and the stores): 268 MB of codes in
-// pages of 32 tokens take 94 us.
+// Memory latency bounds it -- a warp waits for a page's codes before it asks for the next page's -- at 63 % of the issue
+// slots (7 instructions a code and lane, and about 300 a page for the reduction, the stores and the loop): 268 MB of codes
+// in pages of 32 tokens take 94 us.
 struct SummaryParams {
     Pages pg;
     const int32_t *seq_lens, *start;
