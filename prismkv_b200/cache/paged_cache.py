@@ -214,7 +214,7 @@ class PagedKVCache:
                 if top_pages < 1 or sinks < 0 or recent < 0 or sinks + recent > top_pages:
                     raise ValueError("need 0 <= sinks + recent <= top_pages and top_pages >= 1, "
                                      f"got {sinks}, {recent}, {top_pages}")
-                if longest > top_pages or capturing:
+                if (self.max_pages if capturing else longest) > top_pages:
                     pages = codec.select_pages(qp, st.summaries, table, st.lens, self.page_size, top_pages, sinks=sinks,
                                                recent=recent)
             out = codec.paged_attention(qp, st.k, st.v, table, st.lens, scale=scale, pages=pages, weights=weights,
